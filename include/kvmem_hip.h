@@ -536,6 +536,173 @@ typedef struct kvmem_hip_meank_args {
 
 KVMEM_HIP_API int kvmem_hip_score_meank(kvmem_hip_ctx *ctx, const kvmem_hip_meank_args *args);
 
+/* --------------------------------------------- new tokens and attention */
+
+/* The calls of a decode or prefill batch over the pool: kvmem_hip_slot_map
+ * (where the batch's tokens go), then per layer kvmem_hip_qkv_rows (their rows
+ * into the pool) and kvmem_hip_attention (the batch's queries over the pool's
+ * rows).  Lengths, tables and cells stay in device memory and no call waits
+ * for the host, so a batch can be captured into a graph and replayed with
+ * other contents.  In the reference these are llama.cpp's own graph (the
+ * KV cache's cells and its flash attention over quantized rows); the window
+ * they work on is the one the reselect path fills. */
+
+/* A table entry without a slot: its keys do not exist. */
+#define KVMEM_HIP_NO_SLOT 0xffffffffu
+
+/* Block tables, cells and positions of the new tokens of `n_seq` requests
+ * (at most 4096; KVMEM_HIP_ERR_UNSUPPORTED beyond) that share one pool, from
+ * their lengths.  Request s has kv_len[s] tokens in its blocks and brings
+ * n_new[s] more; block b of request s lives in slot table[s*table_stride + b].
+ * Blocks a request starts take the next entries of free_slots, request by
+ * request, block by block:
+ *   table         new blocks' entries are written, all others stay.  A block
+ *                 gets KVMEM_HIP_NO_SLOT when the free list is exhausted; a
+ *                 block beyond table_stride has no entry.
+ *   kv_len_out[s] = kv_len[s] + n_new[s]
+ *   q_start       [n_seq + 1]: first token of each request, then their number
+ *   positions[t]  pos0[s] + i for token i of request s (pos0 NULL: kv_len[s])
+ *   cells[t]      slot * block_tokens + offset, -1 where the block has no slot
+ *   free_used_out entries of free_slots taken so far (free_used + the new ones)
+ *   n_missing     blocks that got no slot or no entry
+ * positions and cells have max_tokens entries; those behind the last token are
+ * 0 and -1, and tokens beyond max_tokens get none.  An entry of free_slots or
+ * table at or beyond n_slots counts as no slot (it is still used up).  Every
+ * array is device memory, 4-byte aligned; outputs do not overlap inputs
+ * (table is both).  The call is idempotent: repeated with the same inputs it
+ * writes the same values. */
+typedef struct kvmem_hip_slot_map_args {
+    uint32_t n_seq;
+    uint32_t block_tokens;
+    uint32_t n_slots;          /* slots of the pool; n_slots*block_tokens < 2^31 */
+    uint32_t table_stride;     /* entries per request; n_seq*table_stride < 2^32 */
+    uint32_t max_tokens;
+    uint32_t n_free;           /* entries of free_slots */
+    const uint32_t *n_new;     /* [n_seq] */
+    const uint32_t *kv_len;    /* [n_seq] */
+    const int32_t *pos0;       /* [n_seq] or NULL */
+    const uint32_t *free_slots;/* [n_free] */
+    const uint32_t *free_used; /* [1] */
+    uint32_t *table;           /* [n_seq][table_stride] */
+    uint32_t *kv_len_out;      /* [n_seq] */
+    uint32_t *q_start;         /* [n_seq + 1] */
+    int32_t *positions;        /* [max_tokens] */
+    int32_t *cells;            /* [max_tokens] */
+    uint32_t *free_used_out;   /* [1] */
+    uint32_t *n_missing;       /* [1] */
+} kvmem_hip_slot_map_args;
+
+KVMEM_HIP_API int kvmem_hip_slot_map(kvmem_hip_ctx *ctx, const kvmem_hip_slot_map_args *args);
+
+/* Rows of new tokens, from a layer's projections to attention's inputs, in
+ * one pass.  Per head of q and k:
+ *   y = x / sqrt(mean(x^2) + eps) * weight   (weight NULL: y = x)
+ *   q_norm / k_norm (if set) receive y: the pre-RoPE rows that
+ *     kvmem_hip_q_window_write and the raw history take
+ *   RoPE and the Walsh-Hadamard rotation of the transform, as the stage-in
+ *     applies them (kvmem_hip_transform; hadamard_k for q and k, hadamard_v
+ *     for v), at positions[t]
+ *   q_out / k_out (if set) receive the result, contiguous
+ *     [n_tokens][heads][head_dim] of out_type
+ * With a pool, k and v rows are quantized into row cells[t] of layer `layer`'s
+ * tensors (n_embd_k = n_embd_v = n_head_kv*head_dim); cells outside the pool
+ * (-1) keep nothing.  Two tokens with the same cell leave one of their rows'
+ * bytes in each part of it.  The transform is `xf`, or the pool's where xf is
+ * NULL (its pos0 is not read); a pool passed for k and v whose rows the
+ * stage-in also writes wants the same transform for both.
+ * q, k, v (any may be NULL) are strided device views: element (d, h, t) at
+ * d*size + h*nb1 + t*nb2 bytes; 16-byte aligned views are read 16 bytes at a
+ * time.  Sums of squares are fp32; rows are fp32 until they are stored, each
+ * output rounded once (nearest even).  Outputs are 16-byte aligned and do not
+ * overlap inputs.  head_dim 64, 128, 256 or 512; at most 2^26 tokens. */
+typedef struct kvmem_hip_qkv_args {
+    const void *q;
+    const void *k;
+    const void *v;
+    int32_t type;              /* of q, k, v: F32, F16 or BF16 */
+    int32_t out_type;          /* of q_out, k_out, q_norm, k_norm */
+    uint32_t n_tokens;
+    uint32_t n_head;
+    uint32_t n_head_kv;
+    uint32_t head_dim;
+    size_t q_nb1, q_nb2;       /* bytes between heads, between tokens */
+    size_t k_nb1, k_nb2;
+    size_t v_nb1, v_nb2;
+    const float *q_weight;     /* device [head_dim], 16-byte aligned */
+    const float *k_weight;
+    float eps;
+    const int32_t *positions;  /* device [n_tokens] (NULL without RoPE) */
+    const int32_t *cells;      /* device [n_tokens] (NULL without a pool) */
+    const kvmem_hip_transform *xf;
+    void *q_out;
+    void *k_out;
+    void *q_norm;
+    void *k_norm;
+} kvmem_hip_qkv_args;
+
+KVMEM_HIP_API int kvmem_hip_qkv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_pool *pool, uint32_t layer,
+                                     const kvmem_hip_qkv_args *args);
+
+/* Attention of new tokens over the pool's rows.  Token i of request s (its
+ * m = q_start[s+1] - q_start[s] tokens are the last m of its kv_len[s] keys)
+ * attends, in query head h, the keys of KV head h / (n_head/n_head_kv):
+ *   key j < kv_len[s], and j <= kv_len[s] - m + i if causal, that
+ *   table[s*table_stride + j/block_tokens] gives a slot
+ *   out = sum_j softmax_j(scale * q . K_j) V_j
+ * K_j, V_j being the values row slot*block_tokens + j%block_tokens of layer
+ * `layer` stands for (Q4_0, Q5_0, Q8_0 or F16, K and V each their own).  Keys
+ * were rotated when they were written (and with hadamard_k, which
+ * kvmem_hip_qkv_rows applies to q as well); where the pool's transform has
+ * hadamard_v, the output is rotated back to the value's own coordinates.
+ * A query without any key gets zeros and lse -inf.  Rows of out and lse behind
+ * the last request's tokens are left as they are, and rows of the pool that
+ * hold no key are not read.
+ *   q       strided device view, element (d, h, t) at d*2 + h*nb1 + t*nb2
+ *           bytes, 16-byte aligned (strides too)
+ *   out     contiguous [n_tokens][n_head][head_dim], 16-byte aligned
+ *   lse     [n_tokens][n_head] log of the softmax's sum, or NULL
+ * q_start NULL: request s has token s.  A request's tokens beyond max_q or
+ * n_tokens, and keys beyond max_kv or the table, are not attended (both bounds
+ * size the launch; device lengths beyond them never reach out of range).
+ * Scores, softmax statistics and sums are fp32.  Rounded on the way: cached
+ * values to f16 once they are scaled (so values beyond f16's range become
+ * infinite), and softmax weights to f16.
+ * head_dim 64, 128 or 256, any n_head that is a multiple of n_head_kv.
+ * Keys are split over workgroups when there are few queries; the parts are
+ * joined from a workspace: the caller's (kvmem_hip_attention_workspace bytes,
+ * 16-byte aligned, contents free) or, where it is NULL, one the context keeps
+ * and grows.  A captured call must bring its own (KVMEM_HIP_ERR_INVALID
+ * otherwise): graphs that can be replayed at the same time need one each.
+ * Results do not depend on the order in which workgroups run. */
+typedef struct kvmem_hip_attn_args {
+    const void *q;
+    int32_t q_type;            /* F16 or BF16 */
+    int32_t out_type;          /* F32, F16 or BF16 */
+    size_t q_nb1, q_nb2;       /* bytes between heads, between tokens */
+    void *out;
+    float *lse;
+    uint32_t n_tokens;         /* tokens of q and out */
+    uint32_t n_seq;
+    uint32_t max_q;            /* most tokens of one request */
+    uint32_t max_kv;           /* most keys of one request */
+    uint32_t n_head;
+    uint32_t n_head_kv;
+    uint32_t head_dim;
+    uint32_t table_stride;
+    const uint32_t *q_start;   /* device [n_seq + 1] or NULL */
+    const uint32_t *kv_len;    /* device [n_seq], the new tokens included */
+    const uint32_t *table;     /* device [n_seq][table_stride] */
+    int32_t causal;
+    float scale;               /* 0 = 1/sqrt(head_dim) */
+    void *workspace;
+    size_t workspace_bytes;
+} kvmem_hip_attn_args;
+
+/* Workspace bytes of a call with these arguments (0 = none needed). */
+KVMEM_HIP_API size_t kvmem_hip_attention_workspace(const kvmem_hip_pool *pool, const kvmem_hip_attn_args *args);
+KVMEM_HIP_API int kvmem_hip_attention(kvmem_hip_ctx *ctx, const kvmem_hip_pool *pool, uint32_t layer,
+                                      const kvmem_hip_attn_args *args);
+
 /* -------------------------------------------------------- self-check */
 
 /* Check, on this device and over every float of their ranges, the two

@@ -33,6 +33,7 @@ TYPE_Q4_0 = 2
 TYPE_Q5_0 = 6
 TYPE_Q8_0 = 8
 TYPE_BF16 = 30
+NO_SLOT = 0xffffffff  # a block table's entry without a slot (KVMEM_HIP_NO_SLOT)
 TYPE_NAMES = {TYPE_F16: "f16", TYPE_Q4_0: "q4_0", TYPE_Q5_0: "q5_0", TYPE_Q8_0: "q8_0"}
 GROUP_BYTES = {TYPE_Q8_0: 34, TYPE_Q4_0: 18, TYPE_Q5_0: 22, TYPE_F16: 64}
 
@@ -114,6 +115,37 @@ class MeanKArgs(C.Structure):
                 ("mean_tokens", C.c_void_p), ("n_layers", C.c_uint32), ("n_blocks", C.c_uint32),
                 ("capacity_blocks", C.c_uint32), ("n_head", C.c_uint32), ("n_head_kv", C.c_uint32),
                 ("head_dim", C.c_uint32), ("scores", C.c_void_p)]
+
+
+class SlotMapArgs(C.Structure):
+    """kvmem_hip_slot_map_args; device pointers as integers (keyword arguments)."""
+    _fields_ = [("n_seq", C.c_uint32), ("block_tokens", C.c_uint32), ("n_slots", C.c_uint32),
+                ("table_stride", C.c_uint32), ("max_tokens", C.c_uint32), ("n_free", C.c_uint32),
+                ("n_new", C.c_void_p), ("kv_len", C.c_void_p), ("pos0", C.c_void_p), ("free_slots", C.c_void_p),
+                ("free_used", C.c_void_p), ("table", C.c_void_p), ("kv_len_out", C.c_void_p),
+                ("q_start", C.c_void_p), ("positions", C.c_void_p), ("cells", C.c_void_p),
+                ("free_used_out", C.c_void_p), ("n_missing", C.c_void_p)]
+
+
+class QkvArgs(C.Structure):
+    """kvmem_hip_qkv_args; device pointers as integers (keyword arguments)."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int32),
+                ("out_type", C.c_int32), ("n_tokens", C.c_uint32), ("n_head", C.c_uint32),
+                ("n_head_kv", C.c_uint32), ("head_dim", C.c_uint32), ("q_nb1", C.c_size_t), ("q_nb2", C.c_size_t),
+                ("k_nb1", C.c_size_t), ("k_nb2", C.c_size_t), ("v_nb1", C.c_size_t), ("v_nb2", C.c_size_t),
+                ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("eps", C.c_float), ("positions", C.c_void_p),
+                ("cells", C.c_void_p), ("xf", C.POINTER(Transform)), ("q_out", C.c_void_p), ("k_out", C.c_void_p),
+                ("q_norm", C.c_void_p), ("k_norm", C.c_void_p)]
+
+
+class AttnArgs(C.Structure):
+    """kvmem_hip_attn_args; device pointers as integers (keyword arguments)."""
+    _fields_ = [("q", C.c_void_p), ("q_type", C.c_int32), ("out_type", C.c_int32), ("q_nb1", C.c_size_t),
+                ("q_nb2", C.c_size_t), ("out", C.c_void_p), ("lse", C.c_void_p), ("n_tokens", C.c_uint32),
+                ("n_seq", C.c_uint32), ("max_q", C.c_uint32), ("max_kv", C.c_uint32), ("n_head", C.c_uint32),
+                ("n_head_kv", C.c_uint32), ("head_dim", C.c_uint32), ("table_stride", C.c_uint32),
+                ("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("table", C.c_void_p), ("causal", C.c_int32),
+                ("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 class ReserveArgs(C.Structure):
@@ -238,6 +270,10 @@ def load_library(path: os.PathLike | str | None = None) -> C.CDLL:
     _sig(lib, "kvmem_hip_q_window_gather", i32, vp, vp, C.c_uint32, C.c_uint32, C.c_uint32,
          C.POINTER(C.c_uint32), C.c_uint32, i32, vp)
     _sig(lib, "kvmem_hip_transfer_get", i32, vp, C.POINTER(TransferStats))
+    _sig(lib, "kvmem_hip_slot_map", i32, vp, C.POINTER(SlotMapArgs))
+    _sig(lib, "kvmem_hip_qkv_rows", i32, vp, C.POINTER(Pool), u32, C.POINTER(QkvArgs))
+    _sig(lib, "kvmem_hip_attention_workspace", sz, C.POINTER(Pool), C.POINTER(AttnArgs))
+    _sig(lib, "kvmem_hip_attention", i32, vp, C.POINTER(Pool), u32, C.POINTER(AttnArgs))
     if path is None:
         _lib = lib
     return lib
@@ -458,6 +494,24 @@ class Context:
         self.check(self.lib.kvmem_hip_topk(self.h, scores_ptr, n, f, nf, need, int(tie_lower_index),
                                            out, C.byref(cnt)), "topk")
         return out[: cnt.value]
+
+    # -- new tokens and attention (argument blocks can be built once and reused)
+    def slot_map(self, args: SlotMapArgs) -> None:
+        """Block tables, cells and positions of a batch's new tokens."""
+        self.check(self.lib.kvmem_hip_slot_map(self.h, C.byref(args)), "slot_map")
+
+    def qkv_rows(self, args: QkvArgs, pool: "Pool | None" = None, layer: int = 0) -> None:
+        """Norm, RoPE and rotation of new tokens' rows; k and v into the pool's cells."""
+        self.check(self.lib.kvmem_hip_qkv_rows(self.h, C.byref(pool) if pool is not None else None, layer,
+                                               C.byref(args)), "qkv_rows")
+
+    def attention_workspace(self, args: AttnArgs, pool: Pool) -> int:
+        """Workspace bytes of attention(args, pool) (0: none needed)."""
+        return self.lib.kvmem_hip_attention_workspace(C.byref(pool), C.byref(args))
+
+    def attention(self, args: AttnArgs, pool: Pool, layer: int = 0) -> None:
+        """Attention of new tokens over the pool's rows."""
+        self.check(self.lib.kvmem_hip_attention(self.h, C.byref(pool), layer, C.byref(args)), "attention")
 
     # -- mean-K cosine scorer (reference semantics)
     def meank_sums(self, hist: History, block_ids, k_sum_ptr: int, mean_tokens_ptr: int) -> None:

@@ -43,6 +43,7 @@ EXTRA = {
     "stagein.hip": ["-ffp-contract=off"],
     "score.hip": ["-ffinite-math-only"],
     "meank.hip": ["-ffp-contract=off"],
+    "qkv_rows.hip": ["-ffp-contract=off"],
 }
 
 

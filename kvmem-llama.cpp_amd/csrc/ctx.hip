@@ -484,6 +484,7 @@ int kvmem_hip_create(int device, kvmem_hip_ctx **out) {
         hipStreamCreateWithFlags(&ctx->copy_stream, hipStreamNonBlocking) != hipSuccess ||
         !load_ctx_kernels() || !load_meank_kernels() || !load_score_kernels() ||
         !load_stagein_kernels() || !load_topk_kernels() || !load_qwindow_kernels() ||
+        !load_slot_map_kernels() || !load_qkv_rows_kernels() || !load_attention_kernels() ||
         !score_scratch_setup(ctx)) {
         kvmem_hip_destroy(ctx);
         return KVMEM_HIP_ERR_RUNTIME;
@@ -510,7 +511,8 @@ void kvmem_hip_destroy(kvmem_hip_ctx *ctx) {
         if (s.done) (void) hipEventDestroy(s.done);
     }
     for (DevBuf *b : {&ctx->score_partial, &ctx->score_layers, &ctx->meank_scratch,
-                      &ctx->move_scratch, &ctx->h2d_ring, &ctx->d2h_ring, &ctx->topk_dev, &ctx->plan}) {
+                      &ctx->move_scratch, &ctx->attn_scratch, &ctx->h2d_ring, &ctx->d2h_ring, &ctx->topk_dev,
+                      &ctx->plan}) {
         if (b->ptr) (void) hipFree(b->ptr);
     }
     if (ctx->topk_sel_host.ptr) (void) hipHostFree(ctx->topk_sel_host.ptr);
@@ -648,7 +650,7 @@ int kvmem_hip_scratch_info(const kvmem_hip_ctx *ctx, kvmem_hip_scratch *out) {
         pin += s.host.bytes;
     }
     for (const DevBuf *b : {&ctx->score_partial, &ctx->score_layers, &ctx->meank_scratch,
-                            &ctx->move_scratch, &ctx->h2d_ring, &ctx->d2h_ring}) {
+                            &ctx->move_scratch, &ctx->attn_scratch, &ctx->h2d_ring, &ctx->d2h_ring}) {
         dev += b->bytes;
     }
     pin += ctx->topk_sel_host.bytes;

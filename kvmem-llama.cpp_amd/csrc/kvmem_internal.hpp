@@ -68,6 +68,7 @@ struct kvmem_hip_ctx {
     kvmem_hip::DevBuf score_layers;     // [L][B] f32 when the caller passes none
     kvmem_hip::DevBuf meank_scratch;    // mean-K scorer: layer cosines, query vectors
     kvmem_hip::DevBuf move_scratch;     // gathered slots for kvmem_hip_move_slots
+    kvmem_hip::DevBuf attn_scratch;     // parts of split attention rows
     // Selection written by the top-k kernel straight into coherent pinned
     // host memory: [n] ids, [n] count, and a completion word the kernel
     // sets to topk_epoch after the rest is visible (topk_flag_index).
@@ -381,6 +382,9 @@ bool load_score_kernels();
 bool load_stagein_kernels();
 bool load_topk_kernels();
 bool load_qwindow_kernels();
+bool load_slot_map_kernels();
+bool load_qkv_rows_kernels();
+bool load_attention_kernels();
 // Looks up, once per device (the context's, made current by the caller),
 // the device address of the static scratch array of
 // kvmem_hip_score_noalloc and keeps it in ctx->noalloc_scratch.
