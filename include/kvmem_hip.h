@@ -667,7 +667,8 @@ KVMEM_HIP_API int kvmem_hip_qkv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_pool *p
  * Scores, softmax statistics and sums are fp32.  Rounded on the way: cached
  * values to f16 once they are scaled (so values beyond f16's range become
  * infinite), and softmax weights to f16.
- * head_dim 64, 128 or 256, any n_head that is a multiple of n_head_kv.
+ * head_dim 64, 128 or 256, any n_head that is a multiple of n_head_kv; at most
+ * 65535 requests, 2^23 (token, head) rows and 2^31 - 1 keys a request.
  * Keys are split over workgroups when there are few queries; the parts are
  * joined from a workspace: the caller's (kvmem_hip_attention_workspace bytes,
  * 16-byte aligned, contents free) or, where it is NULL, one the context keeps

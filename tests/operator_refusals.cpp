@@ -173,7 +173,7 @@ static void attention() {
     call("out address", inv, [](Args &a, kvmem_hip_pool &) { a.out = OFF4; });
     call("lse address", inv, [](Args &a, kvmem_hip_pool &) { a.lse = static_cast<float *>(OFF1); });
     call("too many requests", inv, [](Args &a, kvmem_hip_pool &) { a.n_seq = 65536, a.n_tokens = 65536; });
-    call("too many tokens", inv, [](Args &a, kvmem_hip_pool &) { a.n_tokens = (1u << 24) + 1; });
+    call("too many tokens", inv, [](Args &a, kvmem_hip_pool &) { a.n_tokens = (1u << 20) + 1; });
     call("too many keys", inv, [](Args &a, kvmem_hip_pool &) { a.max_kv = 0x80000000u; });
     call("negative scale", inv, [](Args &a, kvmem_hip_pool &) { a.scale = -1.0f; });
     call("NaN scale", inv, [](Args &a, kvmem_hip_pool &) { a.scale = __builtin_nanf(""); });

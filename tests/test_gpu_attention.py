@@ -201,6 +201,69 @@ def test_repeats_bit_for_bit(ctx, oracle):
             assert torch.equal(c.run().out, a)
 
 
+def test_workspace_and_allocations(ctx, oracle):
+    """The caller's workspace gives the context's results; a second call of the same size allocates nothing."""
+    for m in (1, 30):
+        c = Case(ctx, oracle, [9000, 400], [m, m], 8, 2, 128, 64, seed=27)
+        need = ctx.attention_workspace(c.args, c.pool_c)
+        assert need > 0
+        want = c.run().out.clone()
+        before = ctx.scratch_info()["allocations"]
+        c.out.fill_(0)
+        assert torch.equal(c.run().out, want)
+        assert ctx.scratch_info()["allocations"] == before
+        ws = torch.full((need + 64,), 0x7F, dtype=torch.uint8, device="cuda")
+        c.args.workspace, c.args.workspace_bytes = ws.data_ptr(), need
+        c.out.fill_(0)
+        assert torch.equal(c.run().out, want)
+        assert (ws[need:] == 0x7F).all()
+
+
+@pytest.mark.parametrize("m", [1, 30])
+def test_captured_call(ctx, oracle, m):
+    """Two graphs with a workspace each, replayed by turns and together, follow the lengths and queries they find."""
+    say("graphs", m)
+    cs = [Case(ctx, oracle, [3000, 400], [m, m], 8, 2, 64, 64, seed=28 + i) for i in range(2)]
+    eager = [c.run().out.clone() for c in cs]
+    streams = [torch.cuda.Stream() for _ in cs]
+    graphs, keep = [], []
+    try:
+        for c, st in zip(cs, streams):
+            need = ctx.attention_workspace(c.args, c.pool_c)
+            ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+            keep.append(ws)
+            ctx.set_stream(st.cuda_stream)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                with pytest.raises(kv.KvMemError):
+                    ctx.attention(c.args, c.pool_c, 1)  # no workspace of its own
+                c.args.workspace, c.args.workspace_bytes = ws.data_ptr(), need
+                ctx.attention(c.args, c.pool_c, 1)
+            graphs.append(g)
+        ctx.set_stream(None)
+        for step in range(4):
+            for c in cs:
+                c.out.fill_(0)
+            torch.cuda.synchronize()
+            for g, st in zip(graphs, streams):  # both in flight
+                with torch.cuda.stream(st):
+                    g.replay()
+            torch.cuda.synchronize()
+            for c, e in zip(cs, eager):
+                assert torch.equal(c.out, e), step
+            # shorter requests and other queries for the next replay
+            for i, c in enumerate(cs):
+                c.lens = [a - 301 if a > 400 else a - 40 for a in c.lens]
+                c.dev["lens"].copy_(torch.tensor(c.lens, dtype=torch.int32))
+                c.q.neg_()
+                c.q_host = -c.q_host
+                c.out.fill_(0)
+                c.run().check()
+                eager[i] = c.out.clone()
+    finally:
+        ctx.set_stream(None)
+
+
 def test_other_stream(ctx, oracle):
     """On a caller's stream, behind work queued there."""
     c = Case(ctx, oracle, [300, 90], [1, 1], 4, 2, 64, 32, seed=30)
