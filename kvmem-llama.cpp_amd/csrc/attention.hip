@@ -12,13 +12,16 @@ typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
-constexpr uint32_t kTileKeys = 32;   // keys of one wave's step
+constexpr uint32_t kTileKeys = 32;   // keys of one prefill step
 constexpr uint32_t kRowTile = 16;    // query rows of a workgroup
 constexpr uint32_t kWaves = 4;
 constexpr uint32_t kNoCell = 0xffffffffu;
-// log2 of the factor the softmax weights carry before they are rounded to
-// f16: weights down to 2^-24 of the largest stay normal numbers.
-constexpr float kWeightShift = 10.0f;
+// Softmax weights are 2^(x - top + shift) before they are rounded to f16.  A
+// row's `top` follows its maximum only when that has grown by more than
+// kTopSlack (log2), so the sums are rarely scaled down again; weights then stay
+// below 2^15, and those down to 2^-20 of 2^top are normal f16 numbers.
+constexpr float kWeightShift = 6.0f;
+constexpr float kTopSlack = 9.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnParams {
@@ -87,7 +90,9 @@ struct Slice {
     // LDS bytes between keys: f16 rows are padded so that 16 keys' reads
     // spread over the banks
     static constexpr uint32_t stride = TYPE == KVMEM_TYPE_F16 ? bytes + 16 : bytes;
-    static constexpr uint32_t loads = (kTileKeys * units + 63) / 64;
+    // a wave's load moves whole slices, one lane a unit (the last lanes idle):
+    // the addresses of its loads then differ by constants
+    static constexpr uint32_t per_load = 64 / units;
 };
 
 template <uint32_t UNIT> struct UnitOf;
@@ -95,11 +100,38 @@ template <> struct UnitOf<4> { typedef uint32_t type; };
 template <> struct UnitOf<8> { typedef u32x2_t type; };
 template <> struct UnitOf<16> { typedef u32x4_t type; };
 
-struct __attribute__((packed, aligned(2))) Word2 { uint32_t v; };
-struct __attribute__((packed, aligned(2))) Long2 { uint64_t v; };
-__device__ inline uint32_t lds_word(const uint8_t *p) { return reinterpret_cast<const Word2 *>(p)->v; }
-__device__ inline uint64_t lds_long(const uint8_t *p) { return reinterpret_cast<const Long2 *>(p)->v; }
 __device__ inline uint32_t lds_half(const uint8_t *p) { return *reinterpret_cast<const uint16_t *>(p); }
+
+// N words of LDS from an even address.  Groups of 18, 22 and 34 bytes put every
+// other group's codes 2 bytes off a word; the LDS answers such reads at a
+// fraction of its rate (stalls were three quarters of a step's time), so words are
+// read where they are aligned and shifted together.  The word after the last is
+// read too.
+template <int N>
+__device__ inline void lds_words(const uint8_t *p, uint32_t shift, uint32_t out[N]) {
+    const uint32_t *q = reinterpret_cast<const uint32_t *>(p - shift);
+    uint32_t w[N + 1];
+#pragma unroll
+    for (int i = 0; i <= N; ++i) {
+        w[i] = q[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        out[i] = __builtin_amdgcn_alignbyte(w[i + 1], w[i], shift);
+    }
+}
+// The same where the shift is known: 2 bytes (OFF) or none.
+template <int N, bool OFF>
+__device__ inline void lds_words(const uint8_t *p, uint32_t out[N]) {
+    if constexpr (OFF) {
+        lds_words<N>(p, 2u, out);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            out[i] = reinterpret_cast<const uint32_t *>(p)[i];
+        }
+    }
+}
 
 // Key operand of one group of 32 dims: the 8 elements a lane (key, chunk c of
 // 4) feeds the matrix instruction, as f16.  Quantized codes stay integers:
@@ -109,6 +141,7 @@ __device__ inline uint32_t lds_half(const uint8_t *p) { return *reinterpret_cast
 // that meets it is divided by 16.  The code's offset (8, 16, 128) comes off
 // through the accumulator's start, the group's scale is multiplied into the
 // fp32 sum: keys enter the scores unrounded.
+// OFF: the group's codes lie 2 bytes off a word (groups of even number).
 // Element e is dim piece(c, i) + l % 4 of the group, l = order(e) and i = l / 4:
 // a lane's 8 dims are two runs of four.
 template <int TYPE> struct KeyOp;
@@ -116,8 +149,10 @@ template <int TYPE> struct KeyOp;
 template <> struct KeyOp<KVMEM_TYPE_Q4_0> {
     static constexpr float offset = 8.0f;
     static constexpr bool codes = true;
+    template <bool OFF>
     __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c) {
-        const uint32_t w = lds_word(g + 2 + 4 * c);
+        uint32_t w;
+        lds_words<1, OFF>(g + 2 + 4 * c, &w);
         u32x4_t r;
         r[0] = w & 0x000F000Fu;
         r[1] = w & 0x00F000F0u;
@@ -134,9 +169,12 @@ template <> struct KeyOp<KVMEM_TYPE_Q4_0> {
 template <> struct KeyOp<KVMEM_TYPE_Q5_0> {
     static constexpr float offset = 16.0f;
     static constexpr bool codes = true;
+    template <bool OFF>
     __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c) {
-        const uint32_t h = lds_word(g + 2) >> (4 * c);
-        const uint32_t w = lds_word(g + 6 + 4 * c);
+        uint32_t h, w;
+        lds_words<1, OFF>(g + 2, &h);
+        lds_words<1, OFF>(g + 6 + 4 * c, &w);
+        h >>= 4 * c;
         // bits 0 and 2 of a 4-bit field to bits 4 and 20 (8 and 24 for the
         // upper nibbles): two shifted copies in one product, no carries
         const uint32_t lo = (h & 15u) * 0x00040010u;
@@ -156,10 +194,12 @@ template <> struct KeyOp<KVMEM_TYPE_Q5_0> {
 template <> struct KeyOp<KVMEM_TYPE_Q8_0> {
     static constexpr float offset = 128.0f;
     static constexpr bool codes = true;
+    template <bool OFF>
     __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c) {
-        const uint64_t w = lds_long(g + 2 + 8 * c) ^ 0x8080808080808080ull;
-        const uint32_t a = static_cast<uint32_t>(w);
-        const uint32_t b = static_cast<uint32_t>(w >> 32);
+        uint32_t w[2];
+        lds_words<2, OFF>(g + 2 + 8 * c, w);
+        const uint32_t a = w[0] ^ 0x80808080u;
+        const uint32_t b = w[1] ^ 0x80808080u;
         u32x4_t r;
         r[0] = a & 0x00FF00FFu;
         r[1] = (a >> 8) & 0x00FF00FFu;
@@ -175,6 +215,7 @@ template <> struct KeyOp<KVMEM_TYPE_Q8_0> {
 template <> struct KeyOp<KVMEM_TYPE_F16> {
     static constexpr float offset = 0.0f;
     static constexpr bool codes = false;
+    template <bool OFF>
     __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c) {
         return *reinterpret_cast<const u32x4_t *>(g + 16 * c);
     }
@@ -182,6 +223,12 @@ template <> struct KeyOp<KVMEM_TYPE_F16> {
     __device__ static constexpr uint32_t order(uint32_t e) { return e; }
     __device__ static constexpr float times(uint32_t) { return 1.0f; }
 };
+
+// The operand of group g of a key's slice (an unrolled g).
+template <class KO, uint32_t GB>
+__device__ inline u32x4_t load_key(const uint8_t *slice, int g, uint32_t c) {
+    return (g & 1) ? KO::template load<false>(slice + g * GB, c) : KO::template load<true>(slice + g * GB, c);
+}
 
 __device__ inline half2_t as_half2(uint32_t w) { return __builtin_bit_cast(half2_t, w); }
 __device__ inline uint32_t as_word(half2_t h) { return __builtin_bit_cast(uint32_t, h); }
@@ -207,8 +254,9 @@ __device__ inline uint32_t pair_value_hi(uint32_t codes, float offset, uint32_t 
 // hold consecutive dims of one key and the matrix instruction wants
 // consecutive keys of one dim, so a lane reads its dims of 8 keys and pairs
 // keys with byte permutes, still in packed codes (a nibble permute moves 8
-// elements).  raw(): a key's words and scale; emit(f): f(t, operand) for each of
-// the VD dims;  dim(n, t): which dim that is.
+// elements).  raw(): the keys' words and scales; emit(keep, f): f(t,
+// operands of dims t .. t + 3) over the VD dims, keys cleared in `keep` (16 bits a
+// key, pairs as the operand's words) as zeros;  dim(n, t): which dim t is.
 template <int TYPE, int D> struct ValueOp;
 
 template <int D>
@@ -216,7 +264,6 @@ struct ValueOp<KVMEM_TYPE_Q4_0, D> {
     static constexpr int VD = D / 16;
     static constexpr int NB = VD / 2;  // bytes of codes
     static constexpr int NW = NB < 4 ? 1 : NB / 4;
-    static constexpr uint32_t kHead = 2;
     static constexpr float offset = 8.0f;
     uint32_t w[8][NW];
     uint32_t d[4];
@@ -227,18 +274,15 @@ struct ValueOp<KVMEM_TYPE_Q4_0, D> {
     template <class RowOf>
     __device__ inline void raw(uint32_t n, RowOf row) {
         constexpr uint32_t per = 32 / VD;
+        const uint32_t off = 2u * (~(n / per) & 1u);  // of the lane's group's codes in a word
         uint32_t s[8];
 #pragma unroll
         for (uint32_t e = 0; e < 8; ++e) {
             const uint8_t *g = row(e) + (n / per) * 18u;
             s[e] = lds_half(g);
             const uint8_t *b = g + 2 + NB * (n % per);
-            if constexpr (NB == 8) {
-                const uint64_t x = lds_long(b);
-                w[e][0] = static_cast<uint32_t>(x);
-                w[e][1] = static_cast<uint32_t>(x >> 32);
-            } else if constexpr (NB == 4) {
-                w[e][0] = lds_word(b);
+            if constexpr (NB >= 4) {
+                lds_words<NW>(b, off, w[e]);
             } else {
                 w[e][0] = lds_half(b);
             }
@@ -249,25 +293,22 @@ struct ValueOp<KVMEM_TYPE_Q4_0, D> {
         }
     }
     template <class F>
-    __device__ inline void emit(F f) const {
+    __device__ inline void emit(const u32x4_t &keep, F f) const {
+        const u32x4_t ds{d[0] & keep[0], d[1] & keep[1], d[2] & keep[2], d[3] & keep[3]};
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
 #pragma unroll
             for (int h = 0; h < (NB < 4 ? 1 : 2); ++h) {
-                u32x4_t a, b, c, e;
+                u32x4_t a[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t t = h ? pair_hi(w[2 * j][i], w[2 * j + 1][i]) : pair_lo(w[2 * j][i], w[2 * j + 1][i]);
-                    a[j] = pair_value(t & 0x000F000Fu, offset, d[j]);
-                    b[j] = pair_value_hi(t & 0x00F000F0u, offset, d[j]);
-                    c[j] = pair_value((t >> 8) & 0x000F000Fu, offset, d[j]);
-                    e[j] = pair_value_hi((t >> 8) & 0x00F000F0u, offset, d[j]);
+                    a[0][j] = pair_value(t & 0x000F000Fu, offset, ds[j]);
+                    a[1][j] = pair_value_hi(t & 0x00F000F0u, offset, ds[j]);
+                    a[2][j] = pair_value((t >> 8) & 0x000F000Fu, offset, ds[j]);
+                    a[3][j] = pair_value_hi((t >> 8) & 0x00F000F0u, offset, ds[j]);
                 }
-                const int t0 = 8 * i + 4 * h;
-                f(t0, a);
-                f(t0 + 1, b);
-                f(t0 + 2, c);
-                f(t0 + 3, e);
+                f(8 * i + 4 * h, a);
             }
         }
     }
@@ -286,19 +327,17 @@ struct ValueOp<KVMEM_TYPE_Q5_0, D> {
     template <class RowOf>
     __device__ inline void raw(uint32_t n, RowOf row) {
         constexpr uint32_t per = 32 / VD;
+        const uint32_t off = 2u * (~(n / per) & 1u);  // of the lane's group's codes in a word
         uint32_t s[8];
 #pragma unroll
         for (uint32_t e = 0; e < 8; ++e) {
             const uint8_t *g = row(e) + (n / per) * 22u;
             s[e] = lds_half(g);
-            h[e] = lds_word(g + 2) >> (NB * (n % per));
+            lds_words<1>(g + 2, off, &h[e]);
+            h[e] >>= NB * (n % per);
             const uint8_t *b = g + 6 + NB * (n % per);
-            if constexpr (NB == 8) {
-                const uint64_t x = lds_long(b);
-                w[e][0] = static_cast<uint32_t>(x);
-                w[e][1] = static_cast<uint32_t>(x >> 32);
-            } else if constexpr (NB == 4) {
-                w[e][0] = lds_word(b);
+            if constexpr (NB >= 4) {
+                lds_words<NW>(b, off, w[e]);
             } else {
                 w[e][0] = lds_half(b);
             }
@@ -309,7 +348,8 @@ struct ValueOp<KVMEM_TYPE_Q5_0, D> {
         }
     }
     template <class F>
-    __device__ inline void emit(F f) const {
+    __device__ inline void emit(const u32x4_t &keep, F f) const {
+        const u32x4_t ds{d[0] & keep[0], d[1] & keep[1], d[2] & keep[2], d[3] & keep[3]};
         // the fifth bits of a key pair, in the halves of one word
         uint32_t lo[4], hi[4];
 #pragma unroll
@@ -321,23 +361,19 @@ struct ValueOp<KVMEM_TYPE_Q5_0, D> {
         for (int i = 0; i < NW; ++i) {
 #pragma unroll
             for (int q = 0; q < (NB < 4 ? 1 : 2); ++q) {
-                u32x4_t a, b, c, e;
+                u32x4_t a[4];
                 const int b0 = 4 * i + 2 * q;  // byte of the lane's codes
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t t = q ? pair_hi(w[2 * j][i], w[2 * j + 1][i]) : pair_lo(w[2 * j][i], w[2 * j + 1][i]);
-                    a[j] = pair_value((t & 0x000F000Fu) | (((lo[j] >> b0) & 0x00010001u) << 4), offset, d[j]);
-                    b[j] = pair_value_hi((t & 0x00F000F0u) | (((hi[j] >> b0) & 0x00010001u) << 8), offset, d[j]);
-                    c[j] = pair_value(((t >> 8) & 0x000F000Fu) | (((lo[j] >> (b0 + 1)) & 0x00010001u) << 4), offset,
-                                      d[j]);
-                    e[j] = pair_value_hi(((t >> 8) & 0x00F000F0u) | (((hi[j] >> (b0 + 1)) & 0x00010001u) << 8), offset,
-                                         d[j]);
+                    a[0][j] = pair_value((t & 0x000F000Fu) | (((lo[j] >> b0) & 0x00010001u) << 4), offset, ds[j]);
+                    a[1][j] = pair_value_hi((t & 0x00F000F0u) | (((hi[j] >> b0) & 0x00010001u) << 8), offset, ds[j]);
+                    a[2][j] = pair_value(((t >> 8) & 0x000F000Fu) | (((lo[j] >> (b0 + 1)) & 0x00010001u) << 4), offset,
+                                      ds[j]);
+                    a[3][j] = pair_value_hi(((t >> 8) & 0x00F000F0u) | (((hi[j] >> (b0 + 1)) & 0x00010001u) << 8), offset,
+                                         ds[j]);
                 }
-                const int t0 = 8 * i + 4 * q;
-                f(t0, a);
-                f(t0 + 1, b);
-                f(t0 + 2, c);
-                f(t0 + 3, e);
+                f(8 * i + 4 * q, a);
             }
         }
     }
@@ -353,21 +389,16 @@ struct ValueOp<KVMEM_TYPE_Q8_0, D> {
     template <class RowOf>
     __device__ inline void raw(uint32_t n, RowOf row) {
         constexpr uint32_t per = 32 / VD;
+        const uint32_t off = 2u * (~(n / per) & 1u);  // of the lane's group's codes in a word
         uint32_t s[8];
 #pragma unroll
         for (uint32_t e = 0; e < 8; ++e) {
             const uint8_t *g = row(e) + (n / per) * 34u;
             s[e] = lds_half(g);
-            const uint8_t *b = g + 2 + VD * (n % per);
-            if constexpr (NW == 1) {
-                w[e][0] = lds_word(b) ^ 0x80808080u;
-            } else {
+            lds_words<NW>(g + 2 + VD * (n % per), off, w[e]);
 #pragma unroll
-                for (int i = 0; i < NW; i += 2) {
-                    const uint64_t x = lds_long(b + 4 * i) ^ 0x8080808080808080ull;
-                    w[e][i] = static_cast<uint32_t>(x);
-                    w[e][i + 1] = static_cast<uint32_t>(x >> 32);
-                }
+            for (int i = 0; i < NW; ++i) {
+                w[e][i] ^= 0x80808080u;
             }
         }
 #pragma unroll
@@ -376,20 +407,21 @@ struct ValueOp<KVMEM_TYPE_Q8_0, D> {
         }
     }
     template <class F>
-    __device__ inline void emit(F f) const {
+    __device__ inline void emit(const u32x4_t &keep, F f) const {
+        const u32x4_t ds{d[0] & keep[0], d[1] & keep[1], d[2] & keep[2], d[3] & keep[3]};
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
+            u32x4_t a[4];
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                u32x4_t a;
                 // byte b of both keys, zero-extended to 16 bits
                 const uint32_t sel = 0x0c000c00u | static_cast<uint32_t>(b) | (static_cast<uint32_t>(4 + b) << 16);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    a[j] = pair_value(__builtin_amdgcn_perm(w[2 * j + 1][i], w[2 * j][i], sel), 128.0f, d[j]);
+                    a[b][j] = pair_value(__builtin_amdgcn_perm(w[2 * j + 1][i], w[2 * j][i], sel), 128.0f, ds[j]);
                 }
-                f(4 * i + b, a);
             }
+            f(4 * i, a);
         }
     }
 };
@@ -422,17 +454,18 @@ struct ValueOp<KVMEM_TYPE_F16, D> {
         }
     }
     template <class F>
-    __device__ inline void emit(F f) const {
+    __device__ inline void emit(const u32x4_t &keep, F f) const {
 #pragma unroll
-        for (int i = 0; i < NW; ++i) {
-            u32x4_t a, b;
+        for (int i = 0; i < NW; i += 2) {
+            u32x4_t a[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                a[j] = pair_lo(w[2 * j][i], w[2 * j + 1][i]);
-                b[j] = pair_hi(w[2 * j][i], w[2 * j + 1][i]);
+                a[0][j] = pair_lo(w[2 * j][i], w[2 * j + 1][i]) & keep[j];
+                a[1][j] = pair_hi(w[2 * j][i], w[2 * j + 1][i]) & keep[j];
+                a[2][j] = pair_lo(w[2 * j][i + 1], w[2 * j + 1][i + 1]) & keep[j];
+                a[3][j] = pair_hi(w[2 * j][i + 1], w[2 * j + 1][i + 1]) & keep[j];
             }
             f(2 * i, a);
-            f(2 * i + 1, b);
         }
     }
 };
@@ -447,6 +480,26 @@ __device__ inline float lane_xor32(float v) { return __shfl_xor(v, 32, 64); }
 
 __device__ inline float lane_xor8(float v) {
     return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xF, 0xF, true));  // row_ror:8
+}
+
+// The keys of a block of 32 that exist and lie below `limit` (counted from the
+// block's first key), for a lane whose element e of the block's operand is key
+// 16 (e / 4) + first + e % 4: bit 16 (e / 4) + e % 4.
+__device__ inline uint32_t seen_keys(uint32_t have, int32_t limit, uint32_t first) {
+    const int32_t left = limit - static_cast<int32_t>(first);
+    const uint32_t below = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;
+    return (have >> first) & below;
+}
+
+// Operand masks of those keys: 16 bits a key, pairs as the operand's words.
+__device__ inline u32x4_t keep_keys(uint32_t seen) {
+    u32x4_t keep;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t two = seen >> (16u * (j >> 1) + 2u * (j & 1u));
+        keep[j] = (two & 1u) * 0x0000ffffu + ((two >> 1) & 1u) * 0xffff0000u;
+    }
+    return keep;
 }
 
 // A wave's LDS writes become visible to its own later reads, in order.
@@ -466,29 +519,37 @@ __device__ inline void store_elem(uint8_t *out, int type, uint64_t i, float x) {
     }
 }
 
-// The lane's 8 query elements of a group, in the key operand's order.
+// A lane's 8 query elements of a group as they lie in memory (f16 or bf16 bits).
 template <class KO>
-__device__ inline void load_query(const AttnParams &p, const uint8_t *q, uint32_t g, uint32_t c, float x[8]) {
-    float v[8];
-#pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-        const u32x2_t w = *reinterpret_cast<const u32x2_t *>(q + 64u * g + 2u * KO::piece(c, i));
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            if (p.q_bf16) {
-                v[4 * i + 2 * j] = __uint_as_float(w[j] << 16);
-                v[4 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-            } else {
-                const half2_t h = as_half2(w[j]);
-                v[4 * i + 2 * j] = static_cast<float>(h[0]);
-                v[4 * i + 2 * j + 1] = static_cast<float>(h[1]);
-            }
-        }
-    }
+__device__ inline u32x4_t load_query(const uint8_t *q, uint32_t g, uint32_t c) {
+    const u32x2_t a = *reinterpret_cast<const u32x2_t *>(q + 64u * g + 2u * KO::piece(c, 0));
+    const u32x2_t b = *reinterpret_cast<const u32x2_t *>(q + 64u * g + 2u * KO::piece(c, 1));
+    return u32x4_t{a[0], a[1], b[0], b[1]};
+}
+
+// The larger magnitudes of two pairs (bits: both formats order as integers).
+__device__ inline uint32_t max_magnitude(uint32_t a, uint32_t b) {
+    typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a & 0x7fff7fffu),
+                                                                  __builtin_bit_cast(u16x2_t, b)));
+}
+
+template <bool BF16>
+__device__ inline float query_value(uint32_t bits) {
+    return BF16 ? __uint_as_float(bits << 16)
+                : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+}
+
+// f16 queries in the key operand's order, times `up`.
+template <class KO, bool BF16>
+__device__ inline half8_t query_operand(const u32x4_t &w, float up) {
+    half8_t r;
 #pragma unroll
     for (uint32_t e = 0; e < 8; ++e) {
-        x[e] = v[KO::order(e)];
+        const uint32_t l = KO::order(e);
+        r[e] = static_cast<_Float16>(query_value<BF16>((l & 1u) ? w[l >> 1] >> 16 : w[l >> 1] & 0xffffu) * up);
     }
+    return r;
 }
 
 // Exponent of the power of two that brings a row's largest query magnitude to
@@ -497,7 +558,7 @@ __device__ inline int query_shift(float top) {
     int ex = 0;
     if (top > 0.0f && top < INFINITY) {
         (void) frexpf(top, &ex);
-        ex = 9 - ex;
+        ex = min(9 - ex, 120);  // the power itself stays a normal float
     }
     return ex;
 }
@@ -519,26 +580,43 @@ __device__ inline float rotate_back(float x, uint32_t width, uint32_t d, float *
 
 // ------------------------------------------------------------ few queries
 
+// Keys of a wave's step: about the same bytes for every head size (9 KiB of
+// q4_0 keys and values), enough in flight per compute unit to stream.
+template <int D>
+constexpr uint32_t decode_keys() { return 32u * (256 / D); }
+
 template <int TK, int TV, int D>
 constexpr uint32_t decode_wave_bytes() {
-    return kTileKeys * (Slice<TK, D>::stride + Slice<TV, D>::stride) + D / 32 * kTileKeys * 2;
+    return decode_keys<D>() * (Slice<TK, D>::stride + Slice<TV, D>::stride + (KeyOp<TK>::codes ? D / 16 : 0));
 }
 
 // Rows of one KV head's queries over one part of a request's keys: up to 16
-// (token, head) rows, keys split over the workgroup's four waves in steps of
-// 32.  Scores are held transposed (keys by rows) so that a lane owns one
-// query row: S^T = K Q^T, O^T = V^T P^T, and a lane's 8 weights of S^T are
-// its operand of the second product as they stand.
+// (token, head) rows, keys split over the workgroup's four waves.  Scores are
+// held transposed (keys by rows) so that a lane owns one query row: S^T = K Q^T,
+// O^T = V^T P^T, and a lane's weights of S^T are its operand of the second
+// product as they stand.
+// Two waves per SIMD, but for 16-bit rows of 256: their step's rows take half the
+// registers, and one wave has as many bytes in flight.
+constexpr int decode_occupancy(int tk, int tv, int d) {
+    return d == 256 && (tk == KVMEM_TYPE_F16 || tv == KVMEM_TYPE_F16) ? 1 : 2;
+}
+
 template <int TK, int TV, int D>
-__global__ __launch_bounds__(256) void attn_decode_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_kernel(AttnParams p) {
     using SK = Slice<TK, D>;
     using SV = Slice<TV, D>;
     using KO = KeyOp<TK>;
     using VO = ValueOp<TV, D>;
     constexpr int NG = D / 32;
     constexpr int VD = D / 16;
+    constexpr uint32_t KT = decode_keys<D>();
+    constexpr int NT = KT / 16;  // key tiles of a step
+    constexpr uint32_t NC = KT > 64 ? KT / 64 : 1;  // keys a lane finds the cells of
+    constexpr uint32_t NLK = (KT + SK::per_load - 1) / SK::per_load;  // loads of a step
+    constexpr uint32_t NLV = (KT + SV::per_load - 1) / SV::per_load;
     typedef typename UnitOf<SK::unit>::type UK;
     typedef typename UnitOf<SV::unit>::type UV;
+    typedef uint16_t scales_t __attribute__((ext_vector_type(NG)));
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ float2 wave_ml[kWaves][kRowTile];
 
@@ -558,9 +636,10 @@ __global__ __launch_bounds__(256) void attn_decode_kernel(AttnParams p) {
         return;
     }
     const uint32_t rows = min(kRowTile, m * p.group - row0);
-    // keys any of these rows attends
-    const uint32_t n = key_limit(p, r, (row0 + rows - 1u) / p.group);
-    const uint32_t n_all = key_limit(p, r, row0 / p.group);  // keys all of them attend
+    const uint32_t tok0 = row0 / p.group;  // first and last token of the rows
+    const uint32_t tok1 = (row0 + rows - 1u) / p.group;
+    const uint32_t n = key_limit(p, r, tok1);      // keys any of them attends
+    const uint32_t n_all = key_limit(p, r, tok0);  // keys all of them attend
     const uint32_t n_parts = max(1u, (n + p.chunk - 1u) / p.chunk);
     if (part >= n_parts) {
         return;
@@ -569,117 +648,143 @@ __global__ __launch_bounds__(256) void attn_decode_kernel(AttnParams p) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t nl = lane & 15u;   // query row; dim lane of the values
     const uint32_t c = lane >> 4;     // chunk of the contraction
-    // up to 8 rows: each stands in two columns, for the upper and the lower
-    // half of its weights' digits
-    const bool twice = rows <= 8u;
-    const uint32_t my_row = row0 + min(twice ? (nl & 7u) : nl, rows - 1u);
-    const uint32_t my_tok = my_row / p.group;
-    const uint32_t my_head = hk * p.group + (my_row - my_tok * p.group);
-    const uint32_t limit = key_limit(p, r, my_tok);
-    const uint32_t tok0 = row0 / p.group;  // first and last token of the rows
-    const uint32_t tok1 = (row0 + rows - 1u) / p.group;
-
-    // The row's queries: scaled by a power of two to at most 2^9, so that f16
-    // holds them whatever their exponents.
-    half8_t qf[NG];
-    float q_off[NG];
-    float fac;
-    {
-        const uint8_t *q = p.q + static_cast<uint64_t>(r.first + my_tok) * p.q_nb2 + my_head * p.q_nb1;
-        float x[NG][8];
-        float most = 0.0f;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            load_query<KO>(p, q, g, c, x[g]);
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) {
-                most = fmaxf(most, fabsf(x[g][e]));
-            }
-        }
-        most = fmaxf(most, lane_xor16(most));
-        most = fmaxf(most, lane_xor32(most));
-        const int ex = query_shift(most);
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            float all = 0.0f;
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) {
-                const _Float16 h = static_cast<_Float16>(ldexpf(x[g][e], ex));
-                all += static_cast<float>(h);
-                qf[g][e] = static_cast<_Float16>(static_cast<float>(h) / KO::times(e));
-            }
-            all += lane_xor16(all);
-            all += lane_xor32(all);
-            q_off[g] = -KO::offset * all * 0x1p-24f;
-        }
-        fac = ldexpf(p.scale * kLog2e, (KO::codes ? 24 : 0) - ex);
-    }
-
-    uint8_t *kt = lds + wave * decode_wave_bytes<TK, TV, D>();
-    uint8_t *vt = kt + kTileKeys * SK::stride;
-    _Float16 *ks = reinterpret_cast<_Float16 *>(vt + kTileKeys * SV::stride);  // key scales [group][key]
-
     const uint32_t c0 = part * p.chunk;
     const uint32_t c1 = min(n, c0 + p.chunk);
     const uint8_t *k_head = p.k + static_cast<uint64_t>(hk) * SK::bytes;
     const uint8_t *v_head = p.v + static_cast<uint64_t>(hk) * SV::bytes;
     const uint32_t *table = p.table + static_cast<uint64_t>(s) * p.table_stride;
-    const uint32_t my_key = lane & (kTileKeys - 1u);
 
-    // The cell of this lane's key of the tile at j0 (kNoCell: no such key).
-    auto cell_of = [&](uint32_t j0) {
-        const uint32_t j = j0 + my_key;
-        if (j >= c1) {
-            return kNoCell;
-        }
-        const uint32_t b = j / p.T;
-        const uint32_t slot = table[b];
-        return slot < p.n_slots ? slot * p.T + (j - b * p.T) : kNoCell;
+    // The cells of this lane's keys of the step at j0, and which keys exist
+    // (bit = key); one that does not has cell 0, and is masked where it matters.
+    struct Cells {
+        uint32_t at[NC];
+        uint64_t have[NC];
     };
-    UK rk[SK::loads];
-    UV rv[SV::loads];
-    auto load_tile = [&](uint32_t cell) {
+    auto cells_of = [&](uint32_t j0) {
+        Cells r;
 #pragma unroll
-        for (uint32_t i = 0; i < SK::loads; ++i) {
-            const uint32_t u = i * 64u + lane;
-            const uint32_t key = u / SK::units;
-            const uint32_t at = __shfl(cell, key & (kTileKeys - 1u), 64);
-            rk[i] = UK{};
-            if (key < kTileKeys && at != kNoCell) {
-                rk[i] = *reinterpret_cast<const UK *>(k_head + static_cast<uint64_t>(at) * p.row_k +
-                                                      (u - key * SK::units) * SK::unit);
+        for (uint32_t i = 0; i < NC; ++i) {
+            const uint32_t j = j0 + (lane & (KT - 1u)) + 64u * i;
+            uint32_t slot = KVMEM_HIP_NO_SLOT;
+            const uint32_t b = j / p.T;
+            if (j < c1) {
+                slot = table[b];
             }
+            r.at[i] = slot < p.n_slots ? slot * p.T + (j - b * p.T) : 0u;
+            r.have[i] = __ballot(slot < p.n_slots);
         }
-#pragma unroll
-        for (uint32_t i = 0; i < SV::loads; ++i) {
-            const uint32_t u = i * 64u + lane;
-            const uint32_t key = u / SV::units;
-            const uint32_t at = __shfl(cell, key & (kTileKeys - 1u), 64);
-            rv[i] = UV{};
-            if (key < kTileKeys && at != kNoCell) {
-                rv[i] = *reinterpret_cast<const UV *>(v_head + static_cast<uint64_t>(at) * p.row_v +
-                                                      (u - key * SV::units) * SV::unit);
-            }
-        }
+        return r;
     };
-    auto put_tile = [&]() {
+    auto cell_at = [&](const Cells &cells, uint32_t key) {
+        uint32_t at = __shfl(cells.at[0], key & (KT - 1u) & 63u, 64);
+        if constexpr (NC == 2) {
+            const uint32_t hi = __shfl(cells.at[1], key & 63u, 64);
+            at = key < 64u ? at : hi;
+        }
+        return at;
+    };
+    const uint32_t kk = lane / SK::units;  // this lane's key and unit of a load
+    const uint32_t ku = min(kk, SK::per_load - 1u) == kk ? lane - kk * SK::units : 0u;
+    const uint32_t vk = lane / SV::units;
+    const uint32_t vu = min(vk, SV::per_load - 1u) == vk ? lane - vk * SV::units : 0u;
+    UK rk[NLK];
+    UV rv[NLV];
+    auto load_tile = [&](const Cells &cells) {
 #pragma unroll
-        for (uint32_t i = 0; i < SK::loads; ++i) {
-            const uint32_t u = i * 64u + lane;
-            const uint32_t key = u / SK::units;
-            if (key < kTileKeys) {
-                *reinterpret_cast<UK *>(kt + key * SK::stride + (u - key * SK::units) * SK::unit) = rk[i];
-            }
+        for (uint32_t i = 0; i < NLK; ++i) {
+            const uint32_t at = cell_at(cells, kk + i * SK::per_load);
+            rk[i] = *reinterpret_cast<const UK *>(k_head + static_cast<uint64_t>(at) * p.row_k + ku * SK::unit);
         }
 #pragma unroll
-        for (uint32_t i = 0; i < SV::loads; ++i) {
-            const uint32_t u = i * 64u + lane;
-            const uint32_t key = u / SV::units;
-            if (key < kTileKeys) {
-                *reinterpret_cast<UV *>(vt + key * SV::stride + (u - key * SV::units) * SV::unit) = rv[i];
-            }
+        for (uint32_t i = 0; i < NLV; ++i) {
+            const uint32_t at = cell_at(cells, vk + i * SV::per_load);
+            rv[i] = *reinterpret_cast<const UV *>(v_head + static_cast<uint64_t>(at) * p.row_v + vu * SV::unit);
         }
     };
+    constexpr uint32_t step = kWaves * KT;
+    uint32_t j0 = c0 + wave * KT;
+    Cells cells = cells_of(j0);
+
+    // up to 8 rows: each stands in two columns, for the upper and the lower
+    // digits of its weights
+    const bool twice = rows <= 8u;
+    const uint32_t my_row = row0 + min(twice ? (nl & 7u) : nl, rows - 1u);
+    const uint32_t my_tok = my_row / p.group;
+    const uint32_t my_head = hk * p.group + (my_row - my_tok * p.group);
+    const uint32_t limit = key_limit(p, r, my_tok);
+
+    // The row's queries, scaled into f16's range.  Codes carry an offset: the
+    // sum of a group's queries times it comes off each score, as one more product
+    // of the groups' scales with those sums (in three f16 pieces, 33 bits).
+    half8_t qf[NG];
+    half8_t q_off;
+    float fac;
+    {
+        const uint8_t *q = p.q + static_cast<uint64_t>(r.first + my_tok) * p.q_nb2 + my_head * p.q_nb1;
+        u32x4_t x[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            x[g] = load_query<KO>(q, g, c);
+        }
+        load_tile(cells);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                bits = max_magnitude(x[g][i], bits);
+            }
+        }
+        bits = max(bits & 0xffffu, bits >> 16);
+        float most = p.q_bf16 ? query_value<true>(bits) : query_value<false>(bits);
+        most = fmaxf(most, lane_xor16(most));
+        most = fmaxf(most, lane_xor32(most));
+        const int ex = query_shift(most);
+        const float up = ldexpf(1.0f, ex);
+        if (p.q_bf16) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                qf[g] = query_operand<KO, true>(x[g], up);
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                qf[g] = query_operand<KO, false>(x[g], up);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            q_off[e] = 0;
+        }
+        if constexpr (KO::codes) {
+            // piece c of the sum stands in chunk c of the contraction
+            const _Float16 pick[3] = {static_cast<_Float16>(c == 0 ? 1.0f : 0.0f),
+                                      static_cast<_Float16>(c == 1 ? 1.0f : 0.0f),
+                                      static_cast<_Float16>(c == 2 ? 1.0f : 0.0f)};
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                float all = 0.0f;
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) {
+                    all += static_cast<float>(qf[g][e]);
+                    qf[g][e] *= static_cast<_Float16>(1.0f / KO::times(e));
+                }
+                all += lane_xor16(all);
+                all += lane_xor32(all);
+                all *= -KO::offset * 0x1p-10f;
+                const _Float16 hi = static_cast<_Float16>(all);
+                const float left = all - static_cast<float>(hi);
+                const _Float16 mid = static_cast<_Float16>(left);
+                const _Float16 lo = static_cast<_Float16>(left - static_cast<float>(mid));
+                q_off[g] = hi * pick[0] + mid * pick[1] + lo * pick[2];
+            }
+        }
+        fac = ldexpf(p.scale * kLog2e, (KO::codes ? 24 : 0) - ex);
+    }
+
+    uint8_t *kt = lds + wave * decode_wave_bytes<TK, TV, D>();
+    uint8_t *vt = kt + KT * SK::stride;
+    scales_t *ks = reinterpret_cast<scales_t *>(vt + KT * SV::stride);  // [key] scales of its groups
 
     float top = -INFINITY;  // of the row, log2 units
     float sum = 0.0f;       // of this lane's weights
@@ -689,112 +794,176 @@ __global__ __launch_bounds__(256) void attn_decode_kernel(AttnParams p) {
         o[t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    constexpr uint32_t step = kWaves * kTileKeys;
-    uint32_t j0 = c0 + wave * kTileKeys;
-    uint32_t cell = cell_of(j0);
-    load_tile(cell);
-    uint32_t next = cell_of(j0 + step);
+    Cells next = cells_of(j0 + step);
     for (; j0 < c1; j0 += step) {
-        const uint32_t have = static_cast<uint32_t>(__ballot(cell != kNoCell));  // bit = key (lanes 0..31)
-        wave_lds_sync();  // the last tile's reads are done
-        put_tile();
-        wave_lds_sync();
-        cell = next;
-        load_tile(cell);
-        next = cell_of(j0 + 2u * step);
-        if constexpr (KO::codes) {
+        const Cells now = cells;
+        bool whole = true;
 #pragma unroll
-            for (uint32_t i = 0; i < (NG * kTileKeys + 63u) / 64u; ++i) {
-                const uint32_t u = i * 64u + lane;
-                if (u < NG * kTileKeys) {
-                    const uint32_t key = u & (kTileKeys - 1u);
-                    const uint32_t g = u / kTileKeys;
-                    reinterpret_cast<uint16_t *>(ks)[g * kTileKeys + key] =
-                        static_cast<uint16_t>(lds_half(kt + key * SK::stride + g * SK::GB));
+        for (uint32_t i = 0; i < NC; ++i) {
+            whole = whole && now.have[i] == ~0ull;
+        }
+        wave_lds_sync();  // the last step's reads are done
+        if (kk < SK::per_load) {
+#pragma unroll
+            for (uint32_t i = 0; i < NLK; ++i) {
+                const uint32_t key = kk + i * SK::per_load;
+                if ((i + 1) * SK::per_load <= KT || key < KT) {
+                    *reinterpret_cast<UK *>(kt + key * SK::stride + ku * SK::unit) = rk[i];
+                }
+            }
+        }
+        if (vk < SV::per_load) {
+#pragma unroll
+            for (uint32_t i = 0; i < NLV; ++i) {
+                const uint32_t key = vk + i * SV::per_load;
+                if ((i + 1) * SV::per_load <= KT || key < KT) {
+                    *reinterpret_cast<UV *>(vt + key * SV::stride + vu * SV::unit) = rv[i];
+                }
+            }
+        }
+        wave_lds_sync();
+        cells = next;
+        load_tile(cells);
+        next = cells_of(j0 + 2u * step);
+        if constexpr (KO::codes) {
+            // a key's scales side by side
+            for (uint32_t key = lane % KT; key < KT; key += 64u) {
+                constexpr uint32_t per = KT < 64u ? NG * KT / 64u : NG;  // groups of a lane
+                const uint32_t g0 = KT < 64u ? lane / KT * per : 0u;
+#pragma unroll
+                for (uint32_t g = 0; g < per; ++g) {
+                    reinterpret_cast<uint16_t *>(ks + key)[g0 + g] =
+                        static_cast<uint16_t>(lds_half(kt + key * SK::stride + (g0 + g) * SK::GB));
                 }
             }
             wave_lds_sync();
         }
-        float x[8];
+        float x[NT][4];
 #pragma unroll
-        for (uint32_t a = 0; a < 2; ++a) {
+        for (uint32_t a = 0; a < NT; ++a) {
             const uint8_t *kr = kt + (16u * a + nl) * SK::stride;
             float4_t sc{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (KO::codes) {
+                half8_t kd;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const half8_t kf = __builtin_bit_cast(half8_t, KO::load(kr + g * SK::GB, c));
-                if constexpr (KO::codes) {
-                    const float4_t start{q_off[g], q_off[g], q_off[g], q_off[g]};
-                    const float4_t acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[g], start, 0, 0, 0);
-                    const half4_t d = *reinterpret_cast<const half4_t *>(ks + g * kTileKeys + 16u * a + 4u * c);
+                for (int e = 0; e < 8; ++e) {
+                    kd[e] = 0;
+                }
+                const scales_t mine = ks[16u * a + nl];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    kd[g] = __builtin_bit_cast(_Float16, static_cast<uint16_t>(mine[g]));
+                }
+                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kd, q_off, sc, 0, 0, 0);
+                sc *= 0x1p-14f;
+                scales_t d[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    d[i] = ks[16u * a + 4u * c + i];
+                }
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const half8_t kf = __builtin_bit_cast(half8_t, load_key<KO, SK::GB>(kr, g, c));
+                    const float4_t acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        kf, qf[g], float4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        sc[i] = __builtin_fmaf(static_cast<float>(d[i]), acc[i], sc[i]);
+                        sc[i] = __builtin_fmaf(
+                            static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(d[i][g]))), acc[i],
+                            sc[i]);
                     }
-                } else {
+                }
+            } else {
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const half8_t kf = __builtin_bit_cast(half8_t, load_key<KO, SK::GB>(kr, g, c));
                     sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[g], sc, 0, 0, 0);
                 }
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[4 * a + i] = sc[i] * fac;
+                x[a][i] = sc[i] * fac;
             }
         }
-        if (have != 0xffffffffu || j0 + kTileKeys > n_all) {
+        const bool split = j0 + KT > n_all && tok0 != tok1;  // some rows do not attend all these keys
+        if (!whole || j0 + KT > n_all) {
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) {
-                const uint32_t key = 16u * (e >> 2) + 4u * c + (e & 3u);
-                x[e] = ((have >> key) & 1u) && j0 + key < limit ? x[e] : -INFINITY;
+            for (uint32_t h = 0; h < NT / 2; ++h) {
+                const uint32_t seen = seen_keys(static_cast<uint32_t>(now.have[h >> 1] >> (32u * (h & 1u))),
+                                                static_cast<int32_t>(limit - j0) - static_cast<int32_t>(32u * h), 4u * c);
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) {
+                    float &v = x[2 * h + (e >> 2)][e & 3u];
+                    v = (seen & (1u << (16u * (e >> 2) + (e & 3u)))) ? v : -INFINITY;
+                }
             }
         }
-        float most = x[0];
+        float most = -INFINITY;
 #pragma unroll
-        for (int e = 1; e < 8; ++e) {
-            most = fmaxf(most, x[e]);
+        for (uint32_t a = 0; a < NT; ++a) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                most = fmaxf(most, x[a][i]);
+            }
         }
         most = fmaxf(most, lane_xor16(most));
         most = fmaxf(most, lane_xor32(most));
-        if (__any(most > top)) {
-            const float now = fmaxf(top, most);
-            const float fade = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - now);
+        if (__any(most > top + kTopSlack)) {
+            const float higher = fmaxf(top, most);
+            const float fade = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
             sum *= fade;
 #pragma unroll
             for (int t = 0; t < VD; ++t) {
                 o[t] *= fade;
             }
-            top = now;
+            top = higher;
         }
         const float base = (top == -INFINITY ? 0.0f : top) - kWeightShift;
-        half8_t w;
+        half8_t w[NT / 2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float pe = __builtin_amdgcn_exp2f(x[e] - base);
-            sum += pe;
-            const _Float16 hi = static_cast<_Float16>(pe);
-            w[e] = twice && (nl & 8u) ? static_cast<_Float16>(pe - static_cast<float>(hi)) : hi;
+        for (uint32_t a = 0; a < NT; ++a) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const float pe = __builtin_amdgcn_exp2f(x[a][i] - base);
+                sum += pe;
+                const _Float16 hi = static_cast<_Float16>(pe);
+                w[a >> 1][4u * (a & 1u) + i] =
+                    twice && (nl & 8u) ? static_cast<_Float16>(pe - static_cast<float>(hi)) : hi;
+            }
         }
-        VO vo;
-        vo.raw(nl, [&](uint32_t e) { return vt + (16u * (e >> 2) + 4u * c + (e & 3u)) * SV::stride; });
-        if (j0 + kTileKeys <= n_all || tok0 == tok1) {
-            vo.emit([&](int t, u32x4_t a) {
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), w, o[t], 0, 0, 0);
-            });
-        } else {
-            // some rows do not attend all these keys: a zero weight would still
-            // hand them a NaN or infinity, so each token's rows take the product
-            // with its own later keys cleared
-            for (uint32_t tk = tok0; tk <= tok1; ++tk) {
-                const uint32_t lim = key_limit(p, r, tk);
-                u32x4_t keep;
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    const uint32_t key = j0 + 16u * (j >> 1) + 4u * c + 2u * (j & 1u);
-                    keep[j] = (key < lim ? 0x0000ffffu : 0u) | (key + 1u < lim ? 0xffff0000u : 0u);
+        for (uint32_t h = 0; h < NT / 2; ++h) {  // 32 keys each
+            // A zero weight would still hand a row a NaN or infinity: keys that do
+            // not exist are cleared, and where some rows do not attend all the
+            // others, each token's rows take the product with their later keys
+            // cleared.
+            for (uint32_t tk = split ? tok0 : tok1; tk <= tok1; ++tk) {
+                wave_lds_sync();  // the values are read (and unpacked) once a pass, not kept for all
+                VO vo;
+                vo.raw(nl, [&](uint32_t e) {
+                    return vt + (32u * h + 16u * (e >> 2) + 4u * c + (e & 3u)) * SV::stride;
+                });
+                u32x4_t keep{~0u, ~0u, ~0u, ~0u};
+                if (split || !whole) {
+                    keep = keep_keys(seen_keys(
+                        static_cast<uint32_t>(now.have[h >> 1] >> (32u * (h & 1u))),
+                        static_cast<int32_t>(key_limit(p, r, tk) - j0) - static_cast<int32_t>(32u * h), 4u * c));
                 }
-                vo.emit([&](int t, u32x4_t a) {
-                    const float4_t x = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a & keep), w,
-                                                                              o[t], 0, 0, 0);
-                    o[t] = my_tok == tk ? x : o[t];
+                vo.emit(keep, [&](int t0, const u32x4_t *a) {
+                    if (split) {
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            const float4_t y = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                __builtin_bit_cast(half8_t, a[t]), w[h], o[t0 + t], 0, 0, 0);
+                            o[t0 + t] = my_tok == tk ? y : o[t0 + t];
+                        }
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            o[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a[t]), w[h],
+                                                                               o[t0 + t], 0, 0, 0);
+                        }
+                    }
                 });
             }
         }
@@ -962,25 +1131,33 @@ __global__ __launch_bounds__(256) void attn_prefill_kernel(AttnParams p) {
     float fac;
     {
         const uint8_t *q = p.q + static_cast<uint64_t>(r.first + my_tok) * p.q_nb2 + my_head * p.q_nb1;
-        float most = 0.0f;
+        u32x4_t x[D / 16];
 #pragma unroll
         for (uint32_t st = 0; st < D / 16; ++st) {
-            float x[8];
-            load_query<KO>(p, q, st >> 1, 2u * (st & 1u) + hh, x);
+            x[st] = load_query<KO>(q, st >> 1, 2u * (st & 1u) + hh);
+        }
+        uint32_t bits = 0;
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) {
-                most = fmaxf(most, fabsf(x[e]));
+        for (uint32_t st = 0; st < D / 16; ++st) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                bits = max_magnitude(x[st][i], bits);
             }
         }
+        bits = max(bits & 0xffffu, bits >> 16);
+        float most = p.q_bf16 ? query_value<true>(bits) : query_value<false>(bits);
         most = fmaxf(most, lane_xor32(most));
         const int ex = query_shift(most);
+        const float up = ldexpf(1.0f, ex);
+        if (p.q_bf16) {
 #pragma unroll
-        for (uint32_t st = 0; st < D / 16; ++st) {
-            float x[8];
-            load_query<KO>(p, q, st >> 1, 2u * (st & 1u) + hh, x);
+            for (uint32_t st = 0; st < D / 16; ++st) {
+                qf[st] = query_operand<KO, true>(x[st], up);
+            }
+        } else {
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) {
-                qf[st][e] = static_cast<_Float16>(ldexpf(x[e], ex));
+            for (uint32_t st = 0; st < D / 16; ++st) {
+                qf[st] = query_operand<KO, false>(x[st], up);
             }
         }
         fac = ldexpf(p.scale * kLog2e, -ex);
@@ -1077,7 +1254,7 @@ __global__ __launch_bounds__(256) void attn_prefill_kernel(AttnParams p) {
                 scale = lds_half(g) * 0x00010001u;
             }
             *reinterpret_cast<u32x4_t *>(kt + key * (2 * D + 16) + oct * 16u) =
-                key_values<KO>(KO::load(g, oct & 3u), scale);
+                key_values<KO>((oct & 4u) ? KO::template load<false>(g, oct & 3u) : KO::template load<true>(g, oct & 3u), scale);
         }
         // values: a thread makes 8 keys of D/16 dims; octet q holds keys
         // 16 (q / 2) + 8 (e / 4) + 4 (q % 2) + e % 4, as a lane of the scores does
@@ -1090,12 +1267,15 @@ __global__ __launch_bounds__(256) void attn_prefill_kernel(AttnParams p) {
             vo.raw(dl, [&](uint32_t e) {
                 return raw_v + (16u * (q >> 1) + 8u * (e >> 2) + 4u * (q & 1u) + (e & 3u)) * SV::bytes;
             });
-            vo.emit([&](int t, u32x4_t a) {
-                *reinterpret_cast<u32x4_t *>(vt + (q * D + VO::dim(dl, t)) * 16u) = a;
-                if (partial) {
+            vo.emit(u32x4_t{~0u, ~0u, ~0u, ~0u}, [&](int t0, const u32x4_t *a) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        bad |= ((a[j] & 0x7C00u) == 0x7C00u) | ((a[j] & 0x7C000000u) == 0x7C000000u);
+                for (int t = 0; t < 4; ++t) {
+                    *reinterpret_cast<u32x4_t *>(vt + (q * D + VO::dim(dl, t0 + t)) * 16u) = a[t];
+                    if (partial) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            bad |= ((a[t][j] & 0x7C00u) == 0x7C00u) | ((a[t][j] & 0x7C000000u) == 0x7C000000u);
+                        }
                     }
                 }
             });
@@ -1134,7 +1314,7 @@ __global__ __launch_bounds__(256) void attn_prefill_kernel(AttnParams p) {
             }
         }
         most = fmaxf(most, lane_xor32(most));
-        if (__any(most > top)) {
+        if (__any(most > top + kTopSlack)) {
             const float now = fmaxf(top, most);
             const float fade = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - now);
             sum *= fade;
@@ -1281,14 +1461,20 @@ __global__ __launch_bounds__(256) void attn_prefill_kernel(AttnParams p) {
 
 // ------------------------------------------------------------- joining parts
 
-// One workgroup of D threads per (token, head): the parts' sums, each weighted
-// by its maximum, in the order of the parts.
+// One workgroup per (token, head): the parts' sums, each weighted by its
+// maximum.  Each wave adds the parts k = wave, wave + 4, ... in order, a lane its
+// D/64 dims, then the waves' sums are added in order.
 template <int D>
-__global__ __launch_bounds__(D) void attn_join_kernel(AttnParams p) {
-    __shared__ float turn[D];
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
+    constexpr int E = D / 64;
+    typedef float dims_t __attribute__((ext_vector_type(E)));
+    __shared__ float sums[kWaves][D];
+    __shared__ float turn[256];
     const uint32_t h = blockIdx.x % p.n_head;
     const uint32_t tok = blockIdx.x / p.n_head;
-    const uint32_t d = threadIdx.x;
+    const uint32_t tid = threadIdx.x;
+    const uint32_t lane = tid & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // the request this token belongs to
     uint32_t s = tok;
     if (p.q_start) {
@@ -1323,22 +1509,39 @@ __global__ __launch_bounds__(D) void attn_join_kernel(AttnParams p) {
     const uint64_t at = static_cast<uint64_t>(tok) * p.n_head + h;
     const uint64_t stride = static_cast<uint64_t>(p.n_tokens) * p.n_head;
     float top = -INFINITY;
-    for (uint32_t k = 0; k < n_parts; ++k) {
+    for (uint32_t k = lane; k < n_parts; k += 64u) {
         top = fmaxf(top, p.part_ml[k * stride + at].x);
     }
-    float total = 0.0f, x = 0.0f;
-    for (uint32_t k = 0; k < n_parts; ++k) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        top = fmaxf(top, __shfl_xor(top, d, 64));
+    }
+    const float *po = p.part_o + at * D + lane * E;
+    float total = 0.0f;
+    dims_t x = {};
+#pragma unroll 8
+    for (uint32_t k = wave; k < n_parts; k += kWaves) {
         const float2 ml = p.part_ml[k * stride + at];
         const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);
         total += ml.y * f;
-        x += p.part_o[(k * stride + at) * D + d] * f;
+        x += *reinterpret_cast<const dims_t *>(po + k * stride * D) * f;
     }
-    x = total == 0.0f ? 0.0f : x / total;
+    *reinterpret_cast<dims_t *>(&sums[wave][lane * E]) = x;
+    if (lane == 0) {
+        turn[wave] = total;
+    }
+    __syncthreads();
+    total = (turn[0] + turn[1]) + (turn[2] + turn[3]);
+    const uint32_t d = tid & (D - 1u);  // D < 256: more than one thread a dim, the first one stores
+    float y = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
+    y = total == 0.0f ? 0.0f : y / total;
     if (p.hadamard) {
-        x = rotate_back(x, p.hadamard, d & (p.hadamard - 1u), turn + (d - (d & (p.hadamard - 1u))));
+        y = rotate_back(y, p.hadamard, tid & (p.hadamard - 1u), turn + (tid - (tid & (p.hadamard - 1u))));
     }
-    store_elem(p.out, p.out_type, at * D + d, x);
-    if (d == 0 && p.lse) {
+    if (tid < D) {
+        store_elem(p.out, p.out_type, at * D + d, y);
+    }
+    if (tid == 0 && p.lse) {
         p.lse[at] = total == 0.0f ? -INFINITY : (top - kWeightShift) / kLog2e + logf(total);
     }
 }
@@ -1365,7 +1568,7 @@ static AttnPlan plan_attention(const kvmem_hip_pool *pool, const kvmem_hip_attn_
     pl.prefill = rows > kDecodeRows;
     pl.row_tile = pl.prefill ? kPrefillRows : kRowTile;
     pl.row_tiles = static_cast<uint32_t>((rows + pl.row_tile - 1) / pl.row_tile);
-    const uint32_t quantum = pl.prefill ? kTileKeys : kTileKeys * kWaves;
+    const uint32_t quantum = pl.prefill ? kTileKeys : 32u * (256u / a->head_dim) * kWaves;
     const uint64_t room = static_cast<uint64_t>(a->table_stride) * pool->block_tokens;
     const uint64_t keys = std::max<uint64_t>(1, std::min<uint64_t>(a->max_kv, room));
     const uint64_t groups = static_cast<uint64_t>(a->n_seq) * a->n_head_kv * pl.row_tiles;
@@ -1393,12 +1596,13 @@ static void launch_attention(hipStream_t stream, const AttnPlan &pl, const AttnP
         attn_prefill_kernel<TK, TV, D><<<static_cast<uint32_t>(pl.grid), 256, prefill_bytes<TK, TV, D>(), stream>>>(p);
     } else {
         const uint32_t rows = std::min(kRowTile, p.max_q * p.group);
-        const uint32_t lds = std::max<uint32_t>(kWaves * decode_wave_bytes<TK, TV, D>(),
+        // 16 bytes behind the last slice: its last word is read with the next one
+        const uint32_t lds = std::max<uint32_t>(kWaves * decode_wave_bytes<TK, TV, D>() + 16u,
                                                 std::max<uint32_t>(kWaves * rows * D * 4u, 1024u));
         attn_decode_kernel<TK, TV, D><<<static_cast<uint32_t>(pl.grid), 256, lds, stream>>>(p);
     }
     if (pl.n_parts > 1) {
-        attn_join_kernel<D><<<p.n_tokens * p.n_head, D, 0, stream>>>(p);
+        attn_join_kernel<D><<<p.n_tokens * p.n_head, 256, 0, stream>>>(p);
     }
 }
 
@@ -1463,7 +1667,7 @@ static const char *check_attention(const kvmem_hip_pool *pool, const kvmem_hip_a
     if (!(a->scale >= 0.0f) || std::isinf(a->scale)) {
         return "attention: scale must be finite and not negative";
     }
-    if (pool->block_tokens == 0 || static_cast<uint64_t>(pool->n_slots) * pool->block_tokens > 0x7fffffffu) {
+    if (pool->block_tokens == 0 || pool->n_slots == 0 || static_cast<uint64_t>(pool->n_slots) * pool->block_tokens > 0x7fffffffu) {
         return "attention: the pool's rows must fit 31 bits";
     }
     if (pool->n_embd_k != static_cast<uint64_t>(a->n_head_kv) * D || pool->n_embd_v != pool->n_embd_k) {
