@@ -1,0 +1,122 @@
+// Attention of new tokens over the pool's rows: what the kernels and the host
+// side share (kvmem_hip_attention, attention.hip).
+#pragma once
+
+#include "kvmem_internal.hpp"
+
+namespace kvmem_hip {
+
+constexpr uint32_t kRowTile = 16;    // query rows of a decode workgroup
+constexpr uint32_t kWaves = 4;
+// Softmax weights are 2^(x - top + shift) before they are rounded to f16.  A
+// row's `top` follows its maximum only when that has grown by more than
+// kTopSlack (log2), so the sums are rarely scaled down again; weights then stay
+// below 2^15, and those down to 2^-20 of 2^top are normal f16 numbers.
+constexpr float kWeightShift = 6.0f;
+constexpr float kTopSlack = 9.0f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnParams {
+    const uint8_t *q;
+    uint64_t q_nb1, q_nb2;
+    uint8_t *out;
+    float *lse;
+    const uint8_t *k;
+    const uint8_t *v;
+    const uint32_t *q_start;
+    const uint32_t *kv_len;
+    const uint32_t *table;
+    float *part_o;              // [part][token][head][D] sums of weighted values
+    float2 *part_ml;            // [part][token][head] maximum (log2), sum of weights
+    uint32_t row_k, row_v;      // bytes of a cached row
+    uint32_t n_tokens, n_seq, max_q, max_kv, n_head, n_head_kv, group, T, n_slots, table_stride;
+    uint32_t chunk;             // keys of one part
+    uint32_t n_parts;           // parts of the longest request
+    uint32_t row_tile;          // rows of one workgroup
+    uint32_t row_tiles;         // of the longest request
+    uint32_t units;             // of the grid's fast index, a multiple of 8
+    int32_t causal;
+    int32_t q_bf16;
+    int32_t out_type;
+    uint32_t hadamard;
+    uint32_t join_one;          // rows of a single part are joined (and rotated) too
+    float scale;
+};
+
+// A request's share of the call: its first token, tokens, keys in range.
+struct Span {
+    uint32_t first, m, len, keys;
+};
+
+__device__ inline Span request_span(const AttnParams &p, uint32_t s) {
+    Span r;
+    const uint32_t a = p.q_start ? min(p.q_start[s], p.n_tokens) : s;
+    const uint32_t b = p.q_start ? min(p.q_start[s + 1], p.n_tokens) : s + 1;
+    r.first = a;
+    r.m = b > a ? b - a : 0u;
+    r.len = p.kv_len[s];
+    const uint64_t room = static_cast<uint64_t>(p.table_stride) * p.T;
+    r.keys = static_cast<uint32_t>(min<uint64_t>(min(r.len, p.max_kv), room));
+    return r;
+}
+
+// Keys token i attends: [0, limit).
+__device__ inline uint32_t key_limit(const AttnParams &p, const Span &r, uint32_t i) {
+    if (!p.causal) {
+        return r.keys;
+    }
+    const int64_t last = static_cast<int64_t>(r.len) - r.m + i + 1;
+    return last <= 0 ? 0u : static_cast<uint32_t>(min<int64_t>(r.keys, last));
+}
+
+
+__device__ inline void store_elem(uint8_t *out, int type, uint64_t i, float x) {
+    if (type == KVMEM_TYPE_F32) {
+        reinterpret_cast<float *>(out)[i] = x;
+    } else if (type == KVMEM_TYPE_F16) {
+        reinterpret_cast<_Float16 *>(out)[i] = static_cast<_Float16>(x);
+    } else {
+        reinterpret_cast<__bf16 *>(out)[i] = static_cast<__bf16>(x);
+    }
+}
+
+// Walsh-Hadamard rotation of an output element (dim d of a row, one thread per
+// dim, every thread of the workgroup calls): butterflies of span 1 .. width/2
+// through LDS.
+__device__ inline float rotate_back(float x, uint32_t width, uint32_t d, float *row) {
+    x *= 1.0f / sqrtf(static_cast<float>(width));
+    for (uint32_t s = 1; s < width; s <<= 1) {
+        __syncthreads();
+        row[d] = x;
+        __syncthreads();
+        const float y = row[d ^ s];
+        x = (d & s) ? y - x : x + y;
+    }
+    return x;
+}
+
+// How a call is laid out on the chip.
+struct AttnPlan {
+    uint32_t prefill;          // row tiles of a prefill wave (0: decode kernel)
+    uint32_t row_tile, row_tiles, chunk, n_parts, units;
+    uint64_t grid;
+    bool joined;               // a joining kernel follows
+    size_t o_bytes, ml_bytes;  // workspace: sums, then maxima and weights
+};
+
+// Keys of a step: about the same bytes for every head size (9 KiB of q4_0 keys
+// and values), enough in flight per compute unit to stream.
+constexpr uint32_t step_keys(uint32_t d) { return 32u * (256u / d); }
+// Query rows of a prefill workgroup whose waves hold `tiles` tiles of 32.
+constexpr uint32_t prefill_rows(uint32_t tiles) { return kWaves * 32u * tiles; }
+
+// Launches the decode or prefill kernel of key type TK (one translation unit
+// each).
+template <int TK>
+void launch_attention(hipStream_t stream, int type_v, uint32_t head_dim, const AttnPlan &pl, const AttnParams &p);
+extern template void launch_attention<KVMEM_TYPE_Q4_0>(hipStream_t, int, uint32_t, const AttnPlan &, const AttnParams &);
+extern template void launch_attention<KVMEM_TYPE_Q5_0>(hipStream_t, int, uint32_t, const AttnPlan &, const AttnParams &);
+extern template void launch_attention<KVMEM_TYPE_Q8_0>(hipStream_t, int, uint32_t, const AttnPlan &, const AttnParams &);
+extern template void launch_attention<KVMEM_TYPE_F16>(hipStream_t, int, uint32_t, const AttnPlan &, const AttnParams &);
+
+}  // namespace kvmem_hip

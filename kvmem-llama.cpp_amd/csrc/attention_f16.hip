@@ -1,0 +1,8 @@
+// Attention over f16 keys.
+#include "attention_kernels.hpp"
+
+namespace kvmem_hip {
+
+template void launch_attention<KVMEM_TYPE_F16>(hipStream_t, int, uint32_t, const AttnPlan &, const AttnParams &);
+
+}  // namespace kvmem_hip

@@ -1,0 +1,1464 @@
+// Kernels of kvmem_hip_attention (attention.hip); one translation unit per key
+// type instantiates them.
+#pragma once
+
+#include "attention.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace kvmem_hip {
+
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+// ------------------------------------------------------- cached formats
+
+// A head's slice of a row, moved in units of D/16 bytes (16 for f16): its
+// address is a multiple of that.
+template <int TYPE, int D>
+struct Slice {
+    static constexpr uint32_t GB = TYPE == KVMEM_TYPE_Q8_0 ? 34 : TYPE == KVMEM_TYPE_Q5_0 ? 22
+                                   : TYPE == KVMEM_TYPE_Q4_0 ? 18 : 64;
+    static constexpr uint32_t bytes = D / 32 * GB;
+    static constexpr uint32_t unit = TYPE == KVMEM_TYPE_F16 ? 16 : D / 16;
+    static constexpr uint32_t units = bytes / unit;
+    // LDS bytes between keys: f16 rows are padded so that 16 keys' reads
+    // spread over the banks
+    static constexpr uint32_t stride = TYPE == KVMEM_TYPE_F16 ? bytes + 16 : bytes;
+    // a wave's load moves whole slices, one lane a unit (the last lanes idle):
+    // the addresses of its loads then differ by constants
+    static constexpr uint32_t per_load = 64 / units;
+};
+
+template <uint32_t UNIT> struct UnitOf;
+template <> struct UnitOf<4> { typedef uint32_t type; };
+template <> struct UnitOf<8> { typedef u32x2_t type; };
+template <> struct UnitOf<16> { typedef u32x4_t type; };
+
+__device__ inline uint32_t lds_half(const uint8_t *p) { return *reinterpret_cast<const uint16_t *>(p); }
+
+// N words of LDS from an even address.  Groups of 18, 22 and 34 bytes put every
+// other group's codes 2 bytes off a word; the LDS answers such reads at a
+// fraction of its rate (stalls were three quarters of a step's time), so words are
+// read where they are aligned and shifted together.  The word after the last is
+// read too.
+template <int N>
+__device__ inline void lds_words(const uint8_t *p, uint32_t shift, uint32_t out[N]) {
+    const uint32_t *q = reinterpret_cast<const uint32_t *>(p - shift);
+    uint32_t w[N + 1];
+#pragma unroll
+    for (int i = 0; i <= N; ++i) {
+        w[i] = q[i];  // (a last word that a constant shift of 0 leaves unused is not read)
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        out[i] = __builtin_amdgcn_alignbyte(w[i + 1], w[i], shift);
+    }
+}
+// Key operand of one group of 32 dims: the 8 elements a lane (key, chunk c of
+// 4) feeds the matrix instruction, as f16.  Quantized codes stay integers:
+// an f16 whose bits are the code n is the subnormal n * 2^-24, which the
+// matrix cores multiply exactly, so a masked word is an operand already.
+// A code in the upper nibble is 16 times its value there; the query element
+// that meets it is divided by 16.  The code's offset (8, 16, 128) comes off
+// through the accumulator's start, the group's scale is multiplied into the
+// fp32 sum: keys enter the scores unrounded.
+// shift: the bytes that the group's codes lie off a word (2 in groups of even
+// number).
+// Element e is dim piece(c, i) + l % 4 of the group, l = order(e) and i = l / 4:
+// a lane's 8 dims are two runs of four.
+template <int TYPE> struct KeyOp;
+
+template <> struct KeyOp<KVMEM_TYPE_Q4_0> {
+    static constexpr float offset = 8.0f;
+    static constexpr bool codes = true;
+    __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c, uint32_t shift) {
+        uint32_t w;
+        lds_words<1>(g + 2 + 4 * c, shift, &w);
+        u32x4_t r;
+        r[0] = w & 0x000F000Fu;
+        r[1] = w & 0x00F000F0u;
+        r[2] = (w >> 8) & 0x000F000Fu;
+        r[3] = (w >> 8) & 0x00F000F0u;
+        return r;
+    }
+    __device__ static inline uint32_t piece(uint32_t c, uint32_t i) { return 4 * c + 16 * i; }
+    __device__ static constexpr uint32_t order(uint32_t e) { return 2 * (e & 2u) + 2 * (e & 1u) + (e >> 2); }
+    // the operand's element is this many times the code
+    __device__ static constexpr float times(uint32_t e) { return (e & 2u) ? 16.0f : 1.0f; }
+};
+
+template <> struct KeyOp<KVMEM_TYPE_Q5_0> {
+    static constexpr float offset = 16.0f;
+    static constexpr bool codes = true;
+    __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c, uint32_t shift) {
+        uint32_t h, w;
+        lds_words<1>(g + 2, shift, &h);
+        lds_words<1>(g + 6 + 4 * c, shift, &w);
+        h >>= 4 * c;
+        // bits 0 and 2 of a 4-bit field to bits 4 and 20 (8 and 24 for the
+        // upper nibbles): two shifted copies in one product, no carries
+        const uint32_t lo = (h & 15u) * 0x00040010u;
+        const uint32_t hi = ((h >> 16) & 15u) * 0x00400100u;
+        u32x4_t r;
+        r[0] = (w & 0x000F000Fu) | (lo & 0x00100010u);
+        r[1] = (w & 0x00F000F0u) | (hi & 0x01000100u);
+        r[2] = ((w >> 8) & 0x000F000Fu) | ((lo >> 1) & 0x00100010u);
+        r[3] = ((w >> 8) & 0x00F000F0u) | ((hi >> 1) & 0x01000100u);
+        return r;
+    }
+    __device__ static inline uint32_t piece(uint32_t c, uint32_t i) { return 4 * c + 16 * i; }
+    __device__ static constexpr uint32_t order(uint32_t e) { return 2 * (e & 2u) + 2 * (e & 1u) + (e >> 2); }
+    __device__ static constexpr float times(uint32_t e) { return (e & 2u) ? 16.0f : 1.0f; }
+};
+
+template <> struct KeyOp<KVMEM_TYPE_Q8_0> {
+    static constexpr float offset = 128.0f;
+    static constexpr bool codes = true;
+    __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c, uint32_t shift) {
+        uint32_t w[2];
+        lds_words<2>(g + 2 + 8 * c, shift, w);
+        const uint32_t a = w[0] ^ 0x80808080u;
+        const uint32_t b = w[1] ^ 0x80808080u;
+        u32x4_t r;
+        r[0] = a & 0x00FF00FFu;
+        r[1] = (a >> 8) & 0x00FF00FFu;
+        r[2] = b & 0x00FF00FFu;
+        r[3] = (b >> 8) & 0x00FF00FFu;
+        return r;
+    }
+    __device__ static inline uint32_t piece(uint32_t c, uint32_t i) { return 8 * c + 4 * i; }
+    __device__ static constexpr uint32_t order(uint32_t e) { return (e & 4u) + 2 * (e & 1u) + ((e >> 1) & 1u); }
+    __device__ static constexpr float times(uint32_t) { return 1.0f; }
+};
+
+template <> struct KeyOp<KVMEM_TYPE_F16> {
+    static constexpr float offset = 0.0f;
+    static constexpr bool codes = false;
+    __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c, uint32_t) {
+        return *reinterpret_cast<const u32x4_t *>(g + 16 * c);
+    }
+    __device__ static inline uint32_t piece(uint32_t c, uint32_t i) { return 8 * c + 4 * i; }
+    __device__ static constexpr uint32_t order(uint32_t e) { return e; }
+    __device__ static constexpr float times(uint32_t) { return 1.0f; }
+};
+
+__device__ inline half2_t as_half2(uint32_t w) { return __builtin_bit_cast(half2_t, w); }
+__device__ inline uint32_t as_word(half2_t h) { return __builtin_bit_cast(uint32_t, h); }
+
+// (low halves, high halves) of a key pair's words: a in the lower 16 bits.
+__device__ inline uint32_t pair_lo(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ inline uint32_t pair_hi(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// f16 values of a pair of codes in bits 0..9 of each half: 1024 + n by the
+// bits of 1024, less 1024 + offset (both exact), times the scales (the one
+// rounding).
+__device__ inline uint32_t pair_value(uint32_t codes, float offset, uint32_t scales) {
+    const _Float16 o = static_cast<_Float16>(-(1024.0f + offset));
+    return as_word((as_half2(codes | 0x64006400u) + half2_t{o, o}) * as_half2(scales));
+}
+// The same for codes in bits 4..9: 64 + n by the bits of 64.
+__device__ inline uint32_t pair_value_hi(uint32_t codes, float offset, uint32_t scales) {
+    const _Float16 o = static_cast<_Float16>(-(64.0f + offset));
+    return as_word((as_half2(codes | 0x54005400u) + half2_t{o, o}) * as_half2(scales));
+}
+
+// Value operand: lane n owns VD dims of a key's slice.  Rows
+// hold consecutive dims of one key and the matrix instruction wants
+// consecutive keys of one dim, so a lane reads its dims of 8 keys and pairs
+// keys with byte permutes, still in packed codes (a nibble permute moves 8
+// elements).  raw(): the keys' words and scales; emit(keep, f): f(t,
+// operands of dims t .. t + 3) over the VD dims, keys cleared in `keep` (16 bits a
+// key, pairs as the operand's words) as zeros;  dim(n, t): which dim t is.
+template <int TYPE, int VD> struct ValueOp;
+
+template <int VD>
+struct ValueOp<KVMEM_TYPE_Q4_0, VD> {
+    static constexpr int NB = VD / 2;  // bytes of codes
+    static constexpr int NW = NB < 4 ? 1 : NB / 4;
+    static constexpr float offset = 8.0f;
+    uint32_t w[8][NW];
+    uint32_t d[4];
+    __device__ static inline uint32_t dim(uint32_t n, uint32_t t) {
+        constexpr uint32_t per = 32 / VD;  // lanes of a group
+        return 32 * (n / per) + NB * (n % per) + (t >> 1) + 16 * (t & 1u);
+    }
+    template <class RowOf>
+    __device__ inline void raw(uint32_t n, RowOf row) {
+        constexpr uint32_t per = 32 / VD;
+        const uint32_t off = 2u * (~(n / per) & 1u);  // of the lane's group's codes in a word
+        uint32_t s[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+            const uint8_t *g = row(e) + (n / per) * 18u;
+            s[e] = lds_half(g);
+            const uint8_t *b = g + 2 + NB * (n % per);
+            if constexpr (NB >= 4) {
+                lds_words<NW>(b, off, w[e]);
+            } else {
+                w[e][0] = lds_half(b);
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            d[i] = s[2 * i] | (s[2 * i + 1] << 16);
+        }
+    }
+    template <class F>
+    __device__ inline void emit(const u32x4_t &keep, F f) const {
+        const u32x4_t ds{d[0] & keep[0], d[1] & keep[1], d[2] & keep[2], d[3] & keep[3]};
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+#pragma unroll
+            for (int h = 0; h < (NB < 4 ? 1 : 2); ++h) {
+                u32x4_t a[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t t = h ? pair_hi(w[2 * j][i], w[2 * j + 1][i]) : pair_lo(w[2 * j][i], w[2 * j + 1][i]);
+                    a[0][j] = pair_value(t & 0x000F000Fu, offset, ds[j]);
+                    a[1][j] = pair_value_hi(t & 0x00F000F0u, offset, ds[j]);
+                    a[2][j] = pair_value((t >> 8) & 0x000F000Fu, offset, ds[j]);
+                    a[3][j] = pair_value_hi((t >> 8) & 0x00F000F0u, offset, ds[j]);
+                }
+                f(8 * i + 4 * h, a);
+            }
+        }
+    }
+};
+
+template <int VD>
+struct ValueOp<KVMEM_TYPE_Q5_0, VD> {
+    static constexpr int NB = VD / 2;
+    static constexpr int NW = NB < 4 ? 1 : NB / 4;
+    static constexpr float offset = 16.0f;
+    uint32_t w[8][NW];  // lower four bits, as Q4_0's
+    uint32_t h[8];      // fifth bits: of the lower nibbles from bit 0, of the upper from bit 16
+    uint32_t d[4];
+    __device__ static inline uint32_t dim(uint32_t n, uint32_t t) { return ValueOp<KVMEM_TYPE_Q4_0, VD>::dim(n, t); }
+    template <class RowOf>
+    __device__ inline void raw(uint32_t n, RowOf row) {
+        constexpr uint32_t per = 32 / VD;
+        const uint32_t off = 2u * (~(n / per) & 1u);  // of the lane's group's codes in a word
+        uint32_t s[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+            const uint8_t *g = row(e) + (n / per) * 22u;
+            s[e] = lds_half(g);
+            lds_words<1>(g + 2, off, &h[e]);
+            h[e] >>= NB * (n % per);
+            const uint8_t *b = g + 6 + NB * (n % per);
+            if constexpr (NB >= 4) {
+                lds_words<NW>(b, off, w[e]);
+            } else {
+                w[e][0] = lds_half(b);
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            d[i] = s[2 * i] | (s[2 * i + 1] << 16);
+        }
+    }
+    template <class F>
+    __device__ inline void emit(const u32x4_t &keep, F f) const {
+        const u32x4_t ds{d[0] & keep[0], d[1] & keep[1], d[2] & keep[2], d[3] & keep[3]};
+        // the fifth bits of a key pair, in the halves of one word
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            lo[j] = pair_lo(h[2 * j], h[2 * j + 1]);
+            hi[j] = pair_hi(h[2 * j], h[2 * j + 1]);
+        }
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+#pragma unroll
+            for (int q = 0; q < (NB < 4 ? 1 : 2); ++q) {
+                u32x4_t a[4];
+                const int b0 = 4 * i + 2 * q;  // byte of the lane's codes
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t t = q ? pair_hi(w[2 * j][i], w[2 * j + 1][i]) : pair_lo(w[2 * j][i], w[2 * j + 1][i]);
+                    a[0][j] = pair_value((t & 0x000F000Fu) | (((lo[j] >> b0) & 0x00010001u) << 4), offset, ds[j]);
+                    a[1][j] = pair_value_hi((t & 0x00F000F0u) | (((hi[j] >> b0) & 0x00010001u) << 8), offset, ds[j]);
+                    a[2][j] = pair_value(((t >> 8) & 0x000F000Fu) | (((lo[j] >> (b0 + 1)) & 0x00010001u) << 4), offset,
+                                      ds[j]);
+                    a[3][j] = pair_value_hi(((t >> 8) & 0x00F000F0u) | (((hi[j] >> (b0 + 1)) & 0x00010001u) << 8), offset,
+                                         ds[j]);
+                }
+                f(8 * i + 4 * q, a);
+            }
+        }
+    }
+};
+
+template <int VD>
+struct ValueOp<KVMEM_TYPE_Q8_0, VD> {
+    static constexpr int NW = VD / 4;
+    uint32_t w[8][NW];
+    uint32_t d[4];
+    __device__ static inline uint32_t dim(uint32_t n, uint32_t t) { return VD * n + t; }
+    template <class RowOf>
+    __device__ inline void raw(uint32_t n, RowOf row) {
+        constexpr uint32_t per = 32 / VD;
+        const uint32_t off = 2u * (~(n / per) & 1u);  // of the lane's group's codes in a word
+        uint32_t s[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+            const uint8_t *g = row(e) + (n / per) * 34u;
+            s[e] = lds_half(g);
+            lds_words<NW>(g + 2 + VD * (n % per), off, w[e]);
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                w[e][i] ^= 0x80808080u;
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            d[i] = s[2 * i] | (s[2 * i + 1] << 16);
+        }
+    }
+    template <class F>
+    __device__ inline void emit(const u32x4_t &keep, F f) const {
+        const u32x4_t ds{d[0] & keep[0], d[1] & keep[1], d[2] & keep[2], d[3] & keep[3]};
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            u32x4_t a[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                // byte b of both keys, zero-extended to 16 bits
+                const uint32_t sel = 0x0c000c00u | static_cast<uint32_t>(b) | (static_cast<uint32_t>(4 + b) << 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    a[b][j] = pair_value(__builtin_amdgcn_perm(w[2 * j + 1][i], w[2 * j][i], sel), 128.0f, ds[j]);
+                }
+            }
+            f(4 * i, a);
+        }
+    }
+};
+
+template <int VD>
+struct ValueOp<KVMEM_TYPE_F16, VD> {
+    static constexpr int NW = VD / 2;
+    uint32_t w[8][NW];
+    __device__ static inline uint32_t dim(uint32_t n, uint32_t t) { return VD * n + t; }
+    template <class RowOf>
+    __device__ inline void raw(uint32_t n, RowOf row) {
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+            const uint8_t *b = row(e) + 2u * VD * n;
+            if constexpr (NW == 2) {
+                const u32x2_t x = *reinterpret_cast<const u32x2_t *>(b);
+                w[e][0] = x[0];
+                w[e][1] = x[1];
+            } else {
+#pragma unroll
+                for (int i = 0; i < NW; i += 4) {
+                    const u32x4_t x = *reinterpret_cast<const u32x4_t *>(b + 4 * i);
+                    w[e][i] = x[0];
+                    w[e][i + 1] = x[1];
+                    w[e][i + 2] = x[2];
+                    w[e][i + 3] = x[3];
+                }
+            }
+        }
+    }
+    template <class F>
+    __device__ inline void emit(const u32x4_t &keep, F f) const {
+#pragma unroll
+        for (int i = 0; i < NW; i += 2) {
+            u32x4_t a[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                a[0][j] = pair_lo(w[2 * j][i], w[2 * j + 1][i]) & keep[j];
+                a[1][j] = pair_hi(w[2 * j][i], w[2 * j + 1][i]) & keep[j];
+                a[2][j] = pair_lo(w[2 * j][i + 1], w[2 * j + 1][i + 1]) & keep[j];
+                a[3][j] = pair_hi(w[2 * j][i + 1], w[2 * j + 1][i + 1]) & keep[j];
+            }
+            f(2 * i, a);
+        }
+    }
+};
+
+// ------------------------------------------------------------ wave helpers
+
+// The value of lane ^ 16 (lanes swapped between row pairs) and lane ^ 32.
+__device__ inline float lane_xor16(float v) {
+    return __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(v), 0x1F | (16 << 10)));
+}
+__device__ inline float lane_xor32(float v) { return __shfl_xor(v, 32, 64); }
+
+__device__ inline float lane_xor8(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xF, 0xF, true));  // row_ror:8
+}
+
+// Of a block of 32 keys, those that exist and lie below `limit` (both from the
+// block's first key), for a lane whose element e of the block's operand is key
+// GAP (e / 4) + first + e % 4: bit GAP (e / 4) + e % 4.
+__device__ inline uint32_t seen_keys(uint32_t have, int32_t limit, uint32_t first) {
+    const int32_t left = limit - static_cast<int32_t>(first);
+    const uint32_t below = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;
+    return (have >> first) & below;
+}
+
+// Operand masks of those keys: 16 bits a key, pairs as the operand's words.
+template <uint32_t GAP>
+__device__ inline u32x4_t keep_keys(uint32_t seen) {
+    u32x4_t keep;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t two = seen >> (GAP * (j >> 1) + 2u * (j & 1u));
+        keep[j] = (two & 1u) * 0x0000ffffu + ((two >> 1) & 1u) * 0xffff0000u;
+    }
+    return keep;
+}
+
+// Values that are not finite, where some rows of a workgroup do not attend their
+// key: a weight of zero would still hand those rows the NaN.  Such a value enters
+// the product as zero, its key is noted for its dim (first[dim], the lowest such
+// key), and rows that attend that key get NaN for the dim at the end.  `a`: the
+// operand of one dim for 8 keys, element e key at(e).
+template <class At>
+__device__ inline void clear_odd(u32x4_t &a, uint32_t *first, At at) {
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        const bool lo = (a[j] & 0x7C00u) == 0x7C00u;
+        const bool hi = (a[j] & 0x7C000000u) == 0x7C000000u;
+        if (lo) {
+            atomicMin(first, at(2 * j));
+        }
+        if (hi) {
+            atomicMin(first, at(2 * j + 1));
+        }
+        a[j] &= (lo ? 0u : 0x0000ffffu) | (hi ? 0u : 0xffff0000u);
+    }
+}
+
+// A wave's LDS writes become visible to its own later reads, in order.
+__device__ inline void wave_lds_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A lane's 8 query elements of a group as they lie in memory (f16 or bf16 bits).
+template <class KO>
+__device__ inline u32x4_t load_query(const uint8_t *q, uint32_t g, uint32_t c) {
+    const u32x2_t a = *reinterpret_cast<const u32x2_t *>(q + 64u * g + 2u * KO::piece(c, 0));
+    const u32x2_t b = *reinterpret_cast<const u32x2_t *>(q + 64u * g + 2u * KO::piece(c, 1));
+    return u32x4_t{a[0], a[1], b[0], b[1]};
+}
+
+// The larger magnitudes of two pairs (bits: both formats order as integers).
+__device__ inline uint32_t max_magnitude(uint32_t a, uint32_t b) {
+    typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a & 0x7fff7fffu),
+                                                                  __builtin_bit_cast(u16x2_t, b)));
+}
+
+template <bool BF16>
+__device__ inline float query_value(uint32_t bits) {
+    return BF16 ? __uint_as_float(bits << 16)
+                : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+}
+
+// f16 queries in the key operand's order, times `up`.
+template <class KO, bool BF16>
+__device__ inline half8_t query_operand(const u32x4_t &w, float up) {
+    half8_t r;
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) {
+        const uint32_t l = KO::order(e);
+        r[e] = static_cast<_Float16>(query_value<BF16>((l & 1u) ? w[l >> 1] >> 16 : w[l >> 1] & 0xffffu) * up);
+    }
+    return r;
+}
+
+// Exponent of the power of two that brings a row's largest query magnitude to
+// at most 2^9: f16 then holds the row whatever its exponents.
+__device__ inline int query_shift(float top) {
+    int ex = 0;
+    if (top > 0.0f && top < INFINITY) {
+        (void) frexpf(top, &ex);
+        ex = min(9 - ex, 120);  // the power itself stays a normal float
+    }
+    return ex;
+}
+
+// ------------------------------------------------------------ few queries
+
+template <int TK, int TV, int D>
+constexpr uint32_t decode_wave_bytes() {
+    return step_keys(D) * (Slice<TK, D>::stride + Slice<TV, D>::stride + (KeyOp<TK>::codes ? D / 16 : 0));
+}
+
+// Rows of one KV head's queries over one part of a request's keys: up to 16
+// (token, head) rows, keys split over the workgroup's four waves.  Scores are
+// held transposed (keys by rows) so that a lane owns one query row: S^T = K Q^T,
+// O^T = V^T P^T, and a lane's weights of S^T are its operand of the second
+// product as they stand.
+// Two waves per SIMD, but for 16-bit rows of 256: their step's rows take half the
+// registers, and one wave has as many bytes in flight.
+constexpr int decode_occupancy(int tk, int tv, int d) {
+    return d == 256 && (tk == KVMEM_TYPE_F16 || tv == KVMEM_TYPE_F16) ? 1 : 2;
+}
+
+template <int TK, int TV, int D>
+__global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_kernel(AttnParams p) {
+    using SK = Slice<TK, D>;
+    using SV = Slice<TV, D>;
+    using KO = KeyOp<TK>;
+    constexpr int NG = D / 32;
+    constexpr int VD = D / 16;
+    using VO = ValueOp<TV, VD>;
+    constexpr uint32_t KT = step_keys(D);
+    constexpr int NT = KT / 16;  // key tiles of a step
+    constexpr uint32_t NC = KT > 64 ? KT / 64 : 1;  // keys a lane finds the cells of
+    constexpr uint32_t NLK = (KT + SK::per_load - 1) / SK::per_load;  // loads of a step
+    constexpr uint32_t NLV = (KT + SV::per_load - 1) / SV::per_load;
+    typedef typename UnitOf<SK::unit>::type UK;
+    typedef typename UnitOf<SV::unit>::type UV;
+    typedef uint16_t scales_t __attribute__((ext_vector_type(NG)));
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ float2 wave_ml[kWaves][kRowTile];
+    __shared__ uint32_t first_odd[D];
+
+    const uint32_t unit = blockIdx.x % p.units;
+    const uint32_t y = blockIdx.x / p.units;
+    const uint32_t s = unit / p.n_parts;
+    const uint32_t part = unit - s * p.n_parts;
+    if (s >= p.n_seq) {
+        return;
+    }
+    const uint32_t hk = y % p.n_head_kv;
+    const uint32_t tile = y / p.n_head_kv;
+    const Span r = request_span(p, s);
+    const uint32_t m = min(r.m, p.max_q);
+    const uint32_t row0 = tile * kRowTile;
+    if (row0 >= m * p.group) {
+        return;
+    }
+    const uint32_t rows = min(kRowTile, m * p.group - row0);
+    const uint32_t tok0 = row0 / p.group;  // first and last token of the rows
+    const uint32_t tok1 = (row0 + rows - 1u) / p.group;
+    const uint32_t n = key_limit(p, r, tok1);      // keys any of them attends
+    const uint32_t n_all = key_limit(p, r, tok0);  // keys all of them attend
+    const uint32_t n_parts = max(1u, (n + p.chunk - 1u) / p.chunk);
+    if (part >= n_parts) {
+        return;
+    }
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t nl = lane & 15u;   // query row; dim lane of the values
+    const uint32_t c = lane >> 4;     // chunk of the contraction
+    const uint32_t c0 = part * p.chunk;
+    const uint32_t c1 = min(n, c0 + p.chunk);
+    const uint8_t *k_head = p.k + static_cast<uint64_t>(hk) * SK::bytes;
+    const uint8_t *v_head = p.v + static_cast<uint64_t>(hk) * SV::bytes;
+    const uint32_t *table = p.table + static_cast<uint64_t>(s) * p.table_stride;
+
+    // The cells of this lane's keys of the step at j0, and which keys exist
+    // (bit = key); one that does not has cell 0, and is masked where it matters.
+    struct Cells {
+        uint32_t at[NC];
+        uint64_t have[NC];
+    };
+    auto cells_of = [&](uint32_t j0) {
+        Cells r;
+#pragma unroll
+        for (uint32_t i = 0; i < NC; ++i) {
+            const uint32_t j = j0 + (lane & (KT - 1u)) + 64u * i;
+            uint32_t slot = KVMEM_HIP_NO_SLOT;
+            const uint32_t b = j / p.T;
+            if (j < c1) {
+                slot = table[b];
+            }
+            r.at[i] = slot < p.n_slots ? slot * p.T + (j - b * p.T) : 0u;
+            r.have[i] = __ballot(slot < p.n_slots);
+        }
+        return r;
+    };
+    auto cell_at = [&](const Cells &cells, uint32_t key) {
+        uint32_t at = __shfl(cells.at[0], key & (KT - 1u) & 63u, 64);
+        if constexpr (NC == 2) {
+            const uint32_t hi = __shfl(cells.at[1], key & 63u, 64);
+            at = key < 64u ? at : hi;
+        }
+        return at;
+    };
+    const uint32_t kk = lane / SK::units;  // this lane's key and unit of a load
+    const uint32_t ku = min(kk, SK::per_load - 1u) == kk ? lane - kk * SK::units : 0u;
+    const uint32_t vk = lane / SV::units;
+    const uint32_t vu = min(vk, SV::per_load - 1u) == vk ? lane - vk * SV::units : 0u;
+    UK rk[NLK];
+    UV rv[NLV];
+    auto load_tile = [&](const Cells &cells) {
+#pragma unroll
+        for (uint32_t i = 0; i < NLK; ++i) {
+            const uint32_t at = cell_at(cells, kk + i * SK::per_load);
+            rk[i] = *reinterpret_cast<const UK *>(k_head + static_cast<uint64_t>(at) * p.row_k + ku * SK::unit);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < NLV; ++i) {
+            const uint32_t at = cell_at(cells, vk + i * SV::per_load);
+            rv[i] = *reinterpret_cast<const UV *>(v_head + static_cast<uint64_t>(at) * p.row_v + vu * SV::unit);
+        }
+    };
+    constexpr uint32_t step = kWaves * KT;
+    uint32_t j0 = c0 + wave * KT;
+    Cells cells = cells_of(j0);
+    const bool uneven = tok0 != tok1 && c1 > n_all;  // some rows do not attend all the keys
+    if (uneven) {
+        if (threadIdx.x < D) {
+            first_odd[threadIdx.x] = ~0u;
+        }
+        __syncthreads();
+    }
+
+    // up to 8 rows: each stands in two columns, for the upper and the lower
+    // digits of its weights
+    const bool twice = rows <= 8u;
+    const uint32_t my_row = row0 + min(twice ? (nl & 7u) : nl, rows - 1u);
+    const uint32_t my_tok = my_row / p.group;
+    const uint32_t my_head = hk * p.group + (my_row - my_tok * p.group);
+    const uint32_t limit = key_limit(p, r, my_tok);
+
+    // The row's queries, scaled into f16's range.  Codes carry an offset: the
+    // sum of a group's queries times it comes off each score, as one more product
+    // of the groups' scales with those sums (in three f16 pieces, 33 bits).
+    half8_t qf[NG];
+    half8_t q_off;
+    float fac;
+    {
+        const uint8_t *q = p.q + static_cast<uint64_t>(r.first + my_tok) * p.q_nb2 + my_head * p.q_nb1;
+        u32x4_t x[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            x[g] = load_query<KO>(q, g, c);
+        }
+        load_tile(cells);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                bits = max_magnitude(x[g][i], bits);
+            }
+        }
+        bits = max(bits & 0xffffu, bits >> 16);
+        float most = p.q_bf16 ? query_value<true>(bits) : query_value<false>(bits);
+        most = fmaxf(most, lane_xor16(most));
+        most = fmaxf(most, lane_xor32(most));
+        const int ex = query_shift(most);
+        const float up = ldexpf(1.0f, ex);
+        if (p.q_bf16) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                qf[g] = query_operand<KO, true>(x[g], up);
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                qf[g] = query_operand<KO, false>(x[g], up);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            q_off[e] = 0;
+        }
+        if constexpr (KO::codes) {
+            // piece c of the sum stands in chunk c of the contraction
+            const _Float16 pick[3] = {static_cast<_Float16>(c == 0 ? 1.0f : 0.0f),
+                                      static_cast<_Float16>(c == 1 ? 1.0f : 0.0f),
+                                      static_cast<_Float16>(c == 2 ? 1.0f : 0.0f)};
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                float all = 0.0f;
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) {
+                    all += static_cast<float>(qf[g][e]);
+                    qf[g][e] *= static_cast<_Float16>(1.0f / KO::times(e));
+                }
+                all += lane_xor16(all);
+                all += lane_xor32(all);
+                all *= -KO::offset * 0x1p-10f;
+                const _Float16 hi = static_cast<_Float16>(all);
+                const float left = all - static_cast<float>(hi);
+                const _Float16 mid = static_cast<_Float16>(left);
+                const _Float16 lo = static_cast<_Float16>(left - static_cast<float>(mid));
+                q_off[g] = hi * pick[0] + mid * pick[1] + lo * pick[2];
+            }
+        }
+        fac = ldexpf(p.scale * kLog2e, (KO::codes ? 24 : 0) - ex);
+    }
+
+    uint8_t *kt = lds + wave * decode_wave_bytes<TK, TV, D>();
+    uint8_t *vt = kt + KT * SK::stride;
+    scales_t *ks = reinterpret_cast<scales_t *>(vt + KT * SV::stride);  // [key] scales of its groups
+
+    float top = -INFINITY;  // of the row, log2 units
+    float sum = 0.0f;       // of this lane's weights
+    float4_t o[VD];
+#pragma unroll
+    for (int t = 0; t < VD; ++t) {
+        o[t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    Cells next = cells_of(j0 + step);
+    for (; j0 < c1; j0 += step) {
+        const Cells now = cells;
+        bool whole = true;
+#pragma unroll
+        for (uint32_t i = 0; i < NC; ++i) {
+            whole = whole && now.have[i] == ~0ull;
+        }
+        wave_lds_sync();  // the last step's reads are done
+        if (kk < SK::per_load) {
+#pragma unroll
+            for (uint32_t i = 0; i < NLK; ++i) {
+                const uint32_t key = kk + i * SK::per_load;
+                if ((i + 1) * SK::per_load <= KT || key < KT) {
+                    *reinterpret_cast<UK *>(kt + key * SK::stride + ku * SK::unit) = rk[i];
+                }
+            }
+        }
+        if (vk < SV::per_load) {
+#pragma unroll
+            for (uint32_t i = 0; i < NLV; ++i) {
+                const uint32_t key = vk + i * SV::per_load;
+                if ((i + 1) * SV::per_load <= KT || key < KT) {
+                    *reinterpret_cast<UV *>(vt + key * SV::stride + vu * SV::unit) = rv[i];
+                }
+            }
+        }
+        wave_lds_sync();
+        cells = next;
+        load_tile(cells);
+        next = cells_of(j0 + 2u * step);
+        if constexpr (KO::codes) {
+            // a key's scales side by side
+            for (uint32_t key = lane % KT; key < KT; key += 64u) {
+                constexpr uint32_t per = KT < 64u ? NG * KT / 64u : NG;  // groups of a lane
+                const uint32_t g0 = KT < 64u ? lane / KT * per : 0u;
+#pragma unroll
+                for (uint32_t g = 0; g < per; ++g) {
+                    reinterpret_cast<uint16_t *>(ks + key)[g0 + g] =
+                        static_cast<uint16_t>(lds_half(kt + key * SK::stride + (g0 + g) * SK::GB));
+                }
+            }
+            wave_lds_sync();
+        }
+        float x[NT][4];
+#pragma unroll
+        for (uint32_t a = 0; a < NT; ++a) {
+            const uint8_t *kr = kt + (16u * a + nl) * SK::stride;
+            float4_t sc{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (KO::codes) {
+                half8_t kd;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    kd[e] = 0;
+                }
+                const scales_t mine = ks[16u * a + nl];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    kd[g] = __builtin_bit_cast(_Float16, static_cast<uint16_t>(mine[g]));
+                }
+                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kd, q_off, sc, 0, 0, 0);
+                sc *= 0x1p-14f;
+                scales_t d[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    d[i] = ks[16u * a + 4u * c + i];
+                }
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const half8_t kf = __builtin_bit_cast(half8_t, KO::load(kr + g * SK::GB, c, (g & 1) ? 0u : 2u));
+                    const float4_t acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        kf, qf[g], float4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        sc[i] = __builtin_fmaf(
+                            static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(d[i][g]))), acc[i],
+                            sc[i]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const half8_t kf = __builtin_bit_cast(half8_t, KO::load(kr + g * SK::GB, c, (g & 1) ? 0u : 2u));
+                    sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[g], sc, 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[a][i] = sc[i] * fac;
+            }
+        }
+        if (!whole || j0 + KT > n_all) {
+#pragma unroll
+            for (uint32_t h = 0; h < NT / 2; ++h) {
+                const uint32_t seen = seen_keys(static_cast<uint32_t>(now.have[h >> 1] >> (32u * (h & 1u))),
+                                                static_cast<int32_t>(limit - j0) - static_cast<int32_t>(32u * h), 4u * c);
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) {
+                    float &v = x[2 * h + (e >> 2)][e & 3u];
+                    v = (seen & (1u << (16u * (e >> 2) + (e & 3u)))) ? v : -INFINITY;
+                }
+            }
+        }
+        float most = -INFINITY;
+#pragma unroll
+        for (uint32_t a = 0; a < NT; ++a) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                most = fmaxf(most, x[a][i]);
+            }
+        }
+        most = fmaxf(most, lane_xor16(most));
+        most = fmaxf(most, lane_xor32(most));
+        if (__any(most > top + kTopSlack)) {
+            const float higher = fmaxf(top, most);
+            const float fade = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
+            sum *= fade;
+#pragma unroll
+            for (int t = 0; t < VD; ++t) {
+                o[t] *= fade;
+            }
+            top = higher;
+        }
+        const float base = (top == -INFINITY ? 0.0f : top) - kWeightShift;
+        half8_t w[NT / 2];
+#pragma unroll
+        for (uint32_t a = 0; a < NT; ++a) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const float pe = __builtin_amdgcn_exp2f(x[a][i] - base);
+                sum += pe;
+                const _Float16 hi = static_cast<_Float16>(pe);
+                w[a >> 1][4u * (a & 1u) + i] =
+                    twice && (nl & 8u) ? static_cast<_Float16>(pe - static_cast<float>(hi)) : hi;
+            }
+        }
+#pragma unroll
+        for (uint32_t h = 0; h < NT / 2; ++h) {  // 32 keys each
+            VO vo;
+            vo.raw(nl, [&](uint32_t e) {
+                return vt + (32u * h + 16u * (e >> 2) + 4u * c + (e & 3u)) * SV::stride;
+            });
+            u32x4_t keep{~0u, ~0u, ~0u, ~0u};
+            if (!whole) {  // rows of keys that do not exist are not even finite
+                keep = keep_keys<16>(static_cast<uint32_t>(now.have[h >> 1] >> (32u * (h & 1u))) >> (4u * c));
+            }
+            vo.emit(keep, [&](int t0, u32x4_t *a) {
+                if (uneven && j0 + KT > n_all) {
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        clear_odd(a[t], first_odd + VO::dim(nl, t0 + t),
+                                  [&](uint32_t e) { return j0 + 32u * h + 16u * (e >> 2) + 4u * c + (e & 3u); });
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    o[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a[t]), w[h],
+                                                                       o[t0 + t], 0, 0, 0);
+                }
+            });
+        }
+    }
+
+    // join the chunks' sums and the two columns of a row
+    sum += lane_xor16(sum);
+    sum += lane_xor32(sum);
+    if (twice) {
+#pragma unroll
+        for (int t = 0; t < VD; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                o[t][i] += lane_xor8(o[t][i]);
+            }
+        }
+    }
+    if (c == 0) {
+        wave_ml[wave][nl] = make_float2(top, sum);
+    }
+    __syncthreads();  // every wave has left its tiles
+    float all = wave_ml[0][nl].x;
+#pragma unroll
+    for (uint32_t w = 1; w < kWaves; ++w) {
+        all = fmaxf(all, wave_ml[w][nl].x);
+    }
+    float *ow = reinterpret_cast<float *>(lds) + wave * rows * D;  // [row][dim]
+    const float fade = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - all);
+    if (nl < rows) {
+#pragma unroll
+        for (int t = 0; t < VD; ++t) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                ow[nl * D + VO::dim(4u * c + i, t)] = o[t][i] * fade;
+            }
+        }
+    }
+    __syncthreads();
+    const float *ol = reinterpret_cast<const float *>(lds);
+    const bool last = n_parts == 1;
+    float *turn = reinterpret_cast<float *>(lds);
+    for (uint32_t e0 = 0; e0 < rows * D; e0 += 256u) {
+        const uint32_t e = e0 + threadIdx.x;
+        const bool in = e < rows * D;
+        const uint32_t row = min(e / D, rows - 1u);
+        const uint32_t d = e & (D - 1u);
+        const uint32_t tok = (row0 + row) / p.group;
+        const uint32_t head = hk * p.group + (row0 + row - tok * p.group);
+        const uint64_t at = static_cast<uint64_t>(r.first + tok) * p.n_head + head;
+        float total = 0.0f, mx = -INFINITY, x = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; ++w) {
+            mx = fmaxf(mx, wave_ml[w][row].x);
+        }
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; ++w) {
+            const float2 ml = wave_ml[w][row];
+            total += ml.x == -INFINITY ? 0.0f * ml.y : ml.y * __builtin_amdgcn_exp2f(ml.x - mx);
+            x += in ? ol[w * rows * D + e] : 0.0f;
+        }
+        if (uneven && first_odd[d] < key_limit(p, r, tok)) {
+            x = NAN;
+        }
+        if (!last) {
+            if (in) {
+                const uint64_t pe = (static_cast<uint64_t>(part) * p.n_tokens * p.n_head) + at;
+                p.part_o[pe * D + d] = x;
+                if (d == 0) {
+                    p.part_ml[pe] = make_float2(mx, total);
+                }
+            }
+            continue;
+        }
+        x = total == 0.0f ? 0.0f : x / total;
+        if (p.hadamard) {
+            // this round's own 256 elements of the LDS rows (read above by these threads only)
+            x = rotate_back(x, p.hadamard, e & (p.hadamard - 1u), turn + (e - (e & (p.hadamard - 1u))));
+        }
+        if (in) {
+            store_elem(p.out, p.out_type, at * D + d, x);
+            if (d == 0 && p.lse) {
+                p.lse[at] = total == 0.0f ? -INFINITY : (mx - kWeightShift) / kLog2e + logf(total);
+            }
+        }
+    }
+}
+
+// f16 values of a key operand's codes, scaled (rounded once).
+template <class KO>
+__device__ inline u32x4_t key_values(u32x4_t codes, uint32_t scale) {
+    if constexpr (!KO::codes) {
+        return codes;
+    } else {
+        u32x4_t r;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            r[j] = KO::times(2 * j) == 1.0f ? pair_value(codes[j], KO::offset, scale)
+                                            : pair_value_hi(codes[j], KO::offset, scale);
+        }
+        return r;
+    }
+}
+
+// ------------------------------------------------------------ many queries
+
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+// Four neighbouring output elements.
+__device__ inline void store4(uint8_t *out, int type, uint64_t e, float4_t x) {
+    if (type == KVMEM_TYPE_F32) {
+        *reinterpret_cast<float4_t *>(out + 4 * e) = x;
+    } else if (type == KVMEM_TYPE_F16) {
+        *reinterpret_cast<half4_t *>(out + 2 * e) = __builtin_convertvector(x, half4_t);
+    } else {
+        typedef __bf16 bf4_t __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<bf4_t *>(out + 2 * e) = __builtin_convertvector(x, bf4_t);
+    }
+}
+
+template <int TK, int TV, int D>
+struct PrefillLds {
+    static constexpr uint32_t KT = step_keys(D);
+    static constexpr uint32_t raw_k = KT * Slice<TK, D>::bytes;  // rows as cached
+    static constexpr uint32_t raw = raw_k + KT * Slice<TV, D>::bytes;
+    static constexpr uint32_t key_stride = 2 * D + 16;           // padded against bank conflicts
+    static constexpr uint32_t keys = KT * key_stride;            // keys as f16 [key][D]
+    static constexpr uint32_t values = KT * 2 * D;               // values as f16 [octet of keys][D] operands
+    // two of each: one in use while the next is made; 16 bytes behind the
+    // last row, whose last word is read with the next one
+    static constexpr uint32_t bytes = 2 * (raw + keys + values) + 16;
+};
+
+// Where operand `dim` of an octet stands: neighbours in the writing lanes' and
+// in the reading lanes' order fall into different banks.
+__device__ inline uint32_t value_slot(uint32_t dim) {
+    return dim ^ ((dim >> 5) & 7u) ^ ((dim >> 1) & 8u);
+}
+
+// RT tiles of 32 rows a wave, 4 waves: 128 RT rows of one KV head's queries over
+// one part of a request's keys.  Steps of step_keys(D) keys: their rows come into
+// LDS two steps ahead, are made f16 one step ahead (each thread 8 keys of 4
+// value dims and 4 octets of key dims) between the score products of the
+// present step, and every wave multiplies its rows (transposed products as in
+// the decode kernel, on 32x32 tiles).  One barrier a step.
+template <int TK, int TV, int D, int RT>
+__global__ __launch_bounds__(256, 1) void attn_prefill_kernel(AttnParams p) {
+    using SK = Slice<TK, D>;
+    using SV = Slice<TV, D>;
+    using KO = KeyOp<TK>;
+    using VO = ValueOp<TV, 4>;
+    using L = PrefillLds<TK, TV, D>;
+    constexpr uint32_t KT = L::KT;
+    constexpr int NT = KT / 32;    // key tiles of a step
+    constexpr int QS = D / 16;     // products of a key tile's scores
+    constexpr int NB = D / 32;     // blocks of value dims
+    constexpr uint32_t NC = KT > 64 ? KT / 64 : 1;
+    constexpr uint32_t NK = (KT * SK::units + 255u) / 256u;
+    constexpr uint32_t NV = (KT * SV::units + 255u) / 256u;
+    constexpr uint32_t kRows = prefill_rows(RT);
+    typedef typename UnitOf<SK::unit>::type UK;
+    typedef typename UnitOf<SV::unit>::type UV;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ uint32_t first_odd[D];
+
+    const uint32_t unit = blockIdx.x % p.units;
+    const uint32_t tile = p.row_tiles - 1u - blockIdx.x / p.units;  // long rows first
+    const uint32_t hk = unit % p.n_head_kv;
+    const uint32_t sp = unit / p.n_head_kv;
+    const uint32_t s = sp / p.n_parts;
+    const uint32_t part = sp - s * p.n_parts;
+    if (s >= p.n_seq) {
+        return;
+    }
+    const Span r = request_span(p, s);
+    const uint32_t m = min(r.m, p.max_q);
+    const uint32_t row0 = tile * kRows;
+    if (row0 >= m * p.group) {
+        return;
+    }
+    const uint32_t rows = min(kRows, m * p.group - row0);
+    const uint32_t n = key_limit(p, r, (row0 + rows - 1u) / p.group);
+    const uint32_t n_all = key_limit(p, r, row0 / p.group);
+    const uint32_t n_parts = max(1u, (n + p.chunk - 1u) / p.chunk);
+    if (part >= n_parts) {
+        return;
+    }
+    const uint32_t tid = threadIdx.x;
+    const uint32_t lane = tid & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t nl = lane & 31u;  // query row of a tile
+    const uint32_t hh = lane >> 5;   // half of the contraction
+    const uint32_t c0 = part * p.chunk;
+    const uint32_t c1 = min(n, c0 + p.chunk);
+    const uint8_t *k_head = p.k + static_cast<uint64_t>(hk) * SK::bytes;
+    const uint8_t *v_head = p.v + static_cast<uint64_t>(hk) * SV::bytes;
+    const uint32_t *table = p.table + static_cast<uint64_t>(s) * p.table_stride;
+
+    // as in the decode kernel: cells of a step's keys, and which keys exist
+    struct Cells {
+        uint32_t at[NC];
+        uint64_t have[NC];
+    };
+    auto cells_of = [&](uint32_t j0) {
+        Cells r;
+#pragma unroll
+        for (uint32_t i = 0; i < NC; ++i) {
+            const uint32_t j = j0 + (lane & (KT - 1u)) + 64u * i;
+            uint32_t slot = KVMEM_HIP_NO_SLOT;
+            const uint32_t b = j / p.T;
+            if (j < c1) {
+                slot = table[b];
+            }
+            r.at[i] = slot < p.n_slots ? slot * p.T + (j - b * p.T) : 0u;
+            r.have[i] = __ballot(slot < p.n_slots);
+        }
+        return r;
+    };
+    auto cell_at = [&](const Cells &cells, uint32_t key) {
+        uint32_t at = __shfl(cells.at[0], key & (KT - 1u) & 63u, 64);
+        if constexpr (NC == 2) {
+            const uint32_t hi = __shfl(cells.at[1], key & 63u, 64);
+            at = key < 64u ? at : hi;
+        }
+        return at;
+    };
+    UK rk[NK];
+    UV rv[NV];
+    auto load_tile = [&](const Cells &cells) {
+#pragma unroll
+        for (uint32_t i = 0; i < NK; ++i) {
+            const uint32_t u = i * 256u + tid;
+            const uint32_t key = u / SK::units;
+            const uint32_t at = cell_at(cells, key);
+            rk[i] = *reinterpret_cast<const UK *>(k_head + static_cast<uint64_t>(at) * p.row_k +
+                                                  (u - key * SK::units) * SK::unit);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < NV; ++i) {
+            const uint32_t u = i * 256u + tid;
+            const uint32_t key = u / SV::units;
+            const uint32_t at = cell_at(cells, key);
+            rv[i] = *reinterpret_cast<const UV *>(v_head + static_cast<uint64_t>(at) * p.row_v +
+                                                  (u - key * SV::units) * SV::unit);
+        }
+    };
+    auto put_tile = [&](uint8_t *raw) {
+#pragma unroll
+        for (uint32_t i = 0; i < NK; ++i) {
+            const uint32_t u = i * 256u + tid;
+            if ((i + 1) * 256u <= KT * SK::units || u < KT * SK::units) {
+                *reinterpret_cast<UK *>(raw + u * SK::unit) = rk[i];
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < NV; ++i) {
+            const uint32_t u = i * 256u + tid;
+            if ((i + 1) * 256u <= KT * SV::units || u < KT * SV::units) {
+                *reinterpret_cast<UV *>(raw + L::raw_k + u * SV::unit) = rv[i];
+            }
+        }
+    };
+    uint8_t *const raw0 = lds;
+    uint8_t *const keys0 = lds + 2 * L::raw;
+    uint8_t *const values0 = keys0 + 2 * L::keys;
+
+    // Making f16 of a step's rows, in pieces.  Values: this thread's octet of
+    // keys (keys 16 (q / 2) + 8 (e / 4) + 4 (q % 2) + e % 4, as a lane of the
+    // scores holds them) and its 4 dims.
+    const uint32_t oct = tid / (D / 4);
+    const uint32_t dl = tid % (D / 4);
+    VO vo;
+    auto value_read = [&](const uint8_t *raw) {
+        vo.raw(dl, [&](uint32_t e) {
+            return raw + L::raw_k + (16u * (oct >> 1) + 8u * (e >> 2) + 4u * (oct & 1u) + (e & 3u)) * SV::bytes;
+        });
+    };
+    auto value_write = [&](uint8_t *values, const uint64_t *have, uint32_t j0) {
+        const uint32_t in = static_cast<uint32_t>(have[oct >> 3] >> (16u * ((oct >> 1) & 3u) + 4u * (oct & 1u)));
+        vo.emit(keep_keys<8>(in), [&](int, u32x4_t *a) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const uint32_t dim = VO::dim(dl, t);
+                if (j0 + KT > n_all) {
+                    clear_odd(a[t], first_odd + dim, [&](uint32_t e) {
+                        return j0 + 16u * (oct >> 1) + 8u * (e >> 2) + 4u * (oct & 1u) + (e & 3u);
+                    });
+                }
+                *reinterpret_cast<u32x4_t *>(values + (oct * D + value_slot(dim)) * 16u) = a[t];
+            }
+        });
+    };
+    // Keys: octet i of 4 of this thread.
+    u32x4_t codes;
+    uint32_t key_scale = 0;
+    auto key_read = [&](const uint8_t *raw, uint32_t i) {
+        const uint32_t u = i * 256u + tid;
+        const uint32_t key = u / (D / 8);
+        const uint32_t o = u % (D / 8);
+        const uint8_t *g = raw + key * SK::bytes + (o >> 2) * SK::GB;
+        if constexpr (KO::codes) {
+            key_scale = lds_half(g) * 0x00010001u;
+        }
+        codes = KO::load(g, o & 3u, 2u * (~(o >> 2) & 1u));
+    };
+    auto key_write = [&](uint8_t *keys, uint32_t i) {
+        const uint32_t u = i * 256u + tid;
+        const uint32_t key = u / (D / 8);
+        const uint32_t o = u % (D / 8);
+        *reinterpret_cast<u32x4_t *>(keys + key * L::key_stride + o * 16u) = key_values<KO>(codes, key_scale);
+    };
+
+    Cells cells = cells_of(c0);
+    load_tile(cells);
+    uint64_t have[NC], have1[NC];
+#pragma unroll
+    for (uint32_t i = 0; i < NC; ++i) {
+        have[i] = cells.have[i];
+    }
+    cells = cells_of(c0 + KT);
+
+    // This wave's queries, scaled into f16's range row by row: made operands in
+    // LDS (the step buffers are not in use yet), a tile at a time.
+    half8_t qf[RT][QS];
+    float fac[RT];
+    uint32_t limit[RT];
+    uint64_t at[RT];  // (token, head) row of q and out
+    bool mine[RT];
+    u32x4_t *ql = reinterpret_cast<u32x4_t *>(lds) + wave * QS * 64u + lane;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const uint32_t in_tile = (wave * RT + rt) * 32u + nl;
+        const uint32_t row = row0 + min(in_tile, rows - 1u);
+        mine[rt] = in_tile < rows;
+        const uint32_t tok = row / p.group;
+        const uint32_t head = hk * p.group + (row - tok * p.group);
+        limit[rt] = key_limit(p, r, tok);
+        at[rt] = static_cast<uint64_t>(r.first + tok) * p.n_head + head;
+        const uint8_t *q = p.q + static_cast<uint64_t>(r.first + tok) * p.q_nb2 + head * p.q_nb1;
+        uint32_t bits = 0;
+#pragma unroll 4
+        for (uint32_t st = 0; st < QS; ++st) {
+            const u32x4_t x = load_query<KO>(q, st >> 1, 2u * (st & 1u) + hh);
+            ql[st * 64u] = x;
+            bits = max_magnitude(x[0], max_magnitude(x[1], max_magnitude(x[2], max_magnitude(x[3], bits))));
+        }
+        bits = max(bits & 0xffffu, bits >> 16);
+        float most = p.q_bf16 ? query_value<true>(bits) : query_value<false>(bits);
+        most = fmaxf(most, lane_xor32(most));
+        const int ex = query_shift(most);
+        const float up = ldexpf(1.0f, ex);
+#pragma unroll 1
+        for (uint32_t st = 0; st < QS; ++st) {
+            const u32x4_t x = ql[st * 64u];
+            const half8_t h = p.q_bf16 ? query_operand<KO, true>(x, up) : query_operand<KO, false>(x, up);
+            ql[st * 64u] = __builtin_bit_cast(u32x4_t, h);
+        }
+#pragma unroll
+        for (uint32_t st = 0; st < QS; ++st) {
+            qf[rt][st] = __builtin_bit_cast(half8_t, ql[st * 64u]);
+        }
+        wave_lds_sync();
+        fac[rt] = fmaxf(ldexpf(p.scale * kLog2e, -ex), 0x1p-126f);
+    }
+
+    float top[RT], sum[RT];
+    float16_t o[RT][NB];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        top[rt] = -INFINITY;
+        sum[rt] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                o[rt][b][i] = 0.0f;
+            }
+        }
+    }
+    if (tid < D) {
+        first_odd[tid] = ~0u;
+    }
+    __syncthreads();  // the queries have left the step buffers
+    put_tile(raw0);
+    load_tile(cells);
+#pragma unroll
+    for (uint32_t i = 0; i < NC; ++i) {
+        have1[i] = cells.have[i];
+    }
+    cells = cells_of(c0 + 2u * KT);
+    __syncthreads();
+    put_tile(raw0 + L::raw);
+    value_read(raw0);
+    value_write(values0, have, c0);
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        key_read(raw0, i);
+        key_write(keys0, i);
+    }
+    __syncthreads();
+
+    uint32_t buf = 0;  // step modulo 2
+    for (uint32_t j0 = c0; j0 < c1; j0 += KT) {
+        uint64_t have2[NC];
+        load_tile(cells);
+#pragma unroll
+        for (uint32_t i = 0; i < NC; ++i) {
+            have2[i] = cells.have[i];
+        }
+        cells = cells_of(j0 + 3u * KT);
+        const uint8_t *raw1 = raw0 + (buf ^ 1u) * L::raw;
+        uint8_t *keys1 = keys0 + (buf ^ 1u) * L::keys;
+        uint8_t *values1 = values0 + (buf ^ 1u) * L::values;
+
+        float16_t sc[RT][NT];
+        const uint8_t *kr = keys0 + buf * L::keys + nl * L::key_stride + hh * 16u;
+#pragma unroll
+        for (int a = 0; a < NT; ++a) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    sc[rt][a][i] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int st = 0; st < QS; ++st) {
+                const int z = a * QS + st;  // 16 in all
+                const half8_t kf = *reinterpret_cast<const half8_t *>(kr + a * 32 * L::key_stride + st * 32);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    sc[rt][a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[rt][st], sc[rt][a], 0, 0, 0);
+                }
+                if (z == 0) {
+                    value_read(raw1);
+                } else if (z == 3) {
+                    value_write(values1, have1, j0 + KT);
+                } else if (z >= 4 && (z - 4) % 3 == 0) {
+                    key_read(raw1, (z - 4) / 3);
+                } else if (z >= 5 && (z - 5) % 3 == 0) {
+                    key_write(keys1, (z - 5) / 3);
+                }
+            }
+        }
+        bool whole = j0 + KT <= n_all;
+#pragma unroll
+        for (uint32_t i = 0; i < NC; ++i) {
+            whole = whole && have[i] == ~0ull;
+        }
+        half8_t w[RT][2 * NT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            if (!whole) {
+#pragma unroll
+                for (uint32_t a = 0; a < NT; ++a) {
+                    const uint32_t seen =
+                        seen_keys(static_cast<uint32_t>(have[a >> 1] >> (32u * (a & 1u))),
+                                  static_cast<int32_t>(limit[rt] - j0) - static_cast<int32_t>(32u * a), 4u * hh);
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i) {
+                        sc[rt][a][i] = (seen & (1u << (8u * (i >> 2) + (i & 3u)))) ? sc[rt][a][i] : -INFINITY;
+                    }
+                }
+            }
+            float most = -INFINITY;
+#pragma unroll
+            for (int a = 0; a < NT; ++a) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    most = fmaxf(most, sc[rt][a][i]);
+                }
+            }
+            most *= fac[rt];
+            most = fmaxf(most, lane_xor32(most));
+            if (__any(most > top[rt] + kTopSlack)) {
+                const float higher = fmaxf(top[rt], most);
+                const float fade = top[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[rt] - higher);
+                sum[rt] *= fade;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    o[rt][b] *= fade;
+                }
+                top[rt] = higher;
+            }
+            const float base = (top[rt] == -INFINITY ? 0.0f : top[rt]) - kWeightShift;
+#pragma unroll
+            for (int a = 0; a < NT; ++a) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rt][a][i], fac[rt], -base));
+                    sum[rt] += pe;
+                    w[rt][2 * a + (i >> 3)][i & 7] = static_cast<_Float16>(pe);
+                }
+            }
+        }
+        const uint8_t *vr = values0 + buf * L::values + hh * D * 16u;
+#pragma unroll
+        for (int ks = 0; ks < 2 * NT; ++ks) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const half8_t vf =
+                    *reinterpret_cast<const half8_t *>(vr + (2 * ks * D + value_slot(32u * b + nl)) * 16u);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    o[rt][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, w[rt][ks], o[rt][b], 0, 0, 0);
+                }
+            }
+        }
+        put_tile(raw0 + buf * L::raw);
+#pragma unroll
+        for (uint32_t i = 0; i < NC; ++i) {
+            have[i] = have1[i];
+            have1[i] = have2[i];
+        }
+        buf ^= 1u;
+        __syncthreads();
+    }
+
+    // a lane holds dims 32 b + 8 (i / 4) + 4 hh + i % 4 of its rows
+    const bool uneven = c1 > n_all && __syncthreads_or(tid < D && first_odd[tid] != ~0u);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        sum[rt] += lane_xor32(sum[rt]);
+        // parts, and sums that still have to be rotated, go to the joining kernel
+        const bool joined = n_parts > 1 || p.hadamard;
+        const float f = joined ? 1.0f : sum[rt] == 0.0f ? 0.0f : 1.0f / sum[rt];
+        const uint64_t to = (joined ? static_cast<uint64_t>(part) * p.n_tokens * p.n_head : 0u) + at[rt];
+        uint8_t *out = joined ? reinterpret_cast<uint8_t *>(p.part_o) : p.out;
+        const int type = joined ? static_cast<int>(KVMEM_TYPE_F32) : p.out_type;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const uint32_t dim = 32 * b + 2 * i + 4 * hh;
+                float4_t x{o[rt][b][i] * f, o[rt][b][i + 1] * f, o[rt][b][i + 2] * f, o[rt][b][i + 3] * f};
+                if (uneven) {
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        x[d] = first_odd[dim + d] < limit[rt] ? NAN : x[d];
+                    }
+                }
+                if (mine[rt]) {
+                    store4(out, type, to * D + dim, x);
+                }
+            }
+        }
+        if (mine[rt] && hh == 0) {
+            if (joined) {
+                p.part_ml[to] = make_float2(top[rt], sum[rt]);
+            } else if (p.lse) {
+                p.lse[at[rt]] = sum[rt] == 0.0f ? -INFINITY : (top[rt] - kWeightShift) / kLog2e + logf(sum[rt]);
+            }
+        }
+    }
+}
+
+// -------------------------------------------------------------------- launch
+
+template <int TK, int TV, int D>
+static void launch_types(hipStream_t stream, const AttnPlan &pl, const AttnParams &p) {
+    const uint32_t grid = static_cast<uint32_t>(pl.grid);
+    if (pl.prefill == 2) {
+        if constexpr (D < 256) {  // (256 dims of two tiles are more than a wave's registers)
+            attn_prefill_kernel<TK, TV, D, 2><<<grid, 256, PrefillLds<TK, TV, D>::bytes, stream>>>(p);
+        }
+    } else if (pl.prefill == 1) {
+        attn_prefill_kernel<TK, TV, D, 1><<<grid, 256, PrefillLds<TK, TV, D>::bytes, stream>>>(p);
+    } else {
+        const uint32_t rows = std::min(kRowTile, p.max_q * p.group);
+        // 16 bytes behind the last slice: its last word is read with the next one
+        const uint32_t lds = std::max<uint32_t>(kWaves * decode_wave_bytes<TK, TV, D>() + 16u,
+                                                std::max<uint32_t>(kWaves * rows * D * 4u, 1024u));
+        attn_decode_kernel<TK, TV, D><<<grid, 256, lds, stream>>>(p);
+    }
+}
+
+template <int TK, int TV>
+static void launch_dims(hipStream_t stream, uint32_t d, const AttnPlan &pl, const AttnParams &p) {
+    if (d == 64) {
+        launch_types<TK, TV, 64>(stream, pl, p);
+    } else if (d == 128) {
+        launch_types<TK, TV, 128>(stream, pl, p);
+    } else {
+        launch_types<TK, TV, 256>(stream, pl, p);
+    }
+}
+
+template <int TK>
+void launch_attention(hipStream_t stream, int type_v, uint32_t d, const AttnPlan &pl, const AttnParams &p) {
+    switch (type_v) {
+        case KVMEM_TYPE_Q4_0: launch_dims<TK, KVMEM_TYPE_Q4_0>(stream, d, pl, p); break;
+        case KVMEM_TYPE_Q5_0: launch_dims<TK, KVMEM_TYPE_Q5_0>(stream, d, pl, p); break;
+        case KVMEM_TYPE_Q8_0: launch_dims<TK, KVMEM_TYPE_Q8_0>(stream, d, pl, p); break;
+        default: launch_dims<TK, KVMEM_TYPE_F16>(stream, d, pl, p); break;
+    }
+}
+
+}  // namespace kvmem_hip

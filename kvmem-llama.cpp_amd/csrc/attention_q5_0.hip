@@ -1,0 +1,8 @@
+// Attention over q5_0 keys.
+#include "attention_kernels.hpp"
+
+namespace kvmem_hip {
+
+template void launch_attention<KVMEM_TYPE_Q5_0>(hipStream_t, int, uint32_t, const AttnPlan &, const AttnParams &);
+
+}  // namespace kvmem_hip
