@@ -95,25 +95,40 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
 
 // Query rows of a request above which the prefill kernel takes the call.
 constexpr uint32_t kDecodeRows = 16;
-// Workgroups a launch is split up to.
+// Workgroups a decode launch is split up to.
 constexpr uint32_t kDecodeGroups = 512;
-constexpr uint32_t kPrefillGroups = 256;
+constexpr uint32_t kComputeUnits = 256;
 
 static AttnPlan plan_attention(const kvmem_hip_pool *pool, const kvmem_hip_attn_args *a) {
     AttnPlan pl{};
     const uint32_t max_q = a->q_start ? std::min(a->max_q, a->n_tokens) : 1u;
     const uint32_t group = a->n_head / a->n_head_kv;
     const uint64_t rows = static_cast<uint64_t>(max_q) * group;
-    pl.prefill = rows <= kDecodeRows ? 0u : rows <= prefill_rows(1) || a->head_dim == 256 ? 1u : 2u;
-    pl.row_tile = pl.prefill ? prefill_rows(pl.prefill) : kRowTile;
+    pl.prefill = rows <= kDecodeRows ? 0u : rows <= 128 ? 4u : 8u;
+    pl.row_tile = pl.prefill ? 32u * pl.prefill : kRowTile;
     pl.row_tiles = static_cast<uint32_t>((rows + pl.row_tile - 1) / pl.row_tile);
     const uint32_t quantum = step_keys(a->head_dim) * (pl.prefill ? 1u : kWaves);
     const uint64_t room = static_cast<uint64_t>(a->table_stride) * pool->block_tokens;
     const uint64_t keys = std::max<uint64_t>(1, std::min<uint64_t>(a->max_kv, room));
     const uint64_t groups = static_cast<uint64_t>(a->n_seq) * a->n_head_kv * pl.row_tiles;
-    const uint64_t want = pl.prefill ? kPrefillGroups : kDecodeGroups;
-    uint64_t parts = std::max<uint64_t>(1, want / groups);
-    parts = std::min<uint64_t>(parts, (keys + quantum - 1) / quantum);
+    const uint64_t most = (keys + quantum - 1) / quantum;
+    uint64_t parts = 1;
+    if (pl.prefill) {
+        // rounds of workgroups (one a compute unit) times the keys of each, and
+        // for every part the joining of its rows, in keys' time
+        const uint64_t join = static_cast<uint64_t>(a->n_tokens) * a->n_head / 256 + 64;
+        uint64_t best = ~uint64_t{0};
+        for (uint64_t k = 1; k <= std::min<uint64_t>(most, kComputeUnits) && groups * (k - 1) < 4 * kComputeUnits; ++k) {
+            const uint64_t rounds = (groups * k + kComputeUnits - 1) / kComputeUnits;
+            const uint64_t cost = rounds * ((keys + k - 1) / k) + (k > 1 ? k * join : 0);
+            if (cost < best) {
+                best = cost;
+                parts = k;
+            }
+        }
+    } else {
+        parts = std::min(std::max<uint64_t>(1, kDecodeGroups / groups), most);
+    }
     uint64_t chunk = (keys + parts - 1) / parts;
     chunk = (chunk + quantum - 1) / quantum * quantum;
     pl.chunk = static_cast<uint32_t>(chunk);
@@ -258,6 +273,15 @@ int kvmem_hip_attention(kvmem_hip_ctx *ctx, const kvmem_hip_pool *pool, uint32_t
     p.n_head_kv = a->n_head_kv;
     p.group = a->n_head / a->n_head_kv;
     p.T = pool->block_tokens;
+    if (p.T > 1) {
+        // ceil(2^(31 + l) / T), l = ceil(log2 T): exact for every j < 2^31
+        uint32_t l = 1;
+        while ((uint64_t{1} << l) < p.T) {
+            ++l;
+        }
+        p.T_mul = static_cast<uint32_t>(((uint64_t{1} << (31 + l)) + p.T - 1) / p.T);
+        p.T_shift = l - 1;
+    }
     p.n_slots = pool->n_slots;
     p.table_stride = a->table_stride;
     p.causal = a->causal != 0;

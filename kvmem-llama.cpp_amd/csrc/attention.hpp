@@ -32,6 +32,7 @@ struct AttnParams {
     uint32_t n_tokens, n_seq, max_q, max_kv, n_head, n_head_kv, group, T, n_slots, table_stride;
     uint32_t chunk;             // keys of one part
     uint32_t n_parts;           // parts of the longest request
+    uint32_t T_mul, T_shift;    // j / T as the upper word of j * T_mul, shifted (T > 1)
     uint32_t row_tile;          // rows of one workgroup
     uint32_t row_tiles;         // of the longest request
     uint32_t units;             // of the grid's fast index, a multiple of 8
@@ -42,6 +43,11 @@ struct AttnParams {
     uint32_t join_one;          // rows of a single part are joined (and rotated) too
     float scale;
 };
+
+// The block of key j < 2^31.
+__device__ inline uint32_t block_of(const AttnParams &p, uint32_t j) {
+    return p.T == 1u ? j : __umulhi(j, p.T_mul) >> p.T_shift;
+}
 
 // A request's share of the call: its first token, tokens, keys in range.
 struct Span {
@@ -97,7 +103,7 @@ __device__ inline float rotate_back(float x, uint32_t width, uint32_t d, float *
 
 // How a call is laid out on the chip.
 struct AttnPlan {
-    uint32_t prefill;          // row tiles of a prefill wave (0: decode kernel)
+    uint32_t prefill;          // waves of a prefill workgroup (0: decode kernel)
     uint32_t row_tile, row_tiles, chunk, n_parts, units;
     uint64_t grid;
     bool joined;               // a joining kernel follows
@@ -107,9 +113,6 @@ struct AttnPlan {
 // Keys of a step: about the same bytes for every head size (9 KiB of q4_0 keys
 // and values), enough in flight per compute unit to stream.
 constexpr uint32_t step_keys(uint32_t d) { return 32u * (256u / d); }
-// Query rows of a prefill workgroup whose waves hold `tiles` tiles of 32.
-constexpr uint32_t prefill_rows(uint32_t tiles) { return kWaves * 32u * tiles; }
-
 // Launches the decode or prefill kernel of key type TK (one translation unit
 // each).
 template <int TK>

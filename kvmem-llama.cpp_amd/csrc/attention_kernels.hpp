@@ -566,17 +566,30 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
         uint32_t at[NC];
         uint64_t have[NC];
     };
-    auto cells_of = [&](uint32_t j0) {
+    // Their table entries are read a step before they are looked at: a value of a
+    // load that is waited for here would wait for the rows requested before it.
+    struct Slots {
+        uint32_t of[NC];
+    };
+    auto slots_of = [&](uint32_t j0) {
+        Slots r;
+#pragma unroll
+        for (uint32_t i = 0; i < NC; ++i) {
+            const uint32_t j = j0 + (lane & (KT - 1u)) + 64u * i;
+            r.of[i] = KVMEM_HIP_NO_SLOT;
+            if (j < c1) {
+                r.of[i] = table[block_of(p, j)];
+            }
+        }
+        return r;
+    };
+    auto cells_of = [&](const Slots &slots, uint32_t j0) {
         Cells r;
 #pragma unroll
         for (uint32_t i = 0; i < NC; ++i) {
             const uint32_t j = j0 + (lane & (KT - 1u)) + 64u * i;
-            uint32_t slot = KVMEM_HIP_NO_SLOT;
-            const uint32_t b = j / p.T;
-            if (j < c1) {
-                slot = table[b];
-            }
-            r.at[i] = slot < p.n_slots ? slot * p.T + (j - b * p.T) : 0u;
+            const uint32_t slot = slots.of[i];
+            r.at[i] = slot < p.n_slots ? slot * p.T + (j - block_of(p, j) * p.T) : 0u;
             r.have[i] = __ballot(slot < p.n_slots);
         }
         return r;
@@ -609,7 +622,7 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
     };
     constexpr uint32_t step = kWaves * KT;
     uint32_t j0 = c0 + wave * KT;
-    Cells cells = cells_of(j0);
+    const Slots first_slots = slots_of(j0);
     const bool uneven = tok0 != tok1 && c1 > n_all;  // some rows do not attend all the keys
     if (uneven) {
         if (threadIdx.x < D) {
@@ -629,6 +642,8 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
     // The row's queries, scaled into f16's range.  Codes carry an offset: the
     // sum of a group's queries times it comes off each score, as one more product
     // of the groups' scales with those sums (in three f16 pieces, 33 bits).
+    Cells cells;
+    Slots next;
     half8_t qf[NG];
     half8_t q_off;
     float fac;
@@ -639,7 +654,9 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
         for (int g = 0; g < NG; ++g) {
             x[g] = load_query<KO>(q, g, c);
         }
+        cells = cells_of(first_slots, j0);
         load_tile(cells);
+        next = slots_of(j0 + step);
         uint32_t bits = 0;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -707,7 +724,6 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
         o[t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    Cells next = cells_of(j0 + step);
     for (; j0 < c1; j0 += step) {
         const Cells now = cells;
         bool whole = true;
@@ -735,9 +751,9 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
             }
         }
         wave_lds_sync();
-        cells = next;
+        cells = cells_of(next, j0 + step);
         load_tile(cells);
-        next = cells_of(j0 + 2u * step);
+        next = slots_of(j0 + 2u * step);
         if constexpr (KO::codes) {
             // a key's scales side by side
             for (uint32_t key = lane % KT; key < KT; key += 64u) {
@@ -971,6 +987,13 @@ __device__ inline u32x4_t key_values(u32x4_t codes, uint32_t scale) {
 // ------------------------------------------------------------ many queries
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
+// The same value, of which the compiler knows nothing: what is derived from it is
+// computed anew where it is used instead of being kept in registers.
+__device__ inline uint32_t anew(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+typedef __attribute__((address_space(3))) void lds_void_t;
 
 // Four neighbouring output elements.
 __device__ inline void store4(uint8_t *out, int type, uint64_t e, float4_t x) {
@@ -991,26 +1014,27 @@ struct PrefillLds {
     static constexpr uint32_t raw = raw_k + KT * Slice<TV, D>::bytes;
     static constexpr uint32_t key_stride = 2 * D + 16;           // padded against bank conflicts
     static constexpr uint32_t keys = KT * key_stride;            // keys as f16 [key][D]
-    static constexpr uint32_t values = KT * 2 * D;               // values as f16 [octet of keys][D] operands
+    // values as f16 [octet of keys][D] operands; one operand's room after each 32
+    // keeps the writing lanes (dims of neighbouring groups) on different banks
+    static constexpr uint32_t octet = (D + D / 32) * 16;
+    static constexpr uint32_t values = KT / 8 * octet;
     // two of each: one in use while the next is made; 16 bytes behind the
     // last row, whose last word is read with the next one
     static constexpr uint32_t bytes = 2 * (raw + keys + values) + 16;
 };
 
-// Where operand `dim` of an octet stands: neighbours in the writing lanes' and
-// in the reading lanes' order fall into different banks.
-__device__ inline uint32_t value_slot(uint32_t dim) {
-    return dim ^ ((dim >> 5) & 7u) ^ ((dim >> 1) & 8u);
-}
+// Where operand `dim` of an octet stands.
+__device__ inline uint32_t value_slot(uint32_t dim) { return dim + (dim >> 5); }
 
-// RT tiles of 32 rows a wave, 4 waves: 128 RT rows of one KV head's queries over
-// one part of a request's keys.  Steps of step_keys(D) keys: their rows come into
-// LDS two steps ahead, are made f16 one step ahead (each thread 8 keys of 4
-// value dims and 4 octets of key dims) between the score products of the
-// present step, and every wave multiplies its rows (transposed products as in
-// the decode kernel, on 32x32 tiles).  One barrier a step.
-template <int TK, int TV, int D, int RT>
-__global__ __launch_bounds__(256, 1) void attn_prefill_kernel(AttnParams p) {
+// NW waves of 32 rows of one KV head's queries over one part of a request's keys.
+// Steps of step_keys(D) keys: their rows come into LDS two steps ahead, are made
+// f16 one step ahead (8 keys of 4 value dims for each of 256 threads, and 4
+// octets of key dims for each of 256) between the score products of the present
+// step, and every wave multiplies its rows (transposed products as in the decode
+// kernel, on 32x32 tiles).  One barrier a step.  Two waves per SIMD cover each
+// other's LDS reads and softmax.
+template <int TK, int TV, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) {
     using SK = Slice<TK, D>;
     using SV = Slice<TV, D>;
     using KO = KeyOp<TK>;
@@ -1021,9 +1045,10 @@ __global__ __launch_bounds__(256, 1) void attn_prefill_kernel(AttnParams p) {
     constexpr int QS = D / 16;     // products of a key tile's scores
     constexpr int NB = D / 32;     // blocks of value dims
     constexpr uint32_t NC = KT > 64 ? KT / 64 : 1;
-    constexpr uint32_t NK = (KT * SK::units + 255u) / 256u;
-    constexpr uint32_t NV = (KT * SV::units + 255u) / 256u;
-    constexpr uint32_t kRows = prefill_rows(RT);
+    constexpr uint32_t NTH = 64 * NW;
+    constexpr uint32_t NK = (KT * SK::units + NTH - 1u) / NTH;
+    constexpr uint32_t NV = (KT * SV::units + NTH - 1u) / NTH;
+    constexpr uint32_t kRows = 32 * NW;
     typedef typename UnitOf<SK::unit>::type UK;
     typedef typename UnitOf<SV::unit>::type UV;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -1067,17 +1092,30 @@ __global__ __launch_bounds__(256, 1) void attn_prefill_kernel(AttnParams p) {
         uint32_t at[NC];
         uint64_t have[NC];
     };
-    auto cells_of = [&](uint32_t j0) {
+    // Their table entries are read a step before they are looked at: a value of a
+    // load that is waited for here would wait for the rows requested before it.
+    struct Slots {
+        uint32_t of[NC];
+    };
+    auto slots_of = [&](uint32_t j0) {
+        Slots r;
+#pragma unroll
+        for (uint32_t i = 0; i < NC; ++i) {
+            const uint32_t j = j0 + (lane & (KT - 1u)) + 64u * i;
+            r.of[i] = KVMEM_HIP_NO_SLOT;
+            if (j < c1) {
+                r.of[i] = table[block_of(p, j)];
+            }
+        }
+        return r;
+    };
+    auto cells_of = [&](const Slots &slots, uint32_t j0) {
         Cells r;
 #pragma unroll
         for (uint32_t i = 0; i < NC; ++i) {
             const uint32_t j = j0 + (lane & (KT - 1u)) + 64u * i;
-            uint32_t slot = KVMEM_HIP_NO_SLOT;
-            const uint32_t b = j / p.T;
-            if (j < c1) {
-                slot = table[b];
-            }
-            r.at[i] = slot < p.n_slots ? slot * p.T + (j - b * p.T) : 0u;
+            const uint32_t slot = slots.of[i];
+            r.at[i] = slot < p.n_slots ? slot * p.T + (j - block_of(p, j) * p.T) : 0u;
             r.have[i] = __ballot(slot < p.n_slots);
         }
         return r;
@@ -1090,39 +1128,67 @@ __global__ __launch_bounds__(256, 1) void attn_prefill_kernel(AttnParams p) {
         }
         return at;
     };
-    UK rk[NK];
-    UV rv[NV];
-    auto load_tile = [&](const Cells &cells) {
+    // A step's rows on their way to `raw`.  Slices of 256 dims are whole 16-byte
+    // units: those go straight to LDS (fetch_tile; there are no registers to spare),
+    // narrower ones through registers (load here, store in put_tile).
+    constexpr bool kDirect = D == 256;
+    constexpr uint32_t KU = KT * SK::units;
+    constexpr uint32_t NU = KU + KT * SV::units;
+    UK rk[kDirect ? 1 : NK];
+    UV rv[kDirect ? 1 : NV];
+    auto fetch_tile = [&](const Cells &cells, uint8_t *raw) {
+        if constexpr (kDirect) {
+            const uint32_t t = anew(tid);
 #pragma unroll
-        for (uint32_t i = 0; i < NK; ++i) {
-            const uint32_t u = i * 256u + tid;
-            const uint32_t key = u / SK::units;
-            const uint32_t at = cell_at(cells, key);
-            rk[i] = *reinterpret_cast<const UK *>(k_head + static_cast<uint64_t>(at) * p.row_k +
-                                                  (u - key * SK::units) * SK::unit);
-        }
+            for (uint32_t i = 0; i < (NU + NTH - 1u) / NTH; ++i) {
+                const uint32_t u = i * NTH + t;
+                const bool is_v = u >= KU;
+                const uint32_t w = is_v ? u - KU : u;
+                const uint32_t key = is_v ? w / SV::units : w / SK::units;
+                const uint32_t off = (w - key * (is_v ? SV::units : SK::units)) * 16u;
+                const uint64_t row = static_cast<uint64_t>(cell_at(cells, key)) * (is_v ? p.row_v : p.row_k);
+                const uint8_t *src = (is_v ? v_head : k_head) + row + off;
+                if ((i + 1) * NTH <= NU || u < NU) {
+                    __builtin_amdgcn_global_load_lds(src, (lds_void_t *) (raw + (i * NTH + wave * 64u) * 16u), 16, 0, 0);
+                }
+            }
+        } else {
 #pragma unroll
-        for (uint32_t i = 0; i < NV; ++i) {
-            const uint32_t u = i * 256u + tid;
-            const uint32_t key = u / SV::units;
-            const uint32_t at = cell_at(cells, key);
-            rv[i] = *reinterpret_cast<const UV *>(v_head + static_cast<uint64_t>(at) * p.row_v +
-                                                  (u - key * SV::units) * SV::unit);
-        }
-    };
-    auto put_tile = [&](uint8_t *raw) {
+            for (uint32_t i = 0; i < NK; ++i) {
+                const uint32_t u = i * NTH + tid;
+                const uint32_t key = u / SK::units;
+                const uint32_t at = cell_at(cells, key);
+                rk[i] = *reinterpret_cast<const UK *>(k_head + static_cast<uint64_t>(at) * p.row_k +
+                                                      (u - key * SK::units) * SK::unit);
+            }
 #pragma unroll
-        for (uint32_t i = 0; i < NK; ++i) {
-            const uint32_t u = i * 256u + tid;
-            if ((i + 1) * 256u <= KT * SK::units || u < KT * SK::units) {
-                *reinterpret_cast<UK *>(raw + u * SK::unit) = rk[i];
+            for (uint32_t i = 0; i < NV; ++i) {
+                const uint32_t u = i * NTH + tid;
+                const uint32_t key = u / SV::units;
+                const uint32_t at = cell_at(cells, key);
+                rv[i] = *reinterpret_cast<const UV *>(v_head + static_cast<uint64_t>(at) * p.row_v +
+                                                      (u - key * SV::units) * SV::unit);
             }
         }
+    };
+    // The fetched step is in `raw` once the barrier behind this call is passed.
+    auto put_tile = [&](uint8_t *raw) {
+        if constexpr (kDirect) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        } else {
 #pragma unroll
-        for (uint32_t i = 0; i < NV; ++i) {
-            const uint32_t u = i * 256u + tid;
-            if ((i + 1) * 256u <= KT * SV::units || u < KT * SV::units) {
-                *reinterpret_cast<UV *>(raw + L::raw_k + u * SV::unit) = rv[i];
+            for (uint32_t i = 0; i < NK; ++i) {
+                const uint32_t u = i * NTH + tid;
+                if ((i + 1) * NTH <= KT * SK::units || u < KT * SK::units) {
+                    *reinterpret_cast<UK *>(raw + u * SK::unit) = rk[i];
+                }
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < NV; ++i) {
+                const uint32_t u = i * NTH + tid;
+                if ((i + 1) * NTH <= KT * SV::units || u < KT * SV::units) {
+                    *reinterpret_cast<UV *>(raw + L::raw_k + u * SV::unit) = rv[i];
+                }
             }
         }
     };
@@ -1133,15 +1199,18 @@ __global__ __launch_bounds__(256, 1) void attn_prefill_kernel(AttnParams p) {
     // Making f16 of a step's rows, in pieces.  Values: this thread's octet of
     // keys (keys 16 (q / 2) + 8 (e / 4) + 4 (q % 2) + e % 4, as a lane of the
     // scores holds them) and its 4 dims.
-    const uint32_t oct = tid / (D / 4);
-    const uint32_t dl = tid % (D / 4);
+    const bool for_values = NW == 4 || wave < 4u;  // with 8 waves four make values, four keys
+    const bool for_keys = NW == 4 || wave >= 4u;
     VO vo;
-    auto value_read = [&](const uint8_t *raw) {
-        vo.raw(dl, [&](uint32_t e) {
+    auto value_read = [&](const uint8_t *raw, uint32_t mt) {
+        const uint32_t oct = mt / (D / 4);
+        vo.raw(mt % (D / 4), [&](uint32_t e) {
             return raw + L::raw_k + (16u * (oct >> 1) + 8u * (e >> 2) + 4u * (oct & 1u) + (e & 3u)) * SV::bytes;
         });
     };
-    auto value_write = [&](uint8_t *values, const uint64_t *have, uint32_t j0) {
+    auto value_write = [&](uint8_t *values, const uint64_t *have, uint32_t j0, uint32_t mt) {
+        const uint32_t oct = mt / (D / 4);
+        const uint32_t dl = mt % (D / 4);
         const uint32_t in = static_cast<uint32_t>(have[oct >> 3] >> (16u * ((oct >> 1) & 3u) + 4u * (oct & 1u)));
         vo.emit(keep_keys<8>(in), [&](int, u32x4_t *a) {
 #pragma unroll
@@ -1152,15 +1221,15 @@ __global__ __launch_bounds__(256, 1) void attn_prefill_kernel(AttnParams p) {
                         return j0 + 16u * (oct >> 1) + 8u * (e >> 2) + 4u * (oct & 1u) + (e & 3u);
                     });
                 }
-                *reinterpret_cast<u32x4_t *>(values + (oct * D + value_slot(dim)) * 16u) = a[t];
+                *reinterpret_cast<u32x4_t *>(values + oct * L::octet + value_slot(dim) * 16u) = a[t];
             }
         });
     };
     // Keys: octet i of 4 of this thread.
     u32x4_t codes;
     uint32_t key_scale = 0;
-    auto key_read = [&](const uint8_t *raw, uint32_t i) {
-        const uint32_t u = i * 256u + tid;
+    auto key_read = [&](const uint8_t *raw, uint32_t i, uint32_t mt) {
+        const uint32_t u = i * 256u + mt;
         const uint32_t key = u / (D / 8);
         const uint32_t o = u % (D / 8);
         const uint8_t *g = raw + key * SK::bytes + (o >> 2) * SK::GB;
@@ -1169,208 +1238,213 @@ __global__ __launch_bounds__(256, 1) void attn_prefill_kernel(AttnParams p) {
         }
         codes = KO::load(g, o & 3u, 2u * (~(o >> 2) & 1u));
     };
-    auto key_write = [&](uint8_t *keys, uint32_t i) {
-        const uint32_t u = i * 256u + tid;
+    auto key_write = [&](uint8_t *keys, uint32_t i, uint32_t mt) {
+        const uint32_t u = i * 256u + mt;
         const uint32_t key = u / (D / 8);
         const uint32_t o = u % (D / 8);
         *reinterpret_cast<u32x4_t *>(keys + key * L::key_stride + o * 16u) = key_values<KO>(codes, key_scale);
     };
 
-    Cells cells = cells_of(c0);
-    load_tile(cells);
-    uint64_t have[NC], have1[NC];
-#pragma unroll
-    for (uint32_t i = 0; i < NC; ++i) {
-        have[i] = cells.have[i];
-    }
-    cells = cells_of(c0 + KT);
+    const Slots slots0 = slots_of(c0);
+    const Slots slots1 = slots_of(c0 + KT);
+    Slots next = slots_of(c0 + 2u * KT);
 
     // This wave's queries, scaled into f16's range row by row: made operands in
-    // LDS (the step buffers are not in use yet), a tile at a time.
-    half8_t qf[RT][QS];
-    float fac[RT];
-    uint32_t limit[RT];
-    uint64_t at[RT];  // (token, head) row of q and out
-    bool mine[RT];
-    u32x4_t *ql = reinterpret_cast<u32x4_t *>(lds) + wave * QS * 64u + lane;
+    // LDS (the step buffers are not in use yet).
+    half8_t qf[QS];
+    // token and query head of a lane's row (rows behind the last one repeat it)
+    auto tok_of = [&](uint32_t l) { return (row0 + min(wave * 32u + (l & 31u), rows - 1u)) / p.group; };
+    auto head_of = [&](uint32_t l) { return hk * p.group + (row0 + min(wave * 32u + (l & 31u), rows - 1u)) % p.group; };
+    float fac;
+    {
+        u32x4_t *ql = reinterpret_cast<u32x4_t *>(lds) + (wave & 3u) * QS * 64u + lane;
+        const uint8_t *q = p.q + static_cast<uint64_t>(r.first + tok_of(lane)) * p.q_nb2 + head_of(lane) * p.q_nb1;
+        int ex = 0;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const uint32_t in_tile = (wave * RT + rt) * 32u + nl;
-        const uint32_t row = row0 + min(in_tile, rows - 1u);
-        mine[rt] = in_tile < rows;
-        const uint32_t tok = row / p.group;
-        const uint32_t head = hk * p.group + (row - tok * p.group);
-        limit[rt] = key_limit(p, r, tok);
-        at[rt] = static_cast<uint64_t>(r.first + tok) * p.n_head + head;
-        const uint8_t *q = p.q + static_cast<uint64_t>(r.first + tok) * p.q_nb2 + head * p.q_nb1;
-        uint32_t bits = 0;
+        for (uint32_t turn = 0; turn < NW / 4u; ++turn) {  // four waves' queries fit at a time
+            if (wave / 4u == turn) {
+                uint32_t bits = 0;
 #pragma unroll 4
-        for (uint32_t st = 0; st < QS; ++st) {
-            const u32x4_t x = load_query<KO>(q, st >> 1, 2u * (st & 1u) + hh);
-            ql[st * 64u] = x;
-            bits = max_magnitude(x[0], max_magnitude(x[1], max_magnitude(x[2], max_magnitude(x[3], bits))));
-        }
-        bits = max(bits & 0xffffu, bits >> 16);
-        float most = p.q_bf16 ? query_value<true>(bits) : query_value<false>(bits);
-        most = fmaxf(most, lane_xor32(most));
-        const int ex = query_shift(most);
-        const float up = ldexpf(1.0f, ex);
+                for (uint32_t st = 0; st < QS; ++st) {
+                    const u32x4_t x = load_query<KO>(q, st >> 1, 2u * (st & 1u) + hh);
+                    ql[st * 64u] = x;
+                    bits = max_magnitude(x[0], max_magnitude(x[1], max_magnitude(x[2], max_magnitude(x[3], bits))));
+                }
+                bits = max(bits & 0xffffu, bits >> 16);
+                float most = p.q_bf16 ? query_value<true>(bits) : query_value<false>(bits);
+                most = fmaxf(most, lane_xor32(most));
+                ex = query_shift(most);
+                const float up = ldexpf(1.0f, ex);
 #pragma unroll 1
-        for (uint32_t st = 0; st < QS; ++st) {
-            const u32x4_t x = ql[st * 64u];
-            const half8_t h = p.q_bf16 ? query_operand<KO, true>(x, up) : query_operand<KO, false>(x, up);
-            ql[st * 64u] = __builtin_bit_cast(u32x4_t, h);
-        }
+                for (uint32_t st = 0; st < QS; ++st) {
+                    const u32x4_t x = ql[st * 64u];
+                    const half8_t h = p.q_bf16 ? query_operand<KO, true>(x, up) : query_operand<KO, false>(x, up);
+                    ql[st * 64u] = __builtin_bit_cast(u32x4_t, h);
+                }
 #pragma unroll
-        for (uint32_t st = 0; st < QS; ++st) {
-            qf[rt][st] = __builtin_bit_cast(half8_t, ql[st * 64u]);
+                for (uint32_t st = 0; st < QS; ++st) {
+                    qf[st] = __builtin_bit_cast(half8_t, ql[st * 64u]);
+                }
+            }
+            __syncthreads();  // the queries have left the step buffers
         }
-        wave_lds_sync();
-        fac[rt] = fmaxf(ldexpf(p.scale * kLog2e, -ex), 0x1p-126f);
+        fac = fmaxf(ldexpf(p.scale * kLog2e, -ex), 0x1p-126f);
     }
 
-    float top[RT], sum[RT];
-    float16_t o[RT][NB];
+    float top = -INFINITY;
+    float sum = 0.0f;
+    float16_t o[NB];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        top[rt] = -INFINITY;
-        sum[rt] = 0.0f;
+    for (int b = 0; b < NB; ++b) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                o[rt][b][i] = 0.0f;
-            }
+        for (int i = 0; i < 16; ++i) {
+            o[b][i] = 0.0f;
         }
     }
     if (tid < D) {
         first_odd[tid] = ~0u;
     }
-    __syncthreads();  // the queries have left the step buffers
+    const Cells cells0 = cells_of(slots0, c0);
+    fetch_tile(cells0, raw0);
     put_tile(raw0);
-    load_tile(cells);
+    const Cells cells1 = cells_of(slots1, c0 + KT);
+    fetch_tile(cells1, raw0 + L::raw);
+    put_tile(raw0 + L::raw);
+    uint64_t have[NC], have1[NC];
 #pragma unroll
     for (uint32_t i = 0; i < NC; ++i) {
-        have1[i] = cells.have[i];
+        have[i] = cells0.have[i];
+        have1[i] = cells1.have[i];
     }
-    cells = cells_of(c0 + 2u * KT);
     __syncthreads();
-    put_tile(raw0 + L::raw);
-    value_read(raw0);
-    value_write(values0, have, c0);
+    if (for_values) {
+        value_read(raw0, tid & 255u);
+        value_write(values0, have, c0, tid & 255u);
+    }
+    if (for_keys) {
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        key_read(raw0, i);
-        key_write(keys0, i);
+        for (uint32_t i = 0; i < 4; ++i) {
+            key_read(raw0, i, tid & 255u);
+            key_write(keys0, i, tid & 255u);
+        }
     }
     __syncthreads();
 
     uint32_t buf = 0;  // step modulo 2
     for (uint32_t j0 = c0; j0 < c1; j0 += KT) {
         uint64_t have2[NC];
-        load_tile(cells);
+        const Cells cells = cells_of(next, j0 + 2u * KT);
+        fetch_tile(cells, raw0 + buf * L::raw);  // (its rows were made f16 in the last step)
+        next = slots_of(j0 + 3u * KT);
 #pragma unroll
         for (uint32_t i = 0; i < NC; ++i) {
             have2[i] = cells.have[i];
         }
-        cells = cells_of(j0 + 3u * KT);
+        const uint32_t mt = anew(tid & 255u);
         const uint8_t *raw1 = raw0 + (buf ^ 1u) * L::raw;
         uint8_t *keys1 = keys0 + (buf ^ 1u) * L::keys;
         uint8_t *values1 = values0 + (buf ^ 1u) * L::values;
 
-        float16_t sc[RT][NT];
+        if (for_keys) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                key_read(raw1, i, mt);
+                key_write(keys1, i, mt);
+            }
+        }
+        float16_t sc[NT];
         const uint8_t *kr = keys0 + buf * L::keys + nl * L::key_stride + hh * 16u;
+        auto key_operand = [&](int z) {
+            return *reinterpret_cast<const half8_t *>(kr + z / QS * 32 * L::key_stride + z % QS * 32);
+        };
+        half8_t ring[4];  // operands are read four products ahead
 #pragma unroll
-        for (int a = 0; a < NT; ++a) {
+        for (int z = 0; z < 4; ++z) {
+            ring[z] = key_operand(z);
+        }
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
+        for (int z = 0; z < NT * QS; ++z) {
+            const int a = z / QS;
+            if (z % QS == 0) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    sc[rt][a][i] = 0.0f;
+                    sc[a][i] = 0.0f;
                 }
             }
-#pragma unroll
-            for (int st = 0; st < QS; ++st) {
-                const int z = a * QS + st;  // 16 in all
-                const half8_t kf = *reinterpret_cast<const half8_t *>(kr + a * 32 * L::key_stride + st * 32);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    sc[rt][a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[rt][st], sc[rt][a], 0, 0, 0);
-                }
-                if (z == 0) {
-                    value_read(raw1);
-                } else if (z == 3) {
-                    value_write(values1, have1, j0 + KT);
-                } else if (z >= 4 && (z - 4) % 3 == 0) {
-                    key_read(raw1, (z - 4) / 3);
-                } else if (z >= 5 && (z - 5) % 3 == 0) {
-                    key_write(keys1, (z - 5) / 3);
-                }
+            sc[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[z & 3], qf[z % QS], sc[a], 0, 0, 0);
+            if (z + 4 < NT * QS) {
+                ring[z & 3] = key_operand(z + 4);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
         bool whole = j0 + KT <= n_all;
 #pragma unroll
         for (uint32_t i = 0; i < NC; ++i) {
             whole = whole && have[i] == ~0ull;
         }
-        half8_t w[RT][2 * NT];
+        if (!whole) {
+            const uint32_t limit = key_limit(p, r, tok_of(anew(lane)));
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            if (!whole) {
+            for (uint32_t a = 0; a < NT; ++a) {
+                const uint32_t seen =
+                    seen_keys(static_cast<uint32_t>(have[a >> 1] >> (32u * (a & 1u))),
+                              static_cast<int32_t>(limit - j0) - static_cast<int32_t>(32u * a), 4u * hh);
 #pragma unroll
-                for (uint32_t a = 0; a < NT; ++a) {
-                    const uint32_t seen =
-                        seen_keys(static_cast<uint32_t>(have[a >> 1] >> (32u * (a & 1u))),
-                                  static_cast<int32_t>(limit[rt] - j0) - static_cast<int32_t>(32u * a), 4u * hh);
-#pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i) {
-                        sc[rt][a][i] = (seen & (1u << (8u * (i >> 2) + (i & 3u)))) ? sc[rt][a][i] : -INFINITY;
-                    }
-                }
-            }
-            float most = -INFINITY;
-#pragma unroll
-            for (int a = 0; a < NT; ++a) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    most = fmaxf(most, sc[rt][a][i]);
-                }
-            }
-            most *= fac[rt];
-            most = fmaxf(most, lane_xor32(most));
-            if (__any(most > top[rt] + kTopSlack)) {
-                const float higher = fmaxf(top[rt], most);
-                const float fade = top[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[rt] - higher);
-                sum[rt] *= fade;
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    o[rt][b] *= fade;
-                }
-                top[rt] = higher;
-            }
-            const float base = (top[rt] == -INFINITY ? 0.0f : top[rt]) - kWeightShift;
-#pragma unroll
-            for (int a = 0; a < NT; ++a) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rt][a][i], fac[rt], -base));
-                    sum[rt] += pe;
-                    w[rt][2 * a + (i >> 3)][i & 7] = static_cast<_Float16>(pe);
+                for (uint32_t i = 0; i < 16; ++i) {
+                    sc[a][i] = (seen & (1u << (8u * (i >> 2) + (i & 3u)))) ? sc[a][i] : -INFINITY;
                 }
             }
         }
-        const uint8_t *vr = values0 + buf * L::values + hh * D * 16u;
+        float most = -INFINITY;
 #pragma unroll
-        for (int ks = 0; ks < 2 * NT; ++ks) {
+        for (int a = 0; a < NT; ++a) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                most = fmaxf(most, sc[a][i]);
+            }
+        }
+        most *= fac;
+        most = fmaxf(most, lane_xor32(most));
+        if (__any(most > top + kTopSlack)) {
+            const float higher = fmaxf(top, most);
+            const float fade = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
+            sum *= fade;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const half8_t vf =
-                    *reinterpret_cast<const half8_t *>(vr + (2 * ks * D + value_slot(32u * b + nl)) * 16u);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    o[rt][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, w[rt][ks], o[rt][b], 0, 0, 0);
-                }
+                o[b] *= fade;
             }
+            top = higher;
+        }
+        const float base = (top == -INFINITY ? 0.0f : top) - kWeightShift;
+        half8_t w[2 * NT];
+#pragma unroll
+        for (int a = 0; a < NT; ++a) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[a][i], fac, -base));
+                sum += pe;
+                w[2 * a + (i >> 3)][i & 7] = static_cast<_Float16>(pe);
+            }
+        }
+        const uint8_t *vr = values0 + buf * L::values + hh * L::octet + nl * 16u;
+        auto value_operand = [&](int z) {
+            return *reinterpret_cast<const half8_t *>(vr + 2 * (z / NB) * L::octet + 33 * (z % NB) * 16);
+        };
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+            ring[z] = value_operand(z);
+        }
+#pragma unroll
+        for (int z = 0; z < 2 * NT * NB; ++z) {
+            o[z % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[z & 3], w[z / NB], o[z % NB], 0, 0, 0);
+            if (z + 4 < 2 * NT * NB) {
+                ring[z & 3] = value_operand(z + 4);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (for_values) {
+            value_read(raw1, mt);
+            value_write(values1, have1, j0 + KT, mt);
         }
         put_tile(raw0 + buf * L::raw);
 #pragma unroll
@@ -1382,40 +1456,43 @@ __global__ __launch_bounds__(256, 1) void attn_prefill_kernel(AttnParams p) {
         __syncthreads();
     }
 
-    // a lane holds dims 32 b + 8 (i / 4) + 4 hh + i % 4 of its rows
+    // a lane holds dims 32 b + 8 (i / 4) + 4 hh + i % 4 of its row
     const bool uneven = c1 > n_all && __syncthreads_or(tid < D && first_odd[tid] != ~0u);
+    sum += lane_xor32(sum);
+    const uint32_t end_lane = anew(lane);
+    const uint32_t tok = tok_of(end_lane);
+    const uint32_t head = head_of(end_lane);
+    const uint32_t limit = key_limit(p, r, tok);
+    const bool mine = wave * 32u + (end_lane & 31u) < rows;
+    // parts, and sums that still have to be rotated, go to the joining kernel
+    const bool joined = n_parts > 1 || p.hadamard;
+    const uint64_t at = static_cast<uint64_t>(r.first + tok) * p.n_head + head;
+    const uint64_t to = (joined ? static_cast<uint64_t>(part) * p.n_tokens * p.n_head : 0u) + at;
+    const float f = joined ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint8_t *out = joined ? reinterpret_cast<uint8_t *>(p.part_o) : p.out;
+    const int type = joined ? static_cast<int>(KVMEM_TYPE_F32) : p.out_type;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        sum[rt] += lane_xor32(sum[rt]);
-        // parts, and sums that still have to be rotated, go to the joining kernel
-        const bool joined = n_parts > 1 || p.hadamard;
-        const float f = joined ? 1.0f : sum[rt] == 0.0f ? 0.0f : 1.0f / sum[rt];
-        const uint64_t to = (joined ? static_cast<uint64_t>(part) * p.n_tokens * p.n_head : 0u) + at[rt];
-        uint8_t *out = joined ? reinterpret_cast<uint8_t *>(p.part_o) : p.out;
-        const int type = joined ? static_cast<int>(KVMEM_TYPE_F32) : p.out_type;
+    for (int b = 0; b < NB; ++b) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
+        for (int i = 0; i < 16; i += 4) {
+            const uint32_t dim = 32 * b + 2 * i + 4 * hh;
+            float4_t x{o[b][i] * f, o[b][i + 1] * f, o[b][i + 2] * f, o[b][i + 3] * f};
+            if (uneven) {
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const uint32_t dim = 32 * b + 2 * i + 4 * hh;
-                float4_t x{o[rt][b][i] * f, o[rt][b][i + 1] * f, o[rt][b][i + 2] * f, o[rt][b][i + 3] * f};
-                if (uneven) {
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        x[d] = first_odd[dim + d] < limit[rt] ? NAN : x[d];
-                    }
+                for (int d = 0; d < 4; ++d) {
+                    x[d] = first_odd[dim + d] < limit ? NAN : x[d];
                 }
-                if (mine[rt]) {
-                    store4(out, type, to * D + dim, x);
-                }
+            }
+            if (mine) {
+                store4(out, type, to * D + dim, x);
             }
         }
-        if (mine[rt] && hh == 0) {
-            if (joined) {
-                p.part_ml[to] = make_float2(top[rt], sum[rt]);
-            } else if (p.lse) {
-                p.lse[at[rt]] = sum[rt] == 0.0f ? -INFINITY : (top[rt] - kWeightShift) / kLog2e + logf(sum[rt]);
-            }
+    }
+    if (mine && hh == 0) {
+        if (joined) {
+            p.part_ml[to] = make_float2(top, sum);
+        } else if (p.lse) {
+            p.lse[at] = sum == 0.0f ? -INFINITY : (top - kWeightShift) / kLog2e + logf(sum);
         }
     }
 }
@@ -1425,12 +1502,10 @@ __global__ __launch_bounds__(256, 1) void attn_prefill_kernel(AttnParams p) {
 template <int TK, int TV, int D>
 static void launch_types(hipStream_t stream, const AttnPlan &pl, const AttnParams &p) {
     const uint32_t grid = static_cast<uint32_t>(pl.grid);
-    if (pl.prefill == 2) {
-        if constexpr (D < 256) {  // (256 dims of two tiles are more than a wave's registers)
-            attn_prefill_kernel<TK, TV, D, 2><<<grid, 256, PrefillLds<TK, TV, D>::bytes, stream>>>(p);
-        }
-    } else if (pl.prefill == 1) {
-        attn_prefill_kernel<TK, TV, D, 1><<<grid, 256, PrefillLds<TK, TV, D>::bytes, stream>>>(p);
+    if (pl.prefill == 8) {
+        attn_prefill_kernel<TK, TV, D, 8><<<grid, 512, PrefillLds<TK, TV, D>::bytes, stream>>>(p);
+    } else if (pl.prefill == 4) {
+        attn_prefill_kernel<TK, TV, D, 4><<<grid, 256, PrefillLds<TK, TV, D>::bytes, stream>>>(p);
     } else {
         const uint32_t rows = std::min(kRowTile, p.max_q * p.group);
         // 16 bytes behind the last slice: its last word is read with the next one
