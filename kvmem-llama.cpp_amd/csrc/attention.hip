@@ -133,9 +133,16 @@ static AttnPlan plan_attention(const kvmem_hip_pool *pool, const kvmem_hip_attn_
     chunk = (chunk + quantum - 1) / quantum * quantum;
     pl.chunk = static_cast<uint32_t>(chunk);
     pl.n_parts = static_cast<uint32_t>((keys + chunk - 1) / chunk);
-    const uint64_t units = (static_cast<uint64_t>(a->n_seq) * pl.n_parts * (pl.prefill ? a->n_head_kv : 1u) + 7) / 8 * 8;
-    pl.units = static_cast<uint32_t>(units);
-    pl.grid = units * pl.row_tiles * (pl.prefill ? 1u : a->n_head_kv);
+    if (pl.prefill) {
+        pl.units = static_cast<uint32_t>(static_cast<uint64_t>(a->n_seq) * pl.n_parts * a->n_head_kv);
+        pl.grid = (static_cast<uint64_t>(pl.units) * pl.row_tiles + 7) / 8 * 8;
+    } else {
+        // (request, part) pairs: a multiple of 8, so that the KV heads of one pair,
+        // whose slices share cache lines, go to the same XCD
+        const uint64_t units = (static_cast<uint64_t>(a->n_seq) * pl.n_parts + 7) / 8 * 8;
+        pl.units = static_cast<uint32_t>(units);
+        pl.grid = units * pl.row_tiles * a->n_head_kv;
+    }
     pl.joined = pl.n_parts > 1 || (pl.prefill && pool->xf && pool->xf->hadamard_v);
     if (pl.joined) {
         const size_t heads = static_cast<size_t>(a->n_tokens) * a->n_head * pl.n_parts;

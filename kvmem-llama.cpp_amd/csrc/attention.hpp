@@ -35,7 +35,8 @@ struct AttnParams {
     uint32_t T_mul, T_shift;    // j / T as the upper word of j * T_mul, shifted (T > 1)
     uint32_t row_tile;          // rows of one workgroup
     uint32_t row_tiles;         // of the longest request
-    uint32_t units;             // of the grid's fast index, a multiple of 8
+    uint32_t units;             // decode: (request, part) pairs, padded to a multiple of 8;
+                                // prefill: (request, part, KV head)
     int32_t causal;
     int32_t q_bf16;
     int32_t out_type;

@@ -1054,8 +1054,27 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) 
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ uint32_t first_odd[D];
 
-    const uint32_t unit = blockIdx.x % p.units;
-    const uint32_t tile = p.row_tiles - 1u - blockIdx.x / p.units;  // long rows first
+    // Workgroups go to the 8 XCDs in turn.  A unit (request, part, KV head) stays on
+    // one of them, whose L2 then holds its rows for all row tiles; units that do
+    // not make a round of eight are spread.  Tiles with the most keys come first.
+    const uint32_t xcd = blockIdx.x & 7u;
+    const uint32_t turn_of = blockIdx.x >> 3;
+    const uint32_t per_xcd = p.units >> 3;
+    const uint32_t even = per_xcd * p.row_tiles;
+    uint32_t unit, tile;
+    if (turn_of < even) {
+        unit = (turn_of % per_xcd) * 8u + xcd;
+        tile = turn_of / per_xcd;
+    } else {
+        const uint32_t rest = p.units & 7u;
+        const uint32_t w = (turn_of - even) * 8u + xcd;
+        unit = per_xcd * 8u + w % max(rest, 1u);
+        tile = w / max(rest, 1u);
+    }
+    if (unit >= p.units || tile >= p.row_tiles) {
+        return;
+    }
+    tile = p.row_tiles - 1u - tile;
     const uint32_t hk = unit % p.n_head_kv;
     const uint32_t sp = unit / p.n_head_kv;
     const uint32_t s = sp / p.n_parts;
