@@ -1268,20 +1268,30 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) 
     const Slots slots1 = slots_of(c0 + KT);
     Slots next = slots_of(c0 + 2u * KT);
 
+    // The first rows are on their way while the queries are made.
+    const Cells cells0 = cells_of(slots0, c0);
+    const Cells cells1 = cells_of(slots1, c0 + KT);
+    fetch_tile(cells0, raw0);
+    if constexpr (kDirect) {
+        fetch_tile(cells1, raw0 + L::raw);
+    }
+
     // This wave's queries, scaled into f16's range row by row: made operands in
-    // LDS (the step buffers are not in use yet).
+    // LDS, where the steps' f16 rows will stand.
     half8_t qf[QS];
     // token and query head of a lane's row (rows behind the last one repeat it)
     auto tok_of = [&](uint32_t l) { return (row0 + min(wave * 32u + (l & 31u), rows - 1u)) / p.group; };
     auto head_of = [&](uint32_t l) { return hk * p.group + (row0 + min(wave * 32u + (l & 31u), rows - 1u)) % p.group; };
     float fac;
     {
-        u32x4_t *ql = reinterpret_cast<u32x4_t *>(lds) + (wave & 3u) * QS * 64u + lane;
+        constexpr uint32_t TURNS = NW * QS * 1024u <= 2 * (L::keys + L::values) ? 1 : 2;
+        constexpr uint32_t PER = NW / TURNS;  // waves whose queries fit at a time
+        u32x4_t *ql = reinterpret_cast<u32x4_t *>(lds + 2 * L::raw) + (wave % PER) * QS * 64u + lane;
         const uint8_t *q = p.q + static_cast<uint64_t>(r.first + tok_of(lane)) * p.q_nb2 + head_of(lane) * p.q_nb1;
         int ex = 0;
 #pragma unroll
-        for (uint32_t turn = 0; turn < NW / 4u; ++turn) {  // four waves' queries fit at a time
-            if (wave / 4u == turn) {
+        for (uint32_t turn = 0; turn < TURNS; ++turn) {
+            if (wave / PER == turn) {
                 uint32_t bits = 0;
 #pragma unroll 4
                 for (uint32_t st = 0; st < QS; ++st) {
@@ -1323,12 +1333,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) 
     if (tid < D) {
         first_odd[tid] = ~0u;
     }
-    const Cells cells0 = cells_of(slots0, c0);
-    fetch_tile(cells0, raw0);
     put_tile(raw0);
-    const Cells cells1 = cells_of(slots1, c0 + KT);
-    fetch_tile(cells1, raw0 + L::raw);
-    put_tile(raw0 + L::raw);
+    if constexpr (!kDirect) {
+        fetch_tile(cells1, raw0 + L::raw);
+        put_tile(raw0 + L::raw);
+    }
     uint64_t have[NC], have1[NC];
 #pragma unroll
     for (uint32_t i = 0; i < NC; ++i) {
