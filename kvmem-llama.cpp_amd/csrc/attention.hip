@@ -16,7 +16,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
     constexpr int E = D / 64;
     typedef float dims_t __attribute__((ext_vector_type(E)));
     __shared__ float sums[kWaves][D];
-    __shared__ float turn[256];
+    __shared__ float totals[kWaves];
     const uint32_t h = blockIdx.x % p.n_head;
     const uint32_t tok = blockIdx.x / p.n_head;
     const uint32_t tid = threadIdx.x;
@@ -59,10 +59,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
     for (uint32_t k = lane; k < n_parts; k += 64u) {
         top = fmaxf(top, p.part_ml[k * stride + at].x);
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        top = fmaxf(top, __shfl_xor(top, d, 64));
-    }
+    top = fmaxf(top, lane_xor<1>(top));
+    top = fmaxf(top, lane_xor<2>(top));
+    top = fmaxf(top, lane_xor<4>(top));
+    top = fmaxf(top, lane_xor<8>(top));
+    top = fmaxf(top, lane_xor<16>(top));
+    top = fmaxf(top, lane_xor<32>(top));
     const float *po = p.part_o + at * D + lane * E;
     float total = 0.0f;
     dims_t x = {};
@@ -75,20 +77,25 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
     }
     *reinterpret_cast<dims_t *>(&sums[wave][lane * E]) = x;
     if (lane == 0) {
-        turn[wave] = total;
+        totals[wave] = total;
     }
     __syncthreads();
-    total = (turn[0] + turn[1]) + (turn[2] + turn[3]);
-    const uint32_t d = tid & (D - 1u);  // D < 256: more than one thread a dim, the first one stores
-    float y = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
-    y = total == 0.0f ? 0.0f : y / total;
+    if (wave != 0) {
+        return;
+    }
+    total = (totals[0] + totals[1]) + (totals[2] + totals[3]);
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    float y[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const uint32_t d = lane * E + i;
+        y[i] = ((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) * inv;
+    }
     if (p.hadamard) {
-        y = rotate_back(y, p.hadamard, tid & (p.hadamard - 1u), turn + (tid - (tid & (p.hadamard - 1u))));
+        rotate_lanes<E>(y, p.hadamard, lane);
     }
-    if (tid < D) {
-        store_elem(p.out, p.out_type, at * D + d, y);
-    }
-    if (tid == 0 && p.lse) {
+    store_elems<E>(p.out, p.out_type, at * D + lane * E, y);
+    if (lane == 0 && p.lse) {
         p.lse[at] = total == 0.0f ? -INFINITY : (top - kWeightShift) / kLog2e + logf(total);
     }
 }
@@ -300,6 +307,8 @@ int kvmem_hip_attention(kvmem_hip_ctx *ctx, const kvmem_hip_pool *pool, uint32_t
     if (pl.grid >= 1u << 24) {
         return fail(ctx, KVMEM_HIP_ERR_INVALID, "attention: too many requests of max_q tokens for one launch");
     }
+    p.room = static_cast<uint32_t>(std::max<uint64_t>(
+        1, std::min<uint64_t>(p.max_kv, static_cast<uint64_t>(p.table_stride) * p.T)));
     p.chunk = pl.chunk;
     p.n_parts = pl.n_parts;
     p.row_tile = pl.row_tile;

@@ -30,6 +30,7 @@ struct AttnParams {
     float2 *part_ml;            // [part][token][head] maximum (log2), sum of weights
     uint32_t row_k, row_v;      // bytes of a cached row
     uint32_t n_tokens, n_seq, max_q, max_kv, n_head, n_head_kv, group, T, n_slots, table_stride;
+    uint32_t room;              // keys the table and max_kv leave room for, at least 1
     uint32_t chunk;             // keys of one part
     uint32_t n_parts;           // parts of the longest request
     uint32_t T_mul, T_shift;    // j / T as the upper word of j * T_mul, shifted (T > 1)
@@ -77,29 +78,69 @@ __device__ inline uint32_t key_limit(const AttnParams &p, const Span &r, uint32_
 }
 
 
-__device__ inline void store_elem(uint8_t *out, int type, uint64_t i, float x) {
+// E neighbouring output elements, from element e.
+template <int E>
+__device__ inline void store_elems(uint8_t *out, int type, uint64_t e, const float *x) {
+    typedef float f_t __attribute__((ext_vector_type(E)));
+    typedef _Float16 h_t __attribute__((ext_vector_type(E)));
+    typedef __bf16 b_t __attribute__((ext_vector_type(E)));
+    f_t v;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        v[i] = x[i];
+    }
     if (type == KVMEM_TYPE_F32) {
-        reinterpret_cast<float *>(out)[i] = x;
+        *reinterpret_cast<f_t *>(out + 4 * e) = v;
     } else if (type == KVMEM_TYPE_F16) {
-        reinterpret_cast<_Float16 *>(out)[i] = static_cast<_Float16>(x);
+        *reinterpret_cast<h_t *>(out + 2 * e) = __builtin_convertvector(v, h_t);
     } else {
-        reinterpret_cast<__bf16 *>(out)[i] = static_cast<__bf16>(x);
+        *reinterpret_cast<b_t *>(out + 2 * e) = __builtin_convertvector(v, b_t);
     }
 }
 
-// Walsh-Hadamard rotation of an output element (dim d of a row, one thread per
-// dim, every thread of the workgroup calls): butterflies of span 1 .. width/2
-// through LDS.
-__device__ inline float rotate_back(float x, uint32_t width, uint32_t d, float *row) {
-    x *= 1.0f / sqrtf(static_cast<float>(width));
-    for (uint32_t s = 1; s < width; s <<= 1) {
-        __syncthreads();
-        row[d] = x;
-        __syncthreads();
-        const float y = row[d ^ s];
-        x = (d & s) ? y - x : x + y;
+// Walsh-Hadamard rotation of rows of which each lane holds E neighbouring
+// elements (a run of `width` stands in width / E lanes from a multiple of that):
+// butterflies of span 1 .. E/2 inside the lane, the others with lane ^ span/E.
+// All lanes of the wave call.
+template <uint32_t M, int E>
+__device__ inline void rotate_span(float *x, uint32_t lane) {
+    const bool upper = lane & M;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const float y = lane_xor<M>(x[i]);
+        x[i] = upper ? y - x[i] : x[i] + y;
     }
-    return x;
+}
+template <int E>
+__device__ inline void rotate_lanes(float *x, uint32_t width, uint32_t lane) {
+    const float f = 1.0f / sqrtf(static_cast<float>(width));
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        x[i] *= f;
+    }
+#pragma unroll
+    for (int h = 1; h < E; h <<= 1) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            if (!(i & h)) {
+                const float u = x[i];
+                const float v = x[i + h];
+                x[i] = u + v;
+                x[i + h] = u - v;
+            }
+        }
+    }
+    // width is at least 64
+    rotate_span<1, E>(x, lane);
+    rotate_span<2, E>(x, lane);
+    rotate_span<4, E>(x, lane);
+    rotate_span<8, E>(x, lane);
+    if (width > 16u * E) {
+        rotate_span<16, E>(x, lane);
+    }
+    if (width > 32u * E) {
+        rotate_span<32, E>(x, lane);
+    }
 }
 
 // How a call is laid out on the chip.

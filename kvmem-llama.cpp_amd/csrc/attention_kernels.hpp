@@ -178,6 +178,10 @@ template <int TYPE, int VD> struct ValueOp;
 
 template <int VD>
 struct ValueOp<KVMEM_TYPE_Q4_0, VD> {
+    // dims nth(t) .. nth(t + RUN - 1), t a multiple of RUN, are neighbours: the lower
+    // nibbles' first, then the upper ones'
+    static constexpr int RUN = VD / 2 < 4 ? VD / 2 : 4;
+    static constexpr int nth(int t) { return t < VD / 2 ? 2 * t : 2 * (t - VD / 2) + 1; }
     static constexpr int NB = VD / 2;  // bytes of codes
     static constexpr int NW = NB < 4 ? 1 : NB / 4;
     static constexpr float offset = 8.0f;
@@ -232,6 +236,10 @@ struct ValueOp<KVMEM_TYPE_Q4_0, VD> {
 
 template <int VD>
 struct ValueOp<KVMEM_TYPE_Q5_0, VD> {
+    // dims nth(t) .. nth(t + RUN - 1), t a multiple of RUN, are neighbours: the lower
+    // nibbles' first, then the upper ones'
+    static constexpr int RUN = VD / 2 < 4 ? VD / 2 : 4;
+    static constexpr int nth(int t) { return t < VD / 2 ? 2 * t : 2 * (t - VD / 2) + 1; }
     static constexpr int NB = VD / 2;
     static constexpr int NW = NB < 4 ? 1 : NB / 4;
     static constexpr float offset = 16.0f;
@@ -296,6 +304,8 @@ struct ValueOp<KVMEM_TYPE_Q5_0, VD> {
 
 template <int VD>
 struct ValueOp<KVMEM_TYPE_Q8_0, VD> {
+    static constexpr int RUN = 4;
+    static constexpr int nth(int t) { return t; }
     static constexpr int NW = VD / 4;
     uint32_t w[8][NW];
     uint32_t d[4];
@@ -342,6 +352,8 @@ struct ValueOp<KVMEM_TYPE_Q8_0, VD> {
 
 template <int VD>
 struct ValueOp<KVMEM_TYPE_F16, VD> {
+    static constexpr int RUN = 4;
+    static constexpr int nth(int t) { return t; }
     static constexpr int NW = VD / 2;
     uint32_t w[8][NW];
     __device__ static inline uint32_t dim(uint32_t n, uint32_t t) { return VD * n + t; }
@@ -533,6 +545,28 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
     if (s >= p.n_seq) {
         return;
     }
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t c0 = part * p.chunk;
+    const uint32_t *table = p.table + static_cast<uint64_t>(s) * p.table_stride;
+    constexpr uint32_t step = kWaves * KT;
+    uint32_t j0 = c0 + wave * KT;
+    // Their table entries are read a step before they are looked at: a value of a
+    // load that is waited for here would wait for the rows requested before it.
+    struct Slots {
+        uint32_t of[NC];
+    };
+    auto slots_of = [&](uint32_t j0) {
+        Slots r;
+#pragma unroll
+        for (uint32_t i = 0; i < NC; ++i) {
+            // within the table, whatever the request's length
+            r.of[i] = table[block_of(p, min(j0 + (lane & (KT - 1u)) + 64u * i, p.room - 1u))];
+        }
+        return r;
+    };
+    const Slots first_slots = slots_of(j0);  // on its way with the request's length
+
     const uint32_t hk = y % p.n_head_kv;
     const uint32_t tile = y / p.n_head_kv;
     const Span r = request_span(p, s);
@@ -550,15 +584,11 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
     if (part >= n_parts) {
         return;
     }
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t nl = lane & 15u;   // query row; dim lane of the values
     const uint32_t c = lane >> 4;     // chunk of the contraction
-    const uint32_t c0 = part * p.chunk;
     const uint32_t c1 = min(n, c0 + p.chunk);
     const uint8_t *k_head = p.k + static_cast<uint64_t>(hk) * SK::bytes;
     const uint8_t *v_head = p.v + static_cast<uint64_t>(hk) * SV::bytes;
-    const uint32_t *table = p.table + static_cast<uint64_t>(s) * p.table_stride;
 
     // The cells of this lane's keys of the step at j0, and which keys exist
     // (bit = key); one that does not has cell 0, and is masked where it matters.
@@ -566,31 +596,15 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
         uint32_t at[NC];
         uint64_t have[NC];
     };
-    // Their table entries are read a step before they are looked at: a value of a
-    // load that is waited for here would wait for the rows requested before it.
-    struct Slots {
-        uint32_t of[NC];
-    };
-    auto slots_of = [&](uint32_t j0) {
-        Slots r;
-#pragma unroll
-        for (uint32_t i = 0; i < NC; ++i) {
-            const uint32_t j = j0 + (lane & (KT - 1u)) + 64u * i;
-            r.of[i] = KVMEM_HIP_NO_SLOT;
-            if (j < c1) {
-                r.of[i] = table[block_of(p, j)];
-            }
-        }
-        return r;
-    };
     auto cells_of = [&](const Slots &slots, uint32_t j0) {
         Cells r;
 #pragma unroll
         for (uint32_t i = 0; i < NC; ++i) {
             const uint32_t j = j0 + (lane & (KT - 1u)) + 64u * i;
             const uint32_t slot = slots.of[i];
-            r.at[i] = slot < p.n_slots ? slot * p.T + (j - block_of(p, j) * p.T) : 0u;
-            r.have[i] = __ballot(slot < p.n_slots);
+            const bool in = j < c1 && slot < p.n_slots;
+            r.at[i] = in ? slot * p.T + (j - block_of(p, j) * p.T) : 0u;
+            r.have[i] = __ballot(in);
         }
         return r;
     };
@@ -620,9 +634,6 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
             rv[i] = *reinterpret_cast<const UV *>(v_head + static_cast<uint64_t>(at) * p.row_v + vu * SV::unit);
         }
     };
-    constexpr uint32_t step = kWaves * KT;
-    uint32_t j0 = c0 + wave * KT;
-    const Slots first_slots = slots_of(j0);
     const bool uneven = tok0 != tok1 && c1 > n_all;  // some rows do not attend all the keys
     if (uneven) {
         if (threadIdx.x < D) {
@@ -641,7 +652,7 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
 
     // The row's queries, scaled into f16's range.  Codes carry an offset: the
     // sum of a group's queries times it comes off each score, as one more product
-    // of the groups' scales with those sums (in three f16 pieces, 33 bits).
+    // of the groups' scales with those sums (in two f16 pieces, 22 bits).
     Cells cells;
     Slots next;
     half8_t qf[NG];
@@ -687,26 +698,27 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
             q_off[e] = 0;
         }
         if constexpr (KO::codes) {
-            // piece c of the sum stands in chunk c of the contraction
-            const _Float16 pick[3] = {static_cast<_Float16>(c == 0 ? 1.0f : 0.0f),
-                                      static_cast<_Float16>(c == 1 ? 1.0f : 0.0f),
-                                      static_cast<_Float16>(c == 2 ? 1.0f : 0.0f)};
+            // a group's sum is its product with a key of ones; its upper and lower
+            // f16 digits stand in chunks 0 and 1 of the contraction
+            half8_t ones;
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                ones[e] = static_cast<_Float16>(KO::times(e));
+            }
+            const _Float16 pick_hi = static_cast<_Float16>(c == 0 ? 1.0f : 0.0f);
+            const _Float16 pick_lo = static_cast<_Float16>(c == 1 ? 1.0f : 0.0f);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                float all = 0.0f;
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) {
-                    all += static_cast<float>(qf[g][e]);
                     qf[g][e] *= static_cast<_Float16>(1.0f / KO::times(e));
                 }
-                all += lane_xor16(all);
-                all += lane_xor32(all);
-                all *= -KO::offset * 0x1p-10f;
+                const float all = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                      ones, qf[g], float4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0)[0] *
+                                  (-KO::offset * 0x1p-10f);
                 const _Float16 hi = static_cast<_Float16>(all);
-                const float left = all - static_cast<float>(hi);
-                const _Float16 mid = static_cast<_Float16>(left);
-                const _Float16 lo = static_cast<_Float16>(left - static_cast<float>(mid));
-                q_off[g] = hi * pick[0] + mid * pick[1] + lo * pick[2];
+                const _Float16 lo = static_cast<_Float16>(all - static_cast<float>(hi));
+                q_off[g] = hi * pick_hi + lo * pick_lo;
             }
         }
         fac = ldexpf(p.scale * kLog2e, (KO::codes ? 24 : 0) - ex);
@@ -910,57 +922,68 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
     float *ow = reinterpret_cast<float *>(lds) + wave * rows * D;  // [row][dim]
     const float fade = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - all);
     if (nl < rows) {
+        constexpr int RUN = VO::RUN;  // neighbouring dims among a lane's
 #pragma unroll
-        for (int t = 0; t < VD; ++t) {
+        for (uint32_t i = 0; i < 4; ++i) {
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                ow[nl * D + VO::dim(4u * c + i, t)] = o[t][i] * fade;
+            for (int t = 0; t < VD; t += RUN) {
+                typedef float run_t __attribute__((ext_vector_type(RUN)));
+                run_t v;
+#pragma unroll
+                for (int u = 0; u < RUN; ++u) {
+                    v[u] = o[VO::nth(t + u)][i] * fade;
+                }
+                *reinterpret_cast<run_t *>(ow + nl * D + VO::dim(4u * c + i, VO::nth(t))) = v;
             }
         }
     }
     __syncthreads();
+    // a wave takes 256 elements of the rows, a lane four
     const float *ol = reinterpret_cast<const float *>(lds);
-    const bool last = n_parts == 1;
-    float *turn = reinterpret_cast<float *>(lds);
-    for (uint32_t e0 = 0; e0 < rows * D; e0 += 256u) {
-        const uint32_t e = e0 + threadIdx.x;
-        const bool in = e < rows * D;
-        const uint32_t row = min(e / D, rows - 1u);
+    for (uint32_t e0 = wave * 256u; e0 < rows * D; e0 += 1024u) {
+        const uint32_t e = min(e0 + 4u * lane, rows * D - 4u);
+        const bool in = e == e0 + 4u * lane;
+        const uint32_t row = e / D;
         const uint32_t d = e & (D - 1u);
         const uint32_t tok = (row0 + row) / p.group;
         const uint32_t head = hk * p.group + (row0 + row - tok * p.group);
         const uint64_t at = static_cast<uint64_t>(r.first + tok) * p.n_head + head;
-        float total = 0.0f, mx = -INFINITY, x = 0.0f;
+        float mx = -INFINITY, total = 0.0f;
 #pragma unroll
         for (uint32_t w = 0; w < kWaves; ++w) {
             mx = fmaxf(mx, wave_ml[w][row].x);
         }
+        float4_t x{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (uint32_t w = 0; w < kWaves; ++w) {
             const float2 ml = wave_ml[w][row];
-            total += ml.x == -INFINITY ? 0.0f * ml.y : ml.y * __builtin_amdgcn_exp2f(ml.x - mx);
-            x += in ? ol[w * rows * D + e] : 0.0f;
+            total += ml.y * (ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mx));
+            x += *reinterpret_cast<const float4_t *>(ol + w * rows * D + e);
         }
-        if (uneven && first_odd[d] < key_limit(p, r, tok)) {
-            x = NAN;
+        if (uneven) {
+            const uint32_t limit = key_limit(p, r, tok);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = first_odd[d + i] < limit ? NAN : x[i];
+            }
         }
-        if (!last) {
+        if (n_parts > 1) {
             if (in) {
-                const uint64_t pe = (static_cast<uint64_t>(part) * p.n_tokens * p.n_head) + at;
-                p.part_o[pe * D + d] = x;
+                const uint64_t pe = static_cast<uint64_t>(part) * p.n_tokens * p.n_head + at;
+                *reinterpret_cast<float4_t *>(p.part_o + pe * D + d) = x;
                 if (d == 0) {
                     p.part_ml[pe] = make_float2(mx, total);
                 }
             }
             continue;
         }
-        x = total == 0.0f ? 0.0f : x / total;
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
         if (p.hadamard) {
-            // this round's own 256 elements of the LDS rows (read above by these threads only)
-            x = rotate_back(x, p.hadamard, e & (p.hadamard - 1u), turn + (e - (e & (p.hadamard - 1u))));
+            rotate_lanes<4>(y, p.hadamard, lane);
         }
         if (in) {
-            store_elem(p.out, p.out_type, at * D + d, x);
+            store_elems<4>(p.out, p.out_type, at * D + d, y);
             if (d == 0 && p.lse) {
                 p.lse[at] = total == 0.0f ? -INFINITY : (mx - kWeightShift) / kLog2e + logf(total);
             }
@@ -994,18 +1017,6 @@ __device__ inline uint32_t anew(uint32_t x) {
     return x;
 }
 typedef __attribute__((address_space(3))) void lds_void_t;
-
-// Four neighbouring output elements.
-__device__ inline void store4(uint8_t *out, int type, uint64_t e, float4_t x) {
-    if (type == KVMEM_TYPE_F32) {
-        *reinterpret_cast<float4_t *>(out + 4 * e) = x;
-    } else if (type == KVMEM_TYPE_F16) {
-        *reinterpret_cast<half4_t *>(out + 2 * e) = __builtin_convertvector(x, half4_t);
-    } else {
-        typedef __bf16 bf4_t __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<bf4_t *>(out + 2 * e) = __builtin_convertvector(x, bf4_t);
-    }
-}
 
 template <int TK, int TV, int D>
 struct PrefillLds {
@@ -1120,11 +1131,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) 
         Slots r;
 #pragma unroll
         for (uint32_t i = 0; i < NC; ++i) {
-            const uint32_t j = j0 + (lane & (KT - 1u)) + 64u * i;
-            r.of[i] = KVMEM_HIP_NO_SLOT;
-            if (j < c1) {
-                r.of[i] = table[block_of(p, j)];
-            }
+            // within the table, whatever the request's length
+            r.of[i] = table[block_of(p, min(j0 + (lane & (KT - 1u)) + 64u * i, p.room - 1u))];
         }
         return r;
     };
@@ -1134,8 +1142,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) 
         for (uint32_t i = 0; i < NC; ++i) {
             const uint32_t j = j0 + (lane & (KT - 1u)) + 64u * i;
             const uint32_t slot = slots.of[i];
-            r.at[i] = slot < p.n_slots ? slot * p.T + (j - block_of(p, j) * p.T) : 0u;
-            r.have[i] = __ballot(slot < p.n_slots);
+            const bool in = j < c1 && slot < p.n_slots;
+            r.at[i] = in ? slot * p.T + (j - block_of(p, j) * p.T) : 0u;
+            r.have[i] = __ballot(in);
         }
         return r;
     };
@@ -1504,7 +1513,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) 
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             const uint32_t dim = 32 * b + 2 * i + 4 * hh;
-            float4_t x{o[b][i] * f, o[b][i + 1] * f, o[b][i + 2] * f, o[b][i + 3] * f};
+            float x[4] = {o[b][i] * f, o[b][i + 1] * f, o[b][i + 2] * f, o[b][i + 3] * f};
             if (uneven) {
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
@@ -1512,7 +1521,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) 
                 }
             }
             if (mine) {
-                store4(out, type, to * D + dim, x);
+                store_elems<4>(out, type, to * D + dim, x);
             }
         }
     }

@@ -142,30 +142,6 @@ __device__ inline void rope_sincos(float a, float &sn, float &cs) {
     cs = static_cast<float>(((quadrant + 1) & 2) ? -cv : cv);
 }
 
-// The value of lane ^ M: DPP quad permutes for 1 and 2, a row rotation by
-// 8 (within 16 lanes, the same as ^ 8), ds_swizzle's xor mode for 4 and 16
-// (within 32 lanes; these run on the LDS pipe, off the VALU that bounds the
-// transform), a lane permute for 32.  Every lane of the wave must be active.
-template <uint32_t M>
-__device__ inline float lane_xor(float v) {
-    const int x = __float_as_int(v);
-    int r;
-    if constexpr (M == 1) {
-        r = __builtin_amdgcn_mov_dpp(x, 0xB1, 0xF, 0xF, true);
-    } else if constexpr (M == 2) {
-        r = __builtin_amdgcn_mov_dpp(x, 0x4E, 0xF, 0xF, true);
-    } else if constexpr (M == 4) {
-        r = __builtin_amdgcn_ds_swizzle(x, 0x1F | (4 << 10));
-    } else if constexpr (M == 8) {
-        r = __builtin_amdgcn_mov_dpp(x, 0x128, 0xF, 0xF, true);  // row_ror:8
-    } else if constexpr (M == 16) {
-        r = __builtin_amdgcn_ds_swizzle(x, 0x1F | (16 << 10));
-    } else {
-        r = __shfl_xor(x, static_cast<int>(M), 64);
-    }
-    return __int_as_float(r);
-}
-
 // One butterfly stage of span 8*M across lanes: the lane whose bit M is set
 // holds the upper element and keeps partner - own, the other own + partner
 // (p + (-x) is the IEEE subtraction p - x).
