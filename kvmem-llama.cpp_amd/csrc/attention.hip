@@ -8,20 +8,11 @@ namespace kvmem_hip {
 
 // ------------------------------------------------------------- joining parts
 
-// One workgroup per (token, head): the parts' sums, each weighted by its
-// maximum.  Each wave adds the parts k = wave, wave + 4, ... in order, a lane its
-// D/64 dims, then the waves' sums are added in order.
-template <int D>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
-    constexpr int E = D / 64;
-    typedef float dims_t __attribute__((ext_vector_type(E)));
-    __shared__ float sums[kWaves][D];
-    __shared__ float totals[kWaves];
-    const uint32_t h = blockIdx.x % p.n_head;
-    const uint32_t tok = blockIdx.x / p.n_head;
-    const uint32_t tid = threadIdx.x;
-    const uint32_t lane = tid & 63u;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+// Parts up to which one wave joins a row.
+constexpr uint32_t kJoinParts = 8;
+
+// The parts of a (token, head) row, 0 where this row is not joined.
+__device__ inline uint32_t row_parts(const AttnParams &p, uint32_t tok, uint32_t h) {
     // the request this token belongs to
     uint32_t s = tok;
     if (p.q_start) {
@@ -37,11 +28,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
         s = lo;
     }
     if (s >= p.n_seq) {
-        return;
+        return 0;
     }
     const Span r = request_span(p, s);
     if (tok < r.first || tok - r.first >= min(r.m, p.max_q)) {
-        return;
+        return 0;
     }
     const uint32_t i = tok - r.first;
     // the part count of the row tile this row was in
@@ -50,10 +41,29 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
     const uint32_t rows = min(p.row_tile, min(r.m, p.max_q) * p.group - row0);
     const uint32_t n = key_limit(p, r, (row0 + rows - 1u) / p.group);
     const uint32_t n_parts = max(1u, (n + p.chunk - 1u) / p.chunk);
-    if (n_parts == 1 && !p.join_one) {
+    return n_parts == 1 && !p.join_one ? 0u : n_parts;
+}
+
+// W waves a row, one row a workgroup (W > 1: the parts are dealt to the waves and
+// their sums added in the waves' order) or four (W = 1).  A lane adds D/64 dims of
+// its wave's parts in order, each weighted by its maximum.  Latency-bound for few
+// rows: a wave has all its parts' loads in flight at once.
+template <int D, int W>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void attn_join_kernel(AttnParams p) {
+    constexpr int E = D / 64;
+    typedef float dims_t __attribute__((ext_vector_type(E)));
+    __shared__ float sums[W][D];
+    __shared__ float totals[W];
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t row = W == 1 ? blockIdx.x * 4u + wave : blockIdx.x;
+    const uint32_t tok = row / p.n_head;
+    const uint32_t h = row - tok * p.n_head;
+    const uint32_t n_parts = tok < p.n_tokens ? row_parts(p, tok, h) : 0u;
+    if (n_parts == 0) {
         return;
     }
-    const uint64_t at = static_cast<uint64_t>(tok) * p.n_head + h;
+    const uint64_t at = row;
     const uint64_t stride = static_cast<uint64_t>(p.n_tokens) * p.n_head;
     float top = -INFINITY;
     for (uint32_t k = lane; k < n_parts; k += 64u) {
@@ -68,28 +78,34 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
     const float *po = p.part_o + at * D + lane * E;
     float total = 0.0f;
     dims_t x = {};
+    const uint32_t k0 = W == 1 ? 0u : wave;
 #pragma unroll 8
-    for (uint32_t k = wave; k < n_parts; k += kWaves) {
+    for (uint32_t k = k0; k < n_parts; k += W) {
         const float2 ml = p.part_ml[k * stride + at];
         const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);
         total += ml.y * f;
         x += *reinterpret_cast<const dims_t *>(po + k * stride * D) * f;
     }
-    *reinterpret_cast<dims_t *>(&sums[wave][lane * E]) = x;
-    if (lane == 0) {
-        totals[wave] = total;
+    if constexpr (W > 1) {
+        *reinterpret_cast<dims_t *>(&sums[wave][lane * E]) = x;
+        if (lane == 0) {
+            totals[wave] = total;
+        }
+        __syncthreads();
+        if (wave != 0) {
+            return;
+        }
+#pragma unroll
+        for (int w = 1; w < W; ++w) {
+            total += totals[w];
+            x += *reinterpret_cast<const dims_t *>(&sums[w][lane * E]);
+        }
     }
-    __syncthreads();
-    if (wave != 0) {
-        return;
-    }
-    total = (totals[0] + totals[1]) + (totals[2] + totals[3]);
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     float y[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        const uint32_t d = lane * E + i;
-        y[i] = ((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) * inv;
+        y[i] = x[i] * inv;
     }
     if (p.hadamard) {
         rotate_lanes<E>(y, p.hadamard, lane);
@@ -100,18 +116,51 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
     }
 }
 
-// Query rows of a request above which the prefill kernel takes the call.
-constexpr uint32_t kDecodeRows = 16;
-// Workgroups a decode launch is split up to.
-constexpr uint32_t kDecodeGroups = 512;
+template <int D>
+static void launch_join(hipStream_t stream, const AttnParams &p) {
+    const uint32_t rows = p.n_tokens * p.n_head;
+    if (p.n_parts <= kJoinParts) {
+        attn_join_kernel<D, 1><<<(rows + 3) / 4, 256, 0, stream>>>(p);
+    } else {
+        attn_join_kernel<D, 4><<<rows, 256, 0, stream>>>(p);
+    }
+}
+
 constexpr uint32_t kComputeUnits = 256;
+
+// Rows of a request (tokens x heads of a KV head) above which the prefill kernel
+// takes the call; the decode kernel reads the keys again for every 16 rows.
+// Measured, decode against prefill kernel, q4_0, 4 KV heads of 256:
+//   one request over 32768 keys:  48 rows 46 against 111 us, 72: 61/116, 96: 94/116
+//   eight over 8192:              60 rows 76 against 87 us, 96: 131/89
+static uint32_t decode_rows(uint32_t n_seq) {
+    return n_seq <= 2 ? 96 : 64;
+}
+
+// Workgroups a decode launch is split up to, from the steps (128 keys of 256
+// elements, a step of four waves) of all requests.  Every part costs its joining
+// and the pipeline's first wait: one workgroup a compute unit while there are few
+// steps for each, then two, or three with many requests, which end at different
+// places.  Measured, q4_0 with 4 KV heads of 256, 256 / 512 / 768 workgroups in us:
+//   one request: 16384 keys 17 / 21, 32768 22 / 24, 65536 32 / 32 / 43,
+//                131072 53 / 46 / 61, and with q8_0 keys 65536 57 / 50 / 67
+//   16 of 1024 keys: 17 / 19 / 19; 8 of 2048: 18 / 18 / 18
+//   8 of 8192: 32 / 29 / 27; 16 of 4096: 31 / 30 / 27; 16 of 8192: 48 / 44 / 37
+//   8 ragged ones up to 8192 with 5 tokens, q5_0, 2 KV heads of 64: 35 / 29 / 24
+//   32 ragged ones up to 16384, 8 KV heads of 128: 172 / 142 / 116 (1024: 134)
+static uint64_t decode_groups(uint32_t n_seq, uint64_t steps) {
+    if (n_seq < 8) {
+        return steps <= 4 * kComputeUnits ? kComputeUnits : 2 * kComputeUnits;
+    }
+    return steps <= 2 * kComputeUnits ? kComputeUnits : 3 * kComputeUnits;
+}
 
 static AttnPlan plan_attention(const kvmem_hip_pool *pool, const kvmem_hip_attn_args *a) {
     AttnPlan pl{};
     const uint32_t max_q = a->q_start ? std::min(a->max_q, a->n_tokens) : 1u;
     const uint32_t group = a->n_head / a->n_head_kv;
     const uint64_t rows = static_cast<uint64_t>(max_q) * group;
-    pl.prefill = rows <= kDecodeRows ? 0u : rows <= 128 ? 4u : 8u;
+    pl.prefill = rows <= decode_rows(a->n_seq) ? 0u : rows <= 128 ? 4u : 8u;
     pl.row_tile = pl.prefill ? 32u * pl.prefill : kRowTile;
     pl.row_tiles = static_cast<uint32_t>((rows + pl.row_tile - 1) / pl.row_tile);
     const uint32_t quantum = step_keys(a->head_dim) * (pl.prefill ? 1u : kWaves);
@@ -134,7 +183,7 @@ static AttnPlan plan_attention(const kvmem_hip_pool *pool, const kvmem_hip_attn_
             }
         }
     } else {
-        parts = std::min(std::max<uint64_t>(1, kDecodeGroups / groups), most);
+        parts = std::min(std::max<uint64_t>(1, decode_groups(a->n_seq, groups * most) / groups), most);
     }
     uint64_t chunk = (keys + parts - 1) / parts;
     chunk = (chunk + quantum - 1) / quantum * quantum;
@@ -160,7 +209,7 @@ static AttnPlan plan_attention(const kvmem_hip_pool *pool, const kvmem_hip_attn_
 }
 
 bool load_attention_kernels() {
-    return load_kernel_object(&attn_join_kernel<64>);
+    return load_kernel_object(&attn_join_kernel<64, 1>);
 }
 
 static bool cache_type(int t) {
@@ -349,13 +398,12 @@ int kvmem_hip_attention(kvmem_hip_ctx *ctx, const kvmem_hip_pool *pool, uint32_t
         default: launch_attention<KVMEM_TYPE_F16>(ctx->stream, pool->type_v, a->head_dim, pl, p); break;
     }
     if (pl.joined) {
-        const uint32_t rows = p.n_tokens * p.n_head;
         if (a->head_dim == 64) {
-            attn_join_kernel<64><<<rows, 256, 0, ctx->stream>>>(p);
+            launch_join<64>(ctx->stream, p);
         } else if (a->head_dim == 128) {
-            attn_join_kernel<128><<<rows, 256, 0, ctx->stream>>>(p);
+            launch_join<128>(ctx->stream, p);
         } else {
-            attn_join_kernel<256><<<rows, 256, 0, ctx->stream>>>(p);
+            launch_join<256>(ctx->stream, p);
         }
     }
     return hip_ok(ctx, hipGetLastError(), "attention launch") ? KVMEM_HIP_OK : KVMEM_HIP_ERR_RUNTIME;

@@ -52,13 +52,23 @@ __device__ inline void lds_words(const uint8_t *p, uint32_t shift, uint32_t out[
     uint32_t w[N + 1];
 #pragma unroll
     for (int i = 0; i <= N; ++i) {
-        w[i] = q[i];  // (a last word that a constant shift of 0 leaves unused is not read)
+        w[i] = q[i];
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         out[i] = __builtin_amdgcn_alignbyte(w[i + 1], w[i], shift);
     }
 }
+// The same where the address is known to be a word's.
+struct Aligned {};
+template <int N>
+__device__ inline void lds_words(const uint8_t *p, Aligned, uint32_t out[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        out[i] = reinterpret_cast<const uint32_t *>(p)[i];
+    }
+}
+
 // Key operand of one group of 32 dims: the 8 elements a lane (key, chunk c of
 // 4) feeds the matrix instruction, as f16.  Quantized codes stay integers:
 // an f16 whose bits are the code n is the subnormal n * 2^-24, which the
@@ -68,7 +78,7 @@ __device__ inline void lds_words(const uint8_t *p, uint32_t shift, uint32_t out[
 // through the accumulator's start, the group's scale is multiplied into the
 // fp32 sum: keys enter the scores unrounded.
 // shift: the bytes that the group's codes lie off a word (2 in groups of even
-// number).
+// number, Aligned where that is known).
 // Element e is dim piece(c, i) + l % 4 of the group, l = order(e) and i = l / 4:
 // a lane's 8 dims are two runs of four.
 template <int TYPE> struct KeyOp;
@@ -76,7 +86,8 @@ template <int TYPE> struct KeyOp;
 template <> struct KeyOp<KVMEM_TYPE_Q4_0> {
     static constexpr float offset = 8.0f;
     static constexpr bool codes = true;
-    __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c, uint32_t shift) {
+    template <class Shift>
+    __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c, Shift shift) {
         uint32_t w;
         lds_words<1>(g + 2 + 4 * c, shift, &w);
         u32x4_t r;
@@ -95,7 +106,8 @@ template <> struct KeyOp<KVMEM_TYPE_Q4_0> {
 template <> struct KeyOp<KVMEM_TYPE_Q5_0> {
     static constexpr float offset = 16.0f;
     static constexpr bool codes = true;
-    __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c, uint32_t shift) {
+    template <class Shift>
+    __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c, Shift shift) {
         uint32_t h, w;
         lds_words<1>(g + 2, shift, &h);
         lds_words<1>(g + 6 + 4 * c, shift, &w);
@@ -119,7 +131,8 @@ template <> struct KeyOp<KVMEM_TYPE_Q5_0> {
 template <> struct KeyOp<KVMEM_TYPE_Q8_0> {
     static constexpr float offset = 128.0f;
     static constexpr bool codes = true;
-    __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c, uint32_t shift) {
+    template <class Shift>
+    __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c, Shift shift) {
         uint32_t w[2];
         lds_words<2>(g + 2 + 8 * c, shift, w);
         const uint32_t a = w[0] ^ 0x80808080u;
@@ -139,7 +152,8 @@ template <> struct KeyOp<KVMEM_TYPE_Q8_0> {
 template <> struct KeyOp<KVMEM_TYPE_F16> {
     static constexpr float offset = 0.0f;
     static constexpr bool codes = false;
-    __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c, uint32_t) {
+    template <class Shift>
+    __device__ static inline u32x4_t load(const uint8_t *g, uint32_t c, Shift) {
         return *reinterpret_cast<const u32x4_t *>(g + 16 * c);
     }
     __device__ static inline uint32_t piece(uint32_t c, uint32_t i) { return 8 * c + 4 * i; }
@@ -540,9 +554,11 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
 
     const uint32_t unit = blockIdx.x % p.units;
     const uint32_t y = blockIdx.x / p.units;
-    const uint32_t s = unit / p.n_parts;
-    const uint32_t part = unit - s * p.n_parts;
-    if (s >= p.n_seq) {
+    // part by part, each starting one request further: a request's parts, and the
+    // parts that only long requests have, fall on all XCDs
+    const uint32_t part = unit / p.n_seq;
+    const uint32_t s = (unit + part) % p.n_seq;
+    if (part >= p.n_parts) {
         return;
     }
     const uint32_t lane = threadIdx.x & 63u;
@@ -767,63 +783,84 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
         load_tile(cells);
         next = slots_of(j0 + 2u * step);
         if constexpr (KO::codes) {
-            // a key's scales side by side
-            for (uint32_t key = lane % KT; key < KT; key += 64u) {
-                constexpr uint32_t per = KT < 64u ? NG * KT / 64u : NG;  // groups of a lane
-                const uint32_t g0 = KT < 64u ? lane / KT * per : 0u;
+            // a key's scales side by side: 256 of a step, four a lane
+            constexpr uint32_t per = NG < 4 ? NG : 4;
+            typedef uint16_t some_t __attribute__((ext_vector_type(per)));
+#pragma unroll
+            for (uint32_t i = 0; i < 4u / per; ++i) {
+                const uint32_t key = (lane + 64u * i) % KT;
+                const uint32_t g0 = (lane + 64u * i) / KT * per;
+                some_t d;
 #pragma unroll
                 for (uint32_t g = 0; g < per; ++g) {
-                    reinterpret_cast<uint16_t *>(ks + key)[g0 + g] =
-                        static_cast<uint16_t>(lds_half(kt + key * SK::stride + (g0 + g) * SK::GB));
+                    d[g] = static_cast<uint16_t>(lds_half(kt + key * SK::stride + (g0 + g) * SK::GB));
                 }
+                *reinterpret_cast<some_t *>(reinterpret_cast<uint16_t *>(ks + key) + g0) = d;
             }
             wave_lds_sync();
         }
         float x[NT][4];
 #pragma unroll
-        for (uint32_t a = 0; a < NT; ++a) {
-            const uint8_t *kr = kt + (16u * a + nl) * SK::stride;
-            float4_t sc{0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (KO::codes) {
-                half8_t kd;
+        for (uint32_t a0 = 0; a0 < NT; a0 += 2) {  // two tiles' products wait for one another's
+            const uint8_t *kr[2];
+            float4_t sc[2];
+            scales_t d[2][4];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    kd[e] = 0;
-                }
-                const scales_t mine = ks[16u * a + nl];
+            for (uint32_t i = 0; i < 2; ++i) {
+                kr[i] = kt + (16u * (a0 + i) + nl) * SK::stride;
+                sc[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (KO::codes) {
+                    half8_t kd;
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    kd[g] = __builtin_bit_cast(_Float16, static_cast<uint16_t>(mine[g]));
-                }
-                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kd, q_off, sc, 0, 0, 0);
-                sc *= 0x1p-14f;
-                scales_t d[4];
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    d[i] = ks[16u * a + 4u * c + i];
-                }
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const half8_t kf = __builtin_bit_cast(half8_t, KO::load(kr + g * SK::GB, c, (g & 1) ? 0u : 2u));
-                    const float4_t acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        kf, qf[g], float4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        sc[i] = __builtin_fmaf(
-                            static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(d[i][g]))), acc[i],
-                            sc[i]);
+                    for (int e = 0; e < 8; ++e) {
+                        kd[e] = 0;
                     }
-                }
-            } else {
+                    const scales_t mine = ks[16u * (a0 + i) + nl];
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const half8_t kf = __builtin_bit_cast(half8_t, KO::load(kr + g * SK::GB, c, (g & 1) ? 0u : 2u));
-                    sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[g], sc, 0, 0, 0);
+                    for (int g = 0; g < NG; ++g) {
+                        kd[g] = __builtin_bit_cast(_Float16, static_cast<uint16_t>(mine[g]));
+                    }
+                    sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kd, q_off, sc[i], 0, 0, 0);
+                    sc[i] *= 0x1p-14f;
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        d[i][j] = ks[16u * (a0 + i) + 4u * c + j];
+                    }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[a][i] = sc[i] * fac;
+            for (int g = 0; g < NG; ++g) {
+                float4_t acc[2];
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i) {
+                    const uint8_t *gp = kr[i] + g * SK::GB;
+                    const half8_t kf = __builtin_bit_cast(
+                        half8_t, (g & 1) ? KO::load(gp, c, Aligned{}) : KO::load(gp, c, 2u));
+                    if constexpr (KO::codes) {
+                        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[g], float4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0,
+                                                                        0, 0);
+                    } else {
+                        sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[g], sc[i], 0, 0, 0);
+                    }
+                }
+                if constexpr (KO::codes) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 2; ++i) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            sc[i][j] = __builtin_fmaf(
+                                static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(d[i][j][g]))),
+                                acc[i][j], sc[i][j]);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    x[a0 + i][j] = sc[i][j] * fac;
+                }
             }
         }
         if (!whole || j0 + KT > n_all) {
