@@ -17,7 +17,13 @@
 // cos and sin of a token's rotary pairs are computed once per workgroup into
 // LDS (about 70 double-precision operations a pair).  A workgroup takes several
 // tokens when there are many, so that a pair's angle serves all the token's
-// heads; few tokens are spread over workgroups instead, a unit per wave.
+// heads; few tokens are spread over workgroups instead, a unit per wave.  Norm
+// weights and cells are read from LDS too: loads complete in order, so one
+// inside the loop would wait for the unit that is read ahead.
+//
+// Measured, 24 + 2 x 4 heads of 256 in bf16: 8191 tokens, with the norm, 57.5 us
+// for 268 MB (4.65 TB/s; 83 us without reading ahead and at four waves a SIMD
+// instead of eight), 96 tokens 4.4 us, one token 4.3 us (the launch).
 #include "kvmem_internal.hpp"
 #include "row_transform.hpp"
 
@@ -32,8 +38,12 @@ namespace kvmem_hip {
 constexpr uint32_t kRowThreads = 256;
 constexpr uint32_t kRowWaves = kRowThreads / 64;
 constexpr uint32_t kUnit = 512;       // elements of a wave's unit
-constexpr uint32_t kMaxRot = 512;     // rotary dims
+constexpr uint32_t kMaxRot = 512;     // rotary dims, head_dim
 constexpr uint32_t kMaxRowTokens = 8; // tokens of a workgroup
+// Workgroups for many tokens: two rounds of the eight that a compute unit holds.
+// 8191 tokens of 24 + 2 x 4 heads of 256 (bf16, norm, q8_0 rows): 2048 take 61 us,
+// 4096 and 8192 57.5 us.
+constexpr uint32_t kRowGroups = 4096;
 
 struct Theta {
     float f[kMaxRot / 2];
@@ -66,31 +76,32 @@ struct RowParams {
 };
 
 template <typename T>
-__device__ inline void load_row8(const uint8_t *p, uint32_t vec, float x[8]) {
-    typedef T unit_t __attribute__((ext_vector_type(8)));
+struct Row8 {
+    typedef T type __attribute__((ext_vector_type(8)));
+};
+
+template <typename T>
+__device__ inline typename Row8<T>::type load_row8(const uint8_t *p, uint32_t vec) {
+    typename Row8<T>::type v;
     if (vec) {
-        const unit_t v = *reinterpret_cast<const unit_t *>(p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x[i] = static_cast<float>(v[i]);
-        }
+        v = *reinterpret_cast<const typename Row8<T>::type *>(p);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            x[i] = static_cast<float>(reinterpret_cast<const T *>(p)[i]);
+            v[i] = reinterpret_cast<const T *>(p)[i];
         }
     }
+    return v;
 }
 
 template <typename T>
 __device__ inline void store_row8(uint8_t *p, const float x[8]) {
-    typedef T unit_t __attribute__((ext_vector_type(8)));
-    unit_t v;
+    typename Row8<T>::type v;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         v[i] = static_cast<T>(x[i]);  // round to nearest even
     }
-    *reinterpret_cast<unit_t *>(p) = v;
+    *reinterpret_cast<typename Row8<T>::type *>(p) = v;
 }
 
 
@@ -134,11 +145,37 @@ __device__ inline void put_unit(const float x[8], uint8_t *lds, uint8_t *dst, ui
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// A wave's unit: token of the workgroup, kind, heads [h0, h0 + heads).
+struct Unit {
+    uint32_t tl, kd, h0, heads;
+};
+
+__device__ inline Unit find_unit(const RowParams &p, uint32_t u, uint32_t per_token, uint32_t heads_per_unit) {
+    Unit r;
+    r.tl = u / per_token;
+    uint32_t w = u - r.tl * per_token;
+    r.kd = 0;
+    if (w >= p.kind[0].units) {
+        w -= p.kind[0].units;
+        r.kd = 1;
+        if (w >= p.kind[1].units) {
+            w -= p.kind[1].units;
+            r.kd = 2;
+        }
+    }
+    r.h0 = w * heads_per_unit;
+    r.heads = min(heads_per_unit, p.kind[r.kd].n_head - r.h0);
+    return r;
+}
+
 // TI / TO: element types of the inputs and of the output rows.
 template <typename TI, typename TO>
-__global__ __launch_bounds__(kRowThreads) void qkv_rows_kernel(RowParams p, Theta theta) {
+__global__ __launch_bounds__(kRowThreads, 8) void qkv_rows_kernel(RowParams p, Theta theta) {
     __shared__ __attribute__((aligned(16))) uint8_t staged[kRowWaves][16 * 64];
-    extern __shared__ __attribute__((aligned(16))) float2 tab[];  // [tokens][n_rot / 2] cos, sin
+    // [2][head_dim] norm weights, then [tokens][n_rot / 2] cos, sin
+    extern __shared__ __attribute__((aligned(16))) float weights[];
+    __shared__ uint32_t cells[kMaxRowTokens];
+    float2 *tab = reinterpret_cast<float2 *>(weights + 2u * p.head_dim);
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t group = blockIdx.x / p.splits;
@@ -146,40 +183,71 @@ __global__ __launch_bounds__(kRowThreads) void qkv_rows_kernel(RowParams p, Thet
     const uint32_t t0 = group * p.tokens;
     const uint32_t nt = min(p.tokens, p.n_tokens - t0);
     const uint32_t half = p.n_rot / 2u;
+    const uint32_t e0 = lane * 8u;
+    const uint32_t head_in_unit = e0 / p.head_dim;
+    const uint32_t d0 = e0 & (p.head_dim - 1u);
+    const uint32_t heads_per_unit = kUnit / p.head_dim;
+    const uint32_t per_token = p.kind[0].units + p.kind[1].units + p.kind[2].units;
+    const uint32_t end = nt * per_token;
+    const uint32_t step = p.splits * kRowWaves;
+    // lanes behind the last head read it again, and write nothing
+    const auto read = [&](const Unit &n) {
+        const RowKind &k = p.kind[n.kd];
+        const uint32_t h = n.h0 + min(head_in_unit, n.heads - 1u);
+        return load_row8<TI>(k.src + h * k.nb1 + (t0 + n.tl) * k.nb2 + d0 * sizeof(TI), k.vec);
+    };
+    // the row a unit ahead is on its way while one is worked on, the first while
+    // the angles are
+    uint32_t u = split * kRowWaves + wave;
+    Unit next{};
+    typename Row8<TI>::type ahead{};
+    if (u < end) {
+        next = find_unit(p, u, per_token, heads_per_unit);
+        ahead = read(next);
+    }
+    constexpr uint32_t kWeightsPerThread = 2 * kMaxRot / kRowThreads;
+    float weight[kWeightsPerThread];
+#pragma unroll
+    for (uint32_t j = 0; j < kWeightsPerThread; ++j) {
+        const uint32_t i = threadIdx.x + j * kRowThreads;
+        const float *w = i < p.head_dim ? p.kind[0].weight : p.kind[1].weight;
+        weight[j] = w && i < 2u * p.head_dim ? w[i < p.head_dim ? i : i - p.head_dim] : 1.0f;
+    }
+    const uint32_t cell_ahead = threadIdx.x < nt && p.cells ? static_cast<uint32_t>(p.cells[t0 + threadIdx.x]) : ~0u;
     for (uint32_t i = threadIdx.x; i < nt * half; i += kRowThreads) {
         const uint32_t t = i / half;
         float sn, cs;
         rope_sincos(static_cast<float>(p.positions[t0 + t]) * theta.f[i - t * half], sn, cs);
         tab[i] = make_float2(cs, sn);
     }
+#pragma unroll
+    for (uint32_t j = 0; j < kWeightsPerThread; ++j) {
+        if (threadIdx.x + j * kRowThreads < 2u * p.head_dim) {
+            weights[threadIdx.x + j * kRowThreads] = weight[j];
+        }
+    }
+    if (threadIdx.x < kMaxRowTokens) {
+        cells[threadIdx.x] = cell_ahead;
+    }
     __syncthreads();
 
-    const uint32_t e0 = lane * 8u;
-    const uint32_t head_in_unit = e0 / p.head_dim;
-    const uint32_t d0 = e0 & (p.head_dim - 1u);
-    const uint32_t heads_per_unit = kUnit / p.head_dim;
-    const uint32_t per_token = p.kind[0].units + p.kind[1].units + p.kind[2].units;
-    for (uint32_t u = split * kRowWaves + wave; u < nt * per_token; u += p.splits * kRowWaves) {
-        const uint32_t tl = u / per_token;
-        uint32_t w = u - tl * per_token;
-        uint32_t kd = 0;
-        if (w >= p.kind[0].units) {
-            w -= p.kind[0].units;
-            kd = 1;
-            if (w >= p.kind[1].units) {
-                w -= p.kind[1].units;
-                kd = 2;
-            }
+    while (u < end) {
+        const Unit n = next;
+        const uint32_t kd = n.kd, tl = n.tl, h0 = n.h0, heads = n.heads;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x[i] = static_cast<float>(ahead[i]);
+        }
+        u += step;
+        if (u < end) {
+            next = find_unit(p, u, per_token, heads_per_unit);
+            ahead = read(next);
         }
         const RowKind &k = p.kind[kd];
         const uint32_t t = t0 + tl;
-        const uint32_t h0 = w * heads_per_unit;
-        const uint32_t heads = min(heads_per_unit, k.n_head - h0);
         const bool valid = head_in_unit < heads;
-        // lanes behind the last head read it again, and write nothing
         const uint32_t h = h0 + min(head_in_unit, heads - 1u);
-        float x[8];
-        load_row8<TI>(k.src + h * k.nb1 + t * k.nb2 + d0 * sizeof(TI), k.vec, x);
         if (k.weight) {
             float ss = 0.0f;
 #pragma unroll
@@ -188,8 +256,9 @@ __global__ __launch_bounds__(kRowThreads) void qkv_rows_kernel(RowParams p, Thet
             }
             ss = head_sum(ss, p.head_dim);
             const float r = 1.0f / sqrtf(ss / static_cast<float>(p.head_dim) + p.eps);
-            const float4 w0 = *reinterpret_cast<const float4 *>(k.weight + d0);
-            const float4 w1 = *reinterpret_cast<const float4 *>(k.weight + d0 + 4);
+            const float *wd = weights + kd * p.head_dim + d0;
+            const float4 w0 = *reinterpret_cast<const float4 *>(wd);
+            const float4 w1 = *reinterpret_cast<const float4 *>(wd + 4);
             const float wt[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -225,7 +294,7 @@ __global__ __launch_bounds__(kRowThreads) void qkv_rows_kernel(RowParams p, Thet
             store_row8<TO>(k.out + o * sizeof(TO), x);
         }
         if (k.pool) {
-            const uint32_t cell = static_cast<uint32_t>(p.cells[t]);
+            const uint32_t cell = __builtin_amdgcn_readfirstlane(cells[tl]);
             if (cell < p.n_cells) {  // -1: the token is not kept
                 const uint32_t groups = heads * (p.head_dim / 32u);
                 const uint32_t g0 = h0 * (p.head_dim / 32u);
@@ -395,17 +464,17 @@ int kvmem_hip_qkv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_pool *pool, uint32_t 
     p.n_rot = n_rot;
     p.eps = a->eps;
     const uint32_t units = p.kind[0].units + p.kind[1].units + p.kind[2].units;
-    // tokens of a workgroup: as many as leave about 2048 workgroups; below
+    // tokens of a workgroup: as many as leave kRowGroups workgroups; below
     // that a token's units are spread over workgroups, one unit a wave
-    p.tokens = std::max(1u, std::min(kMaxRowTokens, a->n_tokens / 2048u));
+    p.tokens = std::max(1u, std::min(kMaxRowTokens, (a->n_tokens + kRowGroups - 1) / kRowGroups));
     const uint32_t groups = (a->n_tokens + p.tokens - 1) / p.tokens;
     const uint32_t most = (p.tokens * units + kRowWaves - 1) / kRowWaves;
-    p.splits = std::max(1u, std::min(most, 2048u / groups));
+    p.splits = std::max(1u, std::min(most, kRowGroups / groups));
     Theta theta;
     if (n_rot) {
         std::memcpy(theta.f, xf->theta, sizeof(float) * (n_rot / 2));
     }
-    const size_t lds = sizeof(float2) * p.tokens * (n_rot / 2);
+    const size_t lds = sizeof(float) * 2 * D + sizeof(float2) * p.tokens * (n_rot / 2);
     (void) hipSetDevice(ctx->device);
     if (injected_fail(ctx, KVMEM_HIP_FAIL_LAUNCH, "qkv_rows launch")) {
         return KVMEM_HIP_ERR_RUNTIME;
