@@ -664,11 +664,15 @@ KVMEM_HIP_API int kvmem_hip_qkv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_pool *p
  * q_start NULL: request s has token s.  A request's tokens beyond max_q or
  * n_tokens, and keys beyond max_kv or the table, are not attended (both bounds
  * size the launch; device lengths beyond them never reach out of range).
- * Scores, softmax statistics and sums are fp32.  Rounded on the way: cached
- * values to f16 once they are scaled (so values beyond f16's range become
- * infinite), and softmax weights to f16.
+ * Scores, softmax statistics and sums are fp32.  Rounded on the way, to f16:
+ * softmax weights, cached values once they are scaled (so values beyond f16's
+ * range become infinite), and in calls with many queries the scaled keys.  The
+ * dim of a value that is not finite is not finite either (NaN, or the value) in
+ * the rows that attend it, and only in those.
  * head_dim 64, 128 or 256, any n_head that is a multiple of n_head_kv; at most
- * 65535 requests, 2^23 (token, head) rows and 2^31 - 1 keys a request.
+ * 65535 requests, 2^23 (token, head) rows and 2^31 - 1 keys a request, and
+ * requests x max_q within one launch (KVMEM_HIP_ERR_INVALID otherwise: 2^24
+ * workgroups); the pool has at least one slot.
  * Keys are split over workgroups when there are few queries; the parts are
  * joined from a workspace: the caller's (kvmem_hip_attention_workspace bytes,
  * 16-byte aligned, contents free) or, where it is NULL, one the context keeps

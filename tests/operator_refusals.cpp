@@ -205,6 +205,28 @@ static void attention() {
     call("null layer", inv, [](Args &, kvmem_hip_pool &p) { p.v_layers = no_layer; });
     call("layer address", inv, [](Args &, kvmem_hip_pool &p) { p.k_layers = off_layer; });
     call("no value tensors", inv, [](Args &, kvmem_hip_pool &p) { p.v_layers = nullptr; });
+    call("pool without slots", inv, [](Args &, kvmem_hip_pool &p) { p.n_slots = 0; });
+    call("too large a launch", inv, [](Args &a, kvmem_hip_pool &) {
+        a.n_seq = 65535, a.n_tokens = a.max_q = 1u << 20;
+    });
+    // 8000 keys are split: tokens x heads x parts x (128 floats and two)
+    auto split = [](Args &a, kvmem_hip_pool &p) {
+        a.n_seq = 1, a.max_kv = 8000, a.table_stride = 64, p.n_slots = 64;
+    };
+    Args wide = ok;
+    kvmem_hip_pool slots = pool;
+    split(wide, slots);
+    const size_t need = kvmem_hip_attention_workspace(&slots, &wide);
+    if (need == 0 || need % (wide.n_tokens * 8 * (128 + 2) * sizeof(float)) != 0) {
+        std::printf("workspace of a split call: %zu bytes\n", need);
+        ++bad;
+    }
+    call("workspace too small", inv, [&](Args &a, kvmem_hip_pool &p) {
+        split(a, p), a.workspace = A, a.workspace_bytes = need - 1;
+    });
+    call("workspace address", inv, [&](Args &a, kvmem_hip_pool &p) {
+        split(a, p), a.workspace = OFF4, a.workspace_bytes = need;
+    });
     if (kvmem_hip_attention_workspace(nullptr, &ok) != 0 || kvmem_hip_attention_workspace(&pool, nullptr) != 0) {
         std::printf("workspace of a refused call is not 0\n");
         ++bad;
