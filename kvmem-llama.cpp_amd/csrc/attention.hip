@@ -143,12 +143,18 @@ static uint32_t decode_rows(uint32_t n_seq) {
 // steps for each, then two, or three with many requests, which end at different
 // places.  Measured, q4_0 with 4 KV heads of 256, 256 / 512 / 768 workgroups in us:
 //   one request: 16384 keys 17 / 21, 32768 22 / 24, 65536 32 / 32 / 43,
-//                131072 53 / 46 / 61, and with q8_0 keys 65536 57 / 50 / 67
+//                131072 53 / 46 / 61
 //   16 of 1024 keys: 17 / 19 / 19; 8 of 2048: 18 / 18 / 18
 //   8 of 8192: 32 / 29 / 27; 16 of 4096: 31 / 30 / 27; 16 of 8192: 48 / 44 / 37
 //   8 ragged ones up to 8192 with 5 tokens, q5_0, 2 KV heads of 64: 35 / 29 / 24
 //   32 ragged ones up to 16384, 8 KV heads of 128: 172 / 142 / 116 (1024: 134)
-static uint64_t decode_groups(uint32_t n_seq, uint64_t steps) {
+// Where one wave takes a SIMD, a second workgroup waits for the first:
+//   one request, q8_0 keys, q4_0 values, 65500 keys 42 / 48 / 59, q8_0 131072 75 / 85 / 100,
+//   64 ragged ones up to 2048: 60 / 69 / 69 (16 up to 8192: 64 / 70 / 58)
+static uint64_t decode_groups(uint32_t n_seq, uint64_t steps, int waves) {
+    if (waves == 1) {
+        return kComputeUnits;
+    }
     if (n_seq < 8) {
         return steps <= 4 * kComputeUnits ? kComputeUnits : 2 * kComputeUnits;
     }
@@ -183,7 +189,8 @@ static AttnPlan plan_attention(const kvmem_hip_pool *pool, const kvmem_hip_attn_
             }
         }
     } else {
-        parts = std::min(std::max<uint64_t>(1, decode_groups(a->n_seq, groups * most) / groups), most);
+        const int waves = decode_waves(pool->type_k, pool->type_v, static_cast<int>(a->head_dim));
+        parts = std::min(std::max<uint64_t>(1, decode_groups(a->n_seq, groups * most, waves) / groups), most);
     }
     uint64_t chunk = (keys + parts - 1) / parts;
     chunk = (chunk + quantum - 1) / quantum * quantum;

@@ -16,6 +16,16 @@ constexpr float kWeightShift = 6.0f;
 constexpr float kTopSlack = 9.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Waves of the decode kernel on a SIMD.  Two, but for 16- and 8-bit rows of 256:
+// their step's rows take half the registers, and one wave without spills has as
+// many bytes in flight.  Two / one, a request over 32768 keys, 4 KV heads: q8_0
+// 57 / 31 us, q8_0 keys with q4_0 values over 65500 58 / 42 us; q5_0 over 131072
+// 75 / 82 us.
+constexpr int decode_waves(int tk, int tv, int d) {
+    return d == 256 && (tk == KVMEM_TYPE_F16 || tv == KVMEM_TYPE_F16 || tk == KVMEM_TYPE_Q8_0 ||
+                        tv == KVMEM_TYPE_Q8_0) ? 1 : 2;
+}
+
 struct AttnParams {
     const uint8_t *q;
     uint64_t q_nb1, q_nb2;

@@ -168,17 +168,32 @@ __device__ inline uint32_t as_word(half2_t h) { return __builtin_bit_cast(uint32
 __device__ inline uint32_t pair_lo(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ inline uint32_t pair_hi(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
+// The same value, of which the compiler knows nothing: what is derived from it is
+// computed anew where it is used instead of being kept in registers.
+__device__ inline uint32_t anew(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// The bits of 1024 and of 64 in both halves of a word.
+struct Magic {
+    uint32_t low, high;
+};
+// Constants; in registers (decode, which has some to spare) a mask and these
+// are one instruction: nothing but one scalar register fits in it otherwise.
+constexpr Magic kMagic{0x64006400u, 0x54005400u};
+
 // f16 values of a pair of codes in bits 0..9 of each half: 1024 + n by the
 // bits of 1024, less 1024 + offset (both exact), times the scales (the one
 // rounding).
-__device__ inline uint32_t pair_value(uint32_t codes, float offset, uint32_t scales) {
+__device__ inline uint32_t pair_value(uint32_t codes, uint32_t magic, float offset, uint32_t scales) {
     const _Float16 o = static_cast<_Float16>(-(1024.0f + offset));
-    return as_word((as_half2(codes | 0x64006400u) + half2_t{o, o}) * as_half2(scales));
+    return as_word((as_half2(codes | magic) + half2_t{o, o}) * as_half2(scales));
 }
 // The same for codes in bits 4..9: 64 + n by the bits of 64.
-__device__ inline uint32_t pair_value_hi(uint32_t codes, float offset, uint32_t scales) {
+__device__ inline uint32_t pair_value_hi(uint32_t codes, uint32_t magic, float offset, uint32_t scales) {
     const _Float16 o = static_cast<_Float16>(-(64.0f + offset));
-    return as_word((as_half2(codes | 0x54005400u) + half2_t{o, o}) * as_half2(scales));
+    return as_word((as_half2(codes | magic) + half2_t{o, o}) * as_half2(scales));
 }
 
 // Value operand: lane n owns VD dims of a key's slice.  Rows
@@ -227,7 +242,7 @@ struct ValueOp<KVMEM_TYPE_Q4_0, VD> {
         }
     }
     template <class F>
-    __device__ inline void emit(const u32x4_t &keep, F f) const {
+    __device__ inline void emit(const u32x4_t &keep, const Magic &magic, F f) const {
         const u32x4_t ds{d[0] & keep[0], d[1] & keep[1], d[2] & keep[2], d[3] & keep[3]};
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
@@ -237,10 +252,10 @@ struct ValueOp<KVMEM_TYPE_Q4_0, VD> {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t t = h ? pair_hi(w[2 * j][i], w[2 * j + 1][i]) : pair_lo(w[2 * j][i], w[2 * j + 1][i]);
-                    a[0][j] = pair_value(t & 0x000F000Fu, offset, ds[j]);
-                    a[1][j] = pair_value_hi(t & 0x00F000F0u, offset, ds[j]);
-                    a[2][j] = pair_value((t >> 8) & 0x000F000Fu, offset, ds[j]);
-                    a[3][j] = pair_value_hi((t >> 8) & 0x00F000F0u, offset, ds[j]);
+                    a[0][j] = pair_value(t & 0x000F000Fu, magic.low, offset, ds[j]);
+                    a[1][j] = pair_value_hi(t & 0x00F000F0u, magic.high, offset, ds[j]);
+                    a[2][j] = pair_value((t >> 8) & 0x000F000Fu, magic.low, offset, ds[j]);
+                    a[3][j] = pair_value_hi((t >> 8) & 0x00F000F0u, magic.high, offset, ds[j]);
                 }
                 f(8 * i + 4 * h, a);
             }
@@ -285,7 +300,7 @@ struct ValueOp<KVMEM_TYPE_Q5_0, VD> {
         }
     }
     template <class F>
-    __device__ inline void emit(const u32x4_t &keep, F f) const {
+    __device__ inline void emit(const u32x4_t &keep, const Magic &magic, F f) const {
         const u32x4_t ds{d[0] & keep[0], d[1] & keep[1], d[2] & keep[2], d[3] & keep[3]};
         // the fifth bits of a key pair, in the halves of one word
         uint32_t lo[4], hi[4];
@@ -303,11 +318,11 @@ struct ValueOp<KVMEM_TYPE_Q5_0, VD> {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t t = q ? pair_hi(w[2 * j][i], w[2 * j + 1][i]) : pair_lo(w[2 * j][i], w[2 * j + 1][i]);
-                    a[0][j] = pair_value((t & 0x000F000Fu) | (((lo[j] >> b0) & 0x00010001u) << 4), offset, ds[j]);
-                    a[1][j] = pair_value_hi((t & 0x00F000F0u) | (((hi[j] >> b0) & 0x00010001u) << 8), offset, ds[j]);
-                    a[2][j] = pair_value(((t >> 8) & 0x000F000Fu) | (((lo[j] >> (b0 + 1)) & 0x00010001u) << 4), offset,
+                    a[0][j] = pair_value((t & 0x000F000Fu) | (((lo[j] >> b0) & 0x00010001u) << 4), magic.low, offset, ds[j]);
+                    a[1][j] = pair_value_hi((t & 0x00F000F0u) | (((hi[j] >> b0) & 0x00010001u) << 8), magic.high, offset, ds[j]);
+                    a[2][j] = pair_value(((t >> 8) & 0x000F000Fu) | (((lo[j] >> (b0 + 1)) & 0x00010001u) << 4), magic.low, offset,
                                       ds[j]);
-                    a[3][j] = pair_value_hi(((t >> 8) & 0x00F000F0u) | (((hi[j] >> (b0 + 1)) & 0x00010001u) << 8), offset,
+                    a[3][j] = pair_value_hi(((t >> 8) & 0x00F000F0u) | (((hi[j] >> (b0 + 1)) & 0x00010001u) << 8), magic.high, offset,
                                          ds[j]);
                 }
                 f(8 * i + 4 * q, a);
@@ -345,7 +360,7 @@ struct ValueOp<KVMEM_TYPE_Q8_0, VD> {
         }
     }
     template <class F>
-    __device__ inline void emit(const u32x4_t &keep, F f) const {
+    __device__ inline void emit(const u32x4_t &keep, const Magic &magic, F f) const {
         const u32x4_t ds{d[0] & keep[0], d[1] & keep[1], d[2] & keep[2], d[3] & keep[3]};
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
@@ -356,7 +371,7 @@ struct ValueOp<KVMEM_TYPE_Q8_0, VD> {
                 const uint32_t sel = 0x0c000c00u | static_cast<uint32_t>(b) | (static_cast<uint32_t>(4 + b) << 16);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    a[b][j] = pair_value(__builtin_amdgcn_perm(w[2 * j + 1][i], w[2 * j][i], sel), 128.0f, ds[j]);
+                    a[b][j] = pair_value(__builtin_amdgcn_perm(w[2 * j + 1][i], w[2 * j][i], sel), magic.low, 128.0f, ds[j]);
                 }
             }
             f(4 * i, a);
@@ -393,7 +408,7 @@ struct ValueOp<KVMEM_TYPE_F16, VD> {
         }
     }
     template <class F>
-    __device__ inline void emit(const u32x4_t &keep, F f) const {
+    __device__ inline void emit(const u32x4_t &keep, const Magic &magic, F f) const {
 #pragma unroll
         for (int i = 0; i < NW; i += 2) {
             u32x4_t a[4];
@@ -526,14 +541,8 @@ constexpr uint32_t decode_wave_bytes() {
 // held transposed (keys by rows) so that a lane owns one query row: S^T = K Q^T,
 // O^T = V^T P^T, and a lane's weights of S^T are its operand of the second
 // product as they stand.
-// Two waves per SIMD, but for 16-bit rows of 256: their step's rows take half the
-// registers, and one wave has as many bytes in flight.
-constexpr int decode_occupancy(int tk, int tv, int d) {
-    return d == 256 && (tk == KVMEM_TYPE_F16 || tv == KVMEM_TYPE_F16) ? 1 : 2;
-}
-
 template <int TK, int TV, int D>
-__global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, decode_waves(TK, TV, D)) void attn_decode_kernel(AttnParams p) {
     using SK = Slice<TK, D>;
     using SV = Slice<TV, D>;
     using KO = KeyOp<TK>;
@@ -752,6 +761,9 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
         o[t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
+    // where registers are to spare
+    constexpr bool kSpare = D < 256 || (TK == KVMEM_TYPE_Q4_0 && TV == KVMEM_TYPE_Q4_0);
+    const Magic magic = kSpare ? Magic{anew(kMagic.low), anew(kMagic.high)} : kMagic;
     for (; j0 < c1; j0 += step) {
         const Cells now = cells;
         bool whole = true;
@@ -918,7 +930,7 @@ __global__ __launch_bounds__(256, decode_occupancy(TK, TV, D)) void attn_decode_
             if (!whole) {  // rows of keys that do not exist are not even finite
                 keep = keep_keys<16>(static_cast<uint32_t>(now.have[h >> 1] >> (32u * (h & 1u))) >> (4u * c));
             }
-            vo.emit(keep, [&](int t0, u32x4_t *a) {
+            vo.emit(keep, magic, [&](int t0, u32x4_t *a) {
                 if (uneven && j0 + KT > n_all) {
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
@@ -1037,8 +1049,8 @@ __device__ inline u32x4_t key_values(u32x4_t codes, uint32_t scale) {
         u32x4_t r;
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
-            r[j] = KO::times(2 * j) == 1.0f ? pair_value(codes[j], KO::offset, scale)
-                                            : pair_value_hi(codes[j], KO::offset, scale);
+            r[j] = KO::times(2 * j) == 1.0f ? pair_value(codes[j], kMagic.low, KO::offset, scale)
+                                            : pair_value_hi(codes[j], kMagic.high, KO::offset, scale);
         }
         return r;
     }
@@ -1047,12 +1059,6 @@ __device__ inline u32x4_t key_values(u32x4_t codes, uint32_t scale) {
 // ------------------------------------------------------------ many queries
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
-// The same value, of which the compiler knows nothing: what is derived from it is
-// computed anew where it is used instead of being kept in registers.
-__device__ inline uint32_t anew(uint32_t x) {
-    asm volatile("" : "+v"(x));
-    return x;
-}
 typedef __attribute__((address_space(3))) void lds_void_t;
 
 template <int TK, int TV, int D>
@@ -1277,7 +1283,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) 
         const uint32_t oct = mt / (D / 4);
         const uint32_t dl = mt % (D / 4);
         const uint32_t in = static_cast<uint32_t>(have[oct >> 3] >> (16u * ((oct >> 1) & 3u) + 4u * (oct & 1u)));
-        vo.emit(keep_keys<8>(in), [&](int, u32x4_t *a) {
+        vo.emit(keep_keys<8>(in), kMagic, [&](int, u32x4_t *a) {
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 const uint32_t dim = VO::dim(dl, t);
