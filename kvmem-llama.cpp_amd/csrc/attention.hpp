@@ -16,14 +16,19 @@ constexpr float kWeightShift = 6.0f;
 constexpr float kTopSlack = 9.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Waves of the decode kernel on a SIMD.  Two, but for 16- and 8-bit rows of 256:
-// their step's rows take half the registers, and one wave without spills has as
-// many bytes in flight.  Two / one, a request over 32768 keys, 4 KV heads: q8_0
-// 57 / 31 us, q8_0 keys with q4_0 values over 65500 58 / 42 us; q5_0 over 131072
-// 75 / 82 us.
+// Waves of the decode kernel on a SIMD.  Two, but one where a step's rows, on
+// their way in registers, would make two spill: f16 or q8_0 rows of 256, f16 rows
+// of 128 beside f16 or q8_0 ones.  One has as many bytes in flight.
+// Two / one, in us, one request: q8_0, 256 wide, 32768 keys 57 / 31, q8_0 keys and
+// q4_0 values, 65500 keys 58 / 42; f16, 128 wide, 32768 keys 38 / 31.  32 ragged
+// ones up to 8192 keys, 128 wide: f16 183 / 136, q8_0 keys and f16 values 238 / 131.
+// The other way round: q5_0, 256 wide, 131072 keys 75 / 82, q8_0, 128 wide, the 32
+// 98 / 134.
 constexpr int decode_waves(int tk, int tv, int d) {
-    return d == 256 && (tk == KVMEM_TYPE_F16 || tv == KVMEM_TYPE_F16 || tk == KVMEM_TYPE_Q8_0 ||
-                        tv == KVMEM_TYPE_Q8_0) ? 1 : 2;
+    const bool wide_k = tk == KVMEM_TYPE_F16 || tk == KVMEM_TYPE_Q8_0;
+    const bool wide_v = tv == KVMEM_TYPE_F16 || tv == KVMEM_TYPE_Q8_0;
+    const bool half = tk == KVMEM_TYPE_F16 || tv == KVMEM_TYPE_F16;
+    return (d == 256 && (wide_k || wide_v)) || (d == 128 && wide_k && wide_v && half) ? 1 : 2;
 }
 
 struct AttnParams {

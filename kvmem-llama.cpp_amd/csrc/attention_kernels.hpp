@@ -1272,16 +1272,13 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) 
     // scores holds them) and its 4 dims.
     const bool for_values = NW == 4 || wave < 4u;  // with 8 waves four make values, four keys
     const bool for_keys = NW == 4 || wave >= 4u;
-    VO vo;
-    auto value_read = [&](const uint8_t *raw, uint32_t mt) {
-        const uint32_t oct = mt / (D / 4);
-        vo.raw(mt % (D / 4), [&](uint32_t e) {
-            return raw + L::raw_k + (16u * (oct >> 1) + 8u * (e >> 2) + 4u * (oct & 1u) + (e & 3u)) * SV::bytes;
-        });
-    };
-    auto value_write = [&](uint8_t *values, const uint64_t *have, uint32_t j0, uint32_t mt) {
+    auto make_values = [&](const uint8_t *raw, uint8_t *values, const uint64_t *have, uint32_t j0, uint32_t mt) {
         const uint32_t oct = mt / (D / 4);
         const uint32_t dl = mt % (D / 4);
+        VO vo;
+        vo.raw(dl, [&](uint32_t e) {
+            return raw + L::raw_k + (16u * (oct >> 1) + 8u * (e >> 2) + 4u * (oct & 1u) + (e & 3u)) * SV::bytes;
+        });
         const uint32_t in = static_cast<uint32_t>(have[oct >> 3] >> (16u * ((oct >> 1) & 3u) + 4u * (oct & 1u)));
         vo.emit(keep_keys<8>(in), kMagic, [&](int, u32x4_t *a) {
 #pragma unroll
@@ -1398,8 +1395,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) 
     }
     __syncthreads();
     if (for_values) {
-        value_read(raw0, tid & 255u);
-        value_write(values0, have, c0, tid & 255u);
+        make_values(raw0, values0, have, c0, tid & 255u);
     }
     if (for_keys) {
 #pragma unroll
@@ -1523,8 +1519,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) 
             __builtin_amdgcn_sched_barrier(0);
         }
         if (for_values) {
-            value_read(raw1, mt);
-            value_write(values1, have1, j0 + KT, mt);
+            make_values(raw1, values1, have1, j0 + KT, mt);
         }
         put_tile(raw0 + buf * L::raw);
 #pragma unroll
