@@ -571,7 +571,8 @@ KVMEM_HIP_API int kvmem_hip_score_meank(kvmem_hip_ctx *ctx, const kvmem_hip_mean
  * array is device memory, 4-byte aligned; outputs do not overlap inputs
  * (table is both).  The call is idempotent: repeated with the same inputs it
  * writes the same values. */
-typedef struct kvmem_hip_slot_map_args {
+typedef struct kvmem_hip_slot_map_args kvmem_hip_slot_map_args;
+struct kvmem_hip_slot_map_args {
     uint32_t n_seq;
     uint32_t block_tokens;
     uint32_t n_slots;          /* slots of the pool; n_slots*block_tokens < 2^31 */
@@ -590,7 +591,7 @@ typedef struct kvmem_hip_slot_map_args {
     int32_t *cells;            /* [max_tokens] */
     uint32_t *free_used_out;   /* [1] */
     uint32_t *n_missing;       /* [1] */
-} kvmem_hip_slot_map_args;
+};
 
 KVMEM_HIP_API int kvmem_hip_slot_map(kvmem_hip_ctx *ctx, const kvmem_hip_slot_map_args *args);
 
@@ -615,7 +616,8 @@ KVMEM_HIP_API int kvmem_hip_slot_map(kvmem_hip_ctx *ctx, const kvmem_hip_slot_ma
  * time.  Sums of squares are fp32; rows are fp32 until they are stored, each
  * output rounded once (nearest even).  Outputs are 16-byte aligned and do not
  * overlap inputs.  head_dim 64, 128, 256 or 512; at most 2^26 tokens. */
-typedef struct kvmem_hip_qkv_args {
+typedef struct kvmem_hip_qkv_args kvmem_hip_qkv_args;
+struct kvmem_hip_qkv_args {
     const void *q;
     const void *k;
     const void *v;
@@ -638,7 +640,7 @@ typedef struct kvmem_hip_qkv_args {
     void *k_out;
     void *q_norm;
     void *k_norm;
-} kvmem_hip_qkv_args;
+};
 
 KVMEM_HIP_API int kvmem_hip_qkv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_pool *pool, uint32_t layer,
                                      const kvmem_hip_qkv_args *args);
@@ -679,7 +681,8 @@ KVMEM_HIP_API int kvmem_hip_qkv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_pool *p
  * and grows.  A captured call must bring its own (KVMEM_HIP_ERR_INVALID
  * otherwise): graphs that can be replayed at the same time need one each.
  * Results do not depend on the order in which workgroups run. */
-typedef struct kvmem_hip_attn_args {
+typedef struct kvmem_hip_attn_args kvmem_hip_attn_args;
+struct kvmem_hip_attn_args {
     const void *q;
     int32_t q_type;            /* F16 or BF16 */
     int32_t out_type;          /* F32, F16 or BF16 */
@@ -701,7 +704,7 @@ typedef struct kvmem_hip_attn_args {
     float scale;               /* 0 = 1/sqrt(head_dim) */
     void *workspace;
     size_t workspace_bytes;
-} kvmem_hip_attn_args;
+};
 
 /* Workspace bytes of a call with these arguments (0 = none needed). */
 KVMEM_HIP_API size_t kvmem_hip_attention_workspace(const kvmem_hip_pool *pool, const kvmem_hip_attn_args *args);

@@ -35,15 +35,19 @@ def test_every_bad_call_is_refused(tmp_path):
 
 def test_argument_structs_match_the_header(tmp_path):
     kv = load_pkg()
-    src = tmp_path / "sizes.cpp"
-    src.write_text('#include "kvmem_internal.hpp"\n#include <cstdio>\nint main() { std::printf("%zu %zu %zu %zu %zu %zu", '
-                   "sizeof(kvmem_hip_slot_map_args), sizeof(kvmem_hip_qkv_args), sizeof(kvmem_hip_attn_args), "
-                   "offsetof(kvmem_hip_slot_map_args, n_missing), offsetof(kvmem_hip_qkv_args, xf), "
-                   "offsetof(kvmem_hip_attn_args, workspace)); }\n")
     if not os.path.exists(HIPCC):
         pytest.skip("hipcc is not installed")
+    structs = {"kvmem_hip_slot_map_args": kv.SlotMapArgs, "kvmem_hip_qkv_args": kv.QkvArgs,
+               "kvmem_hip_attn_args": kv.AttnArgs}
+    lines, want = [], []
+    for name, cls in structs.items():
+        lines.append(f'std::printf("%zu\\n", sizeof({name}));')
+        want.append(kv.C.sizeof(cls))
+        for field, _ in cls._fields_:
+            lines.append(f'std::printf("%zu\\n", offsetof({name}, {field}));')
+            want.append(getattr(cls, field).offset)
+    src = tmp_path / "sizes.cpp"
+    src.write_text("#include <cstddef>\n#include <cstdio>\n#include \"kvmem_hip.h\"\nint main() {\n" + "\n".join(lines)
+                   + "\n}\n")
     out = subprocess.run([str(build(tmp_path, src))], capture_output=True, text=True, timeout=120).stdout
-    C = kv.C
-    assert [int(x) for x in out.split()] == [C.sizeof(kv.SlotMapArgs), C.sizeof(kv.QkvArgs), C.sizeof(kv.AttnArgs),
-                                             kv.SlotMapArgs.n_missing.offset, kv.QkvArgs.xf.offset,
-                                             kv.AttnArgs.workspace.offset]
+    assert [int(x) for x in out.split()] == want
