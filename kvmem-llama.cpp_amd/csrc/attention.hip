@@ -8,7 +8,9 @@ namespace kvmem_hip {
 
 // ------------------------------------------------------------- joining parts
 
-// Parts up to which one wave joins a row.
+// Parts up to which one wave joins a row (many rows of few parts: 512 tokens of 24
+// heads in 5 parts, 474 us with the attention against 542 with four waves), four
+// above (few rows of many: 24 rows of 64 parts 14.8 us against 15.6 with sixteen).
 constexpr uint32_t kJoinParts = 8;
 
 // The parts of a (token, head) row, 0 where this row is not joined.
@@ -129,12 +131,15 @@ static void launch_join(hipStream_t stream, const AttnParams &p) {
 constexpr uint32_t kComputeUnits = 256;
 
 // Rows of a request (tokens x heads of a KV head) above which the prefill kernel
-// takes the call; the decode kernel reads the keys again for every 16 rows.
-// Measured, decode against prefill kernel, q4_0, 4 KV heads of 256:
-//   one request over 32768 keys:  48 rows 46 against 111 us, 72: 61/116, 96: 94/116
-//   eight over 8192:              60 rows 76 against 87 us, 96: 131/89
+// takes the call.  The decode kernel reads the keys again for every 16 rows, the
+// prefill kernel takes some 30 us before its second step.  Measured, decode against
+// prefill kernel in us, q4_0, 4 KV heads of 256:
+//   one request: 126 rows over 2048 / 8192 / 32768 keys 22 / 36 / 76 against 45 / 71 / 118,
+//                192 rows over 8192 61 against 75, 384 rows 92 against 82
+//   two over 8192, 120 rows: 50 against 71; four over 2048, 120 rows: 35 against 49
+//   eight over 8192: 60 rows 76 against 87, 96 rows 131 against 89; 96 over 2048: 49 / 49
 static uint32_t decode_rows(uint32_t n_seq) {
-    return n_seq <= 2 ? 96 : 64;
+    return std::max(64u, std::min(192u, 480u / n_seq));
 }
 
 // Workgroups a decode launch is split up to, from the steps (128 keys of 256
@@ -166,8 +171,8 @@ static AttnPlan plan_attention(const kvmem_hip_pool *pool, const kvmem_hip_attn_
     const uint32_t max_q = a->q_start ? std::min(a->max_q, a->n_tokens) : 1u;
     const uint32_t group = a->n_head / a->n_head_kv;
     const uint64_t rows = static_cast<uint64_t>(max_q) * group;
-    pl.prefill = rows <= decode_rows(a->n_seq) ? 0u : rows <= 128 ? 4u : 8u;
-    pl.row_tile = pl.prefill ? 32u * pl.prefill : kRowTile;
+    pl.prefill = rows > decode_rows(a->n_seq);
+    pl.row_tile = pl.prefill ? kPrefillRows : kRowTile;
     pl.row_tiles = static_cast<uint32_t>((rows + pl.row_tile - 1) / pl.row_tile);
     const uint32_t quantum = step_keys(a->head_dim) * (pl.prefill ? 1u : kWaves);
     const uint64_t room = static_cast<uint64_t>(a->table_stride) * pool->block_tokens;

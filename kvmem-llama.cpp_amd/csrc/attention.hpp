@@ -6,8 +6,10 @@
 
 namespace kvmem_hip {
 
-constexpr uint32_t kRowTile = 16;    // query rows of a decode workgroup
-constexpr uint32_t kWaves = 4;
+constexpr uint32_t kRowTile = 16;       // query rows of a decode workgroup
+constexpr uint32_t kPrefillWaves = 8;
+constexpr uint32_t kPrefillRows = 32 * kPrefillWaves;
+constexpr uint32_t kWaves = 4;          // of a decode workgroup
 // Softmax weights are 2^(x - top + shift) before they are rounded to f16.  A
 // row's `top` follows its maximum only when that has grown by more than
 // kTopSlack (log2), so the sums are rarely scaled down again; weights then stay
@@ -160,7 +162,7 @@ __device__ inline void rotate_lanes(float *x, uint32_t width, uint32_t lane) {
 
 // How a call is laid out on the chip.
 struct AttnPlan {
-    uint32_t prefill;          // waves of a prefill workgroup (0: decode kernel)
+    bool prefill;              // the kernel for many queries
     uint32_t row_tile, row_tiles, chunk, n_parts, units;
     uint64_t grid;
     bool joined;               // a joining kernel follows

@@ -540,7 +540,15 @@ constexpr uint32_t decode_wave_bytes() {
 // (token, head) rows, keys split over the workgroup's four waves.  Scores are
 // held transposed (keys by rows) so that a lane owns one query row: S^T = K Q^T,
 // O^T = V^T P^T, and a lane's weights of S^T are its operand of the second
-// product as they stand.
+// product as they stand.  With up to 8 rows the other 8 columns of the second
+// product take what the weights lost to f16.
+//
+// Bound for few keys by the way to them (lengths, table, rows, then the joining:
+// 9 us for a single key, 14 us for 2048), for many by vector instructions, mostly
+// values made f16: q4_0, 24/4 heads of 256, 32768 keys 22 us, 131072 46 us = 3.3
+// TB/s; f16 107 us = 5.0 TB/s; q8_0 75 us = 3.8 TB/s.  32 ragged requests up to
+// 16384 keys, 32/8 heads of 128, q4_0: 122 us = 2.6 TB/s, vector instructions 73 %
+// busy.
 template <int TK, int TV, int D>
 __global__ __launch_bounds__(256, decode_waves(TK, TV, D)) void attn_decode_kernel(AttnParams p) {
     using SK = Slice<TK, D>;
@@ -1080,15 +1088,23 @@ struct PrefillLds {
 // Where operand `dim` of an octet stands.
 __device__ inline uint32_t value_slot(uint32_t dim) { return dim + (dim >> 5); }
 
-// NW waves of 32 rows of one KV head's queries over one part of a request's keys.
+// 256 rows of one KV head's queries over one part of a request's keys, 32 a wave.
 // Steps of step_keys(D) keys: their rows come into LDS two steps ahead, are made
-// f16 one step ahead (8 keys of 4 value dims for each of 256 threads, and 4
-// octets of key dims for each of 256) between the score products of the present
-// step, and every wave multiplies its rows (transposed products as in the decode
-// kernel, on 32x32 tiles).  One barrier a step.  Two waves per SIMD cover each
-// other's LDS reads and softmax.
-template <int TK, int TV, int D, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) {
+// f16 one step ahead (8 keys of 4 value dims for each thread of four waves, and 4
+// octets of key dims for each of the others), and every wave multiplies its rows
+// (transposed products as in the decode kernel, on 32x32 tiles).  One barrier a
+// step.  Two waves per SIMD cover each other's LDS reads and softmax; 128 rows in
+// four waves take as long for 126 rows (118 and 116 us over 32768 keys) and twice
+// as long for many, since making f16 is done twice.
+//
+// Bound by the matrix units and what stands between their products.  512 tokens
+// over 32768 keys, 24/4 heads of 256, q4_0: 457-493 us = 830-896 TFLOP/s, the
+// matrix units 35 % busy, vector instructions 42 %; f16 530 us; 32/8 heads of 128:
+// f16 327 us, q8_0 364 us.  A workgroup takes about 15 us beside its steps (table,
+// first rows and queries in, sums out), which short prompts feel.
+template <int TK, int TV, int D>
+__global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(AttnParams p) {
+    constexpr uint32_t NW = kPrefillWaves;
     using SK = Slice<TK, D>;
     using SV = Slice<TV, D>;
     using KO = KeyOp<TK>;
@@ -1102,7 +1118,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) 
     constexpr uint32_t NTH = 64 * NW;
     constexpr uint32_t NK = (KT * SK::units + NTH - 1u) / NTH;
     constexpr uint32_t NV = (KT * SV::units + NTH - 1u) / NTH;
-    constexpr uint32_t kRows = 32 * NW;
+    constexpr uint32_t kRows = kPrefillRows;
     typedef typename UnitOf<SK::unit>::type UK;
     typedef typename UnitOf<SV::unit>::type UV;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -1270,8 +1286,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) 
     // Making f16 of a step's rows, in pieces.  Values: this thread's octet of
     // keys (keys 16 (q / 2) + 8 (e / 4) + 4 (q % 2) + e % 4, as a lane of the
     // scores holds them) and its 4 dims.
-    const bool for_values = NW == 4 || wave < 4u;  // with 8 waves four make values, four keys
-    const bool for_keys = NW == 4 || wave >= 4u;
+    const bool for_values = wave < 4u;  // four waves make values, four keys
+    const bool for_keys = !for_values;
     auto make_values = [&](const uint8_t *raw, uint8_t *values, const uint64_t *have, uint32_t j0, uint32_t mt) {
         const uint32_t oct = mt / (D / 4);
         const uint32_t dl = mt % (D / 4);
@@ -1577,10 +1593,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prefill_kernel(AttnParams p) 
 template <int TK, int TV, int D>
 static void launch_types(hipStream_t stream, const AttnPlan &pl, const AttnParams &p) {
     const uint32_t grid = static_cast<uint32_t>(pl.grid);
-    if (pl.prefill == 8) {
-        attn_prefill_kernel<TK, TV, D, 8><<<grid, 512, PrefillLds<TK, TV, D>::bytes, stream>>>(p);
-    } else if (pl.prefill == 4) {
-        attn_prefill_kernel<TK, TV, D, 4><<<grid, 256, PrefillLds<TK, TV, D>::bytes, stream>>>(p);
+    if (pl.prefill) {
+        attn_prefill_kernel<TK, TV, D><<<grid, 64 * kPrefillWaves, PrefillLds<TK, TV, D>::bytes, stream>>>(p);
     } else {
         const uint32_t rows = std::min(kRowTile, p.max_q * p.group);
         // 16 bytes behind the last slice: its last word is read with the next one
