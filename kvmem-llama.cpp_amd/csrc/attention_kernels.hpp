@@ -906,7 +906,8 @@ __global__ __launch_bounds__(256, decode_waves(TK, TV, D)) void attn_decode_kern
         most = fmaxf(most, lane_xor16(most));
         most = fmaxf(most, lane_xor32(most));
         if (__any(most > top + kTopSlack)) {
-            const float higher = fmaxf(top, most);
+            // each row by its own maximum: a row's sums do not depend on its neighbours
+            const float higher = most > top + kTopSlack ? most : top;
             const float fade = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
             sum *= fade;
 #pragma unroll
@@ -1498,7 +1499,8 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(Att
         most *= fac;
         most = fmaxf(most, lane_xor32(most));
         if (__any(most > top + kTopSlack)) {
-            const float higher = fmaxf(top, most);
+            // each row by its own maximum: a row's sums do not depend on its neighbours
+            const float higher = most > top + kTopSlack ? most : top;
             const float fade = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
             sum *= fade;
 #pragma unroll
