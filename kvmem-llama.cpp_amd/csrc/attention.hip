@@ -221,7 +221,8 @@ static AttnPlan plan_attention(const kvmem_hip_pool *pool, const kvmem_hip_attn_
 }
 
 bool load_attention_kernels() {
-    return load_kernel_object(&attn_join_kernel<64, 1>);
+    return load_kernel_object(&attn_join_kernel<64, 1>) && load_attention<KVMEM_TYPE_Q4_0>() &&
+           load_attention<KVMEM_TYPE_Q5_0>() && load_attention<KVMEM_TYPE_Q8_0>() && load_attention<KVMEM_TYPE_F16>();
 }
 
 static bool cache_type(int t) {

@@ -176,6 +176,13 @@ constexpr uint32_t step_keys(uint32_t d) { return 32u * (256u / d); }
 // each).
 template <int TK>
 void launch_attention(hipStream_t stream, int type_v, uint32_t head_dim, const AttnPlan &pl, const AttnParams &p);
+// Loads the unit's kernels onto the device (a first launch inside a capture must not).
+template <int TK>
+bool load_attention();
+extern template bool load_attention<KVMEM_TYPE_Q4_0>();
+extern template bool load_attention<KVMEM_TYPE_Q5_0>();
+extern template bool load_attention<KVMEM_TYPE_Q8_0>();
+extern template bool load_attention<KVMEM_TYPE_F16>();
 extern template void launch_attention<KVMEM_TYPE_Q4_0>(hipStream_t, int, uint32_t, const AttnPlan &, const AttnParams &);
 extern template void launch_attention<KVMEM_TYPE_Q5_0>(hipStream_t, int, uint32_t, const AttnPlan &, const AttnParams &);
 extern template void launch_attention<KVMEM_TYPE_Q8_0>(hipStream_t, int, uint32_t, const AttnPlan &, const AttnParams &);

@@ -1627,4 +1627,9 @@ void launch_attention(hipStream_t stream, int type_v, uint32_t d, const AttnPlan
     }
 }
 
+template <int TK>
+bool load_attention() {
+    return load_kernel_object(&attn_decode_kernel<TK, KVMEM_TYPE_Q4_0, 64>);
+}
+
 }  // namespace kvmem_hip

@@ -10,6 +10,11 @@ token's cell, or at another position, is far off), and the attention's output
 against the cached rows and the queries it was given (attention_helpers)."""
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 
@@ -209,6 +214,45 @@ def test_captured_step_follows_the_requests(ctx, oracle):
         torch.cuda.synchronize()
         b.check(oracle)
         b.advance()
+
+
+def test_first_calls_of_a_process_captured(tmp_path):
+    """The calls' first launches in a process may be captured ones: a context holds their kernels from its creation."""
+    print("[decode loop] first calls", flush=True)
+    src = tmp_path / "first.py"
+    src.write_text(FIRST)
+    root = Path(__file__).resolve().parent
+    r = subprocess.run([sys.executable, str(src)], cwd=root, capture_output=True, text=True, timeout=100,
+                       env={**os.environ, "PYTHONPATH": os.pathsep.join([str(root), str(root.parent)])})
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
+
+
+FIRST = """
+import torch
+import conftest
+from test_gpu_decode_loop import Batch, kv
+ctx = kv.Context(0)
+outs = []
+for types in (("q4_0", "q8_0"), ("q5_0", "f16"), ("q8_0", "q4_0"), ("f16", "q5_0")):
+    b = Batch(ctx, 2, 4, 2, 64, 16, 40, 20, 60, types, 64, 64, layers=1, seed=3)
+    b.feed([30, 25])
+    st = torch.cuda.Stream()
+    ws = torch.empty(1 << 22, dtype=torch.uint8, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    ctx.set_stream(st.cuda_stream)
+    with torch.cuda.graph(g, stream=st):
+        b.calls(30, 64, ws)
+    ctx.set_stream(None)
+    g.replay()
+    torch.cuda.synchronize()
+    first = b.out[0].clone()
+    b.out[0].fill_(7.25)
+    b.calls(30, 64)
+    ctx.sync()
+    assert torch.equal(b.out[0], first) and bool((first[:55] != 7.25).any())
+print("same")
+"""
 
 
 def test_new_tokens_over_the_engines_window(oracle):
