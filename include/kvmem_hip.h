@@ -663,6 +663,7 @@ KVMEM_HIP_API int kvmem_hip_qkv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_pool *p
  *           bytes, 16-byte aligned (strides too)
  *   out     contiguous [n_tokens][n_head][head_dim], 16-byte aligned
  *   lse     [n_tokens][n_head] log of the softmax's sum, or NULL
+ * out, lse and the workspace overlap no input and not one another.
  * q_start NULL: request s has token s.  A request's tokens beyond max_q or
  * n_tokens, and keys beyond max_kv or the table, are not attended (both bounds
  * size the launch; device lengths beyond them never reach out of range).
