@@ -1289,6 +1289,7 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(Att
     // scores holds them) and its 4 dims.
     const bool for_values = wave < 4u;  // four waves make values, four keys
     const bool for_keys = !for_values;
+    const bool mixed = c1 > n_all;  // some rows do not attend all the keys
     auto make_values = [&](const uint8_t *raw, uint8_t *values, const uint64_t *have, uint32_t j0, uint32_t mt) {
         const uint32_t oct = mt / (D / 4);
         const uint32_t dl = mt % (D / 4);
@@ -1301,7 +1302,7 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(Att
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 const uint32_t dim = VO::dim(dl, t);
-                if (j0 + KT > n_all) {
+                if (mixed && j0 + KT > n_all) {
                     clear_odd(a[t], first_odd + dim, [&](uint32_t e) {
                         return j0 + 16u * (oct >> 1) + 8u * (e >> 2) + 4u * (oct & 1u) + (e & 3u);
                     });
@@ -1550,7 +1551,7 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(Att
     }
 
     // a lane holds dims 32 b + 8 (i / 4) + 4 hh + i % 4 of its row
-    const bool uneven = c1 > n_all && __syncthreads_or(tid < D && first_odd[tid] != ~0u);
+    const bool uneven = mixed && __syncthreads_or(tid < D && first_odd[tid] != ~0u);
     sum += lane_xor32(sum);
     const uint32_t end_lane = anew(lane);
     const uint32_t tok = tok_of(end_lane);
