@@ -529,6 +529,35 @@ __device__ inline int query_shift(float top) {
     return ex;
 }
 
+// What brings the operands' products back to scores in log2 units: scale * log2(e) *
+// 2^e, which may pass fp32 (queries from 2^112 on, large scales) although the scores
+// do not.  Where a row's does, `more`, a power of two, is split off for all rows of
+// the wave, and 1 nearly always: x * fac * more then passes fp32 only where the score
+// does (a product is 0 or at least 2^-72, so what `more` cannot hold would be
+// infinite anyway).
+struct ScoreFactor {
+    float fac, more;
+};
+__device__ inline ScoreFactor score_factor(float scale, int e) {
+    int ex = 0;
+    const float m = frexpf(scale, &ex) * kLog2e;
+    ex += e;
+    int k = 0;
+    if (__any(ex > 126)) {
+        float most = static_cast<float>(ex);
+        most = fmaxf(most, lane_xor<1>(most));
+        most = fmaxf(most, lane_xor<2>(most));
+        most = fmaxf(most, lane_xor<4>(most));
+        most = fmaxf(most, lane_xor<8>(most));
+        most = fmaxf(most, lane_xor<16>(most));
+        most = fmaxf(most, lane_xor<32>(most));
+        k = min(__builtin_amdgcn_readfirstlane(static_cast<int>(most)) - 126, 127);
+    }
+    // (2^k from its bits: in a scalar register, as k is)
+    return {ldexpf(m, min(ex - k, 126)),
+            __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(127 + k)) << 23)};
+}
+
 // ------------------------------------------------------------ few queries
 
 template <int TK, int TV, int D>
@@ -690,7 +719,7 @@ __global__ __launch_bounds__(256, decode_waves(TK, TV, D)) void attn_decode_kern
     Slots next;
     half8_t qf[NG];
     half8_t q_off;
-    float fac;
+    float fac, more;
     {
         const uint8_t *q = p.q + static_cast<uint64_t>(r.first + my_tok) * p.q_nb2 + my_head * p.q_nb1;
         u32x4_t x[NG];
@@ -754,7 +783,9 @@ __global__ __launch_bounds__(256, decode_waves(TK, TV, D)) void attn_decode_kern
                 q_off[g] = hi * pick_hi + lo * pick_lo;
             }
         }
-        fac = ldexpf(p.scale * kLog2e, (KO::codes ? 24 : 0) - ex);
+        const ScoreFactor f = score_factor(p.scale, (KO::codes ? 24 : 0) - ex);
+        fac = f.fac;
+        more = f.more;
     }
 
     uint8_t *kt = lds + wave * decode_wave_bytes<TK, TV, D>();
@@ -880,6 +911,15 @@ __global__ __launch_bounds__(256, decode_waves(TK, TV, D)) void attn_decode_kern
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     x[a0 + i][j] = sc[i][j] * fac;
+                }
+            }
+        }
+        if (more != 1.0f) {
+#pragma unroll
+            for (uint32_t a = 0; a < NT; ++a) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    x[a][i] *= more;
                 }
             }
         }
