@@ -529,6 +529,12 @@ __device__ inline int query_shift(float top) {
     return ex;
 }
 
+// Scores (log2 units) up to which a fused product less the rounded maximum is as good
+// as the rounded product less the maximum: the rounding is at most 2^-4 there, which a
+// row's weights and their sum have in common.
+constexpr float kFarScore = 0x1p20f;
+__device__ inline bool is_far(float top) { return fabsf(top) > kFarScore && top != -INFINITY; }
+
 // What brings the operands' products back to scores in log2 units: scale * log2(e) *
 // 2^e, which may pass fp32 (queries from 2^112 on, large scales) although the scores
 // do not.  Where a row's does, `more`, a power of two, is split off for all rows of
@@ -1389,7 +1395,7 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(Att
     // token and query head of a lane's row (rows behind the last one repeat it)
     auto tok_of = [&](uint32_t l) { return (row0 + min(wave * 32u + (l & 31u), rows - 1u)) / p.group; };
     auto head_of = [&](uint32_t l) { return hk * p.group + (row0 + min(wave * 32u + (l & 31u), rows - 1u)) % p.group; };
-    float fac;
+    float fac, more;
     {
         constexpr uint32_t TURNS = NW * QS * 1024u <= 2 * (L::keys + L::values) ? 1 : 2;
         constexpr uint32_t PER = NW / TURNS;  // waves whose queries fit at a time
@@ -1424,11 +1430,14 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(Att
             }
             __syncthreads();  // the queries have left the step buffers
         }
-        fac = fmaxf(ldexpf(p.scale * kLog2e, -ex), 0x1p-126f);
+        const ScoreFactor f = score_factor(p.scale, -ex);
+        fac = fmaxf(f.fac, 0x1p-126f);
+        more = f.more;
     }
 
     float top = -INFINITY;
     float sum = 0.0f;
+    bool far = more != 1.0f;  // some row's scores have passed kFarScore (or its factor fp32)
     float16_t o[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -1538,7 +1547,7 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(Att
             }
         }
         most *= fac;
-        most = fmaxf(most, lane_xor32(most));
+        most = fmaxf(most * more, lane_xor32(most * more));
         if (__any(most > top + kTopSlack)) {
             // each row by its own maximum: a row's sums do not depend on its neighbours
             const float higher = most > top + kTopSlack ? most : top;
@@ -1549,14 +1558,32 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(Att
                 o[b] *= fade;
             }
             top = higher;
+            far = far || __any(is_far(top));
         }
         const float base = (top == -INFINITY ? 0.0f : top) - kWeightShift;
         half8_t w[2 * NT];
+        // The maximum is a rounded product.  Beyond kFarScore what its rounding took
+        // off is no longer small against a weight's exponent: products are rounded
+        // there as the maximum's was (row by row, for rows that have come so far).
+        float times = fac, less = base;
+        if (__builtin_expect(far, 0)) {
+            const float all = fac * more;
+            const bool rounded = is_far(top) || all == INFINITY;
+#pragma unroll
+            for (int a = 0; a < NT; ++a) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    sc[a][i] = rounded ? sc[a][i] * fac * more - base : __builtin_fmaf(sc[a][i], all, -base);
+                }
+            }
+            times = 1.0f;
+            less = 0.0f;
+        }
 #pragma unroll
         for (int a = 0; a < NT; ++a) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[a][i], fac, -base));
+                const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[a][i], times, -less));
                 sum += pe;
                 w[2 * a + (i >> 3)][i & 7] = static_cast<_Float16>(pe);
             }

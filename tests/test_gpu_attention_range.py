@@ -1,6 +1,7 @@
 """kvmem_hip_attention at the ends of the numbers' ranges: bf16 queries up to 2^122
 and scales that meet them (the factor that brings their scores back passes fp32,
-the scores do not).
+the scores do not), and scores so large that the rounding of a product is more than
+a weight's whole range.
 
 Where scores lie far apart one key takes a row's whole weight.  The float64 scores
 then have to say so, before the kernel's output is looked at: the best key's lead
@@ -62,7 +63,7 @@ def check_best_key(c, least=0.7):
 
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("type_k", ["q4_0", "q5_0", "q8_0", "f16"])
-@pytest.mark.parametrize("m", [1, 5])
+@pytest.mark.parametrize("m", [1, 5, 100])
 def test_queries_at_bf16s_end(ctx, oracle, m, type_k, D):
     print(f"[range] queries {type_k} {D} {m}", flush=True)
     for f, scale in ((2.0 ** 118, 0.0), (2.0 ** 115, 1.0)):
@@ -72,10 +73,44 @@ def test_queries_at_bf16s_end(ctx, oracle, m, type_k, D):
 
 
 @pytest.mark.parametrize("D", [64, 256])
-@pytest.mark.parametrize("m", [1, 5])
+@pytest.mark.parametrize("m", [1, 100])
 def test_large_scales_of_small_keys(ctx, oracle, m, D):
-    """A large scale takes the factor past fp32 ; keys of 2^-20 bring the scores back."""
+    """A large scale takes the factor past fp32 in either kernel; keys of 2^-20 bring the scores back."""
     print(f"[range] scale {D} {m}", flush=True)
     c = Case(ctx, oracle, [130, 33], [m, min(m, 33)], 4, 2, D, 32, "f16", "f16", scale=2.0 ** 17, k_scale=2.0 ** -20, seed=302)
     times(c, 2.0 ** 118)
     check_best_key(c)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("m", [1, 100])
+def test_scores_past_24_bits(ctx, oracle, m, D):
+    """Scores from 2^24 on: a step of their fp32 is more than the weights' whole range."""
+    print(f"[range] scores {D} {m}", flush=True)
+    for e in (21, 24, 28, 40, 80):
+        c = Case(ctx, oracle, [130, 33], [m, min(m, 33)], 4, 2, D, 32, "f16", "f16", seed=303)
+        times(c, 2.0 ** e)
+        check_best_key(c)
+        # split keys: the parts' maxima lie as far apart
+        c = Case(ctx, oracle, [4000], [m], 4, 2, D, 32, "q8_0", "q8_0", seed=304)
+        times(c, 2.0 ** e)
+        check_best_key(c, 0.5)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("m", [1, 100])
+def test_equal_scores_of_any_size(ctx, oracle, m, D):
+    """Keys that are all the same: each weighs 1/n whatever the score, the output is the values' mean.  Bound: the
+    values' rounding to f16 and the weight's, 2^-10 of the mean magnitude, n + 64 fp32 sums."""
+    print(f"[range] equal keys {D} {m}", flush=True)
+    for e in (0, 24, 33, 60, 100):
+        c = Case(ctx, oracle, [700], [m], 4, 2, D, 32, "q8_0", "f16", causal=False, seed=305)
+        c.pool["k"][:] = c.pool["k"][int(c.table[0, 0]) * 32]
+        c.upload()
+        times(c, 2.0 ** e)
+        j = np.arange(700)
+        rows = c.table[0, j // 32].astype(np.int64) * 32 + j % 32
+        v = decode(oracle, "f16", c.pool["v"][rows], 2 * D).reshape(700, 2, D)[:, [0, 0, 1, 1]]
+        got = c.run().out.cpu().double().numpy()
+        bound = np.abs(v).mean(0) * (2.0 ** -10 + 764 * 2.0 ** -24) + 2.0 ** -24
+        assert np.isfinite(got).all() and (np.abs(got - v.mean(0)) <= bound).all(), e
