@@ -669,9 +669,10 @@ KVMEM_HIP_API int kvmem_hip_qkv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_pool *p
  * size the launch; device lengths beyond them never reach out of range).
  * Scores, softmax statistics and sums are fp32.  Rounded on the way, to f16:
  * softmax weights, cached values once they are scaled (so values beyond f16's
- * range become infinite), and in calls with many queries the scaled keys.  The
- * dim of a value that is not finite is not finite either (NaN, or the value) in
- * the rows that attend it, and only in those.
+ * range become infinite), and in calls with many queries the scaled keys (a
+ * key that passes f16's range as a whole by a power of two: it stays finite).
+ * The dim of a value that is not finite is not finite either (NaN, or the value)
+ * in the rows that attend it, and only in those.
  * head_dim 64, 128 or 256, any n_head that is a multiple of n_head_kv; at most
  * 65535 requests, 2^23 (token, head) rows and 2^31 - 1 keys a request, and
  * requests x max_q within one launch (KVMEM_HIP_ERR_INVALID otherwise: 2^24

@@ -1095,6 +1095,13 @@ __global__ __launch_bounds__(256, decode_waves(TK, TV, D)) void attn_decode_kern
     }
 }
 
+// A group's scale with which some code passes f16 (an infinite scale too).
+template <class KO>
+__device__ inline bool beyond_f16(uint32_t scale) {
+    const _Float16 d = __builtin_bit_cast(_Float16, static_cast<uint16_t>(scale));
+    return __builtin_fabsf16(d) > static_cast<_Float16>(65504.0f / KO::offset);
+}
+
 // f16 values of a key operand's codes, scaled (rounded once).
 template <class KO>
 __device__ inline u32x4_t key_values(u32x4_t codes, uint32_t scale) {
@@ -1170,6 +1177,11 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(Att
     typedef typename UnitOf<SV::unit>::type UV;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ uint32_t first_odd[D];
+    // Of the two steps of f16 keys in LDS: the step whose key has a group beyond f16
+    // and is held times 2^-7 (its elements are then rounded to 2^-18 at the finest, far
+    // below what rounds its largest ones), and the step that has any such key.
+    __shared__ __attribute__((aligned(16))) uint32_t beyond[2][KT];
+    __shared__ uint32_t any_beyond[2];
 
     // Workgroups go to the 8 XCDs in turn.  A unit (request, part, KV head) stays on
     // one of them, whose L2 then holds its rows for all row tiles; units that do
@@ -1370,10 +1382,22 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(Att
         }
         codes = KO::load(g, o & 3u, 2u * (~(o >> 2) & 1u));
     };
-    auto key_write = [&](uint8_t *keys, uint32_t i, uint32_t mt) {
+    auto key_write = [&](uint8_t *keys, uint32_t i, uint32_t mt, uint32_t which, uint32_t j0) {
         const uint32_t u = i * 256u + mt;
         const uint32_t key = u / (D / 8);
         const uint32_t o = u % (D / 8);
+        if constexpr (KO::codes) {
+            // a key's octets are D / 8 neighbouring lanes
+            const uint64_t big = __ballot(beyond_f16<KO>(key_scale));
+            if (__builtin_expect(big != 0, 0)) {
+                const uint32_t at = anew(lane);
+                if ((big >> (at & ~(D / 8u - 1u))) & ((1ull << (D / 8)) - 1u)) {
+                    key_scale = as_word(as_half2(key_scale) * half2_t{0x1p-7f16, 0x1p-7f16});
+                    beyond[which][key] = j0;
+                    any_beyond[which] = j0;
+                }
+            }
+        }
         *reinterpret_cast<u32x4_t *>(keys + key * L::key_stride + o * 16u) = key_values<KO>(codes, key_scale);
     };
 
@@ -1449,6 +1473,14 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(Att
     if (tid < D) {
         first_odd[tid] = ~0u;
     }
+    if constexpr (KO::codes) {
+        if (tid < KT) {
+            beyond[0][tid] = beyond[1][tid] = ~0u;
+        }
+        if (tid < 2u) {
+            any_beyond[tid] = ~0u;
+        }
+    }
     put_tile(raw0);
     if constexpr (!kDirect) {
         fetch_tile(cells1, raw0 + L::raw);
@@ -1468,7 +1500,7 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(Att
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
             key_read(raw0, i, tid & 255u);
-            key_write(keys0, i, tid & 255u);
+            key_write(keys0, i, tid & 255u, 0u, c0);
         }
     }
     __syncthreads();
@@ -1492,8 +1524,12 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(Att
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
                 key_read(raw1, i, mt);
-                key_write(keys1, i, mt);
+                key_write(keys1, i, mt, buf ^ 1u, j0 + KT);
             }
+        }
+        uint32_t far_keys = 0;
+        if constexpr (KO::codes) {
+            far_keys = any_beyond[buf];
         }
         float16_t sc[NT];
         const uint8_t *kr = keys0 + buf * L::keys + nl * L::key_stride + hh * 16u;
@@ -1519,6 +1555,18 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(Att
                 ring[z & 3] = key_operand(z + 4);
             }
             __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (KO::codes) {
+            if (__builtin_expect(__builtin_amdgcn_readfirstlane(far_keys) == j0, 0)) {
+                const uint32_t *of = &beyond[buf][4 * (anew(lane) >> 5)];
+#pragma unroll
+                for (int a = 0; a < NT; ++a) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        sc[a][i] *= of[32 * a + 2 * (i & ~3) + (i & 3)] == j0 ? 0x1p7f : 1.0f;
+                    }
+                }
+            }
         }
         bool whole = j0 + KT <= n_all;
 #pragma unroll

@@ -1,7 +1,7 @@
 """kvmem_hip_attention at the ends of the numbers' ranges: bf16 queries up to 2^122
 and scales that meet them (the factor that brings their scores back passes fp32,
-the scores do not), and scores so large that the rounding of a product is more than
-a weight's whole range.
+the scores do not), scores so large that the rounding of a product is more than a
+weight's whole range, and quantized keys beyond f16.
 
 Where scores lie far apart one key takes a row's whole weight.  The float64 scores
 then have to say so, before the kernel's output is looked at: the best key's lead
@@ -114,3 +114,38 @@ def test_equal_scores_of_any_size(ctx, oracle, m, D):
         got = c.run().out.cpu().double().numpy()
         bound = np.abs(v).mean(0) * (2.0 ** -10 + 764 * 2.0 ** -24) + 2.0 ** -24
         assert np.isfinite(got).all() and (np.abs(got - v.mean(0)) <= bound).all(), e
+
+
+# largest f16 scale that keeps a code times it below f16's end: 65504 / 128, / 16, / 8
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("type_k,above", [("q8_0", [512.0, 4096.0, 65504.0]), ("q5_0", [4100.0, 65504.0]),
+                                          ("q4_0", [8192.0, 65504.0])])
+@pytest.mark.parametrize("m", [1, 100])
+def test_keys_beyond_f16(ctx, oracle, m, type_k, above, D):
+    """Quantized keys larger than f16 holds, in some groups of some keys, beside ordinary ones."""
+    print(f"[range] keys {type_k} {D} {m}", flush=True)
+    rng = np.random.default_rng(D + m)
+    gb = {"q8_0": 34, "q5_0": 22, "q4_0": 18}[type_k]
+    for scale_of in above:
+        for share in (0.01, 0.4, 1.0):
+            c = Case(ctx, oracle, [300, 77], [m, min(m, 77)], 6, 2, D, 32, type_k, "f16",
+                     scale=2.0 ** -12 / scale_of, seed=306)
+            rows = c.pool["k"].reshape(len(c.pool["k"]), -1, gb)
+            live = (rows != 0xFF).any(-1).any(-1)
+            hit = (rng.random(rows.shape[:2]) < share) & live[:, None]
+            d = np.where(rng.random(hit.sum()) < 0.5, -scale_of, scale_of).astype(np.float16)
+            rows[..., :2][hit] = d.view(np.uint8).reshape(-1, 2)
+            c.upload()
+            c.run().check()
+
+
+def test_keys_beyond_f16_in_split_calls(ctx, oracle):
+    """Parts and rotated values, 8-bit scales that stay and change from step to step."""
+    for m, had in ((2, 0), (70, 64)):
+        c = Case(ctx, oracle, [5000, 800], [m, m], 6, 2, 128, 64, "q8_0", "q8_0", scale=2.0 ** -24, hadamard=had, seed=307)
+        rows = c.pool["k"].reshape(len(c.pool["k"]), -1, 34)
+        live = np.flatnonzero((rows != 0xFF).any(-1).any(-1))
+        for r in live[::97]:
+            rows[r, r % rows.shape[1], :2] = np.array([3000.0], np.float16).view(np.uint8)
+        c.upload()
+        c.run().check()
