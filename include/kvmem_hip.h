@@ -675,8 +675,9 @@ KVMEM_HIP_API int kvmem_hip_qkv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_pool *p
  * in the rows that attend it, and only in those.
  * head_dim 64, 128 or 256, any n_head that is a multiple of n_head_kv; at most
  * 65535 requests, 2^23 (token, head) rows and 2^31 - 1 keys a request, and
- * requests x max_q within one launch (KVMEM_HIP_ERR_INVALID otherwise: 2^24
- * workgroups); the pool has at least one slot.
+ * requests x max_q within one launch (KVMEM_HIP_ERR_INVALID otherwise: fewer
+ * than 2^24 workgroups, 2^23 in calls with many queries); the pool has at least
+ * one slot.
  * Keys are split over workgroups when there are few queries; the parts are
  * joined from a workspace: the caller's (kvmem_hip_attention_workspace bytes,
  * 16-byte aligned, contents free) or, where it is NULL, one the context keeps

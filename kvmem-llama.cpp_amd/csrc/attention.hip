@@ -366,7 +366,8 @@ int kvmem_hip_attention(kvmem_hip_ctx *ctx, const kvmem_hip_pool *pool, uint32_t
     p.hadamard = pool->xf ? pool->xf->hadamard_v : 0;
     p.scale = a->scale > 0.0f ? a->scale : 1.0f / sqrtf(static_cast<float>(a->head_dim));
     const AttnPlan pl = plan_attention(pool, a);
-    if (pl.grid >= 1u << 24) {
+    // a dispatch counts its work items in 32 bits
+    if (pl.grid * (pl.prefill ? 64u * kPrefillWaves : 64u * kWaves) >= uint64_t{1} << 32) {
         return fail(ctx, KVMEM_HIP_ERR_INVALID, "attention: too many requests of max_q tokens for one launch");
     }
     p.room = static_cast<uint32_t>(std::max<uint64_t>(
@@ -411,6 +412,10 @@ int kvmem_hip_attention(kvmem_hip_ctx *ctx, const kvmem_hip_pool *pool, uint32_t
         default: launch_attention<KVMEM_TYPE_F16>(ctx->stream, pool->type_v, a->head_dim, pl, p); break;
     }
     if (pl.joined) {
+        // parts that were not written must not be joined into out
+        if (!hip_ok(ctx, hipGetLastError(), "attention launch")) {
+            return KVMEM_HIP_ERR_RUNTIME;
+        }
         if (a->head_dim == 64) {
             launch_join<64>(ctx->stream, p);
         } else if (a->head_dim == 128) {
