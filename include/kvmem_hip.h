@@ -613,8 +613,9 @@ KVMEM_HIP_API int kvmem_hip_slot_map(kvmem_hip_ctx *ctx, const kvmem_hip_slot_ma
  * stage-in also writes wants the same transform for both.
  * q, k, v (any may be NULL) are strided device views: element (d, h, t) at
  * d*size + h*nb1 + t*nb2 bytes; 16-byte aligned views are read 16 bytes at a
- * time.  Sums of squares are fp32; rows are fp32 until they are stored, each
- * output rounded once (nearest even).  Outputs are 16-byte aligned and do not
+ * time.  Sums of squares are fp32, whatever a row's magnitude (a row whose
+ * squares leave fp32's range is scaled by a power of two first); rows are fp32
+ * until they are stored, each output rounded once (nearest even).  Outputs are 16-byte aligned and do not
  * overlap inputs.  head_dim 64, 128, 256 or 512; at most 2^26 tokens. */
 typedef struct kvmem_hip_qkv_args kvmem_hip_qkv_args;
 struct kvmem_hip_qkv_args {

@@ -12,7 +12,8 @@
 // of squares and the butterflies are exchanges inside the wave, the quantizers
 // are shared with the stage-in, and a row that needs no norm gets the bytes the
 // stage-in would give it.  The sum of squares is fp32, 8 elements in order per
-// lane and then a tree over the head's lanes.
+// lane and then a tree over the head's lanes; rows whose squares leave fp32's range
+// are brought into it by a power of two.
 //
 // cos and sin of a token's rotary pairs are computed once per workgroup into
 // LDS (about 70 double-precision operations a pair).  A workgroup takes several
@@ -30,6 +31,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #pragma clang fp contract(off)
 
@@ -255,7 +257,25 @@ __global__ __launch_bounds__(kRowThreads, 8) void qkv_rows_kernel(RowParams p, T
                 ss = ss + x[i] * x[i];
             }
             ss = head_sum(ss, p.head_dim);
-            const float r = 1.0f / sqrtf(ss / static_cast<float>(p.head_dim) + p.eps);
+            float eps = p.eps;
+            // Squares that pass fp32, or fall below it where eps does not cover them: the
+            // row by a power of two first (its largest elements by 2^-80 or 2^100; the
+            // norm is the same, eps goes along).  The heads of a unit decide one by one.
+            const bool large = !(ss < INFINITY);
+            const bool small = ss < 0x1p-80f && eps < 0x1p-94f;
+            // (f16's squares do not leave it)
+            if (!std::is_same<TI, _Float16>::value && __any(large || small)) {
+                const float up = large ? 0x1p-80f : small ? 0x1p100f : 1.0f;
+                float s2 = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x[i] = x[i] * up;
+                    s2 = s2 + x[i] * x[i];
+                }
+                ss = head_sum(s2, p.head_dim);
+                eps = eps * up * up;
+            }
+            const float r = 1.0f / sqrtf(ss / static_cast<float>(p.head_dim) + eps);
             const float *wd = weights + kd * p.head_dim + d0;
             const float4 w0 = *reinterpret_cast<const float4 *>(wd);
             const float4 w1 = *reinterpret_cast<const float4 *>(wd + 4);
