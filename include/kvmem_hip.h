@@ -564,13 +564,13 @@ KVMEM_HIP_API int kvmem_hip_score_meank(kvmem_hip_ctx *ctx, const kvmem_hip_mean
  *   positions[t]  pos0[s] + i for token i of request s (pos0 NULL: kv_len[s])
  *   cells[t]      slot * block_tokens + offset, -1 where the block has no slot
  *   free_used_out entries of free_slots taken so far (free_used + the new ones)
- *   n_missing     blocks that got no slot or no entry
+ *   n_missing     blocks that got no entry, of the free list or of the table
  * positions and cells have max_tokens entries; those behind the last token are
  * 0 and -1, and tokens beyond max_tokens get none.  An entry of free_slots or
- * table at or beyond n_slots counts as no slot (it is still used up).  Every
- * array is device memory, 4-byte aligned; outputs do not overlap inputs
- * (table is both).  The call is idempotent: repeated with the same inputs it
- * writes the same values. */
+ * table at or beyond n_slots counts as no slot (one of free_slots is used up all
+ * the same, and its block is not counted in n_missing).  Every array is device
+ * memory, 4-byte aligned; outputs do not overlap inputs (table is both).  The
+ * call is idempotent: repeated with the same inputs it writes the same values. */
 typedef struct kvmem_hip_slot_map_args kvmem_hip_slot_map_args;
 struct kvmem_hip_slot_map_args {
     uint32_t n_seq;
@@ -658,8 +658,9 @@ KVMEM_HIP_API int kvmem_hip_qkv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_pool *p
  * kvmem_hip_qkv_rows applies to q as well); where the pool's transform has
  * hadamard_v, the output is rotated back to the value's own coordinates.
  * A query without any key gets zeros and lse -inf.  Rows of out and lse behind
- * the last request's tokens are left as they are, and rows of the pool that
- * hold no key are not read.
+ * the last request's tokens are left as they are.  No row of the pool that holds
+ * no key reaches a result, whatever it contains; of such rows only row 0 is read
+ * (in the place of keys that do not exist).
  *   q       strided device view, element (d, h, t) at d*2 + h*nb1 + t*nb2
  *           bytes, 16-byte aligned (strides too)
  *   out     contiguous [n_tokens][n_head][head_dim], 16-byte aligned
