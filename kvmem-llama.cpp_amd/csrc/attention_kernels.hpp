@@ -579,11 +579,15 @@ constexpr uint32_t decode_wave_bytes() {
 // product take what the weights lost to f16.
 //
 // Bound for few keys by the way to them (lengths, table, rows, then the joining:
-// 9 us for a single key, 14 us for 2048), for many by vector instructions, mostly
-// values made f16: q4_0, 24/4 heads of 256, 32768 keys 22 us, 131072 46 us = 3.3
-// TB/s; f16 107 us = 5.0 TB/s; q8_0 75 us = 3.8 TB/s.  32 ragged requests up to
-// 16384 keys, 32/8 heads of 128, q4_0: 122 us = 2.6 TB/s, vector instructions 73 %
-// busy.
+// 9 us for a single key, 14 us for 2011), for many by vector instructions, mostly
+// values made f16, and the waits between them: q4_0, 24/4 heads of 256, 32768 keys
+// 22 us (vector instructions 33 % busy), 131072 47 us = 3.2 TB/s; f16 105 us = 5.1
+// TB/s; q8_0 76 us = 3.8 TB/s.  32 ragged requests up to 16384 keys, 32/8 heads of
+// 128, q4_0: 123 us = 2.5 TB/s, vector instructions 57 % busy where a compute unit is
+// (they are for 72 % of the time: requests are cut by the longest one's keys).
+// Above 8 rows a weight is f16 alone, 2^-11 of itself: a second product for the
+// digits it lost would take as long as the first, and the values beside it are
+// rounded as much.
 template <int TK, int TV, int D>
 __global__ __launch_bounds__(256, decode_waves(TK, TV, D)) void attn_decode_kernel(AttnParams p) {
     using SK = Slice<TK, D>;
@@ -1152,10 +1156,13 @@ __device__ inline uint32_t value_slot(uint32_t dim) { return dim + (dim >> 5); }
 // as long for many, since making f16 is done twice.
 //
 // Bound by the matrix units and what stands between their products.  512 tokens
-// over 32768 keys, 24/4 heads of 256, q4_0: 457-493 us = 830-896 TFLOP/s, the
-// matrix units 35 % busy, vector instructions 42 %; f16 530 us; 32/8 heads of 128:
-// f16 327 us, q8_0 364 us.  A workgroup takes about 15 us beside its steps (table,
-// first rows and queries in, sums out), which short prompts feel.
+// over 32768 keys, 24/4 heads of 256, q4_0: 469-491 us = 835-872 TFLOP/s, the
+// matrix units 41 % busy, vector instructions 50 % (nine for each matrix
+// instruction); f16 521 us; 32/8 heads of 128: f16 328 us, q8_0 370 us.  A workgroup
+// takes about 15 us beside its steps (table, first rows and queries in, sums out),
+// which short prompts feel.  Keys and weights are f16 because the matrix units take
+// that: 2^-11 of each, which averages over a row's keys (against 64 bits this call is
+// off by 1.7e-3 in bf16, as the same arithmetic in fp32 is).
 template <int TK, int TV, int D>
 __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attn_prefill_kernel(AttnParams p) {
     constexpr uint32_t NW = kPrefillWaves;

@@ -22,9 +22,10 @@
 // weights and cells are read from LDS too: loads complete in order, so one
 // inside the loop would wait for the unit that is read ahead.
 //
-// Measured, 24 + 2 x 4 heads of 256 in bf16: 8191 tokens, with the norm, 57.5 us
-// for 268 MB (4.65 TB/s; 83 us without reading ahead and at four waves a SIMD
-// instead of eight), 96 tokens 4.4 us, one token 4.3 us (the launch).
+// Measured, 24 + 2 x 4 heads of 256 in bf16: 8191 tokens, with the norm, into F16
+// cells 56.7 us for 268 MB (4.7 TB/s, vector instructions 86 % busy; 83 us without
+// reading ahead and at four waves a SIMD instead of eight), into q8_0 cells 55 us for
+// 253 MB, rotated 65 us; 96 tokens 4.8 us, one token 4.6 us (the launch).
 #include "kvmem_internal.hpp"
 #include "row_transform.hpp"
 
@@ -43,8 +44,8 @@ constexpr uint32_t kUnit = 512;       // elements of a wave's unit
 constexpr uint32_t kMaxRot = 512;     // rotary dims, head_dim
 constexpr uint32_t kMaxRowTokens = 8; // tokens of a workgroup
 // Workgroups for many tokens: two rounds of the eight that a compute unit holds.
-// 8191 tokens of 24 + 2 x 4 heads of 256 (bf16, norm, q8_0 rows): 2048 take 61 us,
-// 4096 and 8192 57.5 us.
+// 8191 tokens of 24 + 2 x 4 heads of 256 (bf16, norm, F16 cells), 2048 / 4096 / 8192
+// workgroups: 57.7 / 54.8 / 57.3 us, rotated 62.8 / 62.5 / 66.1.
 constexpr uint32_t kRowGroups = 4096;
 
 struct Theta {
