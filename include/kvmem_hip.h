@@ -716,6 +716,195 @@ KVMEM_HIP_API size_t kvmem_hip_attention_workspace(const kvmem_hip_pool *pool, c
 KVMEM_HIP_API int kvmem_hip_attention(kvmem_hip_ctx *ctx, const kvmem_hip_pool *pool, uint32_t layer,
                                       const kvmem_hip_attn_args *args);
 
+/* ------------------------------------ recurrent layers, drafted tokens */
+
+/* What stands between the attention layers of a hybrid model, and what decides
+ * how far a step of drafted tokens advances: per recurrent layer
+ * kvmem_hip_conv_rows (its projections' short convolution) and
+ * kvmem_hip_linear_attention (attention through a state), after the last layer
+ * kvmem_hip_verify_draft.  Its n_keep says on the device how many of a request's
+ * tokens stay, and both layer calls take it as n_use: a step of drafts is first
+ * computed with state_out NULL, then its kept tokens are folded into the states
+ * with out NULL.  As for attention, lengths and slots stay in device memory and
+ * no call waits for the host.  (The reference leaves these layers to llama.cpp
+ * and folds kept tokens into their state with kernels of its patch,
+ * patches/llama-kvmem-current.patch:418-474.)
+ *
+ * Batches: token i of request s is row q_start[s] + i (q_start NULL: request s
+ * has row s).  The first n_use[s] tokens of a request take part (NULL: all);
+ * rows of the others, and rows behind the last request, are left as they are.
+ * Tokens beyond max_q or n_tokens take no part: both bounds size the launch and
+ * device lengths beyond them never reach out of range.  State of request s is
+ * entry slots[s] (NULL: s) of `state`; it goes to the same entry of state_out,
+ * which may be `state` itself, also where no token takes part.  state NULL, or a
+ * slot at or beyond n_slots: the state starts at zero (and such a slot stores
+ * nothing).  Slots of one call are distinct; entries no request names stay as
+ * they are.  Otherwise outputs overlap neither inputs nor one another. */
+
+/* Causal depthwise convolution of rows of n_channels, per token t and channel c
+ *   y = bias[c] + sum_{j<width} weight[c][j] * x[t - (width-1) + j][c]
+ *   y = y / (1 + exp(-y))                            (silu != 0)
+ *   y = y / sqrt(sum y^2 + eps)   over runs of norm_dim channels, for the first
+ *                                 norm_channels channels (queries and keys)
+ * where x before the request's first token are the width-1 rows of its state,
+ * oldest first; the new state is the last width-1 rows of both together.
+ * Sums are fp32 whatever the rows' type (a run whose squares leave fp32's range
+ * is summed in fp64; a run of zeros stays zero), each output is
+ * rounded once (nearest even), and states are the rows' own values.
+ * width 2 to 8; norm_dim 32, 64, 128, 256 or 512.  x is a strided view, element
+ * (c, t) at c*size + t*x_nb bytes; rows, states and outputs that are 16-byte
+ * aligned with n_channels a multiple of 8 are moved 16 bytes at a time. */
+typedef struct kvmem_hip_conv_args kvmem_hip_conv_args;
+struct kvmem_hip_conv_args {
+    const void *x;
+    int32_t type;              /* of x, states and out: F32, F16 or BF16 */
+    int32_t silu;
+    size_t x_nb;               /* bytes between tokens */
+    uint32_t n_tokens;         /* rows of x and out */
+    uint32_t n_seq;            /* at most 65535 */
+    uint32_t max_q;            /* most tokens of one request */
+    uint32_t n_channels;
+    uint32_t width;
+    uint32_t n_slots;
+    uint32_t norm_channels;    /* a multiple of norm_dim (0: no norm) */
+    uint32_t norm_dim;
+    const float *weight;       /* device [n_channels][width]; the last tap meets the token itself */
+    const float *bias;         /* device [n_channels] or NULL */
+    float eps;
+    uint32_t pad0;
+    const uint32_t *q_start;   /* device [n_seq + 1] or NULL */
+    const uint32_t *n_use;     /* device [n_seq] or NULL */
+    const uint32_t *slots;     /* device [n_seq] or NULL */
+    const void *state;         /* device [n_slots][width-1][n_channels] or NULL */
+    void *state_out;           /* the same, or NULL: not stored */
+    void *out;                 /* [n_tokens][n_channels], or NULL: the state alone */
+};
+
+KVMEM_HIP_API int kvmem_hip_conv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_conv_args *args);
+
+/* Linear attention through a state S [head_dim_k][head_dim_v] per request and
+ * head, for each token in order
+ *   S = exp(log_decay) S + k (x) d        d = v
+ *                                         or, with beta (the delta rule),
+ *                                         d = beta (v - exp(log_decay) S^T k)
+ *   out = scale * S^T q
+ * Query and key head of head h: h / (n_head / n_head_k).
+ *   q, k, v  strided device views, element (d, h, t) at d*size + h*nb1 + t*nb2
+ *            bytes, 16-byte aligned (strides too); q may be NULL where out is
+ *   log_decay, beta  f32, element (h, t) at h*4 + t*nb bytes: an nb of 0 is one
+ *            value per head; log_decay NULL: no decay.  -inf clears the state.
+ *   state    f32 [n_slots][n_head][head_dim_k][head_dim_v], 16-byte aligned
+ *   out      contiguous [n_tokens][n_head][head_dim_v], 16-byte aligned
+ * The state, sums and decays are fp32 or wider; out is rounded once.  Calls of
+ * few tokens a request go token by token, longer ones by chunks of tokens on
+ * the matrix cores: there the factors of every product are split into bf16
+ * parts of 24 bits together (16 bits for what reaches only a 16-bit out).
+ * A value that is not finite reaches no earlier token, and where only a v is not
+ * finite no other dim; what it reaches is not finite either (NaN, or the value).
+ * head_dim_k 64, 128 or 256, head_dim_v a multiple of 32 up to 512; at most
+ * 65535 requests and 2^26 tokens, and no more workgroups than one launch holds
+ * (KVMEM_HIP_ERR_INVALID otherwise).  Calls by chunks keep their chunks' factors
+ * in a workspace: the caller's (kvmem_hip_linear_attention_workspace bytes,
+ * 16-byte aligned, contents free) or, where it is NULL, one the context keeps
+ * and grows.  A captured call that needs one must bring its own
+ * (KVMEM_HIP_ERR_INVALID otherwise): graphs that can be replayed at the same time
+ * need one each.  Results do not depend on the order in which workgroups run. */
+typedef struct kvmem_hip_linear_args kvmem_hip_linear_args;
+struct kvmem_hip_linear_args {
+    const void *q;
+    const void *k;
+    const void *v;
+    int32_t type;              /* of q, k, v: F32, F16 or BF16 */
+    int32_t out_type;          /* F32, F16 or BF16 */
+    size_t q_nb1, q_nb2;       /* bytes between heads, between tokens */
+    size_t k_nb1, k_nb2;
+    size_t v_nb1, v_nb2;
+    uint32_t n_tokens;         /* rows of q, k, v and out */
+    uint32_t n_seq;
+    uint32_t max_q;            /* most tokens of one request */
+    uint32_t n_head_k;         /* heads of q and k */
+    uint32_t n_head;           /* heads of v, states and out: a multiple of n_head_k */
+    uint32_t head_dim_k;
+    uint32_t head_dim_v;
+    uint32_t n_slots;
+    const float *log_decay;
+    const float *beta;
+    size_t decay_nb, beta_nb;  /* bytes between tokens */
+    float scale;               /* 0 = 1/sqrt(head_dim_k) */
+    uint32_t pad0;
+    const uint32_t *q_start;   /* device [n_seq + 1] or NULL */
+    const uint32_t *n_use;     /* device [n_seq] or NULL */
+    const uint32_t *slots;     /* device [n_seq] or NULL */
+    const float *state;        /* NULL: zero */
+    float *state_out;          /* NULL: not stored */
+    void *out;                 /* NULL: the state alone */
+    void *workspace;
+    size_t workspace_bytes;
+};
+
+/* Workspace bytes of a call with these arguments (0 = none needed). */
+KVMEM_HIP_API size_t kvmem_hip_linear_attention_workspace(const kvmem_hip_linear_args *args);
+KVMEM_HIP_API int kvmem_hip_linear_attention(kvmem_hip_ctx *ctx, const kvmem_hip_linear_args *args);
+
+/* Verification of drafted tokens.  Request s has rows q_start[s] to
+ * q_start[s+1] - 1 (NULL: max_draft + 1 rows each): row r holds the step's token
+ * tokens[r] and the logits of what follows it, so the request's first token is
+ * given and the next, at most max_draft, are drafts (rows beyond max_draft + 1 or
+ * n_rows are not looked at).  With p = softmax(logits / temperature) and q the
+ * draft's distribution (probs; NULL: the draft had probability 1), in order of
+ * the rows:
+ *   draft x = tokens[r+1] stays where u_accept[r] * q_r(x) < p_r(x)
+ * and at the first that does not the next token is drawn from max(p_r - q_r, 0)
+ * (from p_r without x where probs is NULL; from p_r where that leaves nothing);
+ * where all stay it is drawn from the last row's p.  Drawn from weights w:
+ *   the lowest id whose sum_{i <= id} w_i > u_sample[s] * sum_i w_i and w_id > 0
+ *   (rounded sums that leave none: the last id with w_id > 0)
+ * Exponentials and sums are fp64, so a choice differs from the formula's only
+ * where u falls within about 1e-14 of a border.  Temperature 0 (NULL: 1), and a row with
+ * a logit of +inf: the largest logit (the lowest id of equal ones) has
+ * probability 1, whatever the draft's distribution.  NaN logits count as -inf;
+ * a row of nothing but -inf keeps no draft and gives -1.  A draft outside [0,
+ * n_vocab) does not stay.
+ *   tokens_out[s]  [max_draft + 1]: the drafts that stay, the next token, -1 behind
+ *   n_accepted[s]  drafts that stay
+ *   n_keep[s]      n_accepted + 1: the request's tokens that stay (0 without rows)
+ *   kv_len_out[s]  kv_len[s] - rows + n_keep: the keys that stay of kv_len, which
+ *                  counts all the step's tokens (both may be NULL)
+ * Rows of logits and probs are contiguous, element (v, r) at v*size + r*nb bytes,
+ * size-aligned; 16-byte aligned rows are read 16 bytes at a time.  probs are not
+ * negative; only the rows whose draft is tested, and of these the one that refuses,
+ * are read.
+ * At most 65535 requests, 127 drafts, 2^24 ids.  Parts of rows meet in a workspace
+ * (kvmem_hip_verify_draft_workspace bytes, 16-byte aligned): the rules are
+ * linear attention's. */
+typedef struct kvmem_hip_verify_args kvmem_hip_verify_args;
+struct kvmem_hip_verify_args {
+    const void *logits;
+    const void *probs;
+    int32_t type;              /* of logits: F32, F16 or BF16 */
+    int32_t probs_type;        /* F32, F16 or BF16 */
+    size_t logits_nb, probs_nb; /* bytes between rows */
+    uint32_t n_vocab;
+    uint32_t n_rows;
+    uint32_t n_seq;
+    uint32_t max_draft;
+    const uint32_t *q_start;   /* device [n_seq + 1] or NULL */
+    const int32_t *tokens;     /* device [n_rows] */
+    const float *temperature;  /* device [n_seq] or NULL */
+    const float *u_accept;     /* device [n_rows], in [0, 1) */
+    const float *u_sample;     /* device [n_seq], in [0, 1) */
+    const uint32_t *kv_len;    /* device [n_seq] or NULL */
+    int32_t *tokens_out;       /* device [n_seq][max_draft + 1] */
+    uint32_t *n_accepted;      /* device [n_seq] */
+    uint32_t *n_keep;          /* device [n_seq] or NULL */
+    uint32_t *kv_len_out;      /* device [n_seq] or NULL; may be kv_len */
+    void *workspace;
+    size_t workspace_bytes;
+};
+
+KVMEM_HIP_API size_t kvmem_hip_verify_draft_workspace(const kvmem_hip_verify_args *args);
+KVMEM_HIP_API int kvmem_hip_verify_draft(kvmem_hip_ctx *ctx, const kvmem_hip_verify_args *args);
+
 /* -------------------------------------------------------- self-check */
 
 /* Check, on this device and over every float of their ranges, the two

@@ -148,6 +148,40 @@ class AttnArgs(C.Structure):
                 ("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class ConvArgs(C.Structure):
+    """kvmem_hip_conv_args; device pointers as integers (keyword arguments)."""
+    _fields_ = [("x", C.c_void_p), ("type", C.c_int32), ("silu", C.c_int32), ("x_nb", C.c_size_t),
+                ("n_tokens", C.c_uint32), ("n_seq", C.c_uint32), ("max_q", C.c_uint32), ("n_channels", C.c_uint32),
+                ("width", C.c_uint32), ("n_slots", C.c_uint32), ("norm_channels", C.c_uint32),
+                ("norm_dim", C.c_uint32), ("weight", C.c_void_p), ("bias", C.c_void_p), ("eps", C.c_float),
+                ("pad0", C.c_uint32), ("q_start", C.c_void_p), ("n_use", C.c_void_p), ("slots", C.c_void_p),
+                ("state", C.c_void_p), ("state_out", C.c_void_p), ("out", C.c_void_p)]
+
+
+class LinearArgs(C.Structure):
+    """kvmem_hip_linear_args; device pointers as integers (keyword arguments)."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int32),
+                ("out_type", C.c_int32), ("q_nb1", C.c_size_t), ("q_nb2", C.c_size_t), ("k_nb1", C.c_size_t),
+                ("k_nb2", C.c_size_t), ("v_nb1", C.c_size_t), ("v_nb2", C.c_size_t), ("n_tokens", C.c_uint32),
+                ("n_seq", C.c_uint32), ("max_q", C.c_uint32), ("n_head_k", C.c_uint32), ("n_head", C.c_uint32),
+                ("head_dim_k", C.c_uint32), ("head_dim_v", C.c_uint32), ("n_slots", C.c_uint32),
+                ("log_decay", C.c_void_p), ("beta", C.c_void_p), ("decay_nb", C.c_size_t), ("beta_nb", C.c_size_t),
+                ("scale", C.c_float), ("pad0", C.c_uint32), ("q_start", C.c_void_p), ("n_use", C.c_void_p),
+                ("slots", C.c_void_p), ("state", C.c_void_p), ("state_out", C.c_void_p), ("out", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class VerifyArgs(C.Structure):
+    """kvmem_hip_verify_args; device pointers as integers (keyword arguments)."""
+    _fields_ = [("logits", C.c_void_p), ("probs", C.c_void_p), ("type", C.c_int32), ("probs_type", C.c_int32),
+                ("logits_nb", C.c_size_t), ("probs_nb", C.c_size_t), ("n_vocab", C.c_uint32),
+                ("n_rows", C.c_uint32), ("n_seq", C.c_uint32), ("max_draft", C.c_uint32), ("q_start", C.c_void_p),
+                ("tokens", C.c_void_p), ("temperature", C.c_void_p), ("u_accept", C.c_void_p),
+                ("u_sample", C.c_void_p), ("kv_len", C.c_void_p), ("tokens_out", C.c_void_p),
+                ("n_accepted", C.c_void_p), ("n_keep", C.c_void_p), ("kv_len_out", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 class ReserveArgs(C.Structure):
     _fields_ = [("n_layers", C.c_uint32), ("n_blocks", C.c_uint32), ("n_head", C.c_uint32),
                 ("n_head_kv", C.c_uint32), ("head_dim", C.c_uint32), ("n_q_tokens", C.c_uint32),
@@ -274,6 +308,11 @@ def load_library(path: os.PathLike | str | None = None) -> C.CDLL:
     _sig(lib, "kvmem_hip_qkv_rows", i32, vp, C.POINTER(Pool), u32, C.POINTER(QkvArgs))
     _sig(lib, "kvmem_hip_attention_workspace", sz, C.POINTER(Pool), C.POINTER(AttnArgs))
     _sig(lib, "kvmem_hip_attention", i32, vp, C.POINTER(Pool), u32, C.POINTER(AttnArgs))
+    _sig(lib, "kvmem_hip_conv_rows", i32, vp, C.POINTER(ConvArgs))
+    _sig(lib, "kvmem_hip_linear_attention_workspace", sz, C.POINTER(LinearArgs))
+    _sig(lib, "kvmem_hip_linear_attention", i32, vp, C.POINTER(LinearArgs))
+    _sig(lib, "kvmem_hip_verify_draft_workspace", sz, C.POINTER(VerifyArgs))
+    _sig(lib, "kvmem_hip_verify_draft", i32, vp, C.POINTER(VerifyArgs))
     if path is None:
         _lib = lib
     return lib
@@ -512,6 +551,27 @@ class Context:
     def attention(self, args: AttnArgs, pool: Pool, layer: int = 0) -> None:
         """Attention of new tokens over the pool's rows."""
         self.check(self.lib.kvmem_hip_attention(self.h, C.byref(pool), layer, C.byref(args)), "attention")
+
+    # -- recurrent layers and drafted tokens (argument blocks can be built once and reused)
+    def conv_rows(self, args: ConvArgs) -> None:
+        """Short causal convolution of rows with its state, SiLU, L2 norm of the first heads."""
+        self.check(self.lib.kvmem_hip_conv_rows(self.h, C.byref(args)), "conv_rows")
+
+    def linear_attention_workspace(self, args: LinearArgs) -> int:
+        """Workspace bytes of linear_attention(args) (0: none needed)."""
+        return self.lib.kvmem_hip_linear_attention_workspace(C.byref(args))
+
+    def linear_attention(self, args: LinearArgs) -> None:
+        """Attention of new tokens through their requests' decaying states."""
+        self.check(self.lib.kvmem_hip_linear_attention(self.h, C.byref(args)), "linear_attention")
+
+    def verify_draft_workspace(self, args: VerifyArgs) -> int:
+        """Workspace bytes of verify_draft(args)."""
+        return self.lib.kvmem_hip_verify_draft_workspace(C.byref(args))
+
+    def verify_draft(self, args: VerifyArgs) -> None:
+        """Which drafted tokens stay, and the next token, from given random numbers."""
+        self.check(self.lib.kvmem_hip_verify_draft(self.h, C.byref(args)), "verify_draft")
 
     # -- mean-K cosine scorer (reference semantics)
     def meank_sums(self, hist: History, block_ids, k_sum_ptr: int, mean_tokens_ptr: int) -> None:

@@ -68,6 +68,30 @@ bool ensure_dev(kvmem_hip_ctx *ctx, DevBuf &b, size_t bytes, const char *what) {
     return true;
 }
 
+int call_workspace(kvmem_hip_ctx *ctx, DevBuf &own, void *given, size_t given_bytes, size_t need, const char *call,
+                   uint8_t **out) {
+    if (given) {
+        if ((reinterpret_cast<uintptr_t>(given) & 15u) || given_bytes < need) {
+            return fail(ctx, KVMEM_HIP_ERR_INVALID,
+                        std::string(call) + ": workspace too small or not 16-byte aligned");
+        }
+        *out = static_cast<uint8_t *>(given);
+        return KVMEM_HIP_OK;
+    }
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (!hip_ok(ctx, hipStreamIsCapturing(ctx->stream, &capture), call)) {
+        return KVMEM_HIP_ERR_RUNTIME;
+    }
+    if (capture != hipStreamCaptureStatusNone) {
+        return fail(ctx, KVMEM_HIP_ERR_INVALID, std::string(call) + ": a captured call needs a workspace of its own");
+    }
+    if (!ensure_dev(ctx, own, need, call)) {
+        return KVMEM_HIP_ERR_NOMEM;
+    }
+    *out = static_cast<uint8_t *>(own.ptr);
+    return KVMEM_HIP_OK;
+}
+
 bool ensure_pin(kvmem_hip_ctx *ctx, PinBuf &b, size_t bytes, const char *what, unsigned flags) {
     if (b.ptr && b.bytes >= bytes) {
         return true;
@@ -485,6 +509,7 @@ int kvmem_hip_create(int device, kvmem_hip_ctx **out) {
         !load_ctx_kernels() || !load_meank_kernels() || !load_score_kernels() ||
         !load_stagein_kernels() || !load_topk_kernels() || !load_qwindow_kernels() ||
         !load_slot_map_kernels() || !load_qkv_rows_kernels() || !load_attention_kernels() ||
+        !load_conv_rows_kernels() || !load_linear_kernels() || !load_verify_kernels() ||
         !score_scratch_setup(ctx)) {
         kvmem_hip_destroy(ctx);
         return KVMEM_HIP_ERR_RUNTIME;
@@ -511,8 +536,8 @@ void kvmem_hip_destroy(kvmem_hip_ctx *ctx) {
         if (s.done) (void) hipEventDestroy(s.done);
     }
     for (DevBuf *b : {&ctx->score_partial, &ctx->score_layers, &ctx->meank_scratch,
-                      &ctx->move_scratch, &ctx->attn_scratch, &ctx->h2d_ring, &ctx->d2h_ring, &ctx->topk_dev,
-                      &ctx->plan}) {
+                      &ctx->move_scratch, &ctx->attn_scratch, &ctx->linear_scratch, &ctx->verify_scratch, &ctx->h2d_ring,
+                      &ctx->d2h_ring, &ctx->topk_dev, &ctx->plan}) {
         if (b->ptr) (void) hipFree(b->ptr);
     }
     if (ctx->topk_sel_host.ptr) (void) hipHostFree(ctx->topk_sel_host.ptr);
@@ -650,7 +675,8 @@ int kvmem_hip_scratch_info(const kvmem_hip_ctx *ctx, kvmem_hip_scratch *out) {
         pin += s.host.bytes;
     }
     for (const DevBuf *b : {&ctx->score_partial, &ctx->score_layers, &ctx->meank_scratch,
-                            &ctx->move_scratch, &ctx->attn_scratch, &ctx->h2d_ring, &ctx->d2h_ring}) {
+                            &ctx->move_scratch, &ctx->attn_scratch, &ctx->linear_scratch, &ctx->verify_scratch,
+                            &ctx->h2d_ring, &ctx->d2h_ring}) {
         dev += b->bytes;
     }
     pin += ctx->topk_sel_host.bytes;

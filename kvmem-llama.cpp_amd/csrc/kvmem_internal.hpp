@@ -69,6 +69,8 @@ struct kvmem_hip_ctx {
     kvmem_hip::DevBuf meank_scratch;    // mean-K scorer: layer cosines, query vectors
     kvmem_hip::DevBuf move_scratch;     // gathered slots for kvmem_hip_move_slots
     kvmem_hip::DevBuf attn_scratch;     // parts of split attention rows
+    kvmem_hip::DevBuf linear_scratch;   // chunks' factors of linear attention
+    kvmem_hip::DevBuf verify_scratch;   // parts of logits' rows
     // Selection written by the top-k kernel straight into coherent pinned
     // host memory: [n] ids, [n] count, and a completion word the kernel
     // sets to topk_epoch after the rest is visible (topk_flag_index).
@@ -157,6 +159,11 @@ bool hip_ok(kvmem_hip_ctx *ctx, hipError_t e, const char *what);
 bool injected_fail(kvmem_hip_ctx *ctx, uint32_t kind, const char *what);
 
 bool ensure_dev(kvmem_hip_ctx *ctx, DevBuf &b, size_t bytes, const char *what);
+// The workspace of a call that needs `need` bytes: the caller's, where it brings
+// one (16-byte aligned, large enough), else `own`, which grows; a captured call
+// must bring its own.  0, or the call's status with the error recorded.
+int call_workspace(kvmem_hip_ctx *ctx, DevBuf &own, void *given, size_t given_bytes, size_t need, const char *call,
+                   uint8_t **out);
 bool ensure_pin(kvmem_hip_ctx *ctx, PinBuf &b, size_t bytes, const char *what,
                 unsigned flags = hipHostMallocDefault);
 
@@ -385,6 +392,9 @@ bool load_qwindow_kernels();
 bool load_slot_map_kernels();
 bool load_qkv_rows_kernels();
 bool load_attention_kernels();
+bool load_conv_rows_kernels();
+bool load_linear_kernels();
+bool load_verify_kernels();
 // Looks up, once per device (the context's, made current by the caller),
 // the device address of the static scratch array of
 // kvmem_hip_score_noalloc and keeps it in ctx->noalloc_scratch.
