@@ -9,27 +9,9 @@
 #include <cmath>
 #include <type_traits>
 
-#include "recurrent.hpp"
+#include "linear.hpp"
 
 namespace kvmem_hip {
-
-struct LinearParams {
-    BatchArgs batch;
-    const uint8_t *q, *k, *v;
-    uint64_t q_nb1, q_nb2, k_nb1, k_nb2, v_nb1, v_nb2;
-    const uint8_t *decay, *beta;
-    uint64_t decay_nb, beta_nb;
-    const float *state;
-    float *state_out;
-    uint8_t *out;
-    int out_type;
-    uint32_t n_seq;
-    uint32_t n_head;
-    uint32_t group;   // heads of one key head
-    uint32_t dim_v;
-    uint32_t slices;  // of dim_v
-    float scale;
-};
 
 // ------------------------------------------------------------ token by token
 // A wave owns 32 columns of a head's state for all the request's tokens: lane
@@ -178,7 +160,12 @@ static void launch_step(hipStream_t stream, uint32_t dim_k, const LinearParams &
 }
 
 bool load_linear_kernels() {
-    return load_kernel_object(&linear_step_kernel<float, 64>);
+    return load_kernel_object(&linear_step_kernel<float, 64>) && load_linear_chunk_kernels();
+}
+
+// Tokens of a request, at most.
+static uint32_t most_tokens(const kvmem_hip_linear_args *a) {
+    return std::min(a->q_start ? a->max_q : std::min(a->max_q, 1u), a->n_tokens);
 }
 
 // What is wrong with a call's arguments (null: nothing), and its status.
@@ -235,7 +222,10 @@ static const char *check_linear(const kvmem_hip_linear_args *a, int &code) {
         return "linear_attention: scale must not be negative";
     }
     // a dispatch counts its work items in 32 bits
-    if (static_cast<uint64_t>(a->n_head) * (a->head_dim_v / 32) * 64 * a->n_seq >= uint64_t{1} << 32) {
+    const ChunkPlan pl = plan_chunks(a, most_tokens(a));
+    const uint64_t waves = static_cast<uint64_t>(a->n_head) * (a->head_dim_v / (pl.chunked ? pl.cols : kStepCols));
+    const uint64_t chunks = static_cast<uint64_t>(a->n_head) * pl.chunks;
+    if (std::max(waves * 64, chunks * kPrepThreads) * a->n_seq >= uint64_t{1} << 32) {
         return "linear_attention: too many requests for one launch";
     }
     code = KVMEM_HIP_OK;
@@ -249,8 +239,11 @@ using namespace kvmem_hip;
 extern "C" {
 
 size_t kvmem_hip_linear_attention_workspace(const kvmem_hip_linear_args *a) {
-    (void) a;
-    return 0;
+    int code = 0;
+    if (check_linear(a, code) || a->n_seq == 0) {
+        return 0;
+    }
+    return plan_chunks(a, most_tokens(a)).bytes;
 }
 
 int kvmem_hip_linear_attention(kvmem_hip_ctx *ctx, const kvmem_hip_linear_args *a) {
@@ -288,10 +281,20 @@ int kvmem_hip_linear_attention(kvmem_hip_ctx *ctx, const kvmem_hip_linear_args *
     p.slices = a->head_dim_v / kStepCols;
     p.scale = a->scale > 0.0f ? a->scale : 1.0f / sqrtf(static_cast<float>(a->head_dim_k));
     (void) hipSetDevice(ctx->device);
+    const ChunkPlan pl = plan_chunks(a, most_tokens(a));
+    uint8_t *ws = nullptr;
+    if (pl.chunked) {
+        if (const int rc = call_workspace(ctx, ctx->linear_scratch, a->workspace, a->workspace_bytes, pl.bytes,
+                                          "linear_attention", &ws)) {
+            return rc;
+        }
+    }
     if (injected_fail(ctx, KVMEM_HIP_FAIL_LAUNCH, "linear_attention launch")) {
         return KVMEM_HIP_ERR_RUNTIME;
     }
-    if (a->type == KVMEM_TYPE_F32) {
+    if (pl.chunked) {
+        launch_linear_chunks(ctx->stream, a->type, a->head_dim_k, pl, p, ws);
+    } else if (a->type == KVMEM_TYPE_F32) {
         launch_step<float>(ctx->stream, a->head_dim_k, p);
     } else if (a->type == KVMEM_TYPE_F16) {
         launch_step<_Float16>(ctx->stream, a->head_dim_k, p);
