@@ -609,173 +609,312 @@ __device__ inline __attribute__((always_inline)) void walk_tokens(const ChunkPar
     }
 }
 
-template <int DK, int NT, int PARTS, bool DELTA>
+template <int N>
+__device__ inline void get_frags(const uint8_t *base, uint32_t frag, half8_t (&x)[N]) {
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+        x[i] = get_frag(base, frag + i);
+    }
+}
+
+// What a chunk needs first, requested while the chunk before it is computed.
+template <int NT, int PARTS, int KEYS> struct ChunkRows {
+    half8_t k[KEYS];                       // operands of K (delta rule)
+    uint32_t v[NT][16];                    // values as they lie in memory, rows 16 m + 4 g + r
+    uint32_t by_token;
+};
+
+struct ChunkGates {
+    f32x4_t first[4], last[4];  // e^G, e^(G_last - G) of rows 16 m + 4 g + r
+    float out_first[4];         // e^G of rows 16 m + lane % 16
+    float whole;
+    int exp_k, exp_q, exp_t, exp_p;
+};
+
+template <int DK, int NT, int PARTS, bool DELTA, bool FINE>
 __global__ __launch_bounds__(64, 1) void linear_walk_kernel(const ChunkParams p) {
     constexpr int KS = DK / 32, TILES = DK / 16;
+    // operands of a matrix of keys: all parts requested ahead where registers hold them
+    constexpr bool AHEAD = DK * PARTS <= 128;
+    constexpr bool LATE = DK * PARTS >= 256;  // K^T only once K's registers are free
+    constexpr int KEYS = AHEAD && DELTA ? 4 * KS * PARTS : 1;
+    constexpr int ROWS = AHEAD ? 4 * KS * PARTS : 1;
+    typedef ChunkRows<NT, PARTS, KEYS> Rows;
     const uint32_t lane = threadIdx.x, g = lane >> 4;
     const uint32_t slices = p.a.dim_v / (16u * NT);
     const uint32_t h = blockIdx.x / slices, s_id = blockIdx.y;
     const uint32_t col = (blockIdx.x % slices) * (16u * NT) + (lane & 15u);
     const uint32_t hk = h / p.a.group;
-    const Request rq = request_of(p.a.batch, s_id);
+    Request rq = request_of(p.a.batch, s_id);
+    rq.first = __builtin_amdgcn_readfirstlane(rq.first);
+    rq.count = __builtin_amdgcn_readfirstlane(rq.count);
     const uint64_t at = (static_cast<uint64_t>(rq.slot) * p.a.n_head + h) * DK * p.a.dim_v + col;
+    const uint64_t entry0 = entry_of(rq, s_id, 0);
+    const uint64_t key_step = p.key_bytes * (p.a.n_head / p.a.group), head_step = p.head_bytes * p.a.n_head;
+    const uint8_t *keys = p.keys + entry0 * key_step + hk * p.key_bytes;
+    const uint8_t *head = p.heads + entry0 * head_step + h * p.head_bytes;
+    const uint8_t *values = p.a.v + rq.first * p.a.v_nb2 + h * p.a.v_nb1;
+
+    // operand i of K (at 0), Q (4 KS) or K^T (8 KS), its first or second part
+    auto frag_index = [](uint32_t matrix, uint32_t i, uint32_t part) { return part * 12u * KS + matrix + i; };
+    auto request_rows = [&](uint32_t c, Rows &x) {
+        const uint8_t *kp = keys + c * key_step;
+        const ChunkHead *ch = reinterpret_cast<const ChunkHead *>(head + c * head_step);
+        const uint32_t n = min(kChunk, rq.count - c * kChunk);
+        x.by_token = ch->by_token;
+        if constexpr (AHEAD && DELTA) {
+#pragma unroll
+            for (uint32_t part = 0; part < PARTS; ++part) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4 * KS; ++i) {
+                    x.k[part * 4 * KS + i] = get_frag(kp, frag_index(0, i, part));
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < NT; ++j) {
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) {
+                const uint32_t row = 16u * (i >> 2) + 4u * g + (i & 3u);
+                const uint8_t *to = values + static_cast<uint64_t>(c * kChunk + min(row, n - 1u)) * p.a.v_nb2;
+                if constexpr (PARTS == 2) {
+                    x.v[j][i] = reinterpret_cast<const uint32_t *>(to)[col + 16u * j];
+                } else {
+                    x.v[j][i] = reinterpret_cast<const uint16_t *>(to)[col + 16u * j];
+                }
+            }
+        }
+    };
+
     f32x4_t s[NT][TILES];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
         for (int d = 0; d < TILES; ++d) {
-#pragma unroll
-            for (uint32_t r = 0; r < 4; ++r) {
-                s[j][d][r] = p.a.state && rq.has_slot
-                                 ? p.a.state[at + static_cast<uint64_t>(16u * d + 4u * g + r) * p.a.dim_v + 16u * j]
-                                 : 0.0f;
-            }
+            s[j][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
-    const bool fine = p.p_parts == 2;  // the output takes both parts
-    for (uint32_t c = 0; c * kChunk < rq.count; ++c) {
-        const uint32_t n = min(kChunk, rq.count - c * kChunk);
-        const uint64_t row0 = static_cast<uint64_t>(rq.first) + c * kChunk;
-        const uint64_t entry = entry_of(rq, s_id, c);
-        const uint8_t *keys = p.keys + (entry * (p.a.n_head / p.a.group) + hk) * p.key_bytes;
-        const uint8_t *head = p.heads + (entry * p.a.n_head + h) * p.head_bytes;
-        const ChunkHead *ch = reinterpret_cast<const ChunkHead *>(head);
-        const uint8_t *frag_t = head + kHeadBytes;
-        const uint8_t *frag_p = frag_t + (DELTA ? 2u * kLowerFrags * kFragBytes : 0u);
-        // the chunk's values, rows 16 m + 4 g + r
-        f32x4_t v[NT][4];
-        uint32_t odd = ch->by_token;
+    if (p.a.state && rq.has_slot) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
+            for (int d = 0; d < TILES; ++d) {
 #pragma unroll
                 for (uint32_t r = 0; r < 4; ++r) {
-                    const uint32_t i = 16u * m + 4u * g + r;
-                    v[j][m][r] = i < n ? load_one(p.a.v + (row0 + i) * p.a.v_nb2 + h * p.a.v_nb1, p.type, col + 16u * j)
-                                       : 0.0f;
-                    odd |= mag(v[j][m][r]) >= kInf;
+                    s[j][d][r] =
+                        p.a.state[at + static_cast<uint64_t>(16u * d + 4u * g + r) * p.a.dim_v + 16u * j];
                 }
+            }
+        }
+    }
+    const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    Rows next;
+    if (rq.count) {
+        request_rows(0, next);
+    }
+    for (uint32_t c = 0; c * kChunk < rq.count; ++c) {
+        const Rows x = next;
+        const uint32_t n = min(kChunk, rq.count - c * kChunk);
+        const uint64_t row0 = static_cast<uint64_t>(rq.first) + c * kChunk;
+        const uint8_t *kp = keys + c * key_step;
+        const uint8_t *frag_t = head + c * head_step + kHeadBytes;
+        const uint8_t *frag_p = frag_t + (DELTA ? 2u * kLowerFrags * kFragBytes : 0u);
+        half8_t qf[ROWS], tf[DELTA ? 2 * kLowerFrags : 1], pf[(FINE ? 2 : 1) * kLowerFrags], kt[ROWS];
+        if constexpr (AHEAD) {
+            if (p.outs) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4 * KS * PARTS; ++i) {
+                    qf[i] = get_frag(kp, frag_index(4 * KS, i % (4 * KS), i / (4 * KS)));
+                }
+            }
+        }
+        ChunkGates z;
+        const ChunkHead *ch = reinterpret_cast<const ChunkHead *>(head + c * head_step);
+#pragma unroll
+        for (uint32_t m = 0; m < 4; ++m) {
+            z.first[m] = *reinterpret_cast<const f32x4_t *>(ch->from_first + 16u * m + 4u * g);
+            z.last[m] = *reinterpret_cast<const f32x4_t *>(ch->to_last + 16u * m + 4u * g);
+            z.out_first[m] = ch->from_first[16u * m + (lane & 15u)];
+        }
+        z.exp_k = ch->exp_k, z.exp_q = ch->exp_q, z.exp_t = ch->exp_t, z.exp_p = ch->exp_p;
+        z.whole = ch->from_first[kChunk - 1];
+        if constexpr (DELTA) {
+            get_frags(frag_t, 0, tf);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4_t v[NT][4];
+        uint32_t odd = x.by_token;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) {
+                const uint32_t w = x.v[j][i];
+                const float f = PARTS == 2 ? __uint_as_float(w)
+                                : p.type == KVMEM_TYPE_F16
+                                    ? static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w)))
+                                    : __uint_as_float(w << 16);
+                v[j][i >> 2][i & 3u] = 16u * (i >> 2) + 4u * g + (i & 3u) < n ? f : 0.0f;
+                odd |= mag(v[j][i >> 2][i & 3u]) >= kInf;
             }
         }
         if (__builtin_expect(__any(odd), 0)) {
             walk_tokens<DK, NT>(p, s, row0, n, h, hk, col);
+            if ((c + 1) * kChunk < rq.count) {
+                request_rows(c + 1, next);
+            }
             continue;
         }
-        f32x4_t first[4], last[4];
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            first[m] = *reinterpret_cast<const f32x4_t *>(ch->from_first + 16u * m + 4u * g);
-            last[m] = *reinterpret_cast<const f32x4_t *>(ch->to_last + 16u * m + 4u * g);
-        }
-        const float whole = ch->from_first[kChunk - 1];
-        const int exp_k = ch->exp_k;
+        half8_t hi[NT][KS], lo[NT][KS];
+        int exp_s[NT];
+        f32x4_t d[NT][4], o[NT][4];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            half8_t hi[KS], lo[KS];
-            const int exp_s = split<TILES>(s[j], hi, lo);
-            const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-            f32x4_t o[4] = {zero, zero, zero, zero};
-            if (p.outs) {  // transposed: columns of the state are rows of the accumulator
+            exp_s[j] = split<TILES>(s[j], hi[j], lo[j]);
+            if constexpr (DELTA) {
+#pragma unroll
+                for (uint32_t m = 0; m < 4; ++m) {
+                    d[j][m] = zero;
+                }
 #pragma unroll
                 for (uint32_t k = 0; k < KS; ++k) {
 #pragma unroll
                     for (uint32_t m = 0; m < 4; ++m) {
-                        const half8_t q = get_frag(keys, 4u * KS + m * KS + k);
-                        o[m] = KVMEM_MFMA16(hi[k], q, o[m]);
-                        if (fine) {
-                            o[m] = KVMEM_MFMA16(lo[k], q, o[m]);
+                        const uint32_t i = m * KS + k;
+                        const half8_t a = AHEAD ? x.k[AHEAD ? i : 0] : get_frag(kp, frag_index(0, i, 0));
+                        d[j][m] = KVMEM_MFMA16(a, hi[j][k], d[j][m]);
+                        d[j][m] = KVMEM_MFMA16(a, lo[j][k], d[j][m]);
+                        if constexpr (PARTS == 2) {
+                            const half8_t b =
+                                AHEAD ? x.k[AHEAD ? 4 * KS + i : 0] : get_frag(kp, frag_index(0, i, 1));
+                            d[j][m] = KVMEM_MFMA16(b, hi[j][k], d[j][m]);
+                        }
+                    }
+                }
+            }
+        }
+        if (p.outs) {
+            get_frags(frag_p, 0, pf);
+        }
+        if constexpr (AHEAD && !LATE) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4 * KS * PARTS; ++i) {
+                kt[i] = get_frag(kp, frag_index(8 * KS, i % (4 * KS), i / (4 * KS)));
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (p.outs) {  // transposed: columns of the state are rows of the accumulator
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                for (uint32_t m = 0; m < 4; ++m) {
+                    o[j][m] = zero;
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < KS; ++k) {
+#pragma unroll
+                    for (uint32_t m = 0; m < 4; ++m) {
+                        const uint32_t i = m * KS + k;
+                        const half8_t a = AHEAD ? qf[AHEAD ? i : 0] : get_frag(kp, frag_index(4 * KS, i, 0));
+                        o[j][m] = KVMEM_MFMA16(hi[j][k], a, o[j][m]);
+                        if constexpr (FINE) {
+                            o[j][m] = KVMEM_MFMA16(lo[j][k], a, o[j][m]);
                             if constexpr (PARTS == 2) {
-                                o[m] = KVMEM_MFMA16(hi[k], get_frag(keys, 16u * KS + m * KS + k), o[m]);
+                                const half8_t b =
+                                    AHEAD ? qf[AHEAD ? 4 * KS + i : 0] : get_frag(kp, frag_index(4 * KS, i, 1));
+                                o[j][m] = KVMEM_MFMA16(hi[j][k], b, o[j][m]);
                             }
                         }
                     }
                 }
             }
-            f32x4_t d[4];
-            if constexpr (DELTA) {
-                f32x4_t ks[4] = {zero, zero, zero, zero};
+        }
+        if constexpr (DELTA) {
 #pragma unroll
-                for (uint32_t k = 0; k < KS; ++k) {
-#pragma unroll
-                    for (uint32_t m = 0; m < 4; ++m) {
-                        const half8_t kf = get_frag(keys, m * KS + k);
-                        ks[m] = KVMEM_MFMA16(kf, hi[k], ks[m]);
-                        ks[m] = KVMEM_MFMA16(kf, lo[k], ks[m]);
-                        if constexpr (PARTS == 2) {
-                            ks[m] = KVMEM_MFMA16(get_frag(keys, 12u * KS + m * KS + k), hi[k], ks[m]);
-                        }
-                    }
-                }
+            for (int j = 0; j < NT; ++j) {
                 f32x4_t rest[4];
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        rest[m][r] =
-                            __builtin_fmaf(-first[m][r], __builtin_amdgcn_ldexpf(ks[m][r], exp_k + exp_s), v[j][m][r]);
+                        rest[m][r] = __builtin_fmaf(
+                            -z.first[m][r], __builtin_amdgcn_ldexpf(d[j][m][r], z.exp_k + exp_s[j]), v[j][m][r]);
                     }
                 }
                 half8_t rh[2], rl[2];
-                const int exp_r = split<4>(rest, rh, rl);
+                const int e = z.exp_t + split<4>(rest, rh, rl);
 #pragma unroll
                 for (uint32_t m = 0; m < 4; ++m) {
-                    d[m] = zero;
+                    d[j][m] = zero;
 #pragma unroll
                     for (uint32_t k = 0; k <= m / 2; ++k) {
-                        const half8_t th = get_frag(frag_t, lower_frag(m, k));
-                        const half8_t tl = get_frag(frag_t, kLowerFrags + lower_frag(m, k));
-                        d[m] = KVMEM_MFMA16(th, rh[k], d[m]);
-                        d[m] = KVMEM_MFMA16(th, rl[k], d[m]);
-                        d[m] = KVMEM_MFMA16(tl, rh[k], d[m]);
+                        const uint32_t f = lower_frag(m, k);
+                        d[j][m] = KVMEM_MFMA16(tf[f], rh[k], d[j][m]);
+                        d[j][m] = KVMEM_MFMA16(tf[f], rl[k], d[j][m]);
+                        d[j][m] = KVMEM_MFMA16(tf[kLowerFrags + f], rh[k], d[j][m]);
                     }
                 }
-                const int e = ch->exp_t + exp_r;
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        d[m][r] = __builtin_amdgcn_ldexpf(d[m][r], e);
+                        d[j][m][r] = __builtin_amdgcn_ldexpf(d[j][m][r], e);
                     }
                 }
-            } else {
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
-                    d[m] = v[j][m];
+                    d[j][m] = v[j][m];
                 }
             }
-            half8_t dh[2], dl[2];
-            if (p.outs) {
-                const int exp_d = split<4>(d, dh, dl);
+        }
+        if constexpr (AHEAD && LATE) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4 * KS * PARTS; ++i) {
+                kt[i] = get_frag(kp, frag_index(8 * KS, i % (4 * KS), i / (4 * KS)));
+            }
+        }
+        if constexpr (!LATE) {
+            if ((c + 1) * kChunk < rq.count) {
+                request_rows(c + 1, next);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (p.outs) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                half8_t dh[2], dl[2];
+                const int exp_d = split<4>(d[j], dh, dl);
                 f32x4_t pd[4];
 #pragma unroll
                 for (uint32_t m = 0; m < 4; ++m) {
                     pd[m] = zero;
 #pragma unroll
                     for (uint32_t k = 0; k <= m / 2; ++k) {
-                        const half8_t ph = get_frag(frag_p, lower_frag(m, k));
-                        pd[m] = KVMEM_MFMA16(dh[k], ph, pd[m]);
-                        if (fine) {
-                            pd[m] = KVMEM_MFMA16(dl[k], ph, pd[m]);
-                            pd[m] = KVMEM_MFMA16(dh[k], get_frag(frag_p, kLowerFrags + lower_frag(m, k)), pd[m]);
+                        const uint32_t f = lower_frag(m, k);
+                        pd[m] = KVMEM_MFMA16(dh[k], pf[f], pd[m]);
+                        if constexpr (FINE) {
+                            pd[m] = KVMEM_MFMA16(dl[k], pf[f], pd[m]);
+                            pd[m] = KVMEM_MFMA16(dh[k], pf[kLowerFrags + f], pd[m]);
                         }
                     }
                 }
                 int es[4], ed[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    es[r] = __shfl(exp_s, static_cast<int>(4u * g) + r, 64) + ch->exp_q;
-                    ed[r] = __shfl(exp_d, static_cast<int>(4u * g) + r, 64) + ch->exp_p;
+                    es[r] = __shfl(exp_s[j], static_cast<int>(4u * g) + r, 64) + z.exp_q;
+                    ed[r] = __shfl(exp_d, static_cast<int>(4u * g) + r, 64) + z.exp_p;
                 }
                 const uint32_t dv = col - (lane & 15u) + 16u * j + 4u * g;
 #pragma unroll
                 for (uint32_t m = 0; m < 4; ++m) {
                     const uint32_t i = 16u * m + (lane & 15u);
-                    const float f = ch->from_first[i];
                     float y[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        y[r] = p.a.scale * __builtin_fmaf(f, __builtin_amdgcn_ldexpf(o[m][r], es[r]),
+                        y[r] = p.a.scale * __builtin_fmaf(z.out_first[m], __builtin_amdgcn_ldexpf(o[j][m][r], es[r]),
                                                           __builtin_amdgcn_ldexpf(pd[m][r], ed[r]));
                     }
                     if (i < n) {
@@ -790,27 +929,38 @@ __global__ __launch_bounds__(64, 1) void linear_walk_kernel(const ChunkParams p)
                     }
                 }
             }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                d[m] *= last[m];
+                d[j][m] *= z.last[m];
             }
-            const int exp_d = split<4>(d, dh, dl) + exp_k;
+            half8_t dh[2], dl[2];
+            const int e = split<4>(d[j], dh, dl) + z.exp_k;
 #pragma unroll
             for (uint32_t t = 0; t < TILES; ++t) {
-                f32x4_t x = zero;
+                f32x4_t y = zero;
 #pragma unroll
                 for (uint32_t k = 0; k < 2; ++k) {
-                    const half8_t kt = get_frag(keys, 8u * KS + 2u * t + k);
-                    x = KVMEM_MFMA16(kt, dh[k], x);
-                    x = KVMEM_MFMA16(kt, dl[k], x);
+                    const uint32_t i = 2u * t + k;
+                    const half8_t a = AHEAD ? kt[AHEAD ? i : 0] : get_frag(kp, frag_index(8 * KS, i, 0));
+                    y = KVMEM_MFMA16(a, dh[k], y);
+                    y = KVMEM_MFMA16(a, dl[k], y);
                     if constexpr (PARTS == 2) {
-                        x = KVMEM_MFMA16(get_frag(keys, 20u * KS + 2u * t + k), dh[k], x);
+                        const half8_t b = AHEAD ? kt[AHEAD ? 4 * KS + i : 0] : get_frag(kp, frag_index(8 * KS, i, 1));
+                        y = KVMEM_MFMA16(b, dh[k], y);
                     }
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s[j][t][r] = __builtin_fmaf(whole, s[j][t][r], __builtin_amdgcn_ldexpf(x[r], exp_d));
+                    s[j][t][r] = __builtin_fmaf(z.whole, s[j][t][r], __builtin_amdgcn_ldexpf(y[r], e));
                 }
+            }
+        }
+        if constexpr (LATE) {
+            if ((c + 1) * kChunk < rq.count) {
+                request_rows(c + 1, next);
             }
         }
     }
@@ -836,10 +986,13 @@ static void prepare(hipStream_t stream, const ChunkParams &p) {
 template <int DK, int NT, int PARTS>
 static void walk(hipStream_t stream, const ChunkParams &p) {
     const dim3 grid(p.a.n_head * (p.a.dim_v / (16u * NT)), p.a.n_seq);
+    const bool fine = p.p_parts == 2;  // the output takes both parts
     if (p.delta) {
-        linear_walk_kernel<DK, NT, PARTS, true><<<grid, 64, 0, stream>>>(p);
+        fine ? linear_walk_kernel<DK, NT, PARTS, true, true><<<grid, 64, 0, stream>>>(p)
+             : linear_walk_kernel<DK, NT, PARTS, true, false><<<grid, 64, 0, stream>>>(p);
     } else {
-        linear_walk_kernel<DK, NT, PARTS, false><<<grid, 64, 0, stream>>>(p);
+        fine ? linear_walk_kernel<DK, NT, PARTS, false, true><<<grid, 64, 0, stream>>>(p)
+             : linear_walk_kernel<DK, NT, PARTS, false, false><<<grid, 64, 0, stream>>>(p);
     }
 }
 
@@ -856,9 +1009,9 @@ static void launch(hipStream_t stream, const ChunkParams &p) {
         return;  // factors that were not written must not be read
     }
     if (p.type == KVMEM_TYPE_F32) {
-        p.cols == 16 ? walk<DK, 1, 2>(stream, p) : walk<DK, 2, 2>(stream, p);
+        walk<DK, 1, 2>(stream, p);
     } else {
-        p.cols == 16 ? walk<DK, 1, 1>(stream, p) : walk<DK, 2, 1>(stream, p);
+        walk<DK, 1, 1>(stream, p);
     }
 }
 
