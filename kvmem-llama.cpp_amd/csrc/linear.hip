@@ -160,7 +160,47 @@ static void launch_step(hipStream_t stream, uint32_t dim_k, const LinearParams &
 }
 
 bool load_linear_kernels() {
-    return load_kernel_object(&linear_step_kernel<float, 64>) && load_linear_chunk_kernels();
+    return load_kernel_object(&linear_step_kernel<float, 64>) && load_linear_chunks_f32() &&
+           load_linear_chunks_f16() && load_linear_chunks_bf16();
+}
+
+static ChunkPlan plan_chunks(const kvmem_hip_linear_args *a, uint32_t max_q) {
+    ChunkPlan pl;
+    if (max_q < kChunkFrom) {
+        return pl;
+    }
+    pl.chunked = true;
+    const uint32_t parts = a->type == KVMEM_TYPE_F32 ? 2 : 1;
+    pl.p_parts = !a->out ? 1 : a->out_type == KVMEM_TYPE_BF16 ? 1 : 2;
+    pl.chunks = (max_q + kChunk - 1) / kChunk;
+    pl.entries = a->n_tokens / kChunk + a->n_seq + 1;
+    pl.key_bytes = static_cast<uint64_t>(parts) * 12 * (a->head_dim_k / 32) * kFragBytes;
+    pl.head_bytes = kHeadBytes + ((a->beta ? 2 : 0) + pl.p_parts) * kLowerFrags * kFragBytes;
+    pl.bytes = pl.entries * (pl.key_bytes * a->n_head_k + pl.head_bytes * a->n_head);
+    return pl;
+}
+
+static void launch_linear_chunks(hipStream_t stream, int type, uint32_t dim_k, const ChunkPlan &pl,
+                                 const LinearParams &a, uint8_t *workspace) {
+    ChunkParams p{};
+    p.a = a;
+    p.keys = workspace;
+    p.heads = workspace + pl.entries * pl.key_bytes * (a.n_head / a.group);
+    p.key_bytes = pl.key_bytes;
+    p.head_bytes = pl.head_bytes;
+    p.chunks = pl.chunks;
+    p.type = type;
+    p.dim_k = dim_k;
+    p.delta = a.beta != nullptr;
+    p.outs = a.out != nullptr;
+    p.p_parts = static_cast<uint32_t>(pl.p_parts);
+    if (type == KVMEM_TYPE_F32) {
+        launch_linear_chunks_f32(stream, p);
+    } else if (type == KVMEM_TYPE_F16) {
+        launch_linear_chunks_f16(stream, p);
+    } else {
+        launch_linear_chunks_bf16(stream, p);
+    }
 }
 
 // Tokens of a request, at most.
@@ -223,9 +263,10 @@ static const char *check_linear(const kvmem_hip_linear_args *a, int &code) {
     }
     // a dispatch counts its work items in 32 bits
     const ChunkPlan pl = plan_chunks(a, most_tokens(a));
-    const uint64_t waves = static_cast<uint64_t>(a->n_head) * (a->head_dim_v / (pl.chunked ? pl.cols : kStepCols));
+    const uint64_t waves = static_cast<uint64_t>(a->n_head) * 
+                               ((a->head_dim_v + 31) / 32) + kXcds;
     const uint64_t chunks = static_cast<uint64_t>(a->n_head) * pl.chunks;
-    if (std::max(waves * 64, chunks * kPrepThreads) * a->n_seq >= uint64_t{1} << 32) {
+    if (std::max(waves * 256, chunks * kPrepThreads) * a->n_seq >= uint64_t{1} << 32) {
         return "linear_attention: too many requests for one launch";
     }
     code = KVMEM_HIP_OK;

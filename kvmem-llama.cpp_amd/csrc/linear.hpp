@@ -28,6 +28,7 @@ struct LinearParams {
 // q_start[s] / kChunk + s + c: entries of ascending requests never meet.
 constexpr uint32_t kChunk = 64;
 constexpr uint32_t kPrepThreads = 256;
+constexpr uint32_t kXcds = 8;
 
 constexpr uint32_t kChunkFrom = 24;  // tokens a request from which a call goes by chunks
 
@@ -36,15 +37,32 @@ struct ChunkPlan {
     int p_parts = 0;        // f16 parts of the scores (0: no out)
     uint32_t entries = 0;
     uint32_t chunks = 0;    // most of one request
-    uint32_t cols = 0;      // of dim_v per wave
     uint64_t key_bytes = 0, head_bytes = 0;  // of an entry, per key head and per head
     uint64_t bytes = 0;
 };
 
-bool load_linear_chunk_kernels();
-ChunkPlan plan_chunks(const kvmem_hip_linear_args *a, uint32_t max_q);
-// Both launches of a call by chunks (the second only where the first was made).
-void launch_linear_chunks(hipStream_t stream, int type, uint32_t dim_k, const ChunkPlan &pl, const LinearParams &p,
-                          uint8_t *workspace);
+constexpr uint32_t kFragBytes = 1024;  // a 16 x 32 operand of f16: 16 bytes a lane
+constexpr uint32_t kLowerFrags = 6;    // of a 64 x 64 lower triangle: (0,0) (1,0) (2,0) (2,1) (3,0) (3,1)
+constexpr uint32_t kHeadBytes = 1024;  // a head's entry begins with ChunkHead
+
+struct ChunkParams {
+    LinearParams a;
+    uint8_t *keys;   // [entries][key heads]: fragments of K, Q, K^T
+    uint8_t *heads;  // [entries][heads]: ChunkHead, fragments of T, P
+    uint64_t key_bytes, head_bytes;
+    uint32_t chunks;
+    int type;
+    uint32_t dim_k;
+    uint32_t delta, outs, p_parts;
+};
+
+// Both launches of a call by chunks (the second only where the first was made), and
+// the loading of their code object, for rows of each type.
+void launch_linear_chunks_f32(hipStream_t stream, const ChunkParams &p);
+void launch_linear_chunks_f16(hipStream_t stream, const ChunkParams &p);
+void launch_linear_chunks_bf16(hipStream_t stream, const ChunkParams &p);
+bool load_linear_chunks_f32();
+bool load_linear_chunks_f16();
+bool load_linear_chunks_bf16();
 
 }  // namespace kvmem_hip

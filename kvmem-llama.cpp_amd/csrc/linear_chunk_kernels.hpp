@@ -2,18 +2,18 @@
 // linear.hip; a_t = exp(log_decay_t), G_i the chunk's sum of log_decay up to token i).
 // With S the state before the chunk, D the chunk's rows d_i, and
 //     A_ij = beta_i (k_i . k_j) e^(G_i - G_j)   j < i
-//     P_ij =        (q_i . k_j) e^(G_i - G_j)   j <= i
+//     P_ij = scale (q_i . k_j) e^(G_i - G_j)    j <= i
 // the recurrence is, in products of matrices,
 //     D  = (1 + A)^-1 diag(beta) (V - diag(e^G) K S)      (V itself without beta)
-//     O  = scale (diag(e^G) Q S + P D)
+//     O  = scale diag(e^G) Q S + P D
 //     S' = e^(G_last) S + K^T diag(e^(G_last - G)) D
 // Two launches:
 //   prepare  per (chunk, head): T = (1 + A)^-1 diag(beta) and P, which no state
 //            enters, so all chunks at once; keys and queries as the matrix cores'
 //            operands
-//   walk     per (request, head, 16 or 32 columns of the state): the chunks in
+//   walk     per (request, head, 16 columns of the state a wave): the chunks in
 //            order.  Columns of a state never meet, so a wave needs nothing of any
-//            other: no barrier, no LDS.  It keeps its columns of S in accumulator
+//            other but the operands they share in LDS.  It keeps its columns of S in
 //            registers; a product's accumulator (4 consecutive rows per lane) serves
 //            as the next product's operand as it is, because the order in which a
 //            contraction runs over its 32 indices is free as long as both operands
@@ -32,6 +32,8 @@
 // A chunk with a number that is not finite among its rows, gates or factors goes
 // token by token instead (walk_tokens), as products of masked rows would spread it
 // to earlier tokens.
+#pragma once
+
 #include "kvmem_internal.hpp"
 
 #include <algorithm>
@@ -45,10 +47,6 @@ typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kFragBytes = 1024;  // a 16 x 32 operand of f16: 16 bytes a lane
-constexpr uint32_t kLowerFrags = 6;    // of a 64 x 64 lower triangle: (0,0) (1,0) (2,0) (2,1) (3,0) (3,1)
-constexpr uint32_t kHeadBytes = 1024;  // a head's entry begins with ChunkHead
-
 struct ChunkHead {
     float from_first[kChunk];  // e^G_i
     float to_last[kChunk];     // e^(G_last - G_i)
@@ -56,18 +54,6 @@ struct ChunkHead {
     uint32_t by_token;         // a number that is not finite
 };
 static_assert(sizeof(ChunkHead) <= kHeadBytes, "");
-
-struct ChunkParams {
-    LinearParams a;
-    uint8_t *keys;   // [entries][key heads]: fragments of K, Q, K^T
-    uint8_t *heads;  // [entries][heads]: ChunkHead, fragments of T, P
-    uint64_t key_bytes, head_bytes;
-    uint32_t chunks;
-    int type;
-    uint32_t dim_k;
-    uint32_t delta, outs, p_parts;
-    uint32_t cols;
-};
 
 __device__ inline uint64_t entry_of(const Request &rq, uint32_t s, uint32_t c) {
     return static_cast<uint64_t>(rq.first / kChunk) + s + c;
@@ -357,7 +343,8 @@ __global__ __launch_bounds__(kPrepThreads) void linear_prepare_kernel(const Chun
                     col < i ? __builtin_amdgcn_ldexpf(kk[j][r] * f, 2 * exp_k) * bi : 0.0f;
             }
             if (p.outs) {
-                tri_p[i * kTriPitch + col] = col <= i ? __builtin_amdgcn_ldexpf(qk[j][r] * f, exp_k + exp_q) : 0.0f;
+                tri_p[i * kTriPitch + col] =
+                    col <= i ? __builtin_amdgcn_ldexpf(qk[j][r] * f, exp_k + exp_q) * p.a.scale : 0.0f;
             }
         }
     }
@@ -491,13 +478,8 @@ __global__ __launch_bounds__(kPrepThreads) void linear_prepare_kernel(const Chun
 
 // ---------------------------------------------------------------------- walk
 
-__device__ inline float load_one(const uint8_t *p, int type, uint64_t i) {
-    if (type == KVMEM_TYPE_F32) {
-        return reinterpret_cast<const float *>(p)[i];
-    }
-    const uint16_t x = reinterpret_cast<const uint16_t *>(p)[i];
-    return type == KVMEM_TYPE_F16 ? static_cast<float>(__builtin_bit_cast(_Float16, x))
-                                  : __uint_as_float(static_cast<uint32_t>(x) << 16);
+template <typename T> __device__ inline float load_one(const uint8_t *p) {
+    return static_cast<float>(*reinterpret_cast<const T *>(p));
 }
 
 __device__ inline void store_one(uint8_t *p, int type, uint64_t i, float x) {
@@ -514,42 +496,102 @@ __device__ inline half8_t get_frag(const uint8_t *base, uint32_t frag) {
     return *reinterpret_cast<const half8_t *>(base + frag * kFragBytes + (threadIdx.x & 63u) * 16u);
 }
 
+// The largest of a column's four lanes (l, l ^ 16, l ^ 32, l ^ 48): two exchanges of
+// rows of 16 and of halves of the wave, each of a number with its own copy.
+__device__ inline uint32_t column_max(uint32_t m) {
+    auto x = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+    m = max(static_cast<uint32_t>(x[0]), static_cast<uint32_t>(x[1]));
+    x = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    return max(static_cast<uint32_t>(x[0]), static_cast<uint32_t>(x[1]));
+}
+
+// The largest magnitude of a lane's numbers, NaN left out.
+template <int TILES> __device__ inline float lane_max(const f32x4_t (&x)[TILES]) {
+    float m[4] = {};
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m[2 * (t & 1)]) : "v"(x[t][0]), "v"(x[t][1]));
+        asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m[2 * (t & 1) + 1]) : "v"(x[t][2]), "v"(x[t][3]));
+    }
+    asm("v_max3_f32 %0, %0, %1, %2" : "+v"(m[0]) : "v"(m[1]), "v"(m[2]));
+    return __builtin_fmaxf(m[0], m[3]);
+}
+
 // A column's numbers (tiles of 16 rows, 4 of each in every lane of the column) as
-// two f16 parts of x * 2^-e, e the column's own.
+// two f16 parts of x * 2^-e, e the column's own.  The mixed-precision FMAs round
+// x f and x f - high to f16 without a step in fp32: two instructions a number.  No
+// number here is a matrix instruction's own result (its readers would have to wait
+// inside the block); an instruction stands between a half word's write and its use.
 template <int TILES>
 __device__ inline int split(const f32x4_t (&x)[TILES], half8_t (&hi)[TILES / 2], half8_t (&lo)[TILES / 2]) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            m = max(m, mag(x[t][r]));
-        }
-    }
-    m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 16, 64)));
-    m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 32, 64)));
-    const int e = scale_exp(m);
+    const float m = lane_max<TILES>(x);
+    const int e = scale_exp(column_max(__float_as_uint(m)));
     const float f = pow2(-e);
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) {
+    for (int t = 0; t < TILES; t += 2) {
+        uint32_t h[4], l[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float y = x[t][r] * f;
-            const _Float16 a = static_cast<_Float16>(y);
-            hi[t / 2][4 * (t & 1) + r] = a;
-            lo[t / 2][4 * (t & 1) + r] = static_cast<_Float16>(y - static_cast<float>(a));
+        for (int u = 0; u < 2; ++u) {
+            asm("v_fma_mixlo_f16 %0, %4, %8, 0\n\t"
+                "v_fma_mixlo_f16 %1, %6, %8, 0\n\t"
+                "v_fma_mixhi_f16 %0, %5, %8, 0\n\t"
+                "v_fma_mixhi_f16 %1, %7, %8, 0\n\t"
+                "v_fma_mixlo_f16 %2, %4, %8, -%0 op_sel_hi:[0,0,1]\n\t"
+                "v_fma_mixlo_f16 %3, %6, %8, -%1 op_sel_hi:[0,0,1]\n\t"
+                "v_fma_mixhi_f16 %2, %5, %8, -%0 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+                "v_fma_mixhi_f16 %3, %7, %8, -%1 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+                "s_nop 0"
+                : "=&v"(h[2 * u]), "=&v"(h[2 * u + 1]), "=&v"(l[2 * u]), "=&v"(l[2 * u + 1])
+                : "v"(x[t + u][0]), "v"(x[t + u][1]), "v"(x[t + u][2]), "v"(x[t + u][3]), "v"(f));
         }
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        hi[t / 2] = __builtin_bit_cast(half8_t, u32x4{h[0], h[1], h[2], h[3]});
+        lo[t / 2] = __builtin_bit_cast(half8_t, u32x4{l[0], l[1], l[2], l[3]});
     }
     return e;
 }
 
-#define KVMEM_MFMA16(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0)
+// The high parts alone.
+template <int TILES>
+__device__ inline int split_high(const f32x4_t (&x)[TILES], half8_t (&hi)[TILES / 2]) {
+    const float m = lane_max<TILES>(x);
+    const int e = scale_exp(column_max(__float_as_uint(m)));
+    const float f = pow2(-e);
+#pragma unroll
+    for (int t = 0; t < TILES; t += 2) {
+        uint32_t h[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            asm("v_fma_mixlo_f16 %0, %2, %6, 0\n\t"
+                "v_fma_mixlo_f16 %1, %4, %6, 0\n\t"
+                "v_fma_mixhi_f16 %0, %3, %6, 0\n\t"
+                "v_fma_mixhi_f16 %1, %5, %6, 0\n\t"
+                "s_nop 0"
+                : "=&v"(h[2 * u]), "=&v"(h[2 * u + 1])
+                : "v"(x[t + u][0]), "v"(x[t + u][1]), "v"(x[t + u][2]), "v"(x[t + u][3]), "v"(f));
+        }
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        hi[t / 2] = __builtin_bit_cast(half8_t, u32x4{h[0], h[1], h[2], h[3]});
+    }
+    return e;
+}
 
-// A chunk's tokens one by one, on the wave's NT x 16 columns of the state (rows
-// 16 d + 4 g + r in s[.][d][r]).
-template <int DK, int NT>
-__device__ inline __attribute__((always_inline)) void walk_tokens(const ChunkParams &p, f32x4_t (&s)[NT][DK / 16], uint64_t row0,
-                                                      uint32_t n, uint32_t h, uint32_t hk, uint32_t col) {
+// Lets the scheduler put `valu` vector instructions behind each of `n` matrix ones: a
+// matrix instruction of 16 x 16 x 32 runs 16 cycles, in which four others can start.
+template <int N, int VALU> __device__ inline void interleave() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+    }
+}
+
+// A chunk's tokens one by one, on the wave's 16 columns of the state (rows
+// 16 d + 4 g + r in s[d][r]).
+template <typename T, int DK>
+__device__ inline __attribute__((always_inline)) void walk_tokens(const ChunkParams &p, f32x4_t (&s)[DK / 16],
+                                                                  uint64_t row0, uint32_t n, uint32_t h, uint32_t hk,
+                                                                  uint32_t col) {
     const uint32_t g = (threadIdx.x & 63u) >> 4;
     for (uint32_t t = 0; t < n; ++t) {
         const uint64_t row = row0 + t;
@@ -559,55 +601,58 @@ __device__ inline __attribute__((always_inline)) void walk_tokens(const ChunkPar
         float kd[DK / 16][4];
 #pragma unroll
         for (int d = 0; d < DK / 16; ++d) {
-#pragma unroll
-            for (uint32_t r = 0; r < 4; ++r) {
-                kd[d][r] = load_one(k, p.type, 16u * d + 4u * g + r);
-            }
+            RawRow<T, 4> raw;
+            load_raw<T, 4>(k + (16u * d + 4u * g) * sizeof(T), raw);
+            widen<T, 4>(raw, kd[d]);
         }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            float x = load_one(p.a.v + row * p.a.v_nb2 + h * p.a.v_nb1, p.type, col + 16u * j);
-            if (p.delta) {
-                float u = 0.0f;
-#pragma unroll
-                for (int d = 0; d < DK / 16; ++d) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        u = __builtin_fmaf(s[j][d][r], kd[d][r], u);
-                    }
-                }
-                u += __shfl_xor(u, 16, 64);
-                u += __shfl_xor(u, 32, 64);
-                const float b = *reinterpret_cast<const float *>(p.a.beta + row * p.a.beta_nb + h * 4u);
-                x = b * __builtin_fmaf(-a, u, x);
-            }
+        float x = load_one<T>(p.a.v + row * p.a.v_nb2 + h * p.a.v_nb1 + col * sizeof(T));
+        if (p.delta) {
+            float u = 0.0f;
 #pragma unroll
             for (int d = 0; d < DK / 16; ++d) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s[j][d][r] = __builtin_fmaf(kd[d][r], x, a * s[j][d][r]);
+                    u = __builtin_fmaf(s[d][r], kd[d][r], u);
                 }
             }
-            if (p.outs) {
-                const uint8_t *q = p.a.q + row * p.a.q_nb2 + hk * p.a.q_nb1;
-                float o = 0.0f;
+            u += __shfl_xor(u, 16, 64);
+            u += __shfl_xor(u, 32, 64);
+            const float b = *reinterpret_cast<const float *>(p.a.beta + row * p.a.beta_nb + h * 4u);
+            x = b * __builtin_fmaf(-a, u, x);
+        }
 #pragma unroll
-                for (int d = 0; d < DK / 16; ++d) {
+        for (int d = 0; d < DK / 16; ++d) {
 #pragma unroll
-                    for (uint32_t r = 0; r < 4; ++r) {
-                        o = __builtin_fmaf(s[j][d][r], load_one(q, p.type, 16u * d + 4u * g + r), o);
-                    }
+            for (int r = 0; r < 4; ++r) {
+                s[d][r] = __builtin_fmaf(kd[d][r], x, a * s[d][r]);
+            }
+        }
+        if (p.outs) {
+            const uint8_t *q = p.a.q + row * p.a.q_nb2 + hk * p.a.q_nb1;
+            float o = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DK / 16; ++d) {
+                RawRow<T, 4> raw;
+                float qd[4];
+                load_raw<T, 4>(q + (16u * d + 4u * g) * sizeof(T), raw);
+                widen<T, 4>(raw, qd);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    o = __builtin_fmaf(s[d][r], qd[r], o);
                 }
-                o += __shfl_xor(o, 16, 64);
-                o += __shfl_xor(o, 32, 64);
-                if (g == 0) {
-                    store_one(p.a.out, p.a.out_type, (row * p.a.n_head + h) * p.a.dim_v + col + 16u * j,
-                              p.a.scale * o);
-                }
+            }
+            o += __shfl_xor(o, 16, 64);
+            o += __shfl_xor(o, 32, 64);
+            if (g == 0) {
+                store_one(p.a.out, p.a.out_type, (row * p.a.n_head + h) * p.a.dim_v + col, p.a.scale * o);
             }
         }
     }
 }
+
+#define KVMEM_MFMA16(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0)
+
+typedef __attribute__((address_space(3))) void lds_void_t;
 
 template <int N>
 __device__ inline void get_frags(const uint8_t *base, uint32_t frag, half8_t (&x)[N]) {
@@ -617,362 +662,399 @@ __device__ inline void get_frags(const uint8_t *base, uint32_t frag, half8_t (&x
     }
 }
 
-// What a chunk needs first, requested while the chunk before it is computed.
-template <int NT, int PARTS, int KEYS> struct ChunkRows {
-    half8_t k[KEYS];                       // operands of K (delta rule)
-    uint32_t v[NT][16];                    // values as they lie in memory, rows 16 m + 4 g + r
-    uint32_t by_token;
+// A chunk in LDS: its keys' operands [K Q K^T][part], then its head's (ChunkHead, T, P),
+// as they lie in its entries, then its values.
+template <typename T, int DK, bool DELTA, bool FINE, int WAVES> struct ChunkSpace {
+    static constexpr uint32_t parts = sizeof(T) == 4 ? 2 : 1;
+    static constexpr uint32_t key_frags = 12 * (DK / 32) * parts;
+    static constexpr uint32_t head_frags = 1 + (DELTA ? 2 * kLowerFrags : 0) + (FINE ? 2 : 1) * kLowerFrags;
+    static constexpr uint32_t row_bytes = WAVES * 16 * sizeof(T);  // of the values
+    static constexpr uint32_t rest = head_frags * kFragBytes + kChunk * row_bytes;
+    static constexpr uint32_t most = 160 * 1024;
+    // the keys' operands go through LDS where one chunk fits, chunks alternate between
+    // two places where two fit
+    static constexpr bool keys = key_frags * kFragBytes + rest <= most;
+    static constexpr uint32_t bytes = (keys ? key_frags * kFragBytes : 0) + rest;
+    static constexpr uint32_t places = 2 * bytes <= most ? 2 : 1;
 };
 
-struct ChunkGates {
-    f32x4_t first[4], last[4];  // e^G, e^(G_last - G) of rows 16 m + 4 g + r
-    float out_first[4];         // e^G of rows 16 m + lane % 16
-    float whole;
-    int exp_k, exp_q, exp_t, exp_p;
-};
+// Every wave's LDS reads are done before another may write there.
+__device__ inline void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
-template <int DK, int NT, int PARTS, bool DELTA, bool FINE>
-__global__ __launch_bounds__(64, 1) void linear_walk_kernel(const ChunkParams p) {
-    constexpr int KS = DK / 32, TILES = DK / 16;
-    // operands of a matrix of keys: all parts requested ahead where registers hold them
-    constexpr bool AHEAD = DK * PARTS <= 128;
-    constexpr bool LATE = DK * PARTS >= 256;  // K^T only once K's registers are free
-    constexpr int KEYS = AHEAD && DELTA ? 4 * KS * PARTS : 1;
-    constexpr int ROWS = AHEAD ? 4 * KS * PARTS : 1;
-    typedef ChunkRows<NT, PARTS, KEYS> Rows;
-    const uint32_t lane = threadIdx.x, g = lane >> 4;
-    const uint32_t slices = p.a.dim_v / (16u * NT);
-    const uint32_t h = blockIdx.x / slices, s_id = blockIdx.y;
-    const uint32_t col = (blockIdx.x % slices) * (16u * NT) + (lane & 15u);
+// WAVES waves compute, 16 columns each, and as many bring the next chunk into LDS: a
+// wave issues one instruction at a time, and those for the copies would cost the
+// computing ones a third of a chunk's time.
+template <typename T, int DK, bool DELTA, bool FINE, int WAVES>
+__global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const ChunkParams p) {
+    typedef ChunkSpace<T, DK, DELTA, FINE, WAVES> Space;
+    constexpr int PARTS = Space::parts, KS = DK / 32, TILES = DK / 16;
+    __shared__ __align__(16) uint8_t lds[Space::places * Space::bytes];
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t slices = p.a.dim_v / (16u * WAVES);
+    // workgroups go round the 8 XCDs: each XCD takes neighbouring heads, whose columns
+    // read the same operands through its L2
+    const uint32_t unit = (blockIdx.x % kXcds) * (gridDim.x / kXcds) + blockIdx.x / kXcds;
+    if (unit >= p.a.n_head * slices) {
+        return;
+    }
+    const uint32_t h = unit / slices, s_id = blockIdx.y;
+    const uint32_t col0 = (unit % slices) * (16u * WAVES);
     const uint32_t hk = h / p.a.group;
     Request rq = request_of(p.a.batch, s_id);
     rq.first = __builtin_amdgcn_readfirstlane(rq.first);
     rq.count = __builtin_amdgcn_readfirstlane(rq.count);
-    const uint64_t at = (static_cast<uint64_t>(rq.slot) * p.a.n_head + h) * DK * p.a.dim_v + col;
     const uint64_t entry0 = entry_of(rq, s_id, 0);
     const uint64_t key_step = p.key_bytes * (p.a.n_head / p.a.group), head_step = p.head_bytes * p.a.n_head;
     const uint8_t *keys = p.keys + entry0 * key_step + hk * p.key_bytes;
-    const uint8_t *head = p.heads + entry0 * head_step + h * p.head_bytes;
-    const uint8_t *values = p.a.v + rq.first * p.a.v_nb2 + h * p.a.v_nb1;
+    const uint8_t *heads = p.heads + entry0 * head_step + h * p.head_bytes;
+    constexpr uint32_t head_at = Space::keys ? Space::key_frags * kFragBytes : 0;
+    constexpr uint32_t values_at = head_at + Space::head_frags * kFragBytes;
 
+    if (w >= WAVES) {
+        const uint32_t lw = w - WAVES;
+        const uint32_t lane16 = lane * 16u;
+        constexpr uint32_t lanes = Space::row_bytes / 16;  // of a row of values
+        const uint32_t row = lane / lanes;
+        const uint8_t *values =
+            p.a.v + rq.first * p.a.v_nb2 + h * p.a.v_nb1 + col0 * sizeof(T) + (lane % lanes) * 16u;
+        auto frags = [&](const uint8_t *from, uint8_t *to, auto count) {
+            constexpr uint32_t N = decltype(count)::value;
+#pragma unroll
+            for (uint32_t i = 0; i < (N + WAVES - 1) / WAVES; ++i) {
+                if ((i + 1) * WAVES <= N || i * WAVES + lw < N) {
+                    const uint32_t f = (i * WAVES + lw) * kFragBytes;
+                    __builtin_amdgcn_global_load_lds(as_global(from + f) + lane16, (lds_void_t *) (to + f), 16, 0, 0);
+                }
+            }
+        };
+        auto request = [&](uint32_t c, uint8_t *to) {
+            if constexpr (Space::keys) {
+                frags(keys + c * key_step, to, std::integral_constant<uint32_t, Space::key_frags>{});
+            }
+            frags(heads + c * head_step, to + head_at, std::integral_constant<uint32_t, Space::head_frags>{});
+            const uint32_t n = min(kChunk, rq.count - c * kChunk);
+#pragma unroll
+            for (uint32_t i = 0; i < (lanes + WAVES - 1) / WAVES; ++i) {
+                const uint32_t x = i * WAVES + lw;  // of `lanes` groups of 64 / lanes rows
+                if (x < lanes) {
+                    const uint32_t t = min(x * (64 / lanes) + row, n - 1u);
+                    __builtin_amdgcn_global_load_lds(as_global(values + static_cast<uint64_t>(c * kChunk + t) * p.a.v_nb2),
+                                                     (lds_void_t *) (to + values_at + x * kFragBytes), 16, 0, 0);
+                }
+            }
+        };
+        if (Space::places == 2 && rq.count) {
+            request(0, lds);
+        }
+        for (uint32_t c = 0; c * kChunk < rq.count; ++c) {
+            if (Space::places == 1) {
+                lds_barrier();  // the chunk before is read
+                request(c, lds);
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            lds_barrier();
+            if (Space::places == 2 && (c + 1) * kChunk < rq.count) {
+                request(c + 1, lds + ((c + 1) & 1u) * Space::bytes);
+            }
+        }
+        return;
+    }
+
+    const uint32_t col = col0 + 16u * w + (lane & 15u);
+    const uint64_t at = (static_cast<uint64_t>(rq.slot) * p.a.n_head + h) * DK * p.a.dim_v + col;
     // operand i of K (at 0), Q (4 KS) or K^T (8 KS), its first or second part
     auto frag_index = [](uint32_t matrix, uint32_t i, uint32_t part) { return part * 12u * KS + matrix + i; };
-    auto request_rows = [&](uint32_t c, Rows &x) {
-        const uint8_t *kp = keys + c * key_step;
-        const ChunkHead *ch = reinterpret_cast<const ChunkHead *>(head + c * head_step);
-        const uint32_t n = min(kChunk, rq.count - c * kChunk);
-        x.by_token = ch->by_token;
-        if constexpr (AHEAD && DELTA) {
+    f32x4_t s[TILES];
 #pragma unroll
-            for (uint32_t part = 0; part < PARTS; ++part) {
-#pragma unroll
-                for (uint32_t i = 0; i < 4 * KS; ++i) {
-                    x.k[part * 4 * KS + i] = get_frag(kp, frag_index(0, i, part));
-                }
-            }
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < NT; ++j) {
-#pragma unroll
-            for (uint32_t i = 0; i < 16; ++i) {
-                const uint32_t row = 16u * (i >> 2) + 4u * g + (i & 3u);
-                const uint8_t *to = values + static_cast<uint64_t>(c * kChunk + min(row, n - 1u)) * p.a.v_nb2;
-                if constexpr (PARTS == 2) {
-                    x.v[j][i] = reinterpret_cast<const uint32_t *>(to)[col + 16u * j];
-                } else {
-                    x.v[j][i] = reinterpret_cast<const uint16_t *>(to)[col + 16u * j];
-                }
-            }
-        }
-    };
-
-    f32x4_t s[NT][TILES];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-#pragma unroll
-        for (int d = 0; d < TILES; ++d) {
-            s[j][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        }
+    for (int d = 0; d < TILES; ++d) {
+        s[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
     if (p.a.state && rq.has_slot) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+        for (int d = 0; d < TILES; ++d) {
 #pragma unroll
-            for (int d = 0; d < TILES; ++d) {
-#pragma unroll
-                for (uint32_t r = 0; r < 4; ++r) {
-                    s[j][d][r] =
-                        p.a.state[at + static_cast<uint64_t>(16u * d + 4u * g + r) * p.a.dim_v + 16u * j];
-                }
+            for (uint32_t r = 0; r < 4; ++r) {
+                s[d][r] = p.a.state[at + static_cast<uint64_t>(16u * d + 4u * g + r) * p.a.dim_v];
             }
         }
     }
     const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    Rows next;
-    if (rq.count) {
-        request_rows(0, next);
-    }
+    const uint64_t out_row = static_cast<uint64_t>(p.a.n_head) * p.a.dim_v;
+    const uint32_t esz = FINE && p.a.out_type == KVMEM_TYPE_F32 ? 4u : 2u;
+    const uint32_t out_at = ((lane & 15u) * static_cast<uint32_t>(out_row) + 4u * g) * esz;
     for (uint32_t c = 0; c * kChunk < rq.count; ++c) {
-        const Rows x = next;
         const uint32_t n = min(kChunk, rq.count - c * kChunk);
         const uint64_t row0 = static_cast<uint64_t>(rq.first) + c * kChunk;
+        const uint32_t rows = p.outs ? n : 0u;  // without an out, Q and P are whatever the workspace held
+        const uint8_t *here = lds + (Space::places == 2 ? (c & 1u) * Space::bytes : 0u);
         const uint8_t *kp = keys + c * key_step;
-        const uint8_t *frag_t = head + c * head_step + kHeadBytes;
-        const uint8_t *frag_p = frag_t + (DELTA ? 2u * kLowerFrags * kFragBytes : 0u);
-        half8_t qf[ROWS], tf[DELTA ? 2 * kLowerFrags : 1], pf[(FINE ? 2 : 1) * kLowerFrags], kt[ROWS];
-        if constexpr (AHEAD) {
-            if (p.outs) {
-#pragma unroll
-                for (uint32_t i = 0; i < 4 * KS * PARTS; ++i) {
-                    qf[i] = get_frag(kp, frag_index(4 * KS, i % (4 * KS), i / (4 * KS)));
-                }
-            }
+        if constexpr (Space::keys) {
+            kp = here;
         }
-        ChunkGates z;
-        const ChunkHead *ch = reinterpret_cast<const ChunkHead *>(head + c * head_step);
+        const uint8_t *head = here + head_at;
+        const ChunkHead *ch = reinterpret_cast<const ChunkHead *>(head);
+        const uint8_t *frag_t = head + kHeadBytes;
+        const uint8_t *frag_p = frag_t + (DELTA ? 2u * kLowerFrags * kFragBytes : 0u);
+        if (Space::places == 1) {
+            lds_barrier();  // the chunk before is read
+        }
+        lds_barrier();
+
+        // the products' operands are read 8 at a time, a group ahead of their use
+        half8_t kq[2][8];
+        auto read8 = [&](half8_t(&to)[8], uint32_t matrix, uint32_t k) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {  // K, Q: four row tiles of steps k, k + 1; K^T: operands 4k..4k+7
+                to[i] = get_frag(kp, frag_index(matrix, matrix == 8 * KS ? 4 * k + i : (i & 3u) * KS + k + (i >> 2), 0));
+            }
+        };
+        read8(kq[0], DELTA ? 0 : 4 * KS, 0);
+        const uint8_t *vp = here + values_at + 4u * g * Space::row_bytes + (16u * w + (lane & 15u)) * sizeof(T);
+        f32x4_t v[4];
 #pragma unroll
         for (uint32_t m = 0; m < 4; ++m) {
-            z.first[m] = *reinterpret_cast<const f32x4_t *>(ch->from_first + 16u * m + 4u * g);
-            z.last[m] = *reinterpret_cast<const f32x4_t *>(ch->to_last + 16u * m + 4u * g);
-            z.out_first[m] = ch->from_first[16u * m + (lane & 15u)];
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) {
+                v[m][r] = load_one<T>(vp + (16u * m + r) * Space::row_bytes);
+            }
         }
-        z.exp_k = ch->exp_k, z.exp_q = ch->exp_q, z.exp_t = ch->exp_t, z.exp_p = ch->exp_p;
-        z.whole = ch->from_first[kChunk - 1];
+        half8_t hi[KS], lo[KS];
+        const int exp_s = split<TILES>(s, hi, lo);
+        int es[4];  // of columns 4 g + r
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            es[r] = __shfl(exp_s, static_cast<int>(4u * g) + r, 64);
+        }
+        f32x4_t d[4] = {zero, zero, zero, zero}, o[4] = {zero, zero, zero, zero};
+        half8_t tf[DELTA ? 2 * kLowerFrags : 1], pf[(FINE ? 2 : 1) * kLowerFrags];
         if constexpr (DELTA) {
+#pragma unroll
+            for (uint32_t k = 0; k < KS; k += 2) {
+                if (k + 2 < KS) {
+                    read8(kq[(k / 2 + 1) & 1], 0, k + 2);
+                } else {
+                    read8(kq[(k / 2 + 1) & 1], 4 * KS, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (uint32_t x = 0; x < (PARTS == 2 ? 6 : 4); ++x) {  // sums in between do not wait for each other
+#pragma unroll
+                    for (uint32_t m = 0; m < 4; ++m) {
+                        half8_t a;
+                        if (x >= 4) {
+                            a = get_frag(kp, frag_index(0, m * KS + k + (x & 1u), 1));
+                        } else {
+                            a = kq[(k / 2) & 1][4 * (x & 1u) + m];
+                        }
+                        d[m] = KVMEM_MFMA16(a, x == 2 || x == 3 ? lo[k + (x & 1u)] : hi[k + (x & 1u)], d[m]);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        constexpr int Q0 = DELTA ? (KS / 2) & 1 : 0;  // where Q's first group is
+        f32x4_t first[4];
+        float out_first[4];
+        if constexpr (DELTA) {
+#pragma unroll
+            for (uint32_t m = 0; m < 4; ++m) {
+                first[m] = *reinterpret_cast<const f32x4_t *>(ch->from_first + 16u * m + 4u * g);
+            }
             get_frags(frag_t, 0, tf);
         }
-        __builtin_amdgcn_sched_barrier(0);
-        f32x4_t v[NT][4];
-        uint32_t odd = x.by_token;
+        const int exp_k = ch->exp_k, exp_q = ch->exp_q, exp_t = ch->exp_t, exp_p = ch->exp_p;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+        for (uint32_t k = 0; k < KS; k += 2) {  // transposed: columns of the state are rows of the accumulator
+            constexpr uint32_t KT = 8 * KS;
+            if (k + 2 < KS) {
+                read8(kq[(Q0 + k / 2 + 1) & 1], 4 * KS, k + 2);
+            } else {
+                read8(kq[(Q0 + k / 2 + 1) & 1], KT, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            {
 #pragma unroll
-            for (uint32_t i = 0; i < 16; ++i) {
-                const uint32_t w = x.v[j][i];
-                const float f = PARTS == 2 ? __uint_as_float(w)
-                                : p.type == KVMEM_TYPE_F16
-                                    ? static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w)))
-                                    : __uint_as_float(w << 16);
-                v[j][i >> 2][i & 3u] = 16u * (i >> 2) + 4u * g + (i & 3u) < n ? f : 0.0f;
-                odd |= mag(v[j][i >> 2][i & 3u]) >= kInf;
+                for (uint32_t x = 0; x < (!FINE ? 2 : PARTS == 2 ? 6 : 4); ++x) {
+#pragma unroll
+                    for (uint32_t m = 0; m < 4; ++m) {
+                        half8_t a;
+                        if (x >= 4) {
+                            a = get_frag(kp, frag_index(4 * KS, m * KS + k + (x & 1u), 1));
+                        } else {
+                            a = kq[(Q0 + k / 2) & 1][4 * (x & 1u) + m];
+                        }
+                        o[m] = KVMEM_MFMA16(x == 2 || x == 3 ? lo[k + (x & 1u)] : hi[k + (x & 1u)], a, o[m]);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        constexpr int T0 = (Q0 + KS / 2) & 1;  // where K^T's first group is
+        // rows behind the last token repeat it: the factors' zeros meet them
+        f32x4_t odd = zero;  // NaN where a value is not finite
+#pragma unroll
+        for (uint32_t m = 0; m < 4; ++m) {
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) {
+                odd[r] = __builtin_fmaf(v[m][r], 0.0f, odd[r]);
             }
         }
-        if (__builtin_expect(__any(odd), 0)) {
-            walk_tokens<DK, NT>(p, s, row0, n, h, hk, col);
-            if ((c + 1) * kChunk < rq.count) {
-                request_rows(c + 1, next);
-            }
+        const float any_odd = (odd[0] + odd[1]) + (odd[2] + odd[3]);
+        if (__builtin_expect(__any(any_odd != any_odd || ch->by_token != 0), 0)) {
+            walk_tokens<T, DK>(p, s, row0, n, h, hk, col);
             continue;
         }
-        half8_t hi[NT][KS], lo[NT][KS];
-        int exp_s[NT];
-        f32x4_t d[NT][4], o[NT][4];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            exp_s[j] = split<TILES>(s[j], hi[j], lo[j]);
-            if constexpr (DELTA) {
-#pragma unroll
-                for (uint32_t m = 0; m < 4; ++m) {
-                    d[j][m] = zero;
-                }
-#pragma unroll
-                for (uint32_t k = 0; k < KS; ++k) {
-#pragma unroll
-                    for (uint32_t m = 0; m < 4; ++m) {
-                        const uint32_t i = m * KS + k;
-                        const half8_t a = AHEAD ? x.k[AHEAD ? i : 0] : get_frag(kp, frag_index(0, i, 0));
-                        d[j][m] = KVMEM_MFMA16(a, hi[j][k], d[j][m]);
-                        d[j][m] = KVMEM_MFMA16(a, lo[j][k], d[j][m]);
-                        if constexpr (PARTS == 2) {
-                            const half8_t b =
-                                AHEAD ? x.k[AHEAD ? 4 * KS + i : 0] : get_frag(kp, frag_index(0, i, 1));
-                            d[j][m] = KVMEM_MFMA16(b, hi[j][k], d[j][m]);
-                        }
-                    }
-                }
-            }
-        }
-        if (p.outs) {
-            get_frags(frag_p, 0, pf);
-        }
-        if constexpr (AHEAD && !LATE) {
-#pragma unroll
-            for (uint32_t i = 0; i < 4 * KS * PARTS; ++i) {
-                kt[i] = get_frag(kp, frag_index(8 * KS, i % (4 * KS), i / (4 * KS)));
-            }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        if (p.outs) {  // transposed: columns of the state are rows of the accumulator
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-#pragma unroll
-                for (uint32_t m = 0; m < 4; ++m) {
-                    o[j][m] = zero;
-                }
-#pragma unroll
-                for (uint32_t k = 0; k < KS; ++k) {
-#pragma unroll
-                    for (uint32_t m = 0; m < 4; ++m) {
-                        const uint32_t i = m * KS + k;
-                        const half8_t a = AHEAD ? qf[AHEAD ? i : 0] : get_frag(kp, frag_index(4 * KS, i, 0));
-                        o[j][m] = KVMEM_MFMA16(hi[j][k], a, o[j][m]);
-                        if constexpr (FINE) {
-                            o[j][m] = KVMEM_MFMA16(lo[j][k], a, o[j][m]);
-                            if constexpr (PARTS == 2) {
-                                const half8_t b =
-                                    AHEAD ? qf[AHEAD ? 4 * KS + i : 0] : get_frag(kp, frag_index(4 * KS, i, 1));
-                                o[j][m] = KVMEM_MFMA16(hi[j][k], b, o[j][m]);
-                            }
-                        }
-                    }
-                }
-            }
-        }
+        half8_t dh[2], dl[2];
         if constexpr (DELTA) {
+            f32x4_t rest[4];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                f32x4_t rest[4];
+            for (uint32_t m = 0; m < 4; ++m) {
 #pragma unroll
-                for (int m = 0; m < 4; ++m) {
+                for (int r = 0; r < 4; ++r) {
+                    rest[m][r] =
+                        __builtin_fmaf(-first[m][r], __builtin_amdgcn_ldexpf(d[m][r], exp_k + exp_s), v[m][r]);
+                }
+                d[m] = zero;
+            }
+            const int e = exp_t + split<4>(rest, dh, dl);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        rest[m][r] = __builtin_fmaf(
-                            -z.first[m][r], __builtin_amdgcn_ldexpf(d[j][m][r], z.exp_k + exp_s[j]), v[j][m][r]);
+            for (uint32_t k = 0; k < 2; ++k) {
+#pragma unroll
+                for (uint32_t x = 0; x < 3; ++x) {
+#pragma unroll
+                    for (uint32_t m = 2 * k; m < 4; ++m) {
+                        d[m] = KVMEM_MFMA16(tf[(x == 2 ? kLowerFrags : 0u) + lower_frag(m, k)],
+                                            x == 1 ? dl[k] : dh[k], d[m]);
                     }
                 }
-                half8_t rh[2], rl[2];
-                const int e = z.exp_t + split<4>(rest, rh, rl);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            get_frags(frag_p, 0, pf);
 #pragma unroll
-                for (uint32_t m = 0; m < 4; ++m) {
-                    d[j][m] = zero;
+            for (int m = 0; m < 4; ++m) {
 #pragma unroll
-                    for (uint32_t k = 0; k <= m / 2; ++k) {
-                        const uint32_t f = lower_frag(m, k);
-                        d[j][m] = KVMEM_MFMA16(tf[f], rh[k], d[j][m]);
-                        d[j][m] = KVMEM_MFMA16(tf[f], rl[k], d[j][m]);
-                        d[j][m] = KVMEM_MFMA16(tf[kLowerFrags + f], rh[k], d[j][m]);
-                    }
-                }
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        d[j][m][r] = __builtin_amdgcn_ldexpf(d[j][m][r], e);
-                    }
+                for (int r = 0; r < 4; ++r) {
+                    d[m][r] = __builtin_amdgcn_ldexpf(d[m][r], e);
                 }
             }
         } else {
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    d[j][m] = v[j][m];
-                }
-            }
-        }
-        if constexpr (AHEAD && LATE) {
-#pragma unroll
-            for (uint32_t i = 0; i < 4 * KS * PARTS; ++i) {
-                kt[i] = get_frag(kp, frag_index(8 * KS, i % (4 * KS), i / (4 * KS)));
-            }
-        }
-        if constexpr (!LATE) {
-            if ((c + 1) * kChunk < rq.count) {
-                request_rows(c + 1, next);
-            }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        if (p.outs) {
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                half8_t dh[2], dl[2];
-                const int exp_d = split<4>(d[j], dh, dl);
-                f32x4_t pd[4];
-#pragma unroll
-                for (uint32_t m = 0; m < 4; ++m) {
-                    pd[m] = zero;
-#pragma unroll
-                    for (uint32_t k = 0; k <= m / 2; ++k) {
-                        const uint32_t f = lower_frag(m, k);
-                        pd[m] = KVMEM_MFMA16(dh[k], pf[f], pd[m]);
-                        if constexpr (FINE) {
-                            pd[m] = KVMEM_MFMA16(dl[k], pf[f], pd[m]);
-                            pd[m] = KVMEM_MFMA16(dh[k], pf[kLowerFrags + f], pd[m]);
-                        }
-                    }
-                }
-                int es[4], ed[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    es[r] = __shfl(exp_s[j], static_cast<int>(4u * g) + r, 64) + z.exp_q;
-                    ed[r] = __shfl(exp_d, static_cast<int>(4u * g) + r, 64) + z.exp_p;
-                }
-                const uint32_t dv = col - (lane & 15u) + 16u * j + 4u * g;
-#pragma unroll
-                for (uint32_t m = 0; m < 4; ++m) {
-                    const uint32_t i = 16u * m + (lane & 15u);
-                    float y[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        y[r] = p.a.scale * __builtin_fmaf(z.out_first[m], __builtin_amdgcn_ldexpf(o[j][m][r], es[r]),
-                                                          __builtin_amdgcn_ldexpf(pd[m][r], ed[r]));
-                    }
-                    if (i < n) {
-                        const uint64_t to = ((row0 + i) * p.a.n_head + h) * p.a.dim_v + dv;
-                        if (p.a.out_type == KVMEM_TYPE_F32) {
-                            store_row<float, 4>(p.a.out + to * 4, y);
-                        } else if (p.a.out_type == KVMEM_TYPE_F16) {
-                            store_row<_Float16, 4>(p.a.out + to * 2, y);
-                        } else {
-                            store_row<__bf16, 4>(p.a.out + to * 2, y);
-                        }
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
+            get_frags(frag_p, 0, pf);
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                d[j][m] *= z.last[m];
+                d[m] = v[m];
             }
-            half8_t dh[2], dl[2];
-            const int e = split<4>(d[j], dh, dl) + z.exp_k;
+        }
+        f32x4_t last[4];
 #pragma unroll
-            for (uint32_t t = 0; t < TILES; ++t) {
-                f32x4_t y = zero;
+        for (uint32_t m = 0; m < 4; ++m) {
+            last[m] = *reinterpret_cast<const f32x4_t *>(ch->to_last + 16u * m + 4u * g);
+            out_first[m] = p.a.scale * ch->from_first[16u * m + (lane & 15u)];
+        }
+        const float whole = ch->from_first[kChunk - 1];
+        {
+            f32x4_t pd[4] = {zero, zero, zero, zero};
+            int exp_d;
+            if constexpr (FINE) {
+                exp_d = split<4>(d, dh, dl);
+            } else {
+                exp_d = split_high<4>(d, dh);
+            }
 #pragma unroll
-                for (uint32_t k = 0; k < 2; ++k) {
-                    const uint32_t i = 2u * t + k;
-                    const half8_t a = AHEAD ? kt[AHEAD ? i : 0] : get_frag(kp, frag_index(8 * KS, i, 0));
-                    y = KVMEM_MFMA16(a, dh[k], y);
-                    y = KVMEM_MFMA16(a, dl[k], y);
-                    if constexpr (PARTS == 2) {
-                        const half8_t b = AHEAD ? kt[AHEAD ? 4 * KS + i : 0] : get_frag(kp, frag_index(8 * KS, i, 1));
-                        y = KVMEM_MFMA16(b, dh[k], y);
+            for (uint32_t k = 0; k < 2; ++k) {
+#pragma unroll
+                for (uint32_t x = 0; x < (FINE ? 3 : 1); ++x) {
+#pragma unroll
+                    for (uint32_t m = 2 * k; m < 4; ++m) {
+                        pd[m] = KVMEM_MFMA16(x == 1 ? dl[k] : dh[k], pf[(x == 2 ? kLowerFrags : 0u) + lower_frag(m, k)],
+                                             pd[m]);
                     }
                 }
+            }
+            uint8_t *out = p.a.out + (row0 * out_row + h * p.a.dim_v + col0 + 16u * w) * esz;
+            int ed[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                es[r] += exp_q;
+                ed[r] = __shfl(exp_d, static_cast<int>(4u * g) + r, 64) + exp_p - es[r];
+            }
+#pragma unroll
+            for (uint32_t m = 0; m < 4; ++m) {
+                float y[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s[j][t][r] = __builtin_fmaf(z.whole, s[j][t][r], __builtin_amdgcn_ldexpf(y[r], e));
+                    y[r] = __builtin_amdgcn_ldexpf(
+                        __builtin_fmaf(out_first[m], o[m][r], __builtin_amdgcn_ldexpf(pd[m][r], ed[r])), es[r]);
+                }
+                uint8_t *to = out + m * 16u * out_row * esz;
+                if (16u * m + (lane & 15u) < rows) {
+                    if constexpr (!FINE) {
+                        store_row<__bf16, 4>(to + out_at, y);
+                    } else if (p.a.out_type == KVMEM_TYPE_F32) {
+                        store_row<float, 4>(to + out_at, y);
+                    } else {
+                        store_row<_Float16, 4>(to + out_at, y);
+                    }
                 }
             }
         }
-        if constexpr (LATE) {
-            if ((c + 1) * kChunk < rq.count) {
-                request_rows(c + 1, next);
-            }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            d[m] *= last[m];
         }
+        const int exp_d = split<4>(d, dh, dl) + exp_k;
+        f32x4_t y[2][4];
+        auto update = [&](uint32_t t0) {
+#pragma unroll
+            for (uint32_t t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[t0 + t][r] = __builtin_fmaf(whole, s[t0 + t][r],
+                                                  __builtin_amdgcn_ldexpf(y[(t0 / 4) & 1][t][r], exp_d));
+                }
+            }
+        };
+#pragma unroll
+        for (uint32_t t0 = 0; t0 < TILES; t0 += 4) {  // four sums at a time, the four before added meanwhile
+            if (t0 + 4 < TILES) {
+                read8(kq[(T0 + t0 / 4 + 1) & 1], 8 * KS, t0 / 2 + 2);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (uint32_t k = 0; k < 2; ++k) {
+#pragma unroll
+                for (uint32_t x = 0; x < (PARTS == 2 ? 3 : 2); ++x) {
+#pragma unroll
+                    for (uint32_t t = 0; t < 4; ++t) {
+                        half8_t a;
+                        if (x == 2) {
+                            a = get_frag(kp, frag_index(8 * KS, 2 * (t0 + t) + k, 1));
+                        } else {
+                            a = kq[(T0 + t0 / 4) & 1][2 * t + k];
+                        }
+                        f32x4_t &to = y[(t0 / 4) & 1][t];
+                        to = KVMEM_MFMA16(a, x == 1 ? dl[k] : dh[k], k == 0 && x == 0 ? zero : to);
+                    }
+                }
+            }
+            if (t0 >= 4) {
+                update(t0 - 4);
+                interleave<16, 2>();
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        update(TILES - 4);
     }
     if (p.a.state_out && rq.has_slot) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+        for (int d = 0; d < TILES; ++d) {
 #pragma unroll
-            for (int d = 0; d < TILES; ++d) {
-#pragma unroll
-                for (uint32_t r = 0; r < 4; ++r) {
-                    p.a.state_out[at + static_cast<uint64_t>(16u * d + 4u * g + r) * p.a.dim_v + 16u * j] = s[j][d][r];
-                }
+            for (uint32_t r = 0; r < 4; ++r) {
+                p.a.state_out[at + static_cast<uint64_t>(16u * d + 4u * g + r) * p.a.dim_v] = s[d][r];
             }
         }
     }
@@ -983,80 +1065,47 @@ static void prepare(hipStream_t stream, const ChunkParams &p) {
     linear_prepare_kernel<T, DK><<<dim3(p.chunks * p.a.n_head, p.a.n_seq), kPrepThreads, 0, stream>>>(p);
 }
 
-template <int DK, int NT, int PARTS>
-static void walk(hipStream_t stream, const ChunkParams &p) {
-    const dim3 grid(p.a.n_head * (p.a.dim_v / (16u * NT)), p.a.n_seq);
-    const bool fine = p.p_parts == 2;  // the output takes both parts
-    if (p.delta) {
-        fine ? linear_walk_kernel<DK, NT, PARTS, true, true><<<grid, 64, 0, stream>>>(p)
-             : linear_walk_kernel<DK, NT, PARTS, true, false><<<grid, 64, 0, stream>>>(p);
-    } else {
-        fine ? linear_walk_kernel<DK, NT, PARTS, false, true><<<grid, 64, 0, stream>>>(p)
-             : linear_walk_kernel<DK, NT, PARTS, false, false><<<grid, 64, 0, stream>>>(p);
+// 64 columns a workgroup where a head has them and two chunks of that width fit into
+// LDS, else 32.  A chunk takes a wave the same time either way (8192 tokens, 48 states
+// of 128 x 128: KVM_W32 and KVM_W64 us), and wide workgroups read the operands half as
+// often (eight prompts of up to 4096 tokens, 32 states: KVM_B32 and KVM_B64 us).
+template <typename T, int DK, bool DELTA, bool FINE>
+static void walk_cols(hipStream_t stream, const ChunkParams &p) {
+    constexpr bool wide = ChunkSpace<T, DK, DELTA, FINE, 4>::places == 2;
+    const uint32_t cols = wide && p.a.dim_v % 64 == 0 ? 64u : 32u;
+    const uint32_t units = p.a.n_head * (p.a.dim_v / cols);
+    const dim3 grid((units + kXcds - 1) / kXcds * kXcds, p.a.n_seq);
+    if constexpr (wide) {
+        if (cols == 64) {
+            linear_walk_kernel<T, DK, DELTA, FINE, 4><<<grid, 512, 0, stream>>>(p);
+            return;
+        }
     }
+    linear_walk_kernel<T, DK, DELTA, FINE, 2><<<grid, 256, 0, stream>>>(p);
 }
 
-template <int DK>
-static void launch(hipStream_t stream, const ChunkParams &p) {
-    if (p.type == KVMEM_TYPE_F32) {
-        prepare<float, DK>(stream, p);
-    } else if (p.type == KVMEM_TYPE_F16) {
-        prepare<_Float16, DK>(stream, p);
-    } else {
-        prepare<__bf16, DK>(stream, p);
-    }
+template <typename T, int DK>
+static void launch_type(hipStream_t stream, const ChunkParams &p) {
+    prepare<T, DK>(stream, p);
     if (hipPeekAtLastError() != hipSuccess) {
         return;  // factors that were not written must not be read
     }
-    if (p.type == KVMEM_TYPE_F32) {
-        walk<DK, 1, 2>(stream, p);
+    const bool fine = p.p_parts == 2;  // the output takes both parts
+    if (p.delta) {
+        fine ? walk_cols<T, DK, true, true>(stream, p) : walk_cols<T, DK, true, false>(stream, p);
     } else {
-        walk<DK, 1, 1>(stream, p);
+        fine ? walk_cols<T, DK, false, true>(stream, p) : walk_cols<T, DK, false, false>(stream, p);
     }
 }
 
-bool load_linear_chunk_kernels() {
-    return load_kernel_object(&linear_prepare_kernel<float, 64>);
-}
-
-ChunkPlan plan_chunks(const kvmem_hip_linear_args *a, uint32_t max_q) {
-    ChunkPlan pl;
-    if (max_q < kChunkFrom) {
-        return pl;
-    }
-    pl.chunked = true;
-    const uint32_t parts = a->type == KVMEM_TYPE_F32 ? 2 : 1;
-    pl.p_parts = !a->out ? 0 : a->out_type == KVMEM_TYPE_BF16 ? 1 : 2;
-    pl.chunks = (max_q + kChunk - 1) / kChunk;
-    pl.entries = a->n_tokens / kChunk + a->n_seq + 1;
-    pl.key_bytes = static_cast<uint64_t>(parts) * 12 * (a->head_dim_k / 32) * kFragBytes;
-    pl.head_bytes = kHeadBytes + ((a->beta ? 2 : 0) + pl.p_parts) * kLowerFrags * kFragBytes;
-    pl.cols = 16;
-    pl.bytes = pl.entries * (pl.key_bytes * a->n_head_k + pl.head_bytes * a->n_head);
-    return pl;
-}
-
-void launch_linear_chunks(hipStream_t stream, int type, uint32_t dim_k, const ChunkPlan &pl, const LinearParams &a,
-                          uint8_t *workspace) {
-    ChunkParams p{};
-    p.a = a;
-    p.keys = workspace;
-    p.heads = workspace + pl.entries * pl.key_bytes * (a.n_head / a.group);
-    p.key_bytes = pl.key_bytes;
-    p.head_bytes = pl.head_bytes;
-    p.chunks = pl.chunks;
-    p.type = type;
-    p.dim_k = dim_k;
-    p.delta = a.beta != nullptr;
-    p.outs = a.out != nullptr;
-    p.p_parts = static_cast<uint32_t>(pl.p_parts);
-    p.cols = pl.cols;
-    if (dim_k == 64) {
-        launch<64>(stream, p);
-    } else if (dim_k == 128) {
-        launch<128>(stream, p);
+template <typename T>
+static void launch_dims(hipStream_t stream, const ChunkParams &p) {
+    if (p.dim_k == 64) {
+        launch_type<T, 64>(stream, p);
+    } else if (p.dim_k == 128) {
+        launch_type<T, 128>(stream, p);
     } else {
-        launch<256>(stream, p);
+        launch_type<T, 256>(stream, p);
     }
 }
 
