@@ -23,7 +23,10 @@ namespace kvmem_hip {
 constexpr uint32_t kConvThreads = 256;
 constexpr uint32_t kConvWaves = kConvThreads / 64;
 constexpr uint32_t kConvChannels = 512;  // of a wave
-constexpr uint32_t kConvTile = 16;       // tokens of a wave's tile
+// Tokens of a wave's tile.  8191 tokens x 10240 channels of bf16, tiles of 8 / 16 / 32 /
+// 64: 77.6 / 70.0 / 73.6 / 76.6 us (rows read again where tiles begin, against waves
+// to fill the chip); 32 requests of 6 tokens 8.5 us with each.
+constexpr uint32_t kConvTile = 16;
 constexpr uint32_t kConvMaxWidth = 8;
 
 struct ConvParams {
@@ -43,15 +46,15 @@ struct ConvParams {
     float eps;
     bool silu;
     bool vec;                // 16 bytes at a time
+    bool weight_vec;
+    uint32_t tile;           // tokens
 };
 
-// The lane's 8 channels of a row; `n` of them exist.
-template <typename T>
-__device__ inline void load8(const uint8_t *p, bool vec, uint32_t n, RawRow<T, 8> &r) {
-    if (vec) {
-        if (n) {
-            load_raw<T, 8>(p, r);
-        }
+// The lane's 8 channels of a row; `n` of them exist (all or none where VEC).
+template <typename T, bool VEC>
+__device__ inline void load8(const uint8_t *p, uint32_t n, RawRow<T, 8> &r) {
+    if constexpr (VEC) {
+        load_raw<T, 8>(p, r);
         return;
     }
 #pragma unroll
@@ -65,9 +68,9 @@ __device__ inline void load8(const uint8_t *p, bool vec, uint32_t n, RawRow<T, 8
     }
 }
 
-template <typename T>
-__device__ inline void store8(uint8_t *p, bool vec, uint32_t n, const float x[8]) {
-    if (vec) {
+template <typename T, bool VEC>
+__device__ inline void store8(uint8_t *p, uint32_t n, const float x[8]) {
+    if constexpr (VEC) {
         if (n) {
             store_row<T, 8>(p, x);
         }
@@ -108,7 +111,43 @@ __device__ inline float silu(float y) {
     return y * __builtin_amdgcn_rcpf(1.0f + e);
 }
 
-template <typename T, int W>
+// The norm of a run: 1 / sqrt(sum of squares + eps) times y.
+__device__ inline void norm_run(const ConvParams &p, bool norm, float (&y)[8]) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        s = __builtin_fmaf(y[i], y[i], s);
+    }
+    s = sum_lanes(s, p.norm_lanes);
+    float f = __builtin_amdgcn_rsqf(s + p.eps);
+    // squares beyond fp32, or nothing of them left: fp64 holds them all
+    if (__builtin_expect(__any(norm && !(s < 0x1p126f && s + p.eps > 0x1p-100f)), 0)) {
+        double d = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            d = __builtin_fma(static_cast<double>(y[i]), static_cast<double>(y[i]), d);
+        }
+        for (uint32_t m = 1; m < p.norm_lanes; m <<= 1) {
+            d += __shfl_xor(d, static_cast<int>(m), 64);
+        }
+        d += static_cast<double>(p.eps);
+        const double g = d == 0.0 ? 0.0 : 1.0 / sqrt(d);
+        if (norm) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                y[i] = static_cast<float>(static_cast<double>(y[i]) * g);
+            }
+        }
+        f = 1.0f;
+    }
+    f = norm ? f : 1.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        y[i] *= f;
+    }
+}
+
+template <typename T, int W, bool VEC>
 __global__ __launch_bounds__(kConvThreads) void conv_rows_kernel(const ConvParams p) {
     constexpr int U = 4;  // rows requested together
     const uint32_t lane = threadIdx.x & 63u;
@@ -116,11 +155,12 @@ __global__ __launch_bounds__(kConvThreads) void conv_rows_kernel(const ConvParam
     if (unit >= p.units) {
         return;
     }
-    const uint32_t tile = unit / p.blocks;
-    const uint32_t c0 = ((unit % p.blocks) * 64u + lane) * 8u;
+    const uint32_t tile = unit / p.blocks, block = unit % p.blocks;
+    uint32_t c0 = (block * 64u + lane) * 8u;
     const uint32_t n = c0 < p.n_channels ? (p.n_channels - c0 < 8u ? p.n_channels - c0 : 8u) : 0u;
+    c0 = n ? c0 : 0u;  // lanes without channels read the first ones and store nothing
     const Request rq = request_of(p.batch, blockIdx.y);
-    const uint32_t t0 = tile * kConvTile;
+    const uint32_t t0 = tile * p.tile;
     if (tile != 0 && t0 >= rq.count) {
         return;
     }
@@ -128,16 +168,37 @@ __global__ __launch_bounds__(kConvThreads) void conv_rows_kernel(const ConvParam
     const uint8_t *x = p.x + rq.first * p.x_nb + c0 * sizeof(T);
     const uint64_t entry = static_cast<uint64_t>(rq.slot) * (W - 1) * row_bytes + c0 * sizeof(T);
     const bool old = p.state && rq.has_slot;
+    const uint32_t t1 = rq.count < t0 + p.tile ? rq.count : t0 + p.tile;
 
-    RawRow<T, 8> raw[U];
-    float h[W - 1 + U][8];
-    if (p.out) {
-        float w[W][8];
+    if (p.out && t0 < t1) {
+        float h[W - 1 + U][8];
+        RawRow<T, 8> raw[U];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int u = 0; u < U; ++u) {
+            load8<T, VEC>(x + (t0 + u < t1 ? t0 + u : t1 - 1) * p.x_nb, n, raw[u]);
+        }
+        RawRow<T, 8> before[W - 1];
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                w[j][i] = static_cast<uint32_t>(i) < n ? p.weight[static_cast<uint64_t>(c0 + i) * W + j] : 0.0f;
+        for (int j = 0; j < W - 1; ++j) {
+            before[j] = RawRow<T, 8>{};
+            if (tile != 0) {
+                load8<T, VEC>(x + (t0 - (W - 1) + j) * p.x_nb, n, before[j]);
+            } else if (old) {
+                load8<T, VEC>(p.state + entry + j * row_bytes, n, before[j]);
+            }
+        }
+        float w[8 * W];
+        const float *weight = p.weight + static_cast<uint64_t>(c0) * W;
+        if (VEC && p.weight_vec) {
+#pragma unroll
+            for (int i = 0; i < 2 * W; ++i) {
+                const float4 v = reinterpret_cast<const float4 *>(weight)[i];
+                w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8 * W; ++i) {
+                w[i] = static_cast<uint32_t>(i / W) < n ? weight[i] : 0.0f;
             }
         }
         float bias[8];
@@ -147,30 +208,27 @@ __global__ __launch_bounds__(kConvThreads) void conv_rows_kernel(const ConvParam
         }
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) {
-            RawRow<T, 8> r{};
-            if (tile != 0) {
-                load8<T>(x + (t0 - (W - 1) + j) * p.x_nb, p.vec, n, r);
-            } else if (old) {
-                load8<T>(p.state + entry + j * row_bytes, p.vec, n, r);
-            }
-            widen<T, 8>(r, h[j]);
+            widen<T, 8>(before[j], h[j]);
         }
-        const uint32_t t1 = rq.count < t0 + kConvTile ? rq.count : t0 + kConvTile;
-        const bool norm = c0 < p.norm_channels;
-        const bool any_norm = __builtin_amdgcn_readfirstlane(c0) < p.norm_channels;
+        const bool norm = n && c0 < p.norm_channels;
+        const bool any_norm = block * kConvChannels < p.norm_channels;
+        uint8_t *out = p.out + static_cast<uint64_t>(rq.first) * row_bytes + c0 * sizeof(T);
         for (uint32_t t = t0; t < t1; t += U) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                raw[u] = RawRow<T, 8>{};
-                if (t + u < t1) {
-                    load8<T>(x + (t + u) * p.x_nb, p.vec, n, raw[u]);
+                widen<T, 8>(raw[u], h[W - 1 + u]);
+            }
+            if (t + U < t1) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const uint32_t at = t + U + u;
+                    load8<T, VEC>(x + (at < t1 ? at : t1 - 1) * p.x_nb, n, raw[u]);
                 }
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                widen<T, 8>(raw[u], h[W - 1 + u]);
                 if (t + u >= t1) {
-                    continue;
+                    break;
                 }
                 float y[8];
 #pragma unroll
@@ -178,47 +236,19 @@ __global__ __launch_bounds__(kConvThreads) void conv_rows_kernel(const ConvParam
                     y[i] = bias[i];
 #pragma unroll
                     for (int j = 0; j < W; ++j) {
-                        y[i] = __builtin_fmaf(w[j][i], h[u + j][i], y[i]);
+                        y[i] = __builtin_fmaf(w[i * W + j], h[u + j][i], y[i]);
                     }
-                    if (p.silu) {
+                }
+                if (p.silu) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
                         y[i] = silu<sizeof(T) == 4>(y[i]);
                     }
                 }
                 if (any_norm) {
-                    float s = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        s = __builtin_fmaf(y[i], y[i], s);
-                    }
-                    s = sum_lanes(s, p.norm_lanes);
-                    float f = __builtin_amdgcn_rsqf(s + p.eps);
-                    // squares beyond fp32, or nothing of them left: fp64 holds them all
-                    if (__builtin_expect(__any(norm && !(s < 0x1p126f && s + p.eps > 0x1p-100f)), 0)) {
-                        double d = 0.0;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            d = __builtin_fma(static_cast<double>(y[i]), static_cast<double>(y[i]), d);
-                        }
-                        for (uint32_t m = 1; m < p.norm_lanes; m <<= 1) {
-                            d += __shfl_xor(d, static_cast<int>(m), 64);
-                        }
-                        d += static_cast<double>(p.eps);
-                        const double g = d == 0.0 ? 0.0 : 1.0 / sqrt(d);
-                        if (norm) {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                y[i] = static_cast<float>(static_cast<double>(y[i]) * g);
-                            }
-                        }
-                        f = 1.0f;
-                    }
-                    f = norm ? f : 1.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        y[i] *= f;
-                    }
+                    norm_run(p, norm, y);
                 }
-                store8<T>(p.out + (rq.first + t + u) * row_bytes + c0 * sizeof(T), p.vec, n, y);
+                store8<T, VEC>(out + (t + u) * row_bytes, n, y);
             }
 #pragma unroll
             for (int j = 0; j < W - 1; ++j) {
@@ -237,13 +267,13 @@ __global__ __launch_bounds__(kConvThreads) void conv_rows_kernel(const ConvParam
             const uint32_t at = rq.count + j;
             RawRow<T, 8> r{};
             if (at >= W - 1) {
-                load8<T>(x + static_cast<uint64_t>(at - (W - 1)) * p.x_nb, p.vec, n, r);
+                load8<T, VEC>(x + static_cast<uint64_t>(at - (W - 1)) * p.x_nb, n, r);
             } else if (old) {
-                load8<T>(p.state + entry + at * row_bytes, p.vec, n, r);
+                load8<T, VEC>(p.state + entry + at * row_bytes, n, r);
             }
             float v[8];
             widen<T, 8>(r, v);
-            store8<T>(p.state_out + entry + j * row_bytes, p.vec, n, v);
+            store8<T, VEC>(p.state_out + entry + j * row_bytes, n, v);
         }
     }
 }
@@ -252,7 +282,11 @@ template <typename T, int W>
 static void launch_conv(hipStream_t stream, uint32_t width, dim3 grid, const ConvParams &p) {
     if constexpr (W <= static_cast<int>(kConvMaxWidth)) {
         if (width == W) {
-            conv_rows_kernel<T, W><<<grid, kConvThreads, 0, stream>>>(p);
+            if (p.vec) {
+                conv_rows_kernel<T, W, true><<<grid, kConvThreads, 0, stream>>>(p);
+            } else {
+                conv_rows_kernel<T, W, false><<<grid, kConvThreads, 0, stream>>>(p);
+            }
         } else {
             launch_conv<T, W + 1>(stream, width, grid, p);
         }
@@ -260,7 +294,7 @@ static void launch_conv(hipStream_t stream, uint32_t width, dim3 grid, const Con
 }
 
 bool load_conv_rows_kernels() {
-    return load_kernel_object(&conv_rows_kernel<float, 2>);
+    return load_kernel_object(&conv_rows_kernel<float, 2, true>);
 }
 
 }  // namespace kvmem_hip
@@ -342,7 +376,9 @@ int kvmem_hip_conv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_conv_args *a) {
     p.vec = rows % 16 == 0 && a->n_channels % 8 == 0;
     p.blocks = (a->n_channels + kConvChannels - 1) / kConvChannels;
     const uint32_t most = std::min(p.batch.max_q, a->n_tokens);
-    const uint64_t tiles = a->out ? std::max(1u, (most + kConvTile - 1) / kConvTile) : 1u;
+    p.weight_vec = reinterpret_cast<uintptr_t>(a->weight) % 16 == 0;
+    p.tile = kConvTile;
+    const uint64_t tiles = a->out ? std::max(1u, (most + p.tile - 1) / p.tile) : 1u;
     const uint64_t units = tiles * p.blocks;
     // a dispatch counts its work items in 32 bits
     if ((units + kConvWaves - 1) / kConvWaves * kConvThreads * a->n_seq >= uint64_t{1} << 32) {
