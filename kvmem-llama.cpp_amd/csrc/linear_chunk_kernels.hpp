@@ -21,8 +21,8 @@
 //
 // Precision: operands are f16 parts of scaled fp32 numbers.  Each matrix (for S, D
 // and their like each column) is scaled by a power of two that puts its largest
-// element into [2^11, 2^12), then split into a high and a low f16 part: together 22
-// bits, and what lies below 2^-36 of the largest is cut.  16-bit keys and queries
+// element into [2^14, 2^15), then split into a high and a low f16 part: together 22
+// bits, and what lies below 2^-39 of the largest is cut.  16-bit keys and queries
 // are one part, exactly.  Products of two split factors leave out low x low.  What
 // reaches only a 16-bit result takes fewer parts: for a bf16 out (half a step
 // 2^-9) the scores, D and S enter the output's products by their high part (half a
@@ -60,10 +60,10 @@ __device__ inline uint64_t entry_of(const Request &rq, uint32_t s, uint32_t c) {
 }
 
 // The power of two that brings numbers whose largest magnitude has the bits `m`
-// into [2^11, 2^12): x * 2^-e.  Kept inside what one fp32 factor can be.
+// into [2^14, 2^15): x * 2^-e.  Kept inside what one fp32 factor can be.
 __device__ inline int scale_exp(uint32_t m) {
-    const int e = static_cast<int>(m >> 23) - (127 + 11);
-    return m == 0 ? 0 : e < -100 ? -100 : e > 116 ? 116 : e;
+    const int e = static_cast<int>(m >> 23) - (127 + 14);
+    return m == 0 ? 0 : e < -100 ? -100 : e > 113 ? 113 : e;
 }
 __device__ inline float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 __device__ inline uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
