@@ -164,9 +164,29 @@ bool load_linear_kernels() {
            load_linear_chunks_f16() && load_linear_chunks_bf16();
 }
 
+// Tokens a request from which a call goes by chunks.  A chunk costs the same for one
+// token as for 64, and the chunks' kernels take longer to begin; token by token, a wave
+// alone on its SIMD needs 1.2 us a token, and many share the FMAs.  Measured, us by
+// chunks / by tokens, 48 heads of 128 x 128 (192 waves of states a request):
+//   bf16, 1 request    16 tokens 20.2 /  22.2    12 tokens  20.1 /  17.5
+//   bf16, 8 requests   24 tokens 40.4 /  37.7    32 tokens  40.8 /  47.1
+//   bf16, 64 requests  48 tokens 238  /  233     64 tokens  241  /  303
+//   F32, 1 request     16 tokens 23.5 /  22.1    24 tokens  23.9 /  31.5
+//   F32, 8 requests    32 tokens 61.8 /  47.3    48 tokens  62.5 /  67.2
+//   F32, 64 requests  128 tokens 687  /  599; a chunk of 64 more costs 219 / 284
+// 16 heads of 256 x 256 (64 requests: 56 tokens) and 8 of 64 x 64 cross near there.
+static uint32_t chunk_from(const kvmem_hip_linear_args *a) {
+    const uint64_t waves = static_cast<uint64_t>(a->n_seq) * a->n_head * (a->head_dim_v / kStepCols);
+    const bool f32 = a->type == KVMEM_TYPE_F32;
+    if (waves < 4096) {
+        return f32 && waves >= 1024 ? 48 : 24;
+    }
+    return f32 ? 256 : 56;
+}
+
 static ChunkPlan plan_chunks(const kvmem_hip_linear_args *a, uint32_t max_q) {
     ChunkPlan pl;
-    if (max_q < kChunkFrom) {
+    if (max_q < chunk_from(a)) {
         return pl;
     }
     pl.chunked = true;

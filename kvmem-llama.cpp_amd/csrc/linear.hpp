@@ -30,8 +30,6 @@ constexpr uint32_t kChunk = 64;
 constexpr uint32_t kPrepThreads = 256;
 constexpr uint32_t kXcds = 8;
 
-constexpr uint32_t kChunkFrom = 24;  // tokens a request from which a call goes by chunks
-
 struct ChunkPlan {
     bool chunked = false;
     int p_parts = 0;        // f16 parts of the scores (0: no out)

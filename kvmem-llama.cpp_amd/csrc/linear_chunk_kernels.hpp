@@ -51,6 +51,7 @@ struct ChunkHead {
     float from_first[kChunk];  // e^G_i
     float to_last[kChunk];     // e^(G_last - G_i)
     int32_t exp_k, exp_q, exp_t, exp_p;
+    int32_t exp_last;          // of the largest to_last: 0 unless decays grow
     uint32_t by_token;         // a number that is not finite
 };
 static_assert(sizeof(ChunkHead) <= kHeadBytes, "");
@@ -60,14 +61,13 @@ __device__ inline uint64_t entry_of(const Request &rq, uint32_t s, uint32_t c) {
 }
 
 // The power of two that brings numbers whose largest magnitude has the bits `m`
-// into [2^14, 2^15): x * 2^-e.  Kept inside what one fp32 factor can be.
-__device__ inline int scale_exp(uint32_t m) {
-    const int e = static_cast<int>(m >> 23) - (127 + 14);
-    return m == 0 ? 0 : e < -100 ? -100 : e > 113 ? 113 : e;
-}
+// into [2^14, 2^15): x * 2^-e.  At least -100, so that 2^-e is an fp32 number.
+__device__ inline int scale_exp(uint32_t m) { return max(static_cast<int>(m >> 23) - (127 + 14), -100); }
 __device__ inline float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 __device__ inline uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 constexpr uint32_t kInf = 0x7f800000u;
+
+#define KVMEM_MFMA16(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0)
 
 // ------------------------------------------------------------------- prepare
 
@@ -188,29 +188,72 @@ __device__ inline uint32_t lower_frag(uint32_t m, uint32_t k) { return m < 2 ? m
 
 // c += a b over 16 indices, fp32: a row of `a` is read from LDS rows, b's rows
 // 4g..4g+3 of column lane % 16 are in registers (as an accumulator holds them).
-__device__ inline f32x4_t mul16(const float *a_rows, f32x4_t b, f32x4_t c) {
+// `take`: whether the lane's four numbers of `a` count (else zeros).
+__device__ inline f32x4_t mul16(const float *a_rows, f32x4_t b, f32x4_t c, bool take = true) {
     const uint32_t lane = threadIdx.x & 63u;
-    const float4 a = *reinterpret_cast<const float4 *>(a_rows + (lane & 15u) * kTriPitch + 4u * (lane >> 4));
+    float4 a = *reinterpret_cast<const float4 *>(a_rows + (lane & 15u) * kTriPitch + 4u * (lane >> 4));
+    a.x = take ? a.x : 0.0f, a.y = take ? a.y : 0.0f, a.z = take ? a.z : 0.0f, a.w = take ? a.w : 0.0f;
     c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x, b[0], c, 0, 0, 0);
     c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.y, b[1], c, 0, 0, 0);
     c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.z, b[2], c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a.w, b[3], c, 0, 0, 0);
 }
 
-// K's and Q's parts, later A, T and P.
+// K's and Q's parts, later A (then P) and T.
 template <int DK, int PARTS> constexpr uint32_t prep_lds() {
     constexpr uint32_t rows = 2u * PARTS * kChunk * (DK + 8) * 2u;
-    constexpr uint32_t tri = 3u * kChunk * kTriPitch * 4u;
+    constexpr uint32_t tri = 2u * kChunk * kTriPitch * 4u;
     return rows > tri ? rows : tri;
 }
 
-template <typename T, int DK>
-__global__ __launch_bounds__(kPrepThreads) void linear_prepare_kernel(const ChunkParams p) {
+// Decays and beta of a chunk's tokens in one head, one token a lane (every wave holds
+// them): G is the running sum of log_decay.
+struct ChunkGates {
+    double G;
+    float beta;
+    bool odd;  // a gate that is not finite (or a decay that grows without bound)
+};
+
+__device__ inline ChunkGates load_gates(const ChunkParams &p, uint64_t row0, uint32_t n, uint32_t h) {
+    const uint32_t lane = threadIdx.x & 63u;
+    float decay = 0.0f;
+    ChunkGates x{0.0, 0.0f, false};
+    if (lane < n) {
+        if (p.a.decay) {
+            decay = *reinterpret_cast<const float *>(p.a.decay + (row0 + lane) * p.a.decay_nb + h * 4u);
+        }
+        if (p.delta) {
+            x.beta = *reinterpret_cast<const float *>(p.a.beta + (row0 + lane) * p.a.beta_nb + h * 4u);
+        }
+    }
+    x.odd = !(decay < INFINITY) || !(mag(x.beta) < kInf);
+    x.G = decay < -1e5f ? -1e5 : static_cast<double>(decay);
+    if (p.a.decay) {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const double y = __shfl_up(x.G, d, 64);
+            x.G += lane >= static_cast<uint32_t>(d) ? y : 0.0;
+        }
+    }
+    return x;
+}
+
+// e^x of a difference of sums: the rounding of x log2 e costs |x| 2^-25 of a result
+// that falls as e^x, so at most 2^-25 of 1.
+__device__ inline float exp_diff(double x) {
+    return __builtin_amdgcn_exp2f(static_cast<float>(x * 0x1.71547652b82fep+0));
+}
+
+// A workgroup takes `heads` heads of one key head, for which K K^T and Q K^T are the
+// same: all of them where workgroups are many, one where they are few.
+template <typename T, int DK, bool DELTA>
+__global__ __launch_bounds__(kPrepThreads, DK <= 128 ? 3 : 1) void linear_prepare_kernel(const ChunkParams p, const uint32_t heads) {
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
     constexpr int KS = DK / 32;
     __shared__ __align__(16) uint8_t lds[prep_lds<DK, PARTS>()];
     __shared__ uint32_t words[16];
-    const uint32_t h = blockIdx.x % p.a.n_head, c = blockIdx.x / p.a.n_head, s = blockIdx.y;
+    const uint32_t per = p.a.n_head / heads;
+    const uint32_t h0 = blockIdx.x % per * heads, c = blockIdx.x / per, s = blockIdx.y;
     const Request rq = request_of(p.a.batch, s);
     if (c * kChunk >= rq.count) {
         return;
@@ -218,54 +261,29 @@ __global__ __launch_bounds__(kPrepThreads) void linear_prepare_kernel(const Chun
     const uint32_t n = min(kChunk, rq.count - c * kChunk);
     const uint64_t row0 = static_cast<uint64_t>(rq.first) + c * kChunk;
     const uint64_t entry = entry_of(rq, s, c);
-    const uint32_t hk = h / p.a.group;
+    const uint32_t hk = h0 / p.a.group;
     uint8_t *keys = p.keys + (entry * (p.a.n_head / p.a.group) + hk) * p.key_bytes;
-    uint8_t *head = p.heads + (entry * p.a.n_head + h) * p.head_bytes;
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-    // decays: every wave has all 64 sums, one a lane
-    float decay = 0.0f, beta = 0.0f;
-    if (lane < n) {
-        if (p.a.decay) {
-            decay = *reinterpret_cast<const float *>(p.a.decay + (row0 + lane) * p.a.decay_nb + h * 4u);
-        }
-        if (p.delta) {
-            beta = *reinterpret_cast<const float *>(p.a.beta + (row0 + lane) * p.a.beta_nb + h * 4u);
-        }
-    }
-    bool odd = !(decay < INFINITY) || !(mag(beta) < kInf);
-    double G = decay < -1e5f ? -1e5 : static_cast<double>(decay);
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
-        const double y = __shfl_up(G, x, 64);
-        G += lane >= static_cast<uint32_t>(x) ? y : 0.0;
-    }
-    const double G_last = __shfl(G, 63, 64);
-    const float from_first = expf(static_cast<float>(G));
-    const float to_last = expf(static_cast<float>(G_last - G));
-    odd = odd || !(from_first < INFINITY) || !(to_last < INFINITY);
-
-    RawRow<T, 8> raw_k[KS], raw_q[KS];
+    RawRow<T, 8> raw_k[KS], raw_q[KS] = {};  // without an out: no queries, zeros
     load_rows<T, DK>(p.a.k + row0 * p.a.k_nb2 + hk * p.a.k_nb1, p.a.k_nb2, n, raw_k);
-    uint32_t mk = max_mag<T, DK>(raw_k), mq = 0;
     if (p.outs) {
         load_rows<T, DK>(p.a.q + row0 * p.a.q_nb2 + hk * p.a.q_nb1, p.a.q_nb2, n, raw_q);
-        mq = max_mag<T, DK>(raw_q);
     }
+    ChunkGates gates = load_gates(p, row0, n, h0);
+    uint32_t mk = max_mag<T, DK>(raw_k), mq = max_mag<T, DK>(raw_q);
     block_max2(mk, mq, words);
-    odd = odd || mk >= kInf || mq >= kInf;
+    const bool odd_rows = mk >= kInf || mq >= kInf;
     const int exp_k = scale_exp(mk), exp_q = scale_exp(mq);
     _Float16 *k16 = reinterpret_cast<_Float16 *>(lds);
     _Float16 *q16 = k16 + PARTS * kChunk * (DK + 8);
     put_rows<T, DK, PARTS>(raw_k, pow2(-exp_k), k16);
-    if (p.outs) {
-        put_rows<T, DK, PARTS>(raw_q, pow2(-exp_q), q16);
-    }
+    put_rows<T, DK, PARTS>(raw_q, pow2(-exp_q), q16);
     __syncthreads();
 
     // the key head's operands, by its first head
-    if (h % p.a.group == 0) {
+    if (h0 % p.a.group == 0) {
 #pragma unroll
         for (uint32_t part = 0; part < PARTS; ++part) {
             const _Float16 *kp = k16 + part * kChunk * (DK + 8);
@@ -274,9 +292,7 @@ __global__ __launch_bounds__(kPrepThreads) void linear_prepare_kernel(const Chun
 #pragma unroll
             for (uint32_t k = 0; k < KS; ++k) {
                 put_frag(out, w * KS + k, row_frag<DK>(kp, w, k));
-                if (p.outs) {
-                    put_frag(out, 4u * KS + w * KS + k, row_frag<DK>(qp, w, k));
-                }
+                put_frag(out, 4u * KS + w * KS + k, row_frag<DK>(qp, w, k));
             }
 #pragma unroll
             for (uint32_t i = 0; i < KS; ++i) {  // 2 KS tiles of 16 columns x 2 halves, over 4 waves
@@ -302,153 +318,183 @@ __global__ __launch_bounds__(kPrepThreads) void linear_prepare_kernel(const Chun
             if constexpr (PARTS == 2) {
                 b2 = row_frag<DK>(k16 + kChunk * (DK + 8), j, k);
             }
-            if (p.delta) {
-                kk[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, kk[j], 0, 0, 0);
+            if constexpr (DELTA) {
+                kk[j] = KVMEM_MFMA16(a, b, kk[j]);
                 if constexpr (PARTS == 2) {
                     a2 = row_frag<DK>(k16 + kChunk * (DK + 8), w, k);
-                    kk[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b2, kk[j], 0, 0, 0);
-                    kk[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a2, b, kk[j], 0, 0, 0);
+                    kk[j] = KVMEM_MFMA16(a, b2, kk[j]);
+                    kk[j] = KVMEM_MFMA16(a2, b, kk[j]);
                 }
             }
-            if (p.outs) {
-                const half8_t aq = row_frag<DK>(q16, w, k);
-                qk[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(aq, b, qk[j], 0, 0, 0);
-                if constexpr (PARTS == 2) {
-                    a2 = row_frag<DK>(q16 + kChunk * (DK + 8), w, k);
-                    qk[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(aq, b2, qk[j], 0, 0, 0);
-                    qk[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a2, b, qk[j], 0, 0, 0);
-                }
+            const half8_t aq = row_frag<DK>(q16, w, k);
+            qk[j] = KVMEM_MFMA16(aq, b, qk[j]);
+            if constexpr (PARTS == 2) {
+                a2 = row_frag<DK>(q16 + kChunk * (DK + 8), w, k);
+                qk[j] = KVMEM_MFMA16(aq, b2, qk[j]);
+                qk[j] = KVMEM_MFMA16(a2, b, qk[j]);
             }
         }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            kk[j][r] = __builtin_amdgcn_ldexpf(kk[j][r], 2 * exp_k);
+            qk[j][r] = __builtin_amdgcn_ldexpf(qk[j][r], exp_k + exp_q) * p.a.scale;
+        }
+        __builtin_amdgcn_sched_barrier(0);  // a tile's operands at a time: registers for four waves a SIMD
     }
-    __syncthreads();  // K and Q are read: A, T and P take their place
     float *tri_a = reinterpret_cast<float *>(lds);
     float *tri_t = tri_a + kChunk * kTriPitch;
-    float *tri_p = tri_t + kChunk * kTriPitch;
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-        if (j > w) {
-            continue;
+    for (uint32_t h = h0; h < h0 + heads; ++h) {
+        uint8_t *head = p.heads + (entry * p.a.n_head + h) * p.head_bytes;
+        if (h != h0) {
+            gates = load_gates(p, row0, n, h);
         }
-        const uint32_t col = 16u * j + (lane & 15u);
-        const double Gj = __shfl(G, static_cast<int>(col), 64);
+        const double G = gates.G, G_last = __shfl(G, 63, 64);
+        const float beta = gates.beta;
+        const float from_first = expf(static_cast<float>(G)), to_last = expf(static_cast<float>(G_last - G));
+        bool odd = odd_rows || gates.odd || !(from_first < INFINITY) || !(to_last < INFINITY);
+        __syncthreads();  // K and Q, or the head before, are read: A and T take their place
+        double Gi[4];
+        float bi[4];
 #pragma unroll
         for (uint32_t r = 0; r < 4; ++r) {
-            const uint32_t i = 16u * w + 4u * g + r;
-            const double Gi = __shfl(G, static_cast<int>(i), 64);
-            const float bi = __shfl(beta, static_cast<int>(i), 64);
-            const float f = expf(static_cast<float>(Gi - Gj));
-            if (p.delta) {
-                tri_a[i * kTriPitch + col] =
-                    col < i ? __builtin_amdgcn_ldexpf(kk[j][r] * f, 2 * exp_k) * bi : 0.0f;
-            }
-            if (p.outs) {
-                tri_p[i * kTriPitch + col] =
-                    col <= i ? __builtin_amdgcn_ldexpf(qk[j][r] * f, exp_k + exp_q) * p.a.scale : 0.0f;
-            }
+            const int i = static_cast<int>(16u * w + 4u * g + r);
+            Gi[r] = __shfl(G, i, 64);
+            bi[r] = __shfl(beta, i, 64);
         }
-    }
-    if (p.delta) {
-        __syncthreads();
-        // 1 + A's diagonal blocks inverted by forward substitution: lane (any, c) has
-        // column c of block w
-        const float *a = tri_a + 16u * w * kTriPitch + 16u * w;
-        float x[16];
+        f32x4_t pk[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float y = (lane & 15u) == static_cast<uint32_t>(i) ? 1.0f : 0.0f;
-#pragma unroll
-            for (int k = 0; k < i; ++k) {
-                y = __builtin_fmaf(-a[i * kTriPitch + k], x[k], y);
+        for (uint32_t j = 0; j < 4; ++j) {
+            if (j > w) {
+                continue;
             }
-            x[i] = y;
-        }
-        float *t = tri_t + 16u * w * kTriPitch + 16u * w;
-        if (g == 0) {
+            const uint32_t col = 16u * j + (lane & 15u);
+            const double Gj = __shfl(G, static_cast<int>(col), 64);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                t[i * kTriPitch + lane] = x[i];
+            for (uint32_t r = 0; r < 4; ++r) {
+                const uint32_t i = 16u * w + 4u * g + r;
+                const float f = p.a.decay ? exp_diff(Gi[r] - Gj) : 1.0f;
+                if constexpr (DELTA) {
+                    tri_a[i * kTriPitch + col] = col < i ? kk[j][r] * f * bi[r] : 0.0f;
+                }
+                pk[j][r] = qk[j][r] * f;
             }
         }
-        __syncthreads();
-        // column w of blocks downwards: T_iw = -T_ii sum_k A_ik T_kw
-        f32x4_t col[4];
-        const float bw = __shfl(beta, static_cast<int>(16u * w + (lane & 15u)), 64);
+        if constexpr (DELTA) {
+            __syncthreads();
+            // 1 + A's diagonal block w: its two 8 x 8 diagonal blocks inverted by forward
+            // substitution (lane (any, b, c) has column c of block b), together D; with L the
+            // block below them, the inverse is D - D L D
+            const uint32_t c8 = lane & 7u, b8 = lane & 8u;
+            float *a = tri_a + 16u * w * kTriPitch + 16u * w;
+            float *t = tri_t + 16u * w * kTriPitch + 16u * w;
+            float x[8];
 #pragma unroll
-        for (uint32_t r = 0; r < 4; ++r) {
-            col[0][r] = t[(4u * g + r) * kTriPitch + (lane & 15u)];
-        }
-        f32x4_t first = col[0];
+            for (uint32_t i = 0; i < 8; ++i) {
+                float y = c8 == i ? 1.0f : 0.0f;
 #pragma unroll
-        for (uint32_t d = 1; d < 4; ++d) {
-            col[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            if (w + d < 4) {
-                f32x4_t y = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (uint32_t k = 0; k < i; ++k) {
+                    y = __builtin_fmaf(-a[(b8 + i) * kTriPitch + b8 + k], x[k], y);
+                }
+                x[i] = y;
+            }
+            if (g < 2) {  // group 0 the blocks, group 1 the zeros beside them
 #pragma unroll
-                for (uint32_t k = 0; k < 3; ++k) {
-                    if (k < d) {
-                        y = mul16(tri_a + 16u * (w + d) * kTriPitch + 16u * (w + k), col[k], y);
+                for (uint32_t i = 0; i < 8; ++i) {
+                    t[(b8 + i) * kTriPitch + (g == 0 ? b8 : b8 ^ 8u) + c8] = g == 0 ? x[i] : 0.0f;
+                }
+            }
+            __syncthreads();
+            f32x4_t col[4];
+            const float bw = __shfl(beta, static_cast<int>(16u * w + (lane & 15u)), 64);
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) {
+                col[0][r] = t[(4u * g + r) * kTriPitch + (lane & 15u)];
+            }
+            f32x4_t ld = mul16(a, col[0], f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, (lane & 15u) >= 8u && g < 2);
+            ld = mul16(t, ld, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+            col[0] -= ld;
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) {
+                t[(4u * g + r) * kTriPitch + (lane & 15u)] = col[0][r];
+            }
+            __syncthreads();
+            // column w of blocks downwards: T_iw = -T_ii sum_k A_ik T_kw
+#pragma unroll
+            for (uint32_t d = 1; d < 4; ++d) {
+                col[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                if (w + d < 4) {
+                    f32x4_t y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (uint32_t k = 0; k < 3; ++k) {
+                        if (k < d) {
+                            y = mul16(tri_a + 16u * (w + d) * kTriPitch + 16u * (w + k), col[k], y);
+                        }
+                    }
+                    y = mul16(tri_t + 16u * (w + d) * kTriPitch + 16u * (w + d), y, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+                    col[d] = -y;
+                }
+            }
+            __syncthreads();  // A and the diagonal blocks are read
+#pragma unroll
+            for (uint32_t d = 0; d < 4; ++d) {
+                if (w + d < 4) {
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; ++r) {
+                        tri_t[(16u * (w + d) + 4u * g + r) * kTriPitch + 16u * w + (lane & 15u)] = col[d][r] * bw;
                     }
                 }
-                y = mul16(tri_t + 16u * (w + d) * kTriPitch + 16u * (w + d), y, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
-                col[d] = -y;
             }
         }
-        __syncthreads();  // the diagonal blocks are read: they are scaled by beta now too
 #pragma unroll
-        for (uint32_t d = 0; d < 4; ++d) {
-            if (w + d < 4) {
+        for (uint32_t j = 0; j < 4; ++j) {
+            if (j > w) {
+                continue;
+            }
 #pragma unroll
-                for (uint32_t r = 0; r < 4; ++r) {
-                    const float y = d == 0 ? first[r] : col[d][r];
-                    tri_t[(16u * (w + d) + 4u * g + r) * kTriPitch + 16u * w + (lane & 15u)] = y * bw;
-                }
+            for (uint32_t r = 0; r < 4; ++r) {
+                tri_a[(16u * w + 4u * g + r) * kTriPitch + 16u * j + (lane & 15u)] = pk[j][r];
             }
         }
-    }
-    __syncthreads();
-    float xt[2][8], xp[2][8];
-    uint32_t mt = 0, mp = 0;
+        __syncthreads();
+        float xt[2][8], xp[2][8];
+        uint32_t mt = 0, mp = 0;
 #pragma unroll
-    for (uint32_t k = 0; k < 2; ++k) {
-        if (k > w / 2) {
-            continue;
-        }
-        if (p.delta) {
-            tri_row(tri_t, w, k, xt[k]);
-        }
-        if (p.outs) {
-            tri_row(tri_p, w, k, xp[k]);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            mt = p.delta ? max(mt, mag(xt[k][i])) : 0u;
-            mp = p.outs ? max(mp, mag(xp[k][i])) : 0u;
-        }
-    }
-    block_max2(mt, mp, words + 8);
-    odd = odd || mt >= kInf || mp >= kInf;
-    const int exp_t = scale_exp(mt), exp_p = scale_exp(mp);
-#pragma unroll
-    for (uint32_t k = 0; k < 2; ++k) {
-        if (k > w / 2) {
-            continue;
-        }
-        const uint32_t f = lower_frag(w, k);
-        uint8_t *at = head + kHeadBytes;
-        half8_t hi, lo;
-        if (p.delta) {
+        for (uint32_t k = 0; k < 2; ++k) {
+            if (k > w / 2) {
+                continue;
+            }
+            if constexpr (DELTA) {
+                tri_row(tri_t, w, k, xt[k]);
+            }
+            tri_row(tri_a, w, k, xp[k]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float y = xt[k][i] * pow2(-exp_t);
-                hi[i] = static_cast<_Float16>(y);
-                lo[i] = static_cast<_Float16>(y - static_cast<float>(hi[i]));
+                mt = DELTA ? max(mt, mag(xt[k][i])) : 0u;
+                mp = max(mp, mag(xp[k][i]));
             }
-            put_frag(at, f, hi);
-            put_frag(at, kLowerFrags + f, lo);
-            at += 2u * kLowerFrags * kFragBytes;
         }
-        if (p.outs) {
+        block_max2(mt, mp, words + 8);
+        odd = odd || mt >= kInf || mp >= kInf;
+        const int exp_t = scale_exp(mt), exp_p = scale_exp(mp);
+#pragma unroll
+        for (uint32_t k = 0; k < 2; ++k) {
+            if (k > w / 2) {
+                continue;
+            }
+            const uint32_t f = lower_frag(w, k);
+            uint8_t *at = head + kHeadBytes;
+            half8_t hi, lo;
+            if constexpr (DELTA) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float y = xt[k][i] * pow2(-exp_t);
+                    hi[i] = static_cast<_Float16>(y);
+                    lo[i] = static_cast<_Float16>(y - static_cast<float>(hi[i]));
+                }
+                put_frag(at, f, hi);
+                put_frag(at, kLowerFrags + f, lo);
+                at += 2u * kLowerFrags * kFragBytes;
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float y = xp[k][i] * pow2(-exp_p);
@@ -460,18 +506,26 @@ __global__ __launch_bounds__(kPrepThreads) void linear_prepare_kernel(const Chun
                 put_frag(at, kLowerFrags + f, lo);
             }
         }
-    }
-    if (w == 0) {
-        ChunkHead *out = reinterpret_cast<ChunkHead *>(head);
-        out->from_first[lane] = from_first;
-        out->to_last[lane] = to_last;
-        const bool any = __any(odd);
-        if (lane == 0) {
-            out->exp_k = exp_k;
-            out->exp_q = exp_q;
-            out->exp_t = exp_t;
-            out->exp_p = exp_p;
-            out->by_token = any;
+        if (w == 0) {
+            ChunkHead *out = reinterpret_cast<ChunkHead *>(head);
+            out->from_first[lane] = from_first;
+            out->to_last[lane] = to_last;
+            const bool any = __any(odd);
+            uint32_t top = mag(to_last);
+#pragma unroll
+            for (int x = 1; x < 64; x <<= 1) {
+                top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), x, 64)));
+            }
+            // to_last <= 2^exp_last; the last token's is 1
+            const int exp_last = top == __float_as_uint(1.0f) ? 0 : static_cast<int>(top >> 23) - 126;
+            if (lane == 0) {
+                out->exp_k = exp_k;
+                out->exp_q = exp_q;
+                out->exp_t = exp_t;
+                out->exp_p = exp_p;
+                out->exp_last = exp_last;
+                out->by_token = any;
+            }
         }
     }
 }
@@ -518,14 +572,18 @@ template <int TILES> __device__ inline float lane_max(const f32x4_t (&x)[TILES])
 }
 
 // A column's numbers (tiles of 16 rows, 4 of each in every lane of the column) as
-// two f16 parts of x * 2^-e, e the column's own.  The mixed-precision FMAs round
+// two f16 parts of x * 2^-e, or their high parts alone.  The mixed-precision FMAs round
 // x f and x f - high to f16 without a step in fp32: two instructions a number.  No
 // number here is a matrix instruction's own result (its readers would have to wait
 // inside the block); an instruction stands between a half word's write and its use.
+template <int TILES> __device__ inline int column_exp(const f32x4_t (&x)[TILES]) {
+    return scale_exp(column_max(__float_as_uint(lane_max<TILES>(x))));
+}
+
+typedef uint32_t words4_t __attribute__((ext_vector_type(4)));
+
 template <int TILES>
-__device__ inline int split(const f32x4_t (&x)[TILES], half8_t (&hi)[TILES / 2], half8_t (&lo)[TILES / 2]) {
-    const float m = lane_max<TILES>(x);
-    const int e = scale_exp(column_max(__float_as_uint(m)));
+__device__ inline void split(const f32x4_t (&x)[TILES], int e, half8_t (&hi)[TILES / 2], half8_t (&lo)[TILES / 2]) {
     const float f = pow2(-e);
 #pragma unroll
     for (int t = 0; t < TILES; t += 2) {
@@ -544,18 +602,13 @@ __device__ inline int split(const f32x4_t (&x)[TILES], half8_t (&hi)[TILES / 2],
                 : "=&v"(h[2 * u]), "=&v"(h[2 * u + 1]), "=&v"(l[2 * u]), "=&v"(l[2 * u + 1])
                 : "v"(x[t + u][0]), "v"(x[t + u][1]), "v"(x[t + u][2]), "v"(x[t + u][3]), "v"(f));
         }
-        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-        hi[t / 2] = __builtin_bit_cast(half8_t, u32x4{h[0], h[1], h[2], h[3]});
-        lo[t / 2] = __builtin_bit_cast(half8_t, u32x4{l[0], l[1], l[2], l[3]});
+        hi[t / 2] = __builtin_bit_cast(half8_t, words4_t{h[0], h[1], h[2], h[3]});
+        lo[t / 2] = __builtin_bit_cast(half8_t, words4_t{l[0], l[1], l[2], l[3]});
     }
-    return e;
 }
 
-// The high parts alone.
 template <int TILES>
-__device__ inline int split_high(const f32x4_t (&x)[TILES], half8_t (&hi)[TILES / 2]) {
-    const float m = lane_max<TILES>(x);
-    const int e = scale_exp(column_max(__float_as_uint(m)));
+__device__ inline void split_high(const f32x4_t (&x)[TILES], int e, half8_t (&hi)[TILES / 2]) {
     const float f = pow2(-e);
 #pragma unroll
     for (int t = 0; t < TILES; t += 2) {
@@ -570,10 +623,8 @@ __device__ inline int split_high(const f32x4_t (&x)[TILES], half8_t (&hi)[TILES 
                 : "=&v"(h[2 * u]), "=&v"(h[2 * u + 1])
                 : "v"(x[t + u][0]), "v"(x[t + u][1]), "v"(x[t + u][2]), "v"(x[t + u][3]), "v"(f));
         }
-        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-        hi[t / 2] = __builtin_bit_cast(half8_t, u32x4{h[0], h[1], h[2], h[3]});
+        hi[t / 2] = __builtin_bit_cast(half8_t, words4_t{h[0], h[1], h[2], h[3]});
     }
-    return e;
 }
 
 // Lets the scheduler put `valu` vector instructions behind each of `n` matrix ones: a
@@ -649,8 +700,6 @@ __device__ inline __attribute__((always_inline)) void walk_tokens(const ChunkPar
         }
     }
 }
-
-#define KVMEM_MFMA16(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0)
 
 typedef __attribute__((address_space(3))) void lds_void_t;
 
@@ -790,7 +839,7 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
     for (uint32_t c = 0; c * kChunk < rq.count; ++c) {
         const uint32_t n = min(kChunk, rq.count - c * kChunk);
         const uint64_t row0 = static_cast<uint64_t>(rq.first) + c * kChunk;
-        const uint32_t rows = p.outs ? n : 0u;  // without an out, Q and P are whatever the workspace held
+        const uint32_t rows = p.outs ? n : 0u;  // without an out, Q and P are zeros
         const uint8_t *here = lds + (Space::places == 2 ? (c & 1u) * Space::bytes : 0u);
         const uint8_t *kp = keys + c * key_step;
         if constexpr (Space::keys) {
@@ -824,7 +873,8 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
             }
         }
         half8_t hi[KS], lo[KS];
-        const int exp_s = split<TILES>(s, hi, lo);
+        const int exp_s = column_exp<TILES>(s);
+        split<TILES>(s, exp_s, hi, lo);
         int es[4];  // of columns 4 g + r
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -860,13 +910,6 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
         constexpr int Q0 = DELTA ? (KS / 2) & 1 : 0;  // where Q's first group is
         f32x4_t first[4];
         float out_first[4];
-        if constexpr (DELTA) {
-#pragma unroll
-            for (uint32_t m = 0; m < 4; ++m) {
-                first[m] = *reinterpret_cast<const f32x4_t *>(ch->from_first + 16u * m + 4u * g);
-            }
-            get_frags(frag_t, 0, tf);
-        }
         const int exp_k = ch->exp_k, exp_q = ch->exp_q, exp_t = ch->exp_t, exp_p = ch->exp_p;
 #pragma unroll
         for (uint32_t k = 0; k < KS; k += 2) {  // transposed: columns of the state are rows of the accumulator
@@ -895,6 +938,13 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
             __builtin_amdgcn_sched_barrier(0);
         }
         constexpr int T0 = (Q0 + KS / 2) & 1;  // where K^T's first group is
+        if constexpr (DELTA) {
+#pragma unroll
+            for (uint32_t m = 0; m < 4; ++m) {
+                first[m] = *reinterpret_cast<const f32x4_t *>(ch->from_first + 16u * m + 4u * g);
+            }
+            get_frags(frag_t, 0, tf);
+        }
         // rows behind the last token repeat it: the factors' zeros meet them
         f32x4_t odd = zero;  // NaN where a value is not finite
 #pragma unroll
@@ -921,7 +971,8 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
                 }
                 d[m] = zero;
             }
-            const int e = exp_t + split<4>(rest, dh, dl);
+            const int exp_r = column_exp<4>(rest), e = exp_t + exp_r;
+            split<4>(rest, exp_r, dh, dl);
 #pragma unroll
             for (uint32_t k = 0; k < 2; ++k) {
 #pragma unroll
@@ -956,13 +1007,13 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
             out_first[m] = p.a.scale * ch->from_first[16u * m + (lane & 15u)];
         }
         const float whole = ch->from_first[kChunk - 1];
+        const int exp_d = column_exp<4>(d);
         {
             f32x4_t pd[4] = {zero, zero, zero, zero};
-            int exp_d;
             if constexpr (FINE) {
-                exp_d = split<4>(d, dh, dl);
+                split<4>(d, exp_d, dh, dl);
             } else {
-                exp_d = split_high<4>(d, dh);
+                split_high<4>(d, exp_d, dh);
             }
 #pragma unroll
             for (uint32_t k = 0; k < 2; ++k) {
@@ -1006,7 +1057,11 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
         for (int m = 0; m < 4; ++m) {
             d[m] *= last[m];
         }
-        const int exp_d = split<4>(d, dh, dl) + exp_k;
+        // |d| to_last is at most 2^exp_last times what |d| was scaled to, and a finite
+        // number times 2^-113 at most 2^15
+        const int exp_x = min(exp_d + ch->exp_last, 113);
+        split<4>(d, exp_x, dh, dl);
+        const int exp_y = exp_x + exp_k;
         f32x4_t y[2][4];
         auto update = [&](uint32_t t0) {
 #pragma unroll
@@ -1014,7 +1069,7 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     s[t0 + t][r] = __builtin_fmaf(whole, s[t0 + t][r],
-                                                  __builtin_amdgcn_ldexpf(y[(t0 / 4) & 1][t][r], exp_d));
+                                                  __builtin_amdgcn_ldexpf(y[(t0 / 4) & 1][t][r], exp_y));
                 }
             }
         };
@@ -1060,15 +1115,28 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
     }
 }
 
+// A workgroup takes a chunk of one key head for all its heads where those fill the
+// CUs twice, else for one head.  48 heads of 16 key heads, the whole call: 1024 tokens
+// (256 chunks of key heads) 72.8 us together and 69.3 alone, 2048 tokens 120.6 and 125.3,
+// 8192 tokens 445.2 and 460.1.
+constexpr uint32_t kPrepFull = 512;
+
 template <typename T, int DK>
 static void prepare(hipStream_t stream, const ChunkParams &p) {
-    linear_prepare_kernel<T, DK><<<dim3(p.chunks * p.a.n_head, p.a.n_seq), kPrepThreads, 0, stream>>>(p);
+    const uint64_t groups = static_cast<uint64_t>(p.chunks) * (p.a.n_head / p.a.group) * p.a.n_seq;
+    const uint32_t heads = groups >= kPrepFull ? p.a.group : 1u;
+    const dim3 grid(p.chunks * (p.a.n_head / heads), p.a.n_seq);
+    if (p.delta) {
+        linear_prepare_kernel<T, DK, true><<<grid, kPrepThreads, 0, stream>>>(p, heads);
+    } else {
+        linear_prepare_kernel<T, DK, false><<<grid, kPrepThreads, 0, stream>>>(p, heads);
+    }
 }
 
 // 64 columns a workgroup where a head has them and two chunks of that width fit into
-// LDS, else 32.  A chunk takes a wave the same time either way (8192 tokens, 48 states
-// of 128 x 128: KVM_W32 and KVM_W64 us), and wide workgroups read the operands half as
-// often (eight prompts of up to 4096 tokens, 32 states: KVM_B32 and KVM_B64 us).
+// LDS, else 32.  A chunk takes a wave the same time either way (one request of 8192
+// tokens, 48 heads of 128 x 128: 446 us, 443 by 32), and wide workgroups read the
+// operands half as often (eight of up to 4096 tokens, 32 heads: 397 us, 553 by 32).
 template <typename T, int DK, bool DELTA, bool FINE>
 static void walk_cols(hipStream_t stream, const ChunkParams &p) {
     constexpr bool wide = ChunkSpace<T, DK, DELTA, FINE, 4>::places == 2;

@@ -27,7 +27,7 @@ namespace kvmem_hip {
 constexpr uint32_t kVerifyThreads = 256;
 constexpr uint32_t kVerifyMaxDraft = 127;
 constexpr int kVerifyWide = 4;  // groups of 8 ids a thread, in parts for many rows
-constexpr uint32_t kVerifyFull = 1024;  // parts of many rows
+constexpr uint32_t kVerifyFull = 8192;  // parts of many rows
 constexpr uint32_t kVerifyMaxVocab = 1u << 24;
 
 struct Part {

@@ -192,6 +192,27 @@ def test_many_requests_and_heads(ctx):
         c.check(chunked=max(lengths) >= 24)
 
 
+@pytest.mark.parametrize("n,type_", [(24, "bf16"), (55, "bf16"), (56, "bf16"), (255, "f32"), (256, "f32")])
+def test_calls_of_many_states(ctx, n, type_):
+    """Calls whose states fill the card go by chunks from longer requests on: either way within its bounds."""
+    rq = Requests([n, 1, n - 1] + [2] * 29)
+    c = Linear(ctx, rq, 4, 8, 64, 512, type_, "f32", seed=n)
+    chunked = n >= (256 if type_ == "f32" else 56)
+    assert (ctx.linear_attention_workspace(c.args()) > 0) == chunked
+    c.run()
+    c.check(chunked=chunked)
+
+
+@pytest.mark.parametrize("n,type_", [(47, "f32"), (48, "f32"), (23, "f16"), (24, "f16")])
+def test_calls_of_some_states(ctx, n, type_):
+    rq = Requests([n, 1, n - 1] + [2] * 5)
+    c = Linear(ctx, rq, 4, 8, 64, 512, type_, "f32", seed=n)
+    chunked = n >= (48 if type_ == "f32" else 24)
+    assert (ctx.linear_attention_workspace(c.args()) > 0) == chunked
+    c.run()
+    c.check(chunked=chunked)
+
+
 def test_own_workspace_streams_and_replays(ctx):
     """A captured call brings its workspace; two graphs with one each replay at once; results are the eager ones."""
     calls = [Linear(ctx, Requests([100, 30]), 1, 2, 128, 128, seed=i) for i in range(2)]

@@ -147,6 +147,16 @@ def test_large_vocabularies_and_many_rows(ctx, probs):
         c.check()
 
 
+@pytest.mark.parametrize("type_,probs", [("bf16", None), ("bf16", "bf16"), ("f16", "f32"), ("f32", "f16")])
+def test_the_largest_vocabularies(ctx, type_, probs):
+    """Rows that go by parts of 8192 ids: odd ends, drafts that stay and that do not."""
+    for V, pad in ((2097153, 0), (2100008, 8)):
+        print(f"[verify] {V} {type_} {probs}", flush=True)
+        c = Verify(ctx, [3, 2], V, type_, probs, pad=pad, seed=V)
+        c.run()
+        c.check()
+
+
 @pytest.mark.parametrize("probs", [None, "f32"])
 @pytest.mark.parametrize("noise", [0.0, 0.05, 5.0])
 def test_drafts_from_equal_to_unlike(ctx, probs, noise):
