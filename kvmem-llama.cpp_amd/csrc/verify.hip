@@ -3,18 +3,18 @@
 // the next token is drawn from max(p - q, 0) at the first refusal, else from the
 // last row's p.
 //
-// Every logit is read once: bytes bound it for many rows, three short dependent
-// launches for few.
-//   parts    a workgroup per part of a row: the part's maximum (with its lowest
-//            id) and sum of exponentials relative to it
+// Every logit is read once:
+//   parts    a workgroup per 2048 ids of a row: their maximum (with its lowest id) and
+//            the sum of exponentials relative to it
 //   decide   a workgroup per request: joins its rows' parts, tests its drafts in
 //            order, and draws the next token wherever p alone decides it, from the
 //            part sums first and then inside the one part that holds the border
 //   rest     where a refused draft had probabilities, the parts' sums of
-//            max(p - q, 0), then the draw from those
+//            max(p - q, 0), and
+//   draw     the draw from those
 // Exponentials and sums are fp64: a draw compares a running sum with u times the
 // total, and of 10^5 ids' borders fp32 sums would misplace one in a few hundred
-// draws; fp64 ones none in 10^8.
+// draws; a relative error of 10^-13, one in 10^7.
 #include "kvmem_internal.hpp"
 
 #include <algorithm>
@@ -26,9 +26,10 @@ namespace kvmem_hip {
 
 constexpr uint32_t kVerifyThreads = 256;
 constexpr uint32_t kVerifyMaxDraft = 127;
-constexpr int kVerifyWide = 4;  // groups of 8 ids a thread, in parts for many rows
-constexpr uint32_t kVerifyFull = 8192;  // parts of many rows
+constexpr uint32_t kPartIds = 8 * kVerifyThreads;
 constexpr uint32_t kVerifyMaxVocab = 1u << 24;
+
+constexpr uint32_t kNowhere = 0xffffffffu;
 
 struct Part {
     double sum;   // of exp((logit - max) / temperature); 0: nothing above -inf
@@ -61,9 +62,8 @@ struct VerifyParams {
     uint32_t *n_accepted;
     uint32_t *n_keep;
     uint32_t *kv_len_out;
-    uint32_t part;       // ids of a part
     uint32_t n_parts;    // of a row
-    bool vec, probs_vec; // 16-byte aligned rows
+    uint32_t parts_each; // of a workgroup of the first kernel
     Part *parts;         // [n_seq][max_draft + 1][n_parts]
     double *rest;        // [n_seq][n_parts]
     Choice *choice;      // [n_seq]
@@ -90,76 +90,101 @@ __device__ inline float load_float(const uint8_t *p, int type, uint64_t i) {
                                   : __uint_as_float(static_cast<uint32_t>(h) << 16);
 }
 
-template <typename T>
-__device__ inline void load_eight_of(const uint8_t *row, bool vec, uint32_t v, uint32_t end, float (&x)[8]) {
-    if (vec && v % 8 == 0 && v + 8 <= end) {
-        RawRow<T, 8> raw;
-        load_raw<T, 8>(row + static_cast<uint64_t>(v) * sizeof(T), raw);
-        widen<T, 8>(raw, x);
-        return;
-    }
-#pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) {
-        x[e] = static_cast<float>(reinterpret_cast<const T *>(row)[v + e < end ? v + e : end - 1]);
-    }
-}
-
-// Ids v..v+7 of a row (v < end; ids at or beyond `end` repeat the one before it).
-__device__ inline void load_eight(const uint8_t *row, int type, bool vec, uint32_t v, uint32_t end, float (&x)[8]) {
-    if (type == KVMEM_TYPE_F32) {
-        load_eight_of<float>(row, vec, v, end, x);
-    } else if (type == KVMEM_TYPE_F16) {
-        load_eight_of<_Float16>(row, vec, v, end, x);
-    } else {
-        load_eight_of<__bf16>(row, vec, v, end, x);
-    }
-}
-
-// A logit: NaN counts as -inf.
-__device__ inline float load_logit(const uint8_t *p, int type, uint64_t i) {
-    const float x = load_float(p, type, i);
-    return x == x ? x : -INFINITY;
-}
-
 // exp((x - max) / temperature) for x <= max, inv = 1 / temperature, in fp64: with
-// n = rint(32 t / ln 2), e^t = 2^(n / 32) e^r, |r| <= ln 2 / 64, where e^r's series
-// to r^5 leaves 2e-15 and 2^(n mod 32 / 32) comes from a table in LDS (its 32 entries
-// fill the 64 banks once: lanes never collide).  t is cut at -800, whose weight is 0;
-// that is also where -inf and NaN end.  Thirteen fp64 operations against some 40 of the
+// n = rint(256 t / ln 2), e^t = 2^(n / 256) e^r, |r| <= ln 2 / 512, where e^r's series
+// to r^3 leaves 1.4e-13 and 2^(n mod 256 / 256) comes from a table in LDS.  t is cut at
+// -800, whose weight is 0; that is also where -inf and NaN end.  Eleven fp64 operations
+// (a table of 32, to r^5: thirteen, 5 % of the largest calls) against some 40 of the
 // library's exp, which has to hold for every argument.
+__constant__ double kExpCoarse[16] = {
+    0x1.0000000000000p+0, 0x1.0b5586cf9890fp+0, 0x1.172b83c7d517bp+0, 0x1.2387a6e756238p+0,
+    0x1.306fe0a31b715p+0, 0x1.3dea64c123422p+0, 0x1.4bfdad5362a27p+0, 0x1.5ab07dd485429p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.7a11473eb0187p+0, 0x1.8ace5422aa0dbp+0, 0x1.9c49182a3f090p+0,
+    0x1.ae89f995ad3adp+0, 0x1.c199bdd85529cp+0, 0x1.d5818dcfba487p+0, 0x1.ea4afa2a490dap+0,
+};  // 2^(i / 16)
+__constant__ double kExpFine[16] = {
+    0x1.0000000000000p+0, 0x1.00b1afa5abcbfp+0, 0x1.0163da9fb3335p+0, 0x1.02168143b0281p+0,
+    0x1.02c9a3e778061p+0, 0x1.037d42e11bbccp+0, 0x1.04315e86e7f85p+0, 0x1.04e5f72f654b1p+0,
+    0x1.059b0d3158574p+0, 0x1.0650a0e3c1f89p+0, 0x1.0706b29ddf6dep+0, 0x1.07bd42b72a836p+0,
+    0x1.0874518759bc8p+0, 0x1.092bdf66607e0p+0, 0x1.09e3ecac6f383p+0, 0x1.0a9c79b1f3919p+0,
+};  // 2^(i / 256)
 struct ExpTable {
-    double entry[32];
+    double entry[256];
 };
 __device__ inline void fill_table(ExpTable &t) {
-    if (threadIdx.x < 32) {
-        t.entry[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / 32.0);
-    }
+    t.entry[threadIdx.x] = kExpCoarse[threadIdx.x >> 4] * kExpFine[threadIdx.x & 15u];
     __syncthreads();
 }
 __device__ inline double weight_of(const ExpTable &table, float x, double inv, double max_inv) {
     const double t = fmax(__builtin_fma(static_cast<double>(x), inv, -max_inv), -800.0);
     constexpr double magic = 0x1.8p52;  // leaves n in the low bits
-    const double k = __builtin_fma(t, 0x1.71547652b82fep+5, magic);
+    const double k = __builtin_fma(t, 0x1.71547652b82fep+8, magic);
     const int n = static_cast<int>(__builtin_bit_cast(uint64_t, k));
-    const double r = __builtin_fma(k - magic, -0x1.62e42fefa39efp-6, t);
-    double e = __builtin_fma(r, 1.0 / 120.0, 1.0 / 24.0);
-    e = __builtin_fma(r, e, 1.0 / 6.0);
-    e = __builtin_fma(r, e, 0.5);
+    const double r = __builtin_fma(k - magic, -0x1.62e42fefa39efp-9, t);
+    double e = __builtin_fma(r, 1.0 / 6.0, 0.5);
     e = __builtin_fma(r, e, 1.0);
     e = __builtin_fma(r, e, 1.0);
-    return __builtin_ldexp(e * table.entry[n & 31], n >> 5);
+    return __builtin_ldexp(e * table.entry[n & 255], n >> 8);
 }
 
-__device__ inline bool better(float m, uint32_t at, float m2, uint32_t at2) {
-    return m > m2 || (m == m2 && at < at2);
+// A wave's numbers combined by moves inside its rows of 16 lanes, then of lane 15 and
+// 31 to the rows behind them: six steps of the VALU, where a lane permute a step would
+// wait for LDS each time.  Lane 63 ends with all of them.  Lanes that a step has nothing
+// for get `none`.
+template <int CTRL, int ROWS> __device__ inline uint32_t moved(uint32_t none, uint32_t v) {
+    return static_cast<uint32_t>(
+        __builtin_amdgcn_update_dpp(static_cast<int>(none), static_cast<int>(v), CTRL, ROWS, 0xF, false));
+}
+template <int CTRL, int ROWS> __device__ inline double moved_or_zero(double v) {
+    const uint64_t x = __builtin_bit_cast(uint64_t, v);
+    const uint64_t hi = moved<CTRL, ROWS>(0u, static_cast<uint32_t>(x >> 32));
+    return __builtin_bit_cast(double, hi << 32 | moved<CTRL, ROWS>(0u, static_cast<uint32_t>(x)));
+}
+constexpr int kRowShr = 0x110, kRowBcast15 = 0x142, kRowBcast31 = 0x143;
+
+// Running sum over the wave's lanes, this lane's included.
+__device__ inline double wave_scan(double v) {
+    v += moved_or_zero<kRowShr + 1, 0xF>(v);
+    v += moved_or_zero<kRowShr + 2, 0xF>(v);
+    v += moved_or_zero<kRowShr + 4, 0xF>(v);
+    v += moved_or_zero<kRowShr + 8, 0xF>(v);
+    v += moved_or_zero<kRowBcast15, 0xA>(v);
+    return v + moved_or_zero<kRowBcast31, 0xC>(v);
+}
+__device__ inline double wave_sum(double v) {
+    const uint64_t x = __builtin_bit_cast(uint64_t, wave_scan(v));
+    const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x >> 32), 63));
+    return __builtin_bit_cast(double,
+                              hi << 32 | static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), 63)));
+}
+template <int CTRL, int ROWS> __device__ inline float max_moved(float v) {
+    return __builtin_fmaxf(v, __uint_as_float(moved<CTRL, ROWS>(__float_as_uint(v), __float_as_uint(v))));
+}
+__device__ inline float wave_max(float v) {
+    v = max_moved<kRowShr + 1, 0xF>(v);
+    v = max_moved<kRowShr + 2, 0xF>(v);
+    v = max_moved<kRowShr + 4, 0xF>(v);
+    v = max_moved<kRowShr + 8, 0xF>(v);
+    v = max_moved<kRowBcast15, 0xA>(v);
+    v = max_moved<kRowBcast31, 0xC>(v);
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+template <int CTRL, int ROWS> __device__ inline uint32_t min_moved(uint32_t v) {
+    return min(v, moved<CTRL, ROWS>(v, v));
+}
+__device__ inline uint32_t wave_min(uint32_t v) {
+    v = min_moved<kRowShr + 1, 0xF>(v);
+    v = min_moved<kRowShr + 2, 0xF>(v);
+    v = min_moved<kRowShr + 4, 0xF>(v);
+    v = min_moved<kRowShr + 8, 0xF>(v);
+    v = min_moved<kRowBcast15, 0xA>(v);
+    v = min_moved<kRowBcast31, 0xC>(v);
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
 
-// Sum over the workgroup, in an order that never changes; every thread has it.
+// Over the workgroup, in an order that never changes; every thread has it.
 __device__ inline double block_sum(double v, double *lds) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        v += __shfl_xor(v, m, 64);
-    }
+    v = wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63u) == 0) {
         lds[threadIdx.x >> 6] = v;
@@ -168,222 +193,204 @@ __device__ inline double block_sum(double v, double *lds) {
     return (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
-__device__ inline void block_best(float &m, uint32_t &at, float *lds_m, uint32_t *lds_at) {
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
-        const float m2 = __shfl_xor(m, x, 64);
-        const uint32_t at2 = __shfl_xor(at, x, 64);
-        if (better(m2, at2, m, at)) {
-            m = m2, at = at2;
-        }
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63u) == 0) {
-        lds_m[threadIdx.x >> 6] = m;
-        lds_at[threadIdx.x >> 6] = at;
-    }
-    __syncthreads();
-    m = lds_m[0], at = lds_at[0];
-    for (int i = 1; i < 4; ++i) {
-        if (better(lds_m[i], lds_at[i], m, at)) {
-            m = lds_m[i], at = lds_at[i];
-        }
-    }
-}
-
 __device__ inline double inv_temperature(const VerifyParams &p, uint32_t s, bool &greedy) {
     const float t = p.temperature ? p.temperature[s] : 1.0f;
     greedy = !(t > 0.0f);
     return greedy ? 1.0 : 1.0 / static_cast<double>(t);
 }
 
-// A thread's numbers of a part: groups of 8 (16 bytes of a 16-bit row, 32 of an F32
-// one), the workgroup's side by side.  `first` is the part's first id, ids at or beyond
-// `end` are -inf.
-template <typename T, int GROUPS, bool VEC>
-__device__ inline void load_part(const uint8_t *row, uint32_t first, uint32_t end, float (&x)[GROUPS][8]) {
+// Eight neighbouring elements of a row, which may begin at any element: the card loads
+// 16 bytes from any address.
+template <typename T> __device__ inline void load_eight(const uint8_t *p, float (&x)[8]) {
+    typedef T vec_t __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    const vec_t v = *reinterpret_cast<const vec_t *>(p);
 #pragma unroll
-    for (uint32_t j = 0; j < GROUPS; ++j) {
-        const uint32_t v = first + (j * kVerifyThreads + threadIdx.x) * 8u;
-        if (VEC && v + 8 <= end) {
-            RawRow<T, 8> raw;
-            load_raw<T, 8>(row + static_cast<uint64_t>(v) * sizeof(T), raw);
-            widen<T, 8>(raw, x[j]);
-        } else {
+    for (int i = 0; i < 8; ++i) {
+        x[i] = static_cast<float>(v[i]);
+    }
+}
+
+// A thread's eight numbers of a part (16 bytes of a 16-bit row, 32 of an F32 one).
+// `first` is the part's first id, ids at or beyond `end` are -inf.
+template <typename T>
+__device__ inline void load_part(const uint8_t *row, uint32_t first, uint32_t end, float (&x)[8]) {
+    const uint32_t v = first + threadIdx.x * 8u;
+    if (v + 8 <= end) {
+        load_eight<T>(row + static_cast<uint64_t>(v) * sizeof(T), x);
+    } else {
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                x[j][i] = v + i < end ? static_cast<float>(reinterpret_cast<const T *>(row)[v + i]) : -INFINITY;
-            }
+        for (uint32_t i = 0; i < 8; ++i) {
+            x[i] = v + i < end ? static_cast<float>(reinterpret_cast<const T *>(row)[v + i]) : -INFINITY;
         }
     }
 }
 
-template <typename T, int GROUPS, bool VEC>
+// Each wave sums relative to its own maximum, so that a part costs one barrier; the
+// next part's numbers are on their way meanwhile.
+template <typename T>
 __global__ __launch_bounds__(kVerifyThreads) void verify_parts_kernel(const VerifyParams p) {
     __shared__ ExpTable table;
-    __shared__ double lds_d[4];
-    __shared__ float lds_m[4];
-    __shared__ uint32_t lds_at[4];
-    const uint32_t s = blockIdx.z, i = blockIdx.y, part = blockIdx.x;
+    __shared__ Part waves[2][4];
+    const uint32_t s = blockIdx.z, i = blockIdx.y, wave = threadIdx.x >> 6;
     uint32_t count, all;
     const uint32_t first = rows_of(p, s, count, all);
     if (i >= count) {
         return;
     }
     const uint8_t *row = p.logits + (static_cast<uint64_t>(first) + i) * p.logits_nb;
-    constexpr uint32_t ids = GROUPS * 8 * kVerifyThreads;
-    const uint32_t v0 = part * ids, v1 = p.n_vocab - v0 < ids ? p.n_vocab : v0 + ids;
-    float x[GROUPS][8];
-    load_part<T, GROUPS, VEC>(row, v0, v1, x);
+    Part *parts = p.parts + (static_cast<uint64_t>(s) * (p.max_draft + 1) + i) * p.n_parts;
+    uint32_t part = blockIdx.x * p.parts_each;
+    const uint32_t end = min(p.n_parts, part + p.parts_each);
+    float next[8];
+    load_part<T>(row, part * kPartIds, p.n_vocab, next);
     fill_table(table);
     bool greedy;
     const double inv = inv_temperature(p, s, greedy);
-    float m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < GROUPS; ++j) {
+    for (; part < end; ++part) {
+        float x[8], m = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            m = __builtin_fmaxf(m, x[j][e]);  // NaN is left out
+            x[e] = next[e];
+            m = __builtin_fmaxf(m, x[e]);  // NaN is left out
         }
-    }
+        if (part + 1 < end) {
+            load_part<T>(row, (part + 1) * kPartIds, p.n_vocab, next);
+        }
+        m = wave_max(m);
+        double sum = 0.0;
+        uint32_t at = kNowhere;
+        if (greedy || m == INFINITY) {
 #pragma unroll
-    for (int e = 1; e < 64; e <<= 1) {
-        m = __builtin_fmaxf(m, __shfl_xor(m, e, 64));
-    }
-    if ((threadIdx.x & 63u) == 0) {
-        lds_m[threadIdx.x >> 6] = m;
-    }
-    __syncthreads();
-    m = __builtin_fmaxf(__builtin_fmaxf(lds_m[0], lds_m[1]), __builtin_fmaxf(lds_m[2], lds_m[3]));
-    double sum = 0.0;
-    uint32_t at = 0xffffffffu;
-    if (greedy || m == INFINITY) {
-        if (m > -INFINITY) {
-#pragma unroll
-            for (int j = GROUPS - 1; j >= 0; --j) {
-#pragma unroll
-                for (int e = 7; e >= 0; --e) {
-                    at = x[j][e] == m ? v0 + (static_cast<uint32_t>(j) * kVerifyThreads + threadIdx.x) * 8u +
-                                            static_cast<uint32_t>(e)
-                                      : at;
-                }
+            for (int e = 7; e >= 0; --e) {
+                at = x[e] == m ? part * kPartIds + threadIdx.x * 8u + static_cast<uint32_t>(e) : at;
             }
-            float mine = at == 0xffffffffu ? -INFINITY : m;
-            block_best(mine, at, lds_m, lds_at);
-        }
-    } else if (m > -INFINITY) {
-        const double max_inv = static_cast<double>(m) * inv;
-        double part_sum[2] = {};
-#pragma unroll
-        for (int j = 0; j < GROUPS; ++j) {
+            at = wave_min(m > -INFINITY ? at : kNowhere);
+        } else if (m > -INFINITY) {
+            const double max_inv = static_cast<double>(m) * inv;
+            double part_sum[2] = {};
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                part_sum[e & 1] += weight_of(table, x[j][e], inv, max_inv);
+                part_sum[e & 1] += weight_of(table, x[e], inv, max_inv);
+            }
+            sum = wave_sum(part_sum[0] + part_sum[1]);
+        }
+        Part *mine = waves[part & 1u];
+        if ((threadIdx.x & 63u) == 0) {
+            mine[wave] = Part{sum, m, at};
+        }
+        __syncthreads();  // the other place is read before the next
+        if (wave == 0) {
+            const Part w = mine[threadIdx.x & 3u];
+            m = wave_max(w.max);
+            at = wave_min(w.max == m ? w.at : kNowhere);
+            sum = threadIdx.x < 4 && w.sum > 0.0 && m < INFINITY
+                      ? w.sum * weight_of(table, w.max, inv, static_cast<double>(m) * inv)
+                      : 0.0;
+            sum = wave_sum(sum);
+            if (threadIdx.x == 0) {
+                parts[part] = Part{sum, m, at};
             }
         }
-        sum = block_sum(part_sum[0] + part_sum[1], lds_d);
     }
-    if (threadIdx.x == 0) {
-        p.parts[(static_cast<uint64_t>(s) * (p.max_draft + 1) + i) * p.n_parts + part] = Part{sum, m, at};
-    }
-}
-
-// Sum over ids [a, b) of a part of the weights that `weight` makes of a logit and (where
-// probs are given) a probability; eight are read at a time.
-template <typename F>
-__device__ inline double sum_ids(const VerifyParams &p, const uint8_t *logits, const uint8_t *probs, uint32_t v0,
-                                 uint32_t a, uint32_t b, F weight) {
-    double sum = 0.0;
-    for (; a < b; a += 8) {
-        float x[8], q[8];
-        load_eight(logits, p.type, p.vec, v0 + a, v0 + b, x);
-        if (probs) {
-            load_eight(probs, p.probs_type, p.probs_vec, v0 + a, v0 + b, q);
-        }
-#pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) {
-            sum += a + e < b ? weight(v0 + a + e, x[e], probs ? q[e] : 0.0f) : 0.0;
-        }
-    }
-    return sum;
 }
 
 struct PickLds {
     double sum[4];
+    uint32_t first[4], last[4];
     double before;
-    uint32_t found[4], fallback[4];
+    uint32_t part;
 };
 
-// Running sum over the wave's lanes, this lane's included.
-__device__ inline double wave_scan(double v) {
-    const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
-        const double y = __shfl_up(v, x, 64);
-        v += lane >= static_cast<uint32_t>(x) ? y : 0.0;
-    }
-    return v;
-}
-
-// The first of n weights whose running sum (from `start`) passes `target`, by the whole
-// workgroup; `before` is the running sum in front of it.  Where none passes, the last
-// positive one (n if there is none).  Threads sum runs of `per` weights (sum_of(first,
-// end)), running sums of the runs find one run, and its weights' (w) running sums the
-// place in it (per <= 64).
-template <typename S, typename W>
-__device__ inline uint32_t block_pick(uint32_t n, uint32_t per, double start, double target, S sum_of, W w,
-                                      PickLds &lds, double &before) {
+// The first thread whose running sum (from `start`) passes the target; where none does,
+// the last with a positive sum (kNowhere if there is none).  `front` is the running sum
+// before this thread.  The target is `target` times the sum of all with OF_ALL.
+template <bool OF_ALL>
+__device__ inline uint32_t block_find(double sum, double start, double &target, PickLds &lds, double &front) {
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
-    const uint32_t a = min(n, threadIdx.x * per);
-    const double sum = sum_of(a, min(n, a + per));
-    const bool some = sum > 0.0;
     double run = wave_scan(sum);
-    __syncthreads();
     if (lane == 63) {
         lds.sum[wave] = run;
     }
     __syncthreads();
-    double base = start;
-    for (uint32_t i = 0; i < wave; ++i) {
-        base += lds.sum[i];
+    double all = start;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        run += i == wave ? all : 0.0;
+        all += lds.sum[i];
     }
-    run += base;
-    const uint64_t passed = __ballot(some && run > target), there = __ballot(some);
+    if (OF_ALL) {
+        target *= all;
+    }
+    const uint64_t there = __ballot(sum > 0.0), passed = __ballot(sum > 0.0 && run > target);
     if (lane == 0) {
-        lds.found[wave] = passed ? wave * 64u + static_cast<uint32_t>(__builtin_ctzll(passed)) : kVerifyThreads;
-        lds.fallback[wave] = there ? wave * 64u + 63u - static_cast<uint32_t>(__builtin_clzll(there)) : kVerifyThreads;
+        lds.first[wave] = passed ? wave * 64u + static_cast<uint32_t>(__builtin_ctzll(passed)) : kNowhere;
+        lds.last[wave] = there ? wave * 64u + 64u - static_cast<uint32_t>(__builtin_clzll(there)) : 0u;
     }
     __syncthreads();
-    uint32_t owner = kVerifyThreads;
-    for (int i = 3; i >= 0; --i) {
-        owner = lds.found[i] < kVerifyThreads ? lds.found[i] : owner;
+    const uint32_t first = min(min(lds.first[0], lds.first[1]), min(lds.first[2], lds.first[3]));
+    const uint32_t last = max(max(lds.last[0], lds.last[1]), max(lds.last[2], lds.last[3]));  // and one
+    front = run - sum;
+    return first != kNowhere ? first : last - 1u;
+}
+
+// The part a draw ends in (kNowhere: nothing is positive), `target` turned from a
+// fraction of the parts' weights into a running sum, `before` the one in front of the
+// part.
+template <typename W>
+__device__ inline uint32_t pick_part(uint32_t n_parts, double &target, W weight, PickLds &lds, double &before) {
+    const uint32_t per = (n_parts + kVerifyThreads - 1) / kVerifyThreads, a = threadIdx.x * per;
+    double sum = 0.0;
+    for (uint32_t i = a; i < min(n_parts, a + per); ++i) {
+        sum += weight(i);
     }
-    for (int i = 3; i >= 0 && owner == kVerifyThreads; --i) {
-        owner = lds.fallback[i];
-    }
-    if (owner == kVerifyThreads) {
-        before = start;
-        return n;  // nothing positive
-    }
-    if (threadIdx.x == owner) {
-        lds.before = run - sum;
-    }
-    __syncthreads();
-    const double front = lds.before;
-    if (per == 1) {
+    double front;
+    const uint32_t at = block_find<true>(sum, 0.0, target, lds, front);
+    if (at == threadIdx.x) {
+        // of several parts, the first that passes, else the last positive one
+        uint32_t part = a;
+        double run = front;
         before = front;
-        __syncthreads();
-        return owner;
+        for (uint32_t i = a; per > 1 && i < min(n_parts, a + per); ++i) {
+            const double w = weight(i);
+            if (w > 0.0) {
+                part = i;
+                before = run;
+                run += w;
+                if (run > target) {
+                    break;
+                }
+            }
+        }
+        lds.part = part;
+        lds.before = before;
     }
-    // every wave finds the same place
-    const uint32_t i = owner * per + lane;
-    const double mine = lane < per && i < n ? w(i) : 0.0;
-    const double upto = front + wave_scan(mine);
-    const uint64_t over = __ballot(mine > 0.0 && upto > target), positive = __ballot(mine > 0.0);
-    const int at = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(positive | 1u);
-    before = __shfl(upto - mine, at, 64);
     __syncthreads();
-    return owner * per + static_cast<uint32_t>(at);
+    before = lds.before;
+    return at == kNowhere ? kNowhere : lds.part;
+}
+
+// The id a draw ends in, in a part of which this thread has the weights w[i] of ids
+// v0 + threadIdx.x * 8 + i; its thread writes it.
+__device__ inline void pick_id(uint32_t v0, double before, double target, const double (&w)[8], PickLds &lds,
+                               int32_t *token) {
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        sum += w[i];
+    }
+    double front;
+    if (block_find<false>(sum, before, target, lds, front) != threadIdx.x) {
+        return;
+    }
+    uint32_t found = 0;
+    bool over = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        front += w[i];
+        found = w[i] > 0.0 && !over ? static_cast<uint32_t>(i) : found;
+        over = over || (w[i] > 0.0 && front > target);
+    }
+    *token = static_cast<int32_t>(v0 + threadIdx.x * 8u + found);
 }
 
 struct Row {
@@ -391,37 +398,6 @@ struct Row {
     float max;
     uint32_t at;
 };
-
-// A row's parts together, by one wave.
-__device__ inline Row join_row(const VerifyParams &p, const ExpTable &table, const Part *parts, double inv) {
-    const uint32_t lane = threadIdx.x & 63u;
-    float m = -INFINITY;
-    uint32_t at = 0xffffffffu;
-    for (uint32_t i = lane; i < p.n_parts; i += 64) {
-        const Part x = parts[i];
-        if (better(x.max, x.at, m, at)) {
-            m = x.max, at = x.at;
-        }
-    }
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
-        const float m2 = __shfl_xor(m, x, 64);
-        const uint32_t at2 = __shfl_xor(at, x, 64);
-        if (better(m2, at2, m, at)) {
-            m = m2, at = at2;
-        }
-    }
-    double sum = 0.0;
-    for (uint32_t i = lane; i < p.n_parts; i += 64) {
-        const Part x = parts[i];
-        sum += x.sum > 0.0 ? x.sum * weight_of(table, x.max, inv, static_cast<double>(m) * inv) : 0.0;
-    }
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
-        sum += __shfl_xor(sum, x, 64);
-    }
-    return Row{sum, m, at};
-}
 
 __device__ inline void write_request(const VerifyParams &p, uint32_t s, uint32_t first, uint32_t count, uint32_t all,
                                      uint32_t accepted) {
@@ -441,49 +417,105 @@ __device__ inline void write_request(const VerifyParams &p, uint32_t s, uint32_t
     }
 }
 
-__device__ inline void write_token(const VerifyParams &p, uint32_t s, uint32_t accepted, uint32_t id) {
-    if (threadIdx.x == 0) {
-        p.tokens_out[static_cast<uint64_t>(s) * (p.max_draft + 1) + accepted] = static_cast<int32_t>(id);
-    }
-}
+constexpr int kRowsAtOnce = 2;   // of a wave's rows, so that their loads and sums overlap
+constexpr int kPartsHeld = 2;    // parts a lane keeps of a row; it reads others twice
 
+template <typename T>
 __global__ __launch_bounds__(kVerifyThreads) void verify_decide_kernel(const VerifyParams p) {
     __shared__ Row rows[kVerifyMaxDraft + 1];
     __shared__ uint8_t stays[kVerifyMaxDraft + 1];
     __shared__ PickLds lds;
     __shared__ double lds_d[4];
     __shared__ ExpTable table;
-    fill_table(table);
-    const uint32_t s = blockIdx.x;
+    const uint32_t s = blockIdx.x, lane = threadIdx.x & 63u;
     uint32_t count, all;
     const uint32_t first = rows_of(p, s, count, all);
     bool greedy;
     const double inv = inv_temperature(p, s, greedy);
+    const float u_sample = p.u_sample[s];
+    fill_table(table);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (uint32_t i = wave; i < count; i += kVerifyThreads / 64) {
-        const uint64_t r = static_cast<uint64_t>(first) + i;
-        const Row row =
-            join_row(p, table, p.parts + (static_cast<uint64_t>(s) * (p.max_draft + 1) + i) * p.n_parts, inv);
-        if ((threadIdx.x & 63u) == 0) {
-            rows[i] = row;
-            bool ok = false;
+    for (uint32_t i0 = wave; i0 < count; i0 += 4 * kRowsAtOnce) {
+        Part held[kRowsAtOnce][kPartsHeld];
+        uint32_t id[kRowsAtOnce];
+        float u[kRowsAtOnce], logit[kRowsAtOnce], q[kRowsAtOnce];
+        const Part *parts[kRowsAtOnce];
+        // rows behind the last are the last again
+#pragma unroll
+        for (int x = 0; x < kRowsAtOnce; ++x) {
+            const uint32_t i = min(i0 + 4u * x, count - 1u);
+            parts[x] = p.parts + (static_cast<uint64_t>(s) * (p.max_draft + 1) + i) * p.n_parts;
+#pragma unroll
+            for (int k = 0; k < kPartsHeld; ++k) {
+                const uint32_t at = lane + 64u * k;
+                held[x][k] = at < p.n_parts ? parts[x][at] : Part{0.0, -INFINITY, kNowhere};
+            }
+            const uint64_t r = static_cast<uint64_t>(first) + i;
+            id[x] = kNowhere;
+            u[x] = 0.0f;
             if (i + 1 < count) {
-                const uint32_t x = static_cast<uint32_t>(p.tokens[r + 1]);
-                if (x < p.n_vocab && row.max > -INFINITY) {
-                    if (greedy || row.max == INFINITY) {
-                        ok = x == row.at;
-                    } else {
-                        const double e =
-                            weight_of(table, load_logit(p.logits + r * p.logits_nb, p.type, x), inv,
-                                      static_cast<double>(row.max) * inv) /
-                            row.sum;
-                        const double q =
-                            p.probs ? static_cast<double>(load_float(p.probs + r * p.probs_nb, p.probs_type, x)) : 1.0;
-                        ok = static_cast<double>(p.u_accept[r]) * q < e;
-                    }
+                id[x] = static_cast<uint32_t>(p.tokens[r + 1]);
+                u[x] = p.u_accept[r];
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < kRowsAtOnce; ++x) {
+            const uint64_t r = static_cast<uint64_t>(first) + min(i0 + 4u * x, count - 1u);
+            logit[x] = -INFINITY;
+            q[x] = 1.0f;
+            if (id[x] < p.n_vocab) {  // a NaN has no weight either
+                logit[x] = static_cast<float>(reinterpret_cast<const T *>(p.logits + r * p.logits_nb)[id[x]]);
+                if (p.probs) {
+                    q[x] = load_float(p.probs + r * p.probs_nb, p.probs_type, id[x]);
                 }
             }
-            stays[i] = ok;
+        }
+        Row row[kRowsAtOnce];
+        float m[kRowsAtOnce];
+#pragma unroll
+        for (int x = 0; x < kRowsAtOnce; ++x) {
+            m[x] = held[x][0].max;
+#pragma unroll
+            for (int k = 1; k < kPartsHeld; ++k) {
+                m[x] = __builtin_fmaxf(m[x], held[x][k].max);
+            }
+            for (uint32_t at = lane + 64u * kPartsHeld; at < p.n_parts; at += 64) {
+                m[x] = __builtin_fmaxf(m[x], parts[x][at].max);
+            }
+            row[x].max = wave_max(m[x]);
+        }
+#pragma unroll
+        for (int x = 0; x < kRowsAtOnce; ++x) {
+            const double max_inv = static_cast<double>(row[x].max) * inv;
+            uint32_t id_of_max = kNowhere;
+            double sum = 0.0;
+            auto add = [&](const Part &part) {
+                id_of_max = part.max == row[x].max ? min(id_of_max, part.at) : id_of_max;
+                sum += part.sum > 0.0 ? part.sum * weight_of(table, part.max, inv, max_inv) : 0.0;
+            };
+#pragma unroll
+            for (int k = 0; k < kPartsHeld; ++k) {
+                add(held[x][k]);
+            }
+            for (uint32_t at = lane + 64u * kPartsHeld; at < p.n_parts; at += 64) {
+                add(parts[x][at]);
+            }
+            row[x].sum = wave_sum(sum);
+            row[x].at = wave_min(id_of_max);
+            bool ok = false;
+            if (id[x] < p.n_vocab && row[x].max > -INFINITY) {
+                if (greedy || row[x].max == INFINITY) {
+                    ok = id[x] == row[x].at;
+                } else {
+                    ok = static_cast<double>(u[x]) * static_cast<double>(q[x]) <
+                         weight_of(table, logit[x], inv, max_inv) / row[x].sum;
+                }
+            }
+            const uint32_t i = i0 + 4u * x;
+            if (lane == 0 && i < count) {
+                rows[i] = row[x];
+                stays[i] = ok;
+            }
         }
     }
     __syncthreads();
@@ -492,19 +524,22 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_decide_kernel(const Ver
         ++accepted;
     }
     write_request(p, s, first, count, all, accepted);
-    __syncthreads();  // tokens_out[accepted] is written again below
     if (threadIdx.x == 0) {
         p.choice[s].pending = 0;
     }
     if (count == 0) {
         return;
     }
+    __syncthreads();  // tokens_out[accepted] is written again below
+    int32_t *token = p.tokens_out + static_cast<uint64_t>(s) * (p.max_draft + 1) + accepted;
     const Row row = rows[accepted];
     if (row.max == -INFINITY) {
         return;  // nothing to draw from: -1
     }
     if (greedy || row.max == INFINITY) {
-        write_token(p, s, accepted, row.at);
+        if (threadIdx.x == 0) {
+            *token = static_cast<int32_t>(row.at);
+        }
         return;
     }
     const uint64_t r = static_cast<uint64_t>(first) + accepted;
@@ -519,53 +554,46 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_decide_kernel(const Ver
     const double max_inv = static_cast<double>(row.max) * inv;
     const Part *parts = p.parts + (static_cast<uint64_t>(s) * (p.max_draft + 1) + accepted) * p.n_parts;
     const uint8_t *logits = p.logits + r * p.logits_nb;
-    uint32_t without = refused ? static_cast<uint32_t>(p.tokens[r + 1]) : 0xffffffffu;
-    without = without < p.n_vocab ? without : 0xffffffffu;
-    uint32_t cut = 0xffffffffu;  // its part, and that part's sum without it
+    uint32_t without = refused ? static_cast<uint32_t>(p.tokens[r + 1]) : kNowhere;
+    without = without < p.n_vocab ? without : kNowhere;
+    double w[8];
+    auto load_weights = [&](uint32_t v0) {
+        float x[8];
+        load_part<T>(logits, v0, min(p.n_vocab, v0 + kPartIds), x);
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            const double y = weight_of(table, x[i], inv, max_inv);
+            w[i] = v0 + threadIdx.x * 8u + i == without ? 0.0 : y;
+        }
+    };
+    uint32_t cut = kNowhere;  // the draft's part, and that part's sum without it
     double cut_sum = 0.0;
-    double total = row.sum;
-    auto id_weight = [&](uint32_t v, float x, float) {
-        return v == without ? 0.0 : weight_of(table, x, inv, max_inv);
-    };
     auto part_weight = [&](uint32_t i) {
-        const Part x = parts[i];
-        return i == cut ? cut_sum : x.sum > 0.0 ? x.sum * weight_of(table, x.max, inv, max_inv) : 0.0;
+        const Part part = parts[i];
+        return i == cut ? cut_sum : part.sum > 0.0 ? part.sum * weight_of(table, part.max, inv, max_inv) : 0.0;
     };
-    auto parts_sum = [&](uint32_t a, uint32_t b) {
-        double sum = 0.0;
-        for (; a < b; ++a) {
-            sum += part_weight(a);
+    if (without != kNowhere) {
+        cut = without / kPartIds;
+        load_weights(cut * kPartIds);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            cut_sum += w[i];
         }
-        return sum;
-    };
-    if (without != 0xffffffffu) {
-        cut = without / p.part;
-        const uint32_t v0 = cut * p.part, ids = min(p.part, p.n_vocab - v0), per = p.part / kVerifyThreads;
-        const uint32_t a = min(ids, threadIdx.x * per);
-        cut_sum = block_sum(sum_ids(p, logits, nullptr, v0, a, min(ids, a + per), id_weight), lds_d);
-        total = 0.0;
-        for (uint32_t i = threadIdx.x; i < p.n_parts; i += kVerifyThreads) {
-            total += part_weight(i);
-        }
-        total = block_sum(total, lds_d);
-        if (!(total > 0.0)) {  // the draft was all there is
-            without = cut = 0xffffffffu;
-            total = row.sum;
-        }
+        cut_sum = block_sum(cut_sum, lds_d);
     }
-    const double target = static_cast<double>(p.u_sample[s]) * total;
-    double before;
-    const uint32_t part = block_pick(p.n_parts, (p.n_parts + kVerifyThreads - 1) / kVerifyThreads, 0.0, target,
-                                     parts_sum, part_weight, lds, before);
-    if (part >= p.n_parts) {
+    double target = u_sample, before;
+    uint32_t part = pick_part(p.n_parts, target, part_weight, lds, before);
+    if (part == kNowhere && without != kNowhere) {  // the draft was all there is
+        without = cut = kNowhere;
+        target = u_sample;
+        __syncthreads();
+        part = pick_part(p.n_parts, target, part_weight, lds, before);
+    }
+    if (part == kNowhere) {
         return;
     }
-    const uint32_t v0 = part * p.part;
-    const uint32_t at = block_pick(
-        min(p.part, p.n_vocab - v0), p.part / kVerifyThreads, before, target,
-        [&](uint32_t a, uint32_t b) { return sum_ids(p, logits, nullptr, v0, a, b, id_weight); },
-        [&](uint32_t i) { return id_weight(v0 + i, load_float(logits, p.type, v0 + i), 0.0f); }, lds, before);
-    write_token(p, s, accepted, v0 + at);
+    load_weights(part * kPartIds);
+    pick_id(part * kPartIds, before, target, w, lds, token);
 }
 
 __device__ inline double rest_of(const ExpTable &table, double scale, float logit, float q, double inv,
@@ -574,7 +602,7 @@ __device__ inline double rest_of(const ExpTable &table, double scale, float logi
     return e > 0.0 ? e : 0.0;
 }
 
-template <typename T, typename Q, int GROUPS, bool VEC>
+template <typename T, typename Q>
 __global__ __launch_bounds__(kVerifyThreads) void verify_rest_kernel(const VerifyParams p) {
     __shared__ ExpTable table;
     __shared__ double lds_d[4];
@@ -585,25 +613,19 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rest_kernel(const Verif
     }
     uint32_t count, all;
     const uint64_t r = static_cast<uint64_t>(rows_of(p, s, count, all)) + c.row;
-    constexpr uint32_t ids = GROUPS * 8 * kVerifyThreads;
-    const uint32_t v0 = part * ids, v1 = p.n_vocab - v0 < ids ? p.n_vocab : v0 + ids;
-    float x[GROUPS][8], q[GROUPS][8];
-    load_part<T, GROUPS, VEC>(p.logits + r * p.logits_nb, v0, v1, x);
-    load_part<Q, GROUPS, VEC>(p.probs + r * p.probs_nb, v0, v1, q);
+    const uint32_t v0 = part * kPartIds, v1 = min(p.n_vocab, v0 + kPartIds);
+    float x[8], q[8];
+    load_part<T>(p.logits + r * p.logits_nb, v0, v1, x);
+    load_part<Q>(p.probs + r * p.probs_nb, v0, v1, q);
     fill_table(table);
     bool greedy;
     const double inv = inv_temperature(p, s, greedy);
     const double max_inv = static_cast<double>(c.max) * inv;
     double sum = 0.0;
 #pragma unroll
-    for (uint32_t j = 0; j < GROUPS; ++j) {
-#pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) {
-            // behind the part's end logit and q are -inf
-            sum += v0 + (j * kVerifyThreads + threadIdx.x) * 8u + e < v1
-                       ? rest_of(table, c.scale, x[j][e], q[j][e], inv, max_inv)
-                       : 0.0;
-        }
+    for (uint32_t e = 0; e < 8; ++e) {
+        // behind the part's end logit and q are -inf
+        sum += v0 + threadIdx.x * 8u + e < v1 ? rest_of(table, c.scale, x[e], q[e], inv, max_inv) : 0.0;
     }
     sum = block_sum(sum, lds_d);
     if (threadIdx.x == 0) {
@@ -611,11 +633,10 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rest_kernel(const Verif
     }
 }
 
+template <typename T, typename Q>
 __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const VerifyParams p) {
     __shared__ PickLds lds;
-    __shared__ double lds_d[4];
     __shared__ ExpTable table;
-    fill_table(table);
     const uint32_t s = blockIdx.x;
     const Choice c = p.choice[s];
     if (!c.pending) {
@@ -625,118 +646,82 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
     const uint64_t r = static_cast<uint64_t>(rows_of(p, s, count, all)) + c.row;
     bool greedy;
     const double inv = inv_temperature(p, s, greedy);
-    const uint8_t *logits = p.logits + r * p.logits_nb, *probs = p.probs + r * p.probs_nb;
+    const float u_sample = p.u_sample[s];
+    fill_table(table);
     const double *rest = p.rest + static_cast<uint64_t>(s) * p.n_parts;
     const Part *parts = p.parts + (static_cast<uint64_t>(s) * (p.max_draft + 1) + c.row) * p.n_parts;
     const double max_inv = static_cast<double>(c.max) * inv;
-    double total = 0.0;
-    for (uint32_t i = threadIdx.x; i < p.n_parts; i += kVerifyThreads) {
-        total += rest[i];
-    }
-    total = block_sum(total, lds_d);
-    const bool left = total > 0.0;  // else p itself
+    double target = u_sample, before;
+    uint32_t part = pick_part(p.n_parts, target, [&](uint32_t i) { return rest[i]; }, lds, before);
+    const bool left = part != kNowhere;  // else p itself
     if (!left) {
-        total = 1.0 / c.scale;
+        target = u_sample;
+        __syncthreads();
+        part = pick_part(
+            p.n_parts, target,
+            [&](uint32_t i) {
+                const Part x = parts[i];
+                return x.sum > 0.0 ? x.sum * weight_of(table, x.max, inv, max_inv) : 0.0;
+            },
+            lds, before);
     }
-    const double target = static_cast<double>(p.u_sample[s]) * total;
-    double before;
-    auto part_weight = [&](uint32_t i) {
-        const Part x = parts[i];
-        return left ? rest[i] : x.sum > 0.0 ? x.sum * weight_of(table, x.max, inv, max_inv) : 0.0;
-    };
-    const uint32_t part = block_pick(
-        p.n_parts, (p.n_parts + kVerifyThreads - 1) / kVerifyThreads, 0.0, target,
-        [&](uint32_t a, uint32_t b) {
-            double sum = 0.0;
-            for (; a < b; ++a) {
-                sum += part_weight(a);
-            }
-            return sum;
-        },
-        part_weight, lds, before);
-    if (part >= p.n_parts) {
+    if (part == kNowhere) {
         return;
     }
-    const uint32_t v0 = part * p.part;
-    auto id_weight = [&](uint32_t, float x, float q) {
-        return left ? rest_of(table, c.scale, x, q, inv, max_inv) : weight_of(table, x, inv, max_inv);
-    };
-    const uint32_t at = block_pick(
-        min(p.part, p.n_vocab - v0), p.part / kVerifyThreads, before, target,
-        [&](uint32_t a, uint32_t b) { return sum_ids(p, logits, probs, v0, a, b, id_weight); },
-        [&](uint32_t i) {
-            return id_weight(v0 + i, load_float(logits, p.type, v0 + i), load_float(probs, p.probs_type, v0 + i));
-        },
-        lds, before);
-    write_token(p, s, c.row, v0 + at);
-}
-
-template <typename T, int GROUPS>
-static void launch_parts(hipStream_t stream, const VerifyParams &p) {
-    const dim3 grid(p.n_parts, p.max_draft + 1, p.n_seq);
-    if (p.vec) {
-        verify_parts_kernel<T, GROUPS, true><<<grid, kVerifyThreads, 0, stream>>>(p);
-    } else {
-        verify_parts_kernel<T, GROUPS, false><<<grid, kVerifyThreads, 0, stream>>>(p);
+    const uint32_t v0 = part * kPartIds, v1 = min(p.n_vocab, v0 + kPartIds);
+    float x[8], q[8];
+    double w[8];
+    load_part<T>(p.logits + r * p.logits_nb, v0, v1, x);
+    load_part<Q>(p.probs + r * p.probs_nb, v0, v1, q);
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        const double y = left ? rest_of(table, c.scale, x[i], q[i], inv, max_inv)
+                              : weight_of(table, x[i], inv, max_inv);
+        w[i] = v0 + threadIdx.x * 8u + i < v1 ? y : 0.0;  // behind the end logit and q are -inf
     }
+    pick_id(v0, before, target, w, lds, p.tokens_out + static_cast<uint64_t>(s) * (p.max_draft + 1) + c.row);
 }
 
-template <typename T, typename Q, int GROUPS>
-static void launch_rest_groups(hipStream_t stream, const VerifyParams &p) {
-    const dim3 grid(p.n_parts, p.n_seq);
-    if (p.vec && p.probs_vec) {
-        verify_rest_kernel<T, Q, GROUPS, true><<<grid, kVerifyThreads, 0, stream>>>(p);
-    } else {
-        verify_rest_kernel<T, Q, GROUPS, false><<<grid, kVerifyThreads, 0, stream>>>(p);
-    }
-}
-
-template <typename T>
+template <typename T, typename Q>
 static void launch_rest(hipStream_t stream, const VerifyParams &p) {
-    const bool wide = p.part == 8u * kVerifyWide * kVerifyThreads;
-    if (p.probs_type == KVMEM_TYPE_F32) {
-        wide ? launch_rest_groups<T, float, kVerifyWide>(stream, p) : launch_rest_groups<T, float, 1>(stream, p);
-    } else if (p.probs_type == KVMEM_TYPE_F16) {
-        wide ? launch_rest_groups<T, _Float16, kVerifyWide>(stream, p) : launch_rest_groups<T, _Float16, 1>(stream, p);
-    } else {
-        wide ? launch_rest_groups<T, __bf16, kVerifyWide>(stream, p) : launch_rest_groups<T, __bf16, 1>(stream, p);
+    verify_rest_kernel<T, Q><<<dim3(p.n_parts, p.n_seq), kVerifyThreads, 0, stream>>>(p);
+    if (hipPeekAtLastError() == hipSuccess) {
+        verify_draw_kernel<T, Q><<<p.n_seq, kVerifyThreads, 0, stream>>>(p);
     }
 }
 
 template <typename T>
 static void launch_verify(hipStream_t stream, const VerifyParams &p) {
-    if (p.part == 8u * kVerifyWide * kVerifyThreads) {
-        launch_parts<T, kVerifyWide>(stream, p);
-    } else {
-        launch_parts<T, 1>(stream, p);
-    }
+    verify_parts_kernel<T>
+        <<<dim3((p.n_parts + p.parts_each - 1) / p.parts_each, p.max_draft + 1, p.n_seq), kVerifyThreads, 0, stream>>>(p);
     if (hipPeekAtLastError() != hipSuccess) {
         return;  // parts that were not written must not be read
     }
-    verify_decide_kernel<<<p.n_seq, kVerifyThreads, 0, stream>>>(p);
-    if (p.probs && p.max_draft && hipPeekAtLastError() == hipSuccess) {
-        launch_rest<T>(stream, p);
-        if (hipPeekAtLastError() == hipSuccess) {
-            verify_draw_kernel<<<p.n_seq, kVerifyThreads, 0, stream>>>(p);
-        }
+    verify_decide_kernel<T><<<p.n_seq, kVerifyThreads, 0, stream>>>(p);
+    if (!p.probs || !p.max_draft || hipPeekAtLastError() != hipSuccess) {
+        return;
+    }
+    if (p.probs_type == KVMEM_TYPE_F32) {
+        launch_rest<T, float>(stream, p);
+    } else if (p.probs_type == KVMEM_TYPE_F16) {
+        launch_rest<T, _Float16>(stream, p);
+    } else {
+        launch_rest<T, __bf16>(stream, p);
     }
 }
 
 bool load_verify_kernels() {
-    return load_kernel_object(&verify_decide_kernel);
+    return load_kernel_object(&verify_decide_kernel<float>);
 }
 
 struct VerifyPlan {
-    uint32_t part, n_parts;
+    uint32_t n_parts;
     size_t parts_bytes, rest_bytes, choice_bytes;
 };
 
 static VerifyPlan plan_verify(const kvmem_hip_verify_args *a) {
     VerifyPlan pl;
-    const uint64_t logits = static_cast<uint64_t>(a->n_seq) * (a->max_draft + 1) * a->n_vocab;
-    const uint32_t wide = 8u * kVerifyWide * kVerifyThreads;
-    pl.part = logits / wide >= kVerifyFull || a->n_vocab > (1u << 21) ? wide : 8u * kVerifyThreads;
-    pl.n_parts = (a->n_vocab + pl.part - 1) / pl.part;
+    pl.n_parts = (a->n_vocab + kPartIds - 1) / kPartIds;
     const size_t rows = static_cast<size_t>(a->n_seq) * (a->max_draft + 1);
     pl.parts_bytes = rows * pl.n_parts * sizeof(Part);
     pl.rest_bytes = (static_cast<size_t>(a->n_seq) * pl.n_parts * sizeof(double) + 15) / 16 * 16;
@@ -839,10 +824,12 @@ int kvmem_hip_verify_draft(kvmem_hip_ctx *ctx, const kvmem_hip_verify_args *a) {
     p.n_accepted = a->n_accepted;
     p.n_keep = a->n_keep;
     p.kv_len_out = a->kv_len_out;
-    p.part = pl.part;
     p.n_parts = pl.n_parts;
-    p.vec = ((reinterpret_cast<uintptr_t>(a->logits) | a->logits_nb) & 15u) == 0;
-    p.probs_vec = ((reinterpret_cast<uintptr_t>(a->probs) | a->probs_nb) & 15u) == 0;
+    // up to four parts a workgroup once there are many: 512 rows of 152000 ids (38400
+    // parts) 78.8 us one by one, 74.9 by two, 73.9 by four, 80.5 by eight; 256 rows 51.1,
+    // 49.3, 49.7, 54.0; 8 rows 16.8, 17.8, 19.4, 23.5
+    const uint64_t parts = static_cast<uint64_t>(pl.n_parts) * (a->max_draft + 1) * a->n_seq;
+    p.parts_each = static_cast<uint32_t>(std::clamp<uint64_t>(parts / 8192, 1, 4));
     (void) hipSetDevice(ctx->device);
     uint8_t *ws = nullptr;
     if (const int rc = call_workspace(ctx, ctx->verify_scratch, a->workspace, a->workspace_bytes,

@@ -149,7 +149,7 @@ def test_large_vocabularies_and_many_rows(ctx, probs):
 
 @pytest.mark.parametrize("type_,probs", [("bf16", None), ("bf16", "bf16"), ("f16", "f32"), ("f32", "f16")])
 def test_the_largest_vocabularies(ctx, type_, probs):
-    """Rows that go by parts of 8192 ids: odd ends, drafts that stay and that do not."""
+    """Rows of more than a thousand parts, several to a thread: odd ends, drafts that stay and that do not."""
     for V, pad in ((2097153, 0), (2100008, 8)):
         print(f"[verify] {V} {type_} {probs}", flush=True)
         c = Verify(ctx, [3, 2], V, type_, probs, pad=pad, seed=V)
