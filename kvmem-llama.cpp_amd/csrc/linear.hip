@@ -186,7 +186,7 @@ static uint32_t chunk_from(const kvmem_hip_linear_args *a) {
 
 static ChunkPlan plan_chunks(const kvmem_hip_linear_args *a, uint32_t max_q) {
     ChunkPlan pl;
-    if (max_q < chunk_from(a)) {
+    if (a->n_seq == 0 || max_q < chunk_from(a)) {
         return pl;
     }
     pl.chunked = true;
@@ -197,6 +197,25 @@ static ChunkPlan plan_chunks(const kvmem_hip_linear_args *a, uint32_t max_q) {
     pl.key_bytes = static_cast<uint64_t>(parts) * 12 * (a->head_dim_k / 32) * kFragBytes;
     pl.head_bytes = kHeadBytes + ((a->beta ? 2 : 0) + pl.p_parts) * kLowerFrags * kFragBytes;
     pl.bytes = pl.entries * (pl.key_bytes * a->n_head_k + pl.head_bytes * a->n_head);
+    // Without the delta rule states add up: what a segment of chunks adds is made before
+    // what lies behind it is known, in a first pass, and a second one walks the segments
+    // again.  Worth it where the CUs are a quarter full or less and segments hold enough
+    // chunks to pay for their states' traffic.  One piece / segments, us: F16, heads of
+    // 64 x 64, 8 heads, 1024 tokens 42.9 / 25.1, 8192 tokens 265 / 48, eight requests of
+    // up to 4096 tokens 152 / 97; bf16, 32 heads of 128 x 128, 8192 tokens 326 / 217; F32,
+    // 8 heads of 256 x 256, 2048 tokens 376 / 210; bf16, 16 heads of 256 x 256, which the
+    // conditions leave whole, 1024 tokens 83.5 / 94.6 and 4096 tokens 290 / 307.
+    const bool narrow = a->head_dim_v % 64 || a->head_dim_k * float_type_size(a->type) > 256;  // 32 columns a workgroup
+    const uint64_t groups = static_cast<uint64_t>(a->n_seq) * a->n_head * (a->head_dim_v / (narrow ? 32 : 64));
+    const uint32_t segs = static_cast<uint32_t>(std::min<uint64_t>(256 / groups, pl.chunks / (a->head_dim_k / 32)));
+    if (!a->beta && segs >= 4) {
+        pl.seg_chunks = (pl.chunks + segs - 1) / segs;
+        pl.segs = (pl.chunks + pl.seg_chunks - 1) / pl.seg_chunks;
+        const uint64_t entries = static_cast<uint64_t>(a->n_seq) * pl.segs * a->n_head;
+        pl.seg_states = pl.bytes;
+        pl.seg_decays = pl.seg_states + entries * a->head_dim_k * a->head_dim_v * sizeof(float);
+        pl.bytes = (pl.seg_decays + entries * sizeof(float) + 15) / 16 * 16;
+    }
     return pl;
 }
 
@@ -214,6 +233,10 @@ static void launch_linear_chunks(hipStream_t stream, int type, uint32_t dim_k, c
     p.delta = a.beta != nullptr;
     p.outs = a.out != nullptr;
     p.p_parts = static_cast<uint32_t>(pl.p_parts);
+    p.segs = pl.segs;
+    p.seg_chunks = pl.seg_chunks;
+    p.seg_states = reinterpret_cast<float *>(workspace + pl.seg_states);
+    p.seg_decays = reinterpret_cast<float *>(workspace + pl.seg_decays);
     if (type == KVMEM_TYPE_F32) {
         launch_linear_chunks_f32(stream, p);
     } else if (type == KVMEM_TYPE_F16) {

@@ -36,6 +36,8 @@ struct ChunkPlan {
     uint32_t entries = 0;
     uint32_t chunks = 0;    // most of one request
     uint64_t key_bytes = 0, head_bytes = 0;  // of an entry, per key head and per head
+    uint32_t segs = 1, seg_chunks = 0;       // segments of a request, at most, and their chunks
+    uint64_t seg_decays = 0, seg_states = 0;  // where they are in the workspace
     uint64_t bytes = 0;
 };
 
@@ -52,6 +54,9 @@ struct ChunkParams {
     int type;
     uint32_t dim_k;
     uint32_t delta, outs, p_parts;
+    uint32_t segs, seg_chunks, second_pass;
+    float *seg_states;  // [requests][segs][heads][Dk][Dv]
+    float *seg_decays;  // [requests][segs][heads]
 };
 
 // Both launches of a call by chunks (the second only where the first was made), and

@@ -642,7 +642,7 @@ template <int N, int VALU> __device__ inline void interleave() {
 template <typename T, int DK>
 __device__ inline __attribute__((always_inline)) void walk_tokens(const ChunkParams &p, f32x4_t (&s)[DK / 16],
                                                                   uint64_t row0, uint32_t n, uint32_t h, uint32_t hk,
-                                                                  uint32_t col) {
+                                                                  uint32_t col, bool with_out) {
     const uint32_t g = (threadIdx.x & 63u) >> 4;
     for (uint32_t t = 0; t < n; ++t) {
         const uint64_t row = row0 + t;
@@ -678,7 +678,7 @@ __device__ inline __attribute__((always_inline)) void walk_tokens(const ChunkPar
                 s[d][r] = __builtin_fmaf(kd[d][r], x, a * s[d][r]);
             }
         }
-        if (p.outs) {
+        if (with_out) {
             const uint8_t *q = p.a.q + row * p.a.q_nb2 + hk * p.a.q_nb1;
             float o = 0.0f;
 #pragma unroll
@@ -734,6 +734,51 @@ __device__ inline void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// Segments' states one behind the other, in place: what a segment adds becomes the
+// state behind it, S_x = decay_x S_(x-1) + added_x.  The first one's holds the call's
+// state already, and the last one's is the second pass's.  Four elements a thread;
+// segments are read eight at a time, since a chain of loads would cost each of them a
+// latency.
+constexpr uint32_t kScanThreads = 256;
+constexpr uint32_t kScanAtOnce = 8;
+
+static __global__ __launch_bounds__(kScanThreads) void linear_scan_kernel(const ChunkParams p) {
+    const uint32_t s = blockIdx.y;
+    const Request rq = request_of(p.a.batch, s);
+    const uint32_t last = rq.count ? (rq.count - 1u) / (p.seg_chunks * kChunk) : 0u;
+    if (last < 2) {
+        return;
+    }
+    const uint64_t of_head = static_cast<uint64_t>(p.dim_k) * p.a.dim_v, of_seg = of_head * p.a.n_head;
+    const uint64_t at = (static_cast<uint64_t>(blockIdx.x) * kScanThreads + threadIdx.x) * 4u;
+    if (at >= of_seg) {
+        return;
+    }
+    float *made = p.seg_states + s * p.segs * of_seg + at;
+    const float *decays = p.seg_decays + static_cast<uint64_t>(s) * p.segs * p.a.n_head + at / of_head;
+    f32x4_t state = *reinterpret_cast<const f32x4_t *>(made);
+    for (uint32_t x0 = 1; x0 < last; x0 += kScanAtOnce) {
+        f32x4_t added[kScanAtOnce];
+        float decay[kScanAtOnce];
+#pragma unroll
+        for (uint32_t i = 0; i < kScanAtOnce; ++i) {
+            const uint32_t x = min(x0 + i, last - 1u);
+            added[i] = *reinterpret_cast<const f32x4_t *>(made + x * of_seg);
+            decay[i] = decays[static_cast<uint64_t>(x) * p.a.n_head];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kScanAtOnce; ++i) {
+            if (x0 + i < last) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    state[e] = state[e] == 0.0f ? added[i][e] : __builtin_fmaf(decay[i], state[e], added[i][e]);
+                }
+                *reinterpret_cast<f32x4_t *>(made + (x0 + i) * of_seg) = state;
+            }
+        }
+    }
+}
+
 // WAVES waves compute, 16 columns each, and as many bring the next chunk into LDS: a
 // wave issues one instruction at a time, and those for the copies would cost the
 // computing ones a third of a chunk's time.
@@ -757,6 +802,23 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
     Request rq = request_of(p.a.batch, s_id);
     rq.first = __builtin_amdgcn_readfirstlane(rq.first);
     rq.count = __builtin_amdgcn_readfirstlane(rq.count);
+    // the chunks of this workgroup's segment: the first pass leaves behind every segment
+    // but the last the state that it alone makes, the second starts from those
+    uint32_t c0 = 0, limit = rq.count;
+    uint32_t seg = 0, last_seg = 0;
+    if constexpr (!DELTA) {
+        if (p.segs > 1) {
+            const uint32_t of_seg = p.seg_chunks * kChunk;
+            seg = blockIdx.z;
+            last_seg = rq.count ? (rq.count - 1u) / of_seg : 0u;
+            if (seg > last_seg ||
+                (p.second_pass ? seg == 0 || (!p.outs && seg < last_seg) : seg == last_seg && seg > 0)) {
+                return;
+            }
+            c0 = seg * p.seg_chunks;
+            limit = min(rq.count, (seg + 1) * of_seg);
+        }
+    }
     const uint64_t entry0 = entry_of(rq, s_id, 0);
     const uint64_t key_step = p.key_bytes * (p.a.n_head / p.a.group), head_step = p.head_bytes * p.a.n_head;
     const uint8_t *keys = p.keys + entry0 * key_step + hk * p.key_bytes;
@@ -797,17 +859,17 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
                 }
             }
         };
-        if (Space::places == 2 && rq.count) {
-            request(0, lds);
+        if (Space::places == 2 && c0 * kChunk < limit) {
+            request(c0, lds + (c0 & 1u) * Space::bytes);
         }
-        for (uint32_t c = 0; c * kChunk < rq.count; ++c) {
+        for (uint32_t c = c0; c * kChunk < limit; ++c) {
             if (Space::places == 1) {
                 lds_barrier();  // the chunk before is read
                 request(c, lds);
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             lds_barrier();
-            if (Space::places == 2 && (c + 1) * kChunk < rq.count) {
+            if (Space::places == 2 && (c + 1) * kChunk < limit) {
                 request(c + 1, lds + ((c + 1) & 1u) * Space::bytes);
             }
         }
@@ -823,7 +885,17 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
     for (int d = 0; d < TILES; ++d) {
         s[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    if (p.a.state && rq.has_slot) {
+    const uint64_t seg_at = static_cast<uint64_t>(s_id) * p.segs * p.a.n_head + h;  // the request's first segment
+    if (!DELTA && p.second_pass) {
+        const float *made = p.seg_states + (seg_at + (seg - 1u) * p.a.n_head) * DK * p.a.dim_v + col;
+#pragma unroll
+        for (int d = 0; d < TILES; ++d) {
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) {
+                s[d][r] = made[static_cast<uint64_t>(16u * d + 4u * g + r) * p.a.dim_v];
+            }
+        }
+    } else if (seg == 0 && p.a.state && rq.has_slot) {
 #pragma unroll
         for (int d = 0; d < TILES; ++d) {
 #pragma unroll
@@ -836,10 +908,12 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
     const uint64_t out_row = static_cast<uint64_t>(p.a.n_head) * p.a.dim_v;
     const uint32_t esz = FINE && p.a.out_type == KVMEM_TYPE_F32 ? 4u : 2u;
     const uint32_t out_at = ((lane & 15u) * static_cast<uint32_t>(out_row) + 4u * g) * esz;
-    for (uint32_t c = 0; c * kChunk < rq.count; ++c) {
+    const bool with_out = p.outs && (seg == 0 || p.second_pass);
+    float decayed = 1.0f;  // over the segment
+    for (uint32_t c = c0; c * kChunk < limit; ++c) {
         const uint32_t n = min(kChunk, rq.count - c * kChunk);
         const uint64_t row0 = static_cast<uint64_t>(rq.first) + c * kChunk;
-        const uint32_t rows = p.outs ? n : 0u;  // without an out, Q and P are zeros
+        const uint32_t rows = with_out ? n : 0u;
         const uint8_t *here = lds + (Space::places == 2 ? (c & 1u) * Space::bytes : 0u);
         const uint8_t *kp = keys + c * key_step;
         if constexpr (Space::keys) {
@@ -955,8 +1029,12 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
             }
         }
         const float any_odd = (odd[0] + odd[1]) + (odd[2] + odd[3]);
+        const float whole = ch->from_first[kChunk - 1];
+        if constexpr (!DELTA) {
+            decayed *= whole;
+        }
         if (__builtin_expect(__any(any_odd != any_odd || ch->by_token != 0), 0)) {
-            walk_tokens<T, DK>(p, s, row0, n, h, hk, col);
+            walk_tokens<T, DK>(p, s, row0, n, h, hk, col, with_out);
             continue;
         }
         half8_t dh[2], dl[2];
@@ -1006,7 +1084,6 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
             last[m] = *reinterpret_cast<const f32x4_t *>(ch->to_last + 16u * m + 4u * g);
             out_first[m] = p.a.scale * ch->from_first[16u * m + (lane & 15u)];
         }
-        const float whole = ch->from_first[kChunk - 1];
         const int exp_d = column_exp<4>(d);
         {
             f32x4_t pd[4] = {zero, zero, zero, zero};
@@ -1104,6 +1181,22 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
         }
         update(TILES - 4);
     }
+    if (!DELTA && seg < last_seg) {
+        if (!p.second_pass) {
+            float *made = p.seg_states + (seg_at + seg * p.a.n_head) * DK * p.a.dim_v + col;
+#pragma unroll
+            for (int d = 0; d < TILES; ++d) {
+#pragma unroll
+                for (uint32_t r = 0; r < 4; ++r) {
+                    made[static_cast<uint64_t>(16u * d + 4u * g + r) * p.a.dim_v] = s[d][r];
+                }
+            }
+            if (col == 0 && g == 0) {
+                p.seg_decays[seg_at + seg * p.a.n_head] = decayed;
+            }
+        }
+        return;
+    }
     if (p.a.state_out && rq.has_slot) {
 #pragma unroll
         for (int d = 0; d < TILES; ++d) {
@@ -1142,7 +1235,7 @@ static void walk_cols(hipStream_t stream, const ChunkParams &p) {
     constexpr bool wide = ChunkSpace<T, DK, DELTA, FINE, 4>::places == 2;
     const uint32_t cols = wide && p.a.dim_v % 64 == 0 ? 64u : 32u;
     const uint32_t units = p.a.n_head * (p.a.dim_v / cols);
-    const dim3 grid((units + kXcds - 1) / kXcds * kXcds, p.a.n_seq);
+    const dim3 grid((units + kXcds - 1) / kXcds * kXcds, p.a.n_seq, p.segs);
     if constexpr (wide) {
         if (cols == 64) {
             linear_walk_kernel<T, DK, DELTA, FINE, 4><<<grid, 512, 0, stream>>>(p);
@@ -1161,8 +1254,19 @@ static void launch_type(hipStream_t stream, const ChunkParams &p) {
     const bool fine = p.p_parts == 2;  // the output takes both parts
     if (p.delta) {
         fine ? walk_cols<T, DK, true, true>(stream, p) : walk_cols<T, DK, true, false>(stream, p);
-    } else {
-        fine ? walk_cols<T, DK, false, true>(stream, p) : walk_cols<T, DK, false, false>(stream, p);
+        return;
+    }
+    fine ? walk_cols<T, DK, false, true>(stream, p) : walk_cols<T, DK, false, false>(stream, p);
+    if (p.segs > 1 && hipPeekAtLastError() == hipSuccess) {
+        const uint64_t quads = static_cast<uint64_t>(p.a.n_head) * p.dim_k * p.a.dim_v / 4;
+        const dim3 grid(static_cast<uint32_t>((quads + kScanThreads - 1) / kScanThreads), p.a.n_seq);
+        linear_scan_kernel<<<grid, kScanThreads, 0, stream>>>(p);
+        if (hipPeekAtLastError() != hipSuccess) {
+            return;
+        }
+        ChunkParams second = p;
+        second.second_pass = 1;
+        fine ? walk_cols<T, DK, false, true>(stream, second) : walk_cols<T, DK, false, false>(stream, second);
     }
 }
 

@@ -93,6 +93,9 @@ static void linear() {
     };
     expect("linear: null args", inv, kvmem_hip_linear_attention(&ctx, nullptr));
     size("linear: null args", 0, kvmem_hip_linear_attention_workspace(nullptr));
+    Args none = ok;
+    none.n_seq = 0, none.beta = nullptr, none.max_q = none.n_tokens = 1u << 20;
+    size("linear: no requests", 0, kvmem_hip_linear_attention_workspace(&none));
     call("linear: type", uns, [](Args &a) { a.type = KVMEM_TYPE_Q4_0; });
     call("linear: out type", uns, [](Args &a) { a.out_type = KVMEM_TYPE_Q4_0; });
     for (uint32_t d : {0u, 32u, 96u, 512u}) {

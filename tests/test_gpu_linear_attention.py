@@ -213,6 +213,60 @@ def test_calls_of_some_states(ctx, n, type_):
     c.check(chunked=chunked)
 
 
+@pytest.mark.parametrize("type_,out,dims", [("f16", "f16", (64, 64)), ("bf16", "bf16", (128, 96)), ("f32", "f32", (64, 32)),
+                                            ("bf16", "f32", (256, 64))])
+def test_long_requests_without_the_delta_rule(ctx, type_, out, dims):
+    """Requests in segments: long, short, empty and cut ones, of every kind of decay, states stored in place, missing
+    and not wanted, without an out."""
+    for decay, rate in (("token", 1.0), ("head", 1.0), ("none", 1.0), ("token", 100.0)):
+        rq = Requests([1100, 1, 64, 320, 0, 129, 640], slots=[3, 0, 5, 9, 1, 2, 4], n_slots=6,
+                      use=[1090, 1, 64, 400, 0, 65, 128], tail=1)
+        c = Linear(ctx, rq, 1, 2, *dims, type_, out, delta=False, decay=decay, seed=sum(dims), rate=rate)
+        c.run()
+        c.check()
+        # in place, and without an out
+        want, states = c.out.clone(), c.state_out.clone()
+        for state, more in ((c.state.clone(), {}), (c.state.clone(), dict(out=None, q=None))):
+            before = state.clone()
+            c.out.fill_(FILL)
+            torch.cuda.synchronize()
+            ctx.linear_attention(c.args(state=ptr(state), state_out=ptr(state), **more))
+            ctx.sync()
+            assert torch.equal(c.out, torch.full_like(c.out, FILL) if more else want)
+            for s, slot in enumerate(rq.slots):
+                if slot < rq.n_slots:
+                    assert torch.equal(state[slot], states[slot]), (s, slot)
+            kept = [x for x in range(rq.n_slots) if x not in rq.slots]
+            assert all(torch.equal(state[x], before[x]) for x in kept)
+
+
+def test_segments_with_numbers_that_are_not_finite(ctx):
+    """As in one piece: values stay in their dim, clearing decays clear, gates and keys stay in their head, and no
+    earlier token changes."""
+    n = 1000
+    clean = Linear(ctx, Requests([n]), 2, 2, 64, 64, "bf16", "f32", delta=False, seed=4)
+    clean.run()
+    for t in (0, 130, 700, 999):
+        for what in ("v", "k", "decay"):
+            for x in (float("nan"), float("inf")):
+                c = Linear(ctx, Requests([n]), 2, 2, 64, 64, "bf16", "f32", delta=False, seed=4)
+                if what == "decay":
+                    c.decay[t, 1] = x
+                else:
+                    getattr(c, what)[t, 1, 9] = x
+                c.run()
+                ok = torch.isfinite(c.out)
+                assert ok[:t].all() and ok[:, 0].all() and not ok[t:, 1, 9].any()
+                if what == "v":
+                    assert ok[:, 1, :9].all() and ok[:, 1, 10:].all()
+                assert torch.allclose(torch.where(ok, c.out, 0), torch.where(ok, clean.out, 0), rtol=1e-4, atol=1e-5)
+    c = Linear(ctx, Requests([n]), 2, 2, 64, 64, "bf16", "f32", delta=False, seed=4)
+    c.decay[130] = -float("inf")
+    c.decay[700, 1] = -float("inf")
+    c.run()
+    c.check()
+
+
 def test_own_workspace_streams_and_replays(ctx):
     """A captured call brings its workspace; two graphs with one each replay at once; results are the eager ones."""
     calls = [Linear(ctx, Requests([100, 30]), 1, 2, 128, 128, seed=i) for i in range(2)]
