@@ -27,6 +27,9 @@ namespace kvmem_hip {
 constexpr uint32_t kVerifyThreads = 256;
 constexpr uint32_t kVerifyMaxDraft = 127;
 constexpr uint32_t kPartIds = 8 * kVerifyThreads;
+// Parts from which a wave takes a whole one.  Rows of 152000 ids, by four waves / by one:
+// 64 rows (4800 parts) 26.0 / 25.4 us, 32 rows 21.6 / 21.9, 8 rows 16.8 / 18.3.
+constexpr uint64_t kManyParts = 4096;
 constexpr uint32_t kVerifyMaxVocab = 1u << 24;
 
 constexpr uint32_t kNowhere = 0xffffffffu;
@@ -63,7 +66,6 @@ struct VerifyParams {
     uint32_t *n_keep;
     uint32_t *kv_len_out;
     uint32_t n_parts;    // of a row
-    uint32_t parts_each; // of a workgroup of the first kernel
     Part *parts;         // [n_seq][max_draft + 1][n_parts]
     double *rest;        // [n_seq][n_parts]
     Choice *choice;      // [n_seq]
@@ -111,8 +113,11 @@ __constant__ double kExpFine[16] = {
 struct ExpTable {
     double entry[256];
 };
-__device__ inline void fill_table(ExpTable &t) {
-    t.entry[threadIdx.x] = kExpCoarse[threadIdx.x >> 4] * kExpFine[threadIdx.x & 15u];
+template <uint32_t THREADS = kVerifyThreads> __device__ inline void fill_table(ExpTable &t) {
+#pragma unroll
+    for (uint32_t i = threadIdx.x; i < 256; i += THREADS) {
+        t.entry[i] = kExpCoarse[i >> 4] * kExpFine[i & 15u];
+    }
     __syncthreads();
 }
 __device__ inline double weight_of(const ExpTable &table, float x, double inv, double max_inv) {
@@ -225,72 +230,84 @@ __device__ inline void load_part(const uint8_t *row, uint32_t first, uint32_t en
     }
 }
 
-// Each wave sums relative to its own maximum, so that a part costs one barrier; the
-// next part's numbers are on their way meanwhile.
-template <typename T>
-__global__ __launch_bounds__(kVerifyThreads) void verify_parts_kernel(const VerifyParams p) {
+// A thread has GROUPS groups of eight ids.  Each wave sums relative to its own maximum,
+// and the first joins them.  Bound by vector instructions, twelve fp64 ones and two more
+// an id and some ninety a wave to combine its lanes: with four groups a wave takes the
+// whole part and combines a quarter as often.  512 rows of 152000 bf16 ids, the whole
+// call: 78.3 us with one group, 71.7 with two, 67.9 with four (this kernel 49 us, 3.2
+// TB/s); 8 rows of 32000 ids: 13.1, 13.8, 16.4.
+template <typename T, int GROUPS>
+__global__ __launch_bounds__(kVerifyThreads / GROUPS) void verify_parts_kernel(const VerifyParams p) {
+    constexpr uint32_t waves = 4 / GROUPS, threads = kVerifyThreads / GROUPS;
     __shared__ ExpTable table;
-    __shared__ Part waves[2][4];
-    const uint32_t s = blockIdx.z, i = blockIdx.y, wave = threadIdx.x >> 6;
+    __shared__ Part of_waves[waves];
+    const uint32_t s = blockIdx.z, i = blockIdx.y, v0 = blockIdx.x * kPartIds;
     uint32_t count, all;
     const uint32_t first = rows_of(p, s, count, all);
     if (i >= count) {
         return;
     }
     const uint8_t *row = p.logits + (static_cast<uint64_t>(first) + i) * p.logits_nb;
-    Part *parts = p.parts + (static_cast<uint64_t>(s) * (p.max_draft + 1) + i) * p.n_parts;
-    uint32_t part = blockIdx.x * p.parts_each;
-    const uint32_t end = min(p.n_parts, part + p.parts_each);
-    float next[8];
-    load_part<T>(row, part * kPartIds, p.n_vocab, next);
-    fill_table(table);
+    float x[GROUPS][8];
+#pragma unroll
+    for (uint32_t j = 0; j < GROUPS; ++j) {
+        load_part<T>(row, v0 + j * threads * 8u, p.n_vocab, x[j]);
+    }
+    fill_table<threads>(table);
     bool greedy;
     const double inv = inv_temperature(p, s, greedy);
-    for (; part < end; ++part) {
-        float x[8], m = -INFINITY;
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            x[e] = next[e];
-            m = __builtin_fmaxf(m, x[e]);  // NaN is left out
+            m = __builtin_fmaxf(m, x[j][e]);  // NaN is left out
         }
-        if (part + 1 < end) {
-            load_part<T>(row, (part + 1) * kPartIds, p.n_vocab, next);
-        }
-        m = wave_max(m);
-        double sum = 0.0;
-        uint32_t at = kNowhere;
-        if (greedy || m == INFINITY) {
+    }
+    m = wave_max(m);
+    double sum = 0.0;
+    uint32_t at = kNowhere;
+    if (greedy || m == INFINITY) {
+#pragma unroll
+        for (int j = GROUPS - 1; j >= 0; --j) {
 #pragma unroll
             for (int e = 7; e >= 0; --e) {
-                at = x[e] == m ? part * kPartIds + threadIdx.x * 8u + static_cast<uint32_t>(e) : at;
+                at = x[j][e] == m ? v0 + (static_cast<uint32_t>(j) * threads + threadIdx.x) * 8u +
+                                        static_cast<uint32_t>(e)
+                                  : at;
             }
-            at = wave_min(m > -INFINITY ? at : kNowhere);
-        } else if (m > -INFINITY) {
-            const double max_inv = static_cast<double>(m) * inv;
-            double part_sum[2] = {};
+        }
+        at = wave_min(m > -INFINITY ? at : kNowhere);
+    } else if (m > -INFINITY) {
+        const double max_inv = static_cast<double>(m) * inv;
+        double part_sum[2] = {};
+#pragma unroll
+        for (int j = 0; j < GROUPS; ++j) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                part_sum[e & 1] += weight_of(table, x[e], inv, max_inv);
+                part_sum[e & 1] += weight_of(table, x[j][e], inv, max_inv);
             }
-            sum = wave_sum(part_sum[0] + part_sum[1]);
         }
-        Part *mine = waves[part & 1u];
+        sum = wave_sum(part_sum[0] + part_sum[1]);
+    }
+    if constexpr (waves > 1) {
         if ((threadIdx.x & 63u) == 0) {
-            mine[wave] = Part{sum, m, at};
+            of_waves[threadIdx.x >> 6] = Part{sum, m, at};
         }
-        __syncthreads();  // the other place is read before the next
-        if (wave == 0) {
-            const Part w = mine[threadIdx.x & 3u];
-            m = wave_max(w.max);
-            at = wave_min(w.max == m ? w.at : kNowhere);
-            sum = threadIdx.x < 4 && w.sum > 0.0 && m < INFINITY
-                      ? w.sum * weight_of(table, w.max, inv, static_cast<double>(m) * inv)
-                      : 0.0;
-            sum = wave_sum(sum);
-            if (threadIdx.x == 0) {
-                parts[part] = Part{sum, m, at};
-            }
+        __syncthreads();
+        if (threadIdx.x >= 64) {
+            return;
         }
+        const Part w = of_waves[threadIdx.x % waves];
+        m = wave_max(w.max);
+        at = wave_min(w.max == m ? w.at : kNowhere);
+        sum = threadIdx.x < waves && w.sum > 0.0 && m < INFINITY
+                  ? w.sum * weight_of(table, w.max, inv, static_cast<double>(m) * inv)
+                  : 0.0;
+        sum = wave_sum(sum);
+    }
+    if (threadIdx.x == 0) {
+        p.parts[(static_cast<uint64_t>(s) * (p.max_draft + 1) + i) * p.n_parts + blockIdx.x] = Part{sum, m, at};
     }
 }
 
@@ -692,8 +709,12 @@ static void launch_rest(hipStream_t stream, const VerifyParams &p) {
 
 template <typename T>
 static void launch_verify(hipStream_t stream, const VerifyParams &p) {
-    verify_parts_kernel<T>
-        <<<dim3((p.n_parts + p.parts_each - 1) / p.parts_each, p.max_draft + 1, p.n_seq), kVerifyThreads, 0, stream>>>(p);
+    const dim3 grid(p.n_parts, p.max_draft + 1, p.n_seq);
+    if (static_cast<uint64_t>(p.n_parts) * (p.max_draft + 1) * p.n_seq >= kManyParts) {
+        verify_parts_kernel<T, 4><<<grid, kVerifyThreads / 4, 0, stream>>>(p);
+    } else {
+        verify_parts_kernel<T, 1><<<grid, kVerifyThreads, 0, stream>>>(p);
+    }
     if (hipPeekAtLastError() != hipSuccess) {
         return;  // parts that were not written must not be read
     }
@@ -825,11 +846,6 @@ int kvmem_hip_verify_draft(kvmem_hip_ctx *ctx, const kvmem_hip_verify_args *a) {
     p.n_keep = a->n_keep;
     p.kv_len_out = a->kv_len_out;
     p.n_parts = pl.n_parts;
-    // up to four parts a workgroup once there are many: 512 rows of 152000 ids (38400
-    // parts) 78.8 us one by one, 74.9 by two, 73.9 by four, 80.5 by eight; 256 rows 51.1,
-    // 49.3, 49.7, 54.0; 8 rows 16.8, 17.8, 19.4, 23.5
-    const uint64_t parts = static_cast<uint64_t>(pl.n_parts) * (a->max_draft + 1) * a->n_seq;
-    p.parts_each = static_cast<uint32_t>(std::clamp<uint64_t>(parts / 8192, 1, 4));
     (void) hipSetDevice(ctx->device);
     uint8_t *ws = nullptr;
     if (const int rc = call_workspace(ctx, ctx->verify_scratch, a->workspace, a->workspace_bytes,
