@@ -797,8 +797,10 @@ KVMEM_HIP_API int kvmem_hip_conv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_conv_a
  *   out      contiguous [n_tokens][n_head][head_dim_v], 16-byte aligned
  * The state, sums and decays are fp32 or wider; out is rounded once.  Calls of
  * few tokens a request go token by token, longer ones by chunks of tokens on
- * the matrix cores: there the factors of every product are split into bf16
- * parts of 24 bits together (16 bits for what reaches only a 16-bit out).
+ * the matrix cores: there every factor is scaled by a power of two (states,
+ * values and their like column by column) and taken as two f16 parts of 22 bits
+ * together, cut 2^-39 below the largest; what reaches only a bf16 out is one part
+ * of 11 bits.
  * A value that is not finite reaches no earlier token, and where only a v is not
  * finite no other dim; what it reaches is not finite either (NaN, or the value).
  * head_dim_k 64, 128 or 256, head_dim_v a multiple of 32 up to 512; at most
@@ -860,9 +862,9 @@ KVMEM_HIP_API int kvmem_hip_linear_attention(kvmem_hip_ctx *ctx, const kvmem_hip
  *   the lowest id whose sum_{i <= id} w_i > u_sample[s] * sum_i w_i and w_id > 0
  *   (rounded sums that leave none: the last id with w_id > 0)
  * Exponentials and sums are fp64, so a choice differs from the formula's only
- * where u falls within about 1e-14 of a border.  Temperature 0 (NULL: 1), and a row with
- * a logit of +inf: the largest logit (the lowest id of equal ones) has
- * probability 1, whatever the draft's distribution.  NaN logits count as -inf;
+ * where u falls within about 1e-13 of a border.  A temperature that is not above
+ * 0 (NULL: 1), and a row with a logit of +inf: the largest logit (the lowest id of
+ * equal ones) has probability 1, whatever the draft's distribution.  NaN logits count as -inf;
  * a row of nothing but -inf keeps no draft and gives -1.  A draft outside [0,
  * n_vocab) does not stay.
  *   tokens_out[s]  [max_draft + 1]: the drafts that stay, the next token, -1 behind
@@ -871,7 +873,7 @@ KVMEM_HIP_API int kvmem_hip_linear_attention(kvmem_hip_ctx *ctx, const kvmem_hip
  *   kv_len_out[s]  kv_len[s] - rows + n_keep: the keys that stay of kv_len, which
  *                  counts all the step's tokens (both may be NULL)
  * Rows of logits and probs are contiguous, element (v, r) at v*size + r*nb bytes,
- * size-aligned; 16-byte aligned rows are read 16 bytes at a time.  probs are not
+ * size-aligned.  probs are not
  * negative; only the rows whose draft is tested, and of these the one that refuses,
  * are read.
  * At most 65535 requests, 127 drafts, 2^24 ids.  Parts of rows meet in a workspace

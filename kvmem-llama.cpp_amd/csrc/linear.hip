@@ -20,7 +20,10 @@ namespace kvmem_hip {
 // state never meet (S^T k and S^T q are sums over rows): waves need nothing of
 // each other, and a token costs one exchange over the 8 row groups, S^T k and
 // S^T q together (o follows from the old state: S' ^T q = a S^T q + (k . q) d).
-// Bytes bound it: the state is read once and written once.
+// Bytes bound it: the state is read once and written once.  Measured, 48 heads of 128 x
+// 128: 64 requests of a token 80 us = 5.0 TB/s of 405 MB (a copy kernel reaches 6.07);
+// 8 requests of 6 tokens 15.3 us, 52 MB, then a wave's 1.2 us a token, dependent
+// products and exchanges; one token of one request 4.1 us.
 constexpr uint32_t kStepCols = 32;
 
 template <typename T, int R> struct StepRows {
