@@ -22,8 +22,9 @@ namespace kvmem_hip {
 // S^T q together (o follows from the old state: S' ^T q = a S^T q + (k . q) d).
 // Bytes bound it: the state is read once and written once.  Measured, 48 heads of 128 x
 // 128: 64 requests of a token 80 us = 5.0 TB/s of 405 MB (a copy kernel reaches 6.07);
-// 8 requests of 6 tokens 15.3 us, 52 MB, then a wave's 1.2 us a token, dependent
+// 8 requests of 6 tokens 14.6 us, 52 MB, then a wave's 1.2 us a token, dependent
 // products and exchanges; one token of one request 4.1 us.
+// By 16 columns a wave, whose rows are half lines: 107, 16.8 and 3.9 us.
 constexpr uint32_t kStepCols = 32;
 
 template <typename T, int R> struct StepRows {
@@ -44,10 +45,14 @@ __device__ inline void load_step(const LinearParams &p, uint64_t row, uint32_t h
     s.beta = p.beta ? *reinterpret_cast<const float *>(p.beta + row * p.beta_nb + h * 4u) : 0.0f;
 }
 
+// Moves between lanes by the VALU: through LDS six tokens of eight requests take 15.2
+// us for 14.6.
 __device__ inline float sum_row_groups(float v) {
     v += lane_xor<8>(v);
-    v += lane_xor<16>(v);
-    return v + lane_xor<32>(v);
+    auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
 }
 
 template <typename T, int DK>

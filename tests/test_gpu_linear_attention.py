@@ -304,6 +304,46 @@ def test_own_workspace_streams_and_replays(ctx):
         calls[0].run()
 
 
+def test_segments_replayed_in_place(ctx):
+    """A captured call in segments that updates its state: every replay is the eager call's next one."""
+    c = Linear(ctx, Requests([1100, 300, 64]), 1, 2, 64, 64, "f16", "f32", delta=False, seed=6)
+    need = ctx.linear_attention_workspace(c.args())
+    st, g, ws = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    eager, state = c.state.clone(), c.state.clone()
+    torch.cuda.synchronize()
+    ctx.set_stream(st.cuda_stream)
+    try:
+        with torch.cuda.graph(g, stream=st):
+            ctx.linear_attention(c.args(workspace=ptr(ws), workspace_bytes=need, state=ptr(state), state_out=ptr(state)))
+    finally:
+        ctx.set_stream(None)
+    for _ in range(4):
+        ctx.linear_attention(c.args(state=ptr(eager), state_out=ptr(eager)))
+        ctx.sync()
+        want = c.out.clone()
+        c.out.fill_(FILL)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(c.out, want) and torch.equal(state, eager)
+
+
+def test_segments_cut_by_the_call(ctx):
+    """max_q, n_use and n_tokens cut requests inside a segment; requests behind the last token have none."""
+    for most in (1000, 513, 512, 511, 130):
+        rq = Requests([1100, 700, 3])
+        c = Linear(ctx, rq, 1, 1, 64, 64, "f16", "f32", delta=False, seed=2)
+        rq.use = [min(most, n) for n in rq.lengths]
+        c.run(max_q=most)
+        c.check(chunked=True)
+    rq = Requests([1100, 700, 3])
+    c = Linear(ctx, rq, 1, 1, 64, 64, "f16", "f32", delta=False, seed=2)
+    rq.use = [1100, 1200 - 1100, 0]
+    c.run(n_tokens=1200)
+    c.check()
+
+
 def test_two_contexts_at_once(ctx):
     other = kv.Context(0)
     try:
