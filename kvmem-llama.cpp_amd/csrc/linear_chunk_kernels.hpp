@@ -787,6 +787,23 @@ static __global__ __launch_bounds__(kScanThreads) void linear_scan_kernel(const 
     }
 }
 
+// The request that the workgroups of `rank` take: the longest ones first, so that the
+// last to end are short (eight bf16 prompts of up to 4096 tokens, 32 heads of 128 x 128:
+// 378 us, 409 in their own order).  Beyond a wave's lanes of requests, in their own order.
+__device__ inline uint32_t request_by_length(const LinearParams &a, uint32_t rank) {
+    if (a.n_seq == 1 || a.n_seq > 64) {
+        return rank;
+    }
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t count = lane < a.n_seq ? request_of(a.batch, lane).count : 0u;
+    uint32_t before = 0;  // longer ones, and as long ones in front of it
+    for (uint32_t j = 0; j < a.n_seq; ++j) {
+        const uint32_t other = __builtin_amdgcn_readlane(count, j);
+        before += other > count || (other == count && j < lane) ? 1u : 0u;
+    }
+    return static_cast<uint32_t>(__builtin_ctzll(__ballot(lane < a.n_seq && before == rank)));
+}
+
 // WAVES waves compute, 16 columns each, and as many bring the next chunk into LDS: a
 // wave issues one instruction at a time, and those for the copies would cost the
 // computing ones a third of a chunk's time (8192 tokens, 48 heads of 128 x 128: 728 us
@@ -811,7 +828,7 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
     if (unit >= p.a.n_head * slices) {
         return;
     }
-    const uint32_t h = unit / slices, s_id = blockIdx.y;
+    const uint32_t h = unit / slices, s_id = request_by_length(p.a, blockIdx.y);
     const uint32_t col0 = (unit % slices) * (16u * WAVES);
     const uint32_t hk = h / p.a.group;
     Request rq = request_of(p.a.batch, s_id);
@@ -1244,7 +1261,8 @@ static void prepare(hipStream_t stream, const ChunkParams &p) {
 // 64 columns a workgroup where a head has them and two chunks of that width fit into
 // LDS, else 32.  A chunk takes a wave the same time either way (one request of 8192
 // tokens, 48 heads of 128 x 128: 446 us, 443 by 32), and wide workgroups read the
-// operands half as often (eight of up to 4096 tokens, 32 heads: 397 us, 553 by 32).
+// operands half as often (eight of up to 4096 tokens, 32 heads, at an earlier step: 397
+// us, 553 by 32).
 template <typename T, int DK, bool DELTA, bool FINE>
 static void walk_cols(hipStream_t stream, const ChunkParams &p) {
     constexpr bool wide = ChunkSpace<T, DK, DELTA, FINE, 4>::places == 2;

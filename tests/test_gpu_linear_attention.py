@@ -344,6 +344,16 @@ def test_segments_cut_by_the_call(ctx):
     c.check()
 
 
+@pytest.mark.parametrize("S", [2, 63, 64, 65, 90])
+def test_requests_of_every_order(ctx, S):
+    """Chunked requests in and out of order of their lengths, equal and empty ones, around a wave's lanes of them."""
+    g = np.random.default_rng(S)
+    for lengths in (sorted(int(x) for x in g.integers(0, 140, S)), [70] * S, [int(x) for x in g.integers(0, 3, S) * 65]):
+        c = Linear(ctx, Requests(lengths, slots=[int(x) for x in g.permutation(S)], tail=1), 1, 1, 64, 32, "f16", "f32", seed=S)
+        c.run(max_q=140)
+        c.check(chunked=True)
+
+
 def test_two_contexts_at_once(ctx):
     other = kv.Context(0)
     try:
