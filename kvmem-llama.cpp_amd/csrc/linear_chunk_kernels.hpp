@@ -1140,15 +1140,17 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 es[r] += exp_q;
-                ed[r] = __shfl(exp_d, static_cast<int>(4u * g) + r, 64) + exp_p - es[r];
+                ed[r] = __shfl(exp_d, static_cast<int>(4u * g) + r, 64) + exp_p;
             }
 #pragma unroll
             for (uint32_t m = 0; m < 4; ++m) {
                 float y[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    y[r] = __builtin_amdgcn_ldexpf(
-                        __builtin_fmaf(out_first[m], o[m][r], __builtin_amdgcn_ldexpf(pd[m][r], ed[r])), es[r]);
+                    // both terms as they are: the scale of a column of zeros or next to nothing
+                    // would carry P D beyond fp32
+                    y[r] = __builtin_fmaf(out_first[m], __builtin_amdgcn_ldexpf(o[m][r], es[r]),
+                                          __builtin_amdgcn_ldexpf(pd[m][r], ed[r]));
                 }
                 uint8_t *to = out + m * 16u * out_row * esz;
                 if (16u * m + (lane & 15u) < rows) {
