@@ -92,11 +92,13 @@ __device__ inline float load_float(const uint8_t *p, int type, uint64_t i) {
                                   : __uint_as_float(static_cast<uint32_t>(h) << 16);
 }
 
-// exp((x - max) / temperature) for x <= max, inv = 1 / temperature, in fp64: with
+// exp((x - max) / temperature) for x <= max, inv = 1 / temperature, in fp64, the
+// difference first: it is 0 at the maximum and rounded once elsewhere, however small the
+// temperature (max / temperature, rounded by itself, is off by 2^-53 of its size).  With
 // n = rint(256 t / ln 2), e^t = 2^(n / 256) e^r, |r| <= ln 2 / 512, where e^r's series
 // to r^3 leaves 1.4e-13 and 2^(n mod 256 / 256) comes from a table in LDS.  t is cut at
-// -800, whose weight is 0; that is also where -inf and NaN end.  Eleven fp64 operations
-// (a table of 32, to r^5: thirteen, 5 % of the largest calls) against some 40 of the
+// -800, whose weight is 0; that is also where -inf and NaN end.  Twelve fp64 operations
+// (a table of 32, to r^5: fourteen, 5 % of the largest calls) against some 40 of the
 // library's exp, which has to hold for every argument.
 __constant__ double kExpCoarse[16] = {
     0x1.0000000000000p+0, 0x1.0b5586cf9890fp+0, 0x1.172b83c7d517bp+0, 0x1.2387a6e756238p+0,
@@ -120,8 +122,8 @@ template <uint32_t THREADS = kVerifyThreads> __device__ inline void fill_table(E
     }
     __syncthreads();
 }
-__device__ inline double weight_of(const ExpTable &table, float x, double inv, double max_inv) {
-    const double t = fmax(__builtin_fma(static_cast<double>(x), inv, -max_inv), -800.0);
+__device__ inline double weight_of(const ExpTable &table, float x, double inv, double max) {
+    const double t = fmax((static_cast<double>(x) - max) * inv, -800.0);
     constexpr double magic = 0x1.8p52;  // leaves n in the low bits
     const double k = __builtin_fma(t, 0x1.71547652b82fep+8, magic);
     const int n = static_cast<int>(__builtin_bit_cast(uint64_t, k));
@@ -279,13 +281,13 @@ __global__ __launch_bounds__(kVerifyThreads / GROUPS) void verify_parts_kernel(c
         }
         at = wave_min(m > -INFINITY ? at : kNowhere);
     } else if (m > -INFINITY) {
-        const double max_inv = static_cast<double>(m) * inv;
+        const double max = m;
         double part_sum[2] = {};
 #pragma unroll
         for (int j = 0; j < GROUPS; ++j) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                part_sum[e & 1] += weight_of(table, x[j][e], inv, max_inv);
+                part_sum[e & 1] += weight_of(table, x[j][e], inv, max);
             }
         }
         sum = wave_sum(part_sum[0] + part_sum[1]);
@@ -302,7 +304,7 @@ __global__ __launch_bounds__(kVerifyThreads / GROUPS) void verify_parts_kernel(c
         m = wave_max(w.max);
         at = wave_min(w.max == m ? w.at : kNowhere);
         sum = threadIdx.x < waves && w.sum > 0.0 && m < INFINITY
-                  ? w.sum * weight_of(table, w.max, inv, static_cast<double>(m) * inv)
+                  ? w.sum * weight_of(table, w.max, inv, static_cast<double>(m))
                   : 0.0;
         sum = wave_sum(sum);
     }
@@ -503,12 +505,12 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_decide_kernel(const Ver
         }
 #pragma unroll
         for (int x = 0; x < kRowsAtOnce; ++x) {
-            const double max_inv = static_cast<double>(row[x].max) * inv;
+            const double max = row[x].max;
             uint32_t id_of_max = kNowhere;
             double sum = 0.0;
             auto add = [&](const Part &part) {
                 id_of_max = part.max == row[x].max ? min(id_of_max, part.at) : id_of_max;
-                sum += part.sum > 0.0 ? part.sum * weight_of(table, part.max, inv, max_inv) : 0.0;
+                sum += part.sum > 0.0 ? part.sum * weight_of(table, part.max, inv, max) : 0.0;
             };
 #pragma unroll
             for (int k = 0; k < kPartsHeld; ++k) {
@@ -525,7 +527,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_decide_kernel(const Ver
                     ok = id[x] == row[x].at;
                 } else {
                     ok = static_cast<double>(u[x]) * static_cast<double>(q[x]) <
-                         weight_of(table, logit[x], inv, max_inv) / row[x].sum;
+                         weight_of(table, logit[x], inv, max) / row[x].sum;
                 }
             }
             const uint32_t i = i0 + 4u * x;
@@ -568,7 +570,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_decide_kernel(const Ver
         return;
     }
     // the draw from p, without the refused draft
-    const double max_inv = static_cast<double>(row.max) * inv;
+    const double max = row.max;
     const Part *parts = p.parts + (static_cast<uint64_t>(s) * (p.max_draft + 1) + accepted) * p.n_parts;
     const uint8_t *logits = p.logits + r * p.logits_nb;
     uint32_t without = refused ? static_cast<uint32_t>(p.tokens[r + 1]) : kNowhere;
@@ -579,7 +581,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_decide_kernel(const Ver
         load_part<T>(logits, v0, min(p.n_vocab, v0 + kPartIds), x);
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i) {
-            const double y = weight_of(table, x[i], inv, max_inv);
+            const double y = weight_of(table, x[i], inv, max);
             w[i] = v0 + threadIdx.x * 8u + i == without ? 0.0 : y;
         }
     };
@@ -587,7 +589,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_decide_kernel(const Ver
     double cut_sum = 0.0;
     auto part_weight = [&](uint32_t i) {
         const Part part = parts[i];
-        return i == cut ? cut_sum : part.sum > 0.0 ? part.sum * weight_of(table, part.max, inv, max_inv) : 0.0;
+        return i == cut ? cut_sum : part.sum > 0.0 ? part.sum * weight_of(table, part.max, inv, max) : 0.0;
     };
     if (without != kNowhere) {
         cut = without / kPartIds;
@@ -614,8 +616,8 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_decide_kernel(const Ver
 }
 
 __device__ inline double rest_of(const ExpTable &table, double scale, float logit, float q, double inv,
-                                 double max_inv) {
-    const double e = weight_of(table, logit, inv, max_inv) * scale - static_cast<double>(q);
+                                 double max) {
+    const double e = weight_of(table, logit, inv, max) * scale - static_cast<double>(q);
     return e > 0.0 ? e : 0.0;
 }
 
@@ -637,12 +639,12 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_rest_kernel(const Verif
     fill_table(table);
     bool greedy;
     const double inv = inv_temperature(p, s, greedy);
-    const double max_inv = static_cast<double>(c.max) * inv;
+    const double max = c.max;
     double sum = 0.0;
 #pragma unroll
     for (uint32_t e = 0; e < 8; ++e) {
         // behind the part's end logit and q are -inf
-        sum += v0 + threadIdx.x * 8u + e < v1 ? rest_of(table, c.scale, x[e], q[e], inv, max_inv) : 0.0;
+        sum += v0 + threadIdx.x * 8u + e < v1 ? rest_of(table, c.scale, x[e], q[e], inv, max) : 0.0;
     }
     sum = block_sum(sum, lds_d);
     if (threadIdx.x == 0) {
@@ -667,7 +669,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
     fill_table(table);
     const double *rest = p.rest + static_cast<uint64_t>(s) * p.n_parts;
     const Part *parts = p.parts + (static_cast<uint64_t>(s) * (p.max_draft + 1) + c.row) * p.n_parts;
-    const double max_inv = static_cast<double>(c.max) * inv;
+    const double max = c.max;
     double target = u_sample, before;
     uint32_t part = pick_part(p.n_parts, target, [&](uint32_t i) { return rest[i]; }, lds, before);
     const bool left = part != kNowhere;  // else p itself
@@ -678,7 +680,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
             p.n_parts, target,
             [&](uint32_t i) {
                 const Part x = parts[i];
-                return x.sum > 0.0 ? x.sum * weight_of(table, x.max, inv, max_inv) : 0.0;
+                return x.sum > 0.0 ? x.sum * weight_of(table, x.max, inv, max) : 0.0;
             },
             lds, before);
     }
@@ -692,8 +694,8 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(const Verif
     load_part<Q>(p.probs + r * p.probs_nb, v0, v1, q);
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
-        const double y = left ? rest_of(table, c.scale, x[i], q[i], inv, max_inv)
-                              : weight_of(table, x[i], inv, max_inv);
+        const double y = left ? rest_of(table, c.scale, x[i], q[i], inv, max)
+                              : weight_of(table, x[i], inv, max);
         w[i] = v0 + threadIdx.x * 8u + i < v1 ? y : 0.0;  // behind the end logit and q are -inf
     }
     pick_id(v0, before, target, w, lds, p.tokens_out + static_cast<uint64_t>(s) * (p.max_draft + 1) + c.row);
