@@ -799,8 +799,7 @@ KVMEM_HIP_API int kvmem_hip_conv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_conv_a
  * few tokens a request go token by token, longer ones by chunks of tokens on
  * the matrix cores: there every factor is scaled by a power of two (states,
  * values and their like column by column) and taken as two f16 parts of 22 bits
- * together, cut 2^-39 below the largest; what reaches only a bf16 out is one part
- * of 11 bits.
+ * together, cut 2^-39 below the largest, whatever the type of out.
  * A value that is not finite reaches no earlier token, and where only a v is not
  * finite no other dim; what it reaches is not finite either (NaN, or the value).
  * head_dim_k 64, 128 or 256, head_dim_v a multiple of 32 up to 512; at most

@@ -199,11 +199,10 @@ static ChunkPlan plan_chunks(const kvmem_hip_linear_args *a, uint32_t max_q) {
     }
     pl.chunked = true;
     const uint32_t parts = a->type == KVMEM_TYPE_F32 ? 2 : 1;
-    pl.p_parts = !a->out ? 1 : a->out_type == KVMEM_TYPE_BF16 ? 1 : 2;
     pl.chunks = (max_q + kChunk - 1) / kChunk;
     pl.entries = a->n_tokens / kChunk + a->n_seq + 1;
     pl.key_bytes = static_cast<uint64_t>(parts) * 12 * (a->head_dim_k / 32) * kFragBytes;
-    pl.head_bytes = kHeadBytes + ((a->beta ? 2 : 0) + pl.p_parts) * kLowerFrags * kFragBytes;
+    pl.head_bytes = kHeadBytes + ((a->beta ? 2 : 0) + (a->out ? 2 : 0)) * kLowerFrags * kFragBytes;
     pl.bytes = pl.entries * (pl.key_bytes * a->n_head_k + pl.head_bytes * a->n_head);
     // Without the delta rule states add up: what a segment of chunks adds is made before
     // what lies behind it is known, in a first pass, and a second one walks the segments
@@ -240,7 +239,6 @@ static void launch_linear_chunks(hipStream_t stream, int type, uint32_t dim_k, c
     p.dim_k = dim_k;
     p.delta = a.beta != nullptr;
     p.outs = a.out != nullptr;
-    p.p_parts = static_cast<uint32_t>(pl.p_parts);
     p.segs = pl.segs;
     p.seg_chunks = pl.seg_chunks;
     p.seg_states = reinterpret_cast<float *>(workspace + pl.seg_states);

@@ -32,7 +32,6 @@ constexpr uint32_t kXcds = 8;
 
 struct ChunkPlan {
     bool chunked = false;
-    int p_parts = 0;        // f16 parts of the scores (0: no out)
     uint32_t entries = 0;
     uint32_t chunks = 0;    // most of one request
     uint64_t key_bytes = 0, head_bytes = 0;  // of an entry, per key head and per head
@@ -42,18 +41,18 @@ struct ChunkPlan {
 };
 
 constexpr uint32_t kFragBytes = 1024;  // a 16 x 32 operand of f16: 16 bytes a lane
-constexpr uint32_t kLowerFrags = 6;    // of a 64 x 64 lower triangle: (0,0) (1,0) (2,0) (2,1) (3,0) (3,1)
+constexpr uint32_t kLowerFrags = 5;    // of a 64 x 64 lower triangle (lower_frag)
 constexpr uint32_t kHeadBytes = 1024;  // a head's entry begins with ChunkHead
 
 struct ChunkParams {
     LinearParams a;
     uint8_t *keys;   // [entries][key heads]: fragments of K, Q, K^T
-    uint8_t *heads;  // [entries][heads]: ChunkHead, fragments of T, P
+    uint8_t *heads;  // [entries][heads]: ChunkHead, fragments of T (delta), P (outs)
     uint64_t key_bytes, head_bytes;
     uint32_t chunks;
     int type;
     uint32_t dim_k;
-    uint32_t delta, outs, p_parts;
+    uint32_t delta, outs;
     uint32_t segs, seg_chunks, second_pass;
     float *seg_states;  // [requests][segs][heads][Dk][Dv]
     float *seg_decays;  // [requests][segs][heads]

@@ -23,11 +23,11 @@
 // and their like each column) is scaled by a power of two that puts its largest
 // element into [2^14, 2^15), then split into a high and a low f16 part: together 22
 // bits, and what lies below 2^-39 of the largest is cut.  16-bit keys and queries
-// are one part, exactly.  Products of two split factors leave out low x low.  What
-// reaches only a 16-bit result takes fewer parts: for a bf16 out (half a step
-// 2^-9) the scores, D and S enter the output's products by their high part (half a
-// step 2^-12).  Sums of log_decay are fp64: e^(G_i - G_j) of far apart sums
-// keeps its digits, and a decay of zero (-inf, taken as -10^5) stays zero.
+// are one part, exactly.  Products of two split factors leave out low x low.  A 16-bit
+// out is rounded from the same sums as an fp32 one: with single parts (half a step
+// 2^-12) small outputs of large terms would be off by more than their own rounding.
+// Sums of log_decay are fp64: e^(G_i - G_j) of far apart sums keeps its digits, and a
+// decay of zero (-inf, taken as -10^5) stays zero.
 //
 // A chunk with a number that is not finite among its rows, gates or factors goes
 // token by token instead (walk_tokens), as products of masked rows would spread it
@@ -184,7 +184,35 @@ __device__ inline void tri_row(const float *tri, uint32_t m, uint32_t k, float x
     }
 }
 
-__device__ inline uint32_t lower_frag(uint32_t m, uint32_t k) { return m < 2 ? m : 2u * m - 2u + k; }
+// The 16 x 32 operands of a 64 x 64 lower triangle, (row tile m, columns [32 k, 32 k + 32)):
+// (1,0) (2,0) (3,0) (3,1) whole; (0,0) and (2,1), whose second 16 columns are zeros, share
+// the last by their first halves.
+__device__ inline constexpr bool lower_half(uint32_t m, uint32_t k) { return m == 2u * k; }
+__device__ inline constexpr uint32_t lower_frag(uint32_t m, uint32_t k) { return m - 1u + k; }
+constexpr uint32_t kHalvesFrag = 4;
+
+__device__ inline void put_lower(uint8_t *base, uint32_t m, uint32_t k, half8_t x) {
+    if (lower_half(m, k)) {
+        *reinterpret_cast<half4_t *>(base + kHalvesFrag * kFragBytes + (threadIdx.x & 63u) * 16u + k * 8u) =
+            half4_t{x[0], x[1], x[2], x[3]};
+    } else {
+        put_frag(base, lower_frag(m, k), x);
+    }
+}
+
+// c += tile (m, k) of a lower triangle times x, or (FLIP) x times its transpose.
+template <bool FLIP>
+__device__ inline f32x4_t mul_lower(const half8_t *tri, uint32_t m, uint32_t k, half8_t x, f32x4_t c) {
+    if (lower_half(m, k)) {
+        const half8_t f = tri[kHalvesFrag];
+        const half4_t a = k == 0 ? half4_t{f[0], f[1], f[2], f[3]} : half4_t{f[4], f[5], f[6], f[7]};
+        const half4_t b = {x[0], x[1], x[2], x[3]};
+        return FLIP ? __builtin_amdgcn_mfma_f32_16x16x16f16(b, a, c, 0, 0, 0)
+                    : __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+    }
+    const half8_t a = tri[lower_frag(m, k)];
+    return FLIP ? KVMEM_MFMA16(x, a, c) : KVMEM_MFMA16(a, x, c);
+}
 
 // c += a b over 16 indices, fp32: a row of `a` is read from LDS rows, b's rows
 // 4g..4g+3 of column lane % 16 are in registers (as an accumulator holds them).
@@ -489,7 +517,6 @@ __global__ __launch_bounds__(kPrepThreads, DK <= 128 ? 3 : 1) void linear_prepar
             if (k > w / 2) {
                 continue;
             }
-            const uint32_t f = lower_frag(w, k);
             uint8_t *at = head + kHeadBytes;
             half8_t hi, lo;
             if constexpr (DELTA) {
@@ -499,19 +526,19 @@ __global__ __launch_bounds__(kPrepThreads, DK <= 128 ? 3 : 1) void linear_prepar
                     hi[i] = static_cast<_Float16>(y);
                     lo[i] = static_cast<_Float16>(y - static_cast<float>(hi[i]));
                 }
-                put_frag(at, f, hi);
-                put_frag(at, kLowerFrags + f, lo);
+                put_lower(at, w, k, hi);
+                put_lower(at + kLowerFrags * kFragBytes, w, k, lo);
                 at += 2u * kLowerFrags * kFragBytes;
             }
+            if (p.outs) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float y = xp[k][i] * pow2(-exp_p);
-                hi[i] = static_cast<_Float16>(y);
-                lo[i] = static_cast<_Float16>(y - static_cast<float>(hi[i]));
-            }
-            put_frag(at, f, hi);
-            if (p.p_parts == 2) {
-                put_frag(at, kLowerFrags + f, lo);
+                for (int i = 0; i < 8; ++i) {
+                    const float y = xp[k][i] * pow2(-exp_p);
+                    hi[i] = static_cast<_Float16>(y);
+                    lo[i] = static_cast<_Float16>(y - static_cast<float>(hi[i]));
+                }
+                put_lower(at, w, k, hi);
+                put_lower(at + kLowerFrags * kFragBytes, w, k, lo);
             }
         }
         if (w == 0) {
@@ -580,7 +607,7 @@ template <int TILES> __device__ inline float lane_max(const f32x4_t (&x)[TILES])
 }
 
 // A column's numbers (tiles of 16 rows, 4 of each in every lane of the column) as
-// two f16 parts of x * 2^-e, or their high parts alone.  The mixed-precision FMAs round
+// two f16 parts of x * 2^-e.  The mixed-precision FMAs round
 // x f and x f - high to f16 without a step in fp32: two instructions a number.  No
 // number here is a matrix instruction's own result (its readers would have to wait
 // inside the block); an instruction stands between a half word's write and its use.
@@ -612,26 +639,6 @@ __device__ inline void split(const f32x4_t (&x)[TILES], int e, half8_t (&hi)[TIL
         }
         hi[t / 2] = __builtin_bit_cast(half8_t, words4_t{h[0], h[1], h[2], h[3]});
         lo[t / 2] = __builtin_bit_cast(half8_t, words4_t{l[0], l[1], l[2], l[3]});
-    }
-}
-
-template <int TILES>
-__device__ inline void split_high(const f32x4_t (&x)[TILES], int e, half8_t (&hi)[TILES / 2]) {
-    const float f = pow2(-e);
-#pragma unroll
-    for (int t = 0; t < TILES; t += 2) {
-        uint32_t h[4];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            asm("v_fma_mixlo_f16 %0, %2, %6, 0\n\t"
-                "v_fma_mixlo_f16 %1, %4, %6, 0\n\t"
-                "v_fma_mixhi_f16 %0, %3, %6, 0\n\t"
-                "v_fma_mixhi_f16 %1, %5, %6, 0\n\t"
-                "s_nop 0"
-                : "=&v"(h[2 * u]), "=&v"(h[2 * u + 1])
-                : "v"(x[t + u][0]), "v"(x[t + u][1]), "v"(x[t + u][2]), "v"(x[t + u][3]), "v"(f));
-        }
-        hi[t / 2] = __builtin_bit_cast(half8_t, words4_t{h[0], h[1], h[2], h[3]});
     }
 }
 
@@ -709,6 +716,24 @@ __device__ inline __attribute__((always_inline)) void walk_tokens(const ChunkPar
     }
 }
 
+// Four numbers of rows `row`, row + 16, row + 32 and row + 48, of which `rows` exist.
+template <typename T>
+__device__ inline void store_rows(uint8_t *to, uint64_t step, uint32_t row, uint32_t rows, const float (&y)[4][4]) {
+    if (rows == kChunk) {
+#pragma unroll
+        for (uint32_t m = 0; m < 4; ++m) {
+            store_row<T, 4>(to + m * step, y[m]);
+        }
+        return;
+    }
+#pragma unroll
+    for (uint32_t m = 0; m < 4; ++m) {
+        if (16u * m + row < rows) {
+            store_row<T, 4>(to + m * step, y[m]);
+        }
+    }
+}
+
 typedef __attribute__((address_space(3))) void lds_void_t;
 
 template <int N>
@@ -721,10 +746,10 @@ __device__ inline void get_frags(const uint8_t *base, uint32_t frag, half8_t (&x
 
 // A chunk in LDS: its keys' operands [K Q K^T][part], then its head's (ChunkHead, T, P),
 // as they lie in its entries, then its values.
-template <typename T, int DK, bool DELTA, bool FINE, int WAVES> struct ChunkSpace {
+template <typename T, int DK, bool DELTA, bool OUT, int WAVES> struct ChunkSpace {
     static constexpr uint32_t parts = sizeof(T) == 4 ? 2 : 1;
     static constexpr uint32_t key_frags = 12 * (DK / 32) * parts;
-    static constexpr uint32_t head_frags = 1 + (DELTA ? 2 * kLowerFrags : 0) + (FINE ? 2 : 1) * kLowerFrags;
+    static constexpr uint32_t head_frags = 1 + (DELTA ? 2 * kLowerFrags : 0) + (OUT ? 2 * kLowerFrags : 0);
     static constexpr uint32_t row_bytes = WAVES * 16 * sizeof(T);  // of the values
     static constexpr uint32_t rest = head_frags * kFragBytes + kChunk * row_bytes;
     static constexpr uint32_t most = 160 * 1024;
@@ -814,9 +839,9 @@ __device__ inline uint32_t request_by_length(const LinearParams &a, uint32_t ran
 // each product waits for the one before, 6400 cycles = 2.8 us in all.  8192 tokens take
 // 128 of these, one behind the other: 362-373 us on 96 compute units (a column of the
 // state needs the whole chunk before it), 48 heads of 128 x 128.
-template <typename T, int DK, bool DELTA, bool FINE, int WAVES>
+template <typename T, int DK, bool DELTA, bool OUT, int WAVES>
 __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const ChunkParams p) {
-    typedef ChunkSpace<T, DK, DELTA, FINE, WAVES> Space;
+    typedef ChunkSpace<T, DK, DELTA, OUT, WAVES> Space;
     constexpr int PARTS = Space::parts, KS = DK / 32, TILES = DK / 16;
     __shared__ __align__(16) uint8_t lds[Space::places * Space::bytes];
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
@@ -844,7 +869,7 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
             seg = blockIdx.z;
             last_seg = rq.count ? (rq.count - 1u) / of_seg : 0u;
             if (seg > last_seg ||
-                (p.second_pass ? seg == 0 || (!p.outs && seg < last_seg) : seg == last_seg && seg > 0)) {
+                (p.second_pass ? seg == 0 || (!OUT && seg < last_seg) : seg == last_seg && seg > 0)) {
                 return;
             }
             c0 = seg * p.seg_chunks;
@@ -938,9 +963,9 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
     }
     const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
     const uint64_t out_row = static_cast<uint64_t>(p.a.n_head) * p.a.dim_v;
-    const uint32_t esz = FINE && p.a.out_type == KVMEM_TYPE_F32 ? 4u : 2u;
+    const uint32_t esz = p.a.out_type == KVMEM_TYPE_F32 ? 4u : 2u;
     const uint32_t out_at = ((lane & 15u) * static_cast<uint32_t>(out_row) + 4u * g) * esz;
-    const bool with_out = p.outs && (seg == 0 || p.second_pass);
+    const bool with_out = OUT && (seg == 0 || p.second_pass);
     float decayed = 1.0f;  // over the segment
     for (uint32_t c = c0; c * kChunk < limit; ++c) {
         const uint32_t n = min(kChunk, rq.count - c * kChunk);
@@ -968,7 +993,8 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
                 to[i] = get_frag(kp, frag_index(matrix, matrix == 8 * KS ? 4 * k + i : (i & 3u) * KS + k + (i >> 2), 0));
             }
         };
-        read8(kq[0], DELTA ? 0 : 4 * KS, 0);
+        constexpr uint32_t behind_k = OUT ? 4 * KS : 8 * KS;  // what the first product's operands are followed by
+        read8(kq[0], DELTA ? 0 : behind_k, 0);
         const uint8_t *vp = here + values_at + 4u * g * Space::row_bytes + (16u * w + (lane & 15u)) * sizeof(T);
         f32x4_t v[4];
 #pragma unroll
@@ -987,14 +1013,14 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
             es[r] = __shfl(exp_s, static_cast<int>(4u * g) + r, 64);
         }
         f32x4_t d[4] = {zero, zero, zero, zero}, o[4] = {zero, zero, zero, zero};
-        half8_t tf[DELTA ? 2 * kLowerFrags : 1], pf[(FINE ? 2 : 1) * kLowerFrags];
+        half8_t tf[DELTA ? 2 * kLowerFrags : 1], pf[OUT ? 2 * kLowerFrags : 1];
         if constexpr (DELTA) {
 #pragma unroll
             for (uint32_t k = 0; k < KS; k += 2) {
                 if (k + 2 < KS) {
                     read8(kq[(k / 2 + 1) & 1], 0, k + 2);
                 } else {
-                    read8(kq[(k / 2 + 1) & 1], 4 * KS, 0);
+                    read8(kq[(k / 2 + 1) & 1], behind_k, 0);
                 }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -1017,18 +1043,18 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
         f32x4_t first[4];
         float out_first[4];
         const int exp_k = ch->exp_k, exp_q = ch->exp_q, exp_t = ch->exp_t, exp_p = ch->exp_p;
+        if constexpr (OUT) {
 #pragma unroll
-        for (uint32_t k = 0; k < KS; k += 2) {  // transposed: columns of the state are rows of the accumulator
-            constexpr uint32_t KT = 8 * KS;
-            if (k + 2 < KS) {
-                read8(kq[(Q0 + k / 2 + 1) & 1], 4 * KS, k + 2);
-            } else {
-                read8(kq[(Q0 + k / 2 + 1) & 1], KT, 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            {
+            for (uint32_t k = 0; k < KS; k += 2) {  // transposed: columns of the state are rows of the accumulator
+                constexpr uint32_t KT = 8 * KS;
+                if (k + 2 < KS) {
+                    read8(kq[(Q0 + k / 2 + 1) & 1], 4 * KS, k + 2);
+                } else {
+                    read8(kq[(Q0 + k / 2 + 1) & 1], KT, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (uint32_t x = 0; x < (!FINE ? 2 : PARTS == 2 ? 6 : 4); ++x) {
+                for (uint32_t x = 0; x < (PARTS == 2 ? 6 : 4); ++x) {
 #pragma unroll
                     for (uint32_t m = 0; m < 4; ++m) {
                         half8_t a;
@@ -1040,10 +1066,10 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
                         o[m] = KVMEM_MFMA16(x == 2 || x == 3 ? lo[k + (x & 1u)] : hi[k + (x & 1u)], a, o[m]);
                     }
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
         }
-        constexpr int T0 = (Q0 + KS / 2) & 1;  // where K^T's first group is
+        constexpr int T0 = OUT ? (Q0 + KS / 2) & 1 : Q0;  // where K^T's first group is
         if constexpr (DELTA) {
 #pragma unroll
             for (uint32_t m = 0; m < 4; ++m) {
@@ -1089,13 +1115,14 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
                 for (uint32_t x = 0; x < 3; ++x) {
 #pragma unroll
                     for (uint32_t m = 2 * k; m < 4; ++m) {
-                        d[m] = KVMEM_MFMA16(tf[(x == 2 ? kLowerFrags : 0u) + lower_frag(m, k)],
-                                            x == 1 ? dl[k] : dh[k], d[m]);
+                        d[m] = mul_lower<false>(tf + (x == 2 ? kLowerFrags : 0u), m, k, x == 1 ? dl[k] : dh[k], d[m]);
                     }
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-            get_frags(frag_p, 0, pf);
+            if constexpr (OUT) {
+                get_frags(frag_p, 0, pf);
+            }
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
 #pragma unroll
@@ -1104,7 +1131,9 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
                 }
             }
         } else {
-            get_frags(frag_p, 0, pf);
+            if constexpr (OUT) {
+                get_frags(frag_p, 0, pf);
+            }
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 d[m] = v[m];
@@ -1117,21 +1146,16 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
             out_first[m] = p.a.scale * ch->from_first[16u * m + (lane & 15u)];
         }
         const int exp_d = column_exp<4>(d);
-        {
+        if constexpr (OUT) {
             f32x4_t pd[4] = {zero, zero, zero, zero};
-            if constexpr (FINE) {
-                split<4>(d, exp_d, dh, dl);
-            } else {
-                split_high<4>(d, exp_d, dh);
-            }
+            split<4>(d, exp_d, dh, dl);
 #pragma unroll
             for (uint32_t k = 0; k < 2; ++k) {
 #pragma unroll
-                for (uint32_t x = 0; x < (FINE ? 3 : 1); ++x) {
+                for (uint32_t x = 0; x < 3; ++x) {
 #pragma unroll
                     for (uint32_t m = 2 * k; m < 4; ++m) {
-                        pd[m] = KVMEM_MFMA16(x == 1 ? dl[k] : dh[k], pf[(x == 2 ? kLowerFrags : 0u) + lower_frag(m, k)],
-                                             pd[m]);
+                        pd[m] = mul_lower<true>(pf + (x == 2 ? kLowerFrags : 0u), m, k, x == 1 ? dl[k] : dh[k], pd[m]);
                     }
                 }
             }
@@ -1142,26 +1166,24 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
                 es[r] += exp_q;
                 ed[r] = __shfl(exp_d, static_cast<int>(4u * g) + r, 64) + exp_p;
             }
+            float y[4][4];
 #pragma unroll
             for (uint32_t m = 0; m < 4; ++m) {
-                float y[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     // both terms as they are: the scale of a column of zeros or next to nothing
                     // would carry P D beyond fp32
-                    y[r] = __builtin_fmaf(out_first[m], __builtin_amdgcn_ldexpf(o[m][r], es[r]),
-                                          __builtin_amdgcn_ldexpf(pd[m][r], ed[r]));
+                    y[m][r] = __builtin_fmaf(out_first[m], __builtin_amdgcn_ldexpf(o[m][r], es[r]),
+                                             __builtin_amdgcn_ldexpf(pd[m][r], ed[r]));
                 }
-                uint8_t *to = out + m * 16u * out_row * esz;
-                if (16u * m + (lane & 15u) < rows) {
-                    if constexpr (!FINE) {
-                        store_row<__bf16, 4>(to + out_at, y);
-                    } else if (p.a.out_type == KVMEM_TYPE_F32) {
-                        store_row<float, 4>(to + out_at, y);
-                    } else {
-                        store_row<_Float16, 4>(to + out_at, y);
-                    }
-                }
+            }
+            // one choice of the type for all four rows
+            if (p.a.out_type == KVMEM_TYPE_F32) {
+                store_rows<float>(out + out_at, 16u * out_row * esz, lane & 15u, rows, y);
+            } else if (p.a.out_type == KVMEM_TYPE_F16) {
+                store_rows<_Float16>(out + out_at, 16u * out_row * esz, lane & 15u, rows, y);
+            } else {
+                store_rows<__bf16>(out + out_at, 16u * out_row * esz, lane & 15u, rows, y);
             }
         }
 #pragma unroll
@@ -1265,19 +1287,19 @@ static void prepare(hipStream_t stream, const ChunkParams &p) {
 // tokens, 48 heads of 128 x 128: 446 us, 443 by 32), and wide workgroups read the
 // operands half as often (eight of up to 4096 tokens, 32 heads, at an earlier step: 397
 // us, 553 by 32).
-template <typename T, int DK, bool DELTA, bool FINE>
+template <typename T, int DK, bool DELTA, bool OUT>
 static void walk_cols(hipStream_t stream, const ChunkParams &p) {
-    constexpr bool wide = ChunkSpace<T, DK, DELTA, FINE, 4>::places == 2;
+    constexpr bool wide = ChunkSpace<T, DK, DELTA, OUT, 4>::places == 2;
     const uint32_t cols = wide && p.a.dim_v % 64 == 0 ? 64u : 32u;
     const uint32_t units = p.a.n_head * (p.a.dim_v / cols);
     const dim3 grid((units + kXcds - 1) / kXcds * kXcds, p.a.n_seq, p.segs);
     if constexpr (wide) {
         if (cols == 64) {
-            linear_walk_kernel<T, DK, DELTA, FINE, 4><<<grid, 512, 0, stream>>>(p);
+            linear_walk_kernel<T, DK, DELTA, OUT, 4><<<grid, 512, 0, stream>>>(p);
             return;
         }
     }
-    linear_walk_kernel<T, DK, DELTA, FINE, 2><<<grid, 256, 0, stream>>>(p);
+    linear_walk_kernel<T, DK, DELTA, OUT, 2><<<grid, 256, 0, stream>>>(p);
 }
 
 template <typename T, int DK>
@@ -1286,12 +1308,11 @@ static void launch_type(hipStream_t stream, const ChunkParams &p) {
     if (hipPeekAtLastError() != hipSuccess) {
         return;  // factors that were not written must not be read
     }
-    const bool fine = p.p_parts == 2;  // the output takes both parts
     if (p.delta) {
-        fine ? walk_cols<T, DK, true, true>(stream, p) : walk_cols<T, DK, true, false>(stream, p);
+        p.outs ? walk_cols<T, DK, true, true>(stream, p) : walk_cols<T, DK, true, false>(stream, p);
         return;
     }
-    fine ? walk_cols<T, DK, false, true>(stream, p) : walk_cols<T, DK, false, false>(stream, p);
+    p.outs ? walk_cols<T, DK, false, true>(stream, p) : walk_cols<T, DK, false, false>(stream, p);
     if (p.segs > 1 && hipPeekAtLastError() == hipSuccess) {
         const uint64_t quads = static_cast<uint64_t>(p.a.n_head) * p.dim_k * p.a.dim_v / 4;
         const dim3 grid(static_cast<uint32_t>((quads + kScanThreads - 1) / kScanThreads), p.a.n_seq);
@@ -1301,7 +1322,7 @@ static void launch_type(hipStream_t stream, const ChunkParams &p) {
         }
         ChunkParams second = p;
         second.second_pass = 1;
-        fine ? walk_cols<T, DK, false, true>(stream, second) : walk_cols<T, DK, false, false>(stream, second);
+        p.outs ? walk_cols<T, DK, false, true>(stream, second) : walk_cols<T, DK, false, false>(stream, second);
     }
 }
 
