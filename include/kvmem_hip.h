@@ -731,8 +731,9 @@ KVMEM_HIP_API int kvmem_hip_attention(kvmem_hip_ctx *ctx, const kvmem_hip_pool *
  * patches/llama-kvmem-current.patch:418-474.)
  *
  * Batches: token i of request s is row q_start[s] + i (q_start NULL: request s
- * has row s).  The first n_use[s] tokens of a request take part (NULL: all);
- * rows of the others, and rows behind the last request, are left as they are.
+ * has row s); requests lie in any order and share no row, and one whose next start
+ * is below its own has no tokens.  The first n_use[s] tokens of a request take part
+ * (NULL: all); rows of the others, and rows of no request, are left as they are.
  * Tokens beyond max_q or n_tokens take no part: both bounds size the launch and
  * device lengths beyond them never reach out of range.  State of request s is
  * entry slots[s] (NULL: s) of `state`; it goes to the same entry of state_out,

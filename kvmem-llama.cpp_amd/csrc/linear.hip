@@ -200,7 +200,7 @@ static ChunkPlan plan_chunks(const kvmem_hip_linear_args *a, uint32_t max_q) {
     pl.chunked = true;
     const uint32_t parts = a->type == KVMEM_TYPE_F32 ? 2 : 1;
     pl.chunks = (max_q + kChunk - 1) / kChunk;
-    pl.entries = a->n_tokens / kChunk + a->n_seq + 1;
+    pl.entries = a->n_tokens / kChunk + a->n_seq;
     pl.key_bytes = static_cast<uint64_t>(parts) * 12 * (a->head_dim_k / 32) * kFragBytes;
     pl.head_bytes = kHeadBytes + ((a->beta ? 2 : 0) + (a->out ? 2 : 0)) * kLowerFrags * kFragBytes;
     pl.bytes = pl.entries * (pl.key_bytes * a->n_head_k + pl.head_bytes * a->n_head);

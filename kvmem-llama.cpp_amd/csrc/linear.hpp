@@ -24,8 +24,10 @@ struct LinearParams {
     float scale;
 };
 
-// Calls by chunks of tokens.  Request s's chunk c keeps its factors in entry
-// q_start[s] / kChunk + s + c: entries of ascending requests never meet.
+// Calls by chunks of tokens.  A whole chunk keeps its factors in the entry of its first
+// row over kChunk, a request's last and shorter one in entry n_tokens / kChunk + s:
+// whole chunks of other requests begin at least kChunk rows away, so requests that share
+// no row share no entry, in whatever order they lie.
 constexpr uint32_t kChunk = 64;
 constexpr uint32_t kPrepThreads = 256;
 constexpr uint32_t kXcds = 8;

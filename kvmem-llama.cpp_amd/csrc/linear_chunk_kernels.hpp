@@ -56,8 +56,8 @@ struct ChunkHead {
 };
 static_assert(sizeof(ChunkHead) <= kHeadBytes, "");
 
-__device__ inline uint64_t entry_of(const Request &rq, uint32_t s, uint32_t c) {
-    return static_cast<uint64_t>(rq.first / kChunk) + s + c;
+__device__ inline uint64_t entry_of(const LinearParams &a, const Request &rq, uint32_t s, uint32_t c) {
+    return (c + 1) * kChunk <= rq.count ? rq.first / kChunk + c : a.batch.n_tokens / kChunk + s;
 }
 
 // The power of two that brings numbers whose largest magnitude has the bits `m`
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(kPrepThreads, DK <= 128 ? 3 : 1) void linear_prepar
     }
     const uint32_t n = min(kChunk, rq.count - c * kChunk);
     const uint64_t row0 = static_cast<uint64_t>(rq.first) + c * kChunk;
-    const uint64_t entry = entry_of(rq, s, c);
+    const uint64_t entry = entry_of(p.a, rq, s, c);
     const uint32_t hk = h0 / p.a.group;
     uint8_t *keys = p.keys + (entry * (p.a.n_head / p.a.group) + hk) * p.key_bytes;
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
@@ -876,10 +876,8 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
             limit = min(rq.count, (seg + 1) * of_seg);
         }
     }
-    const uint64_t entry0 = entry_of(rq, s_id, 0);
     const uint64_t key_step = p.key_bytes * (p.a.n_head / p.a.group), head_step = p.head_bytes * p.a.n_head;
-    const uint8_t *keys = p.keys + entry0 * key_step + hk * p.key_bytes;
-    const uint8_t *heads = p.heads + entry0 * head_step + h * p.head_bytes;
+    const uint8_t *keys = p.keys + hk * p.key_bytes, *heads = p.heads + h * p.head_bytes;  // of entry 0
     constexpr uint32_t head_at = Space::keys ? Space::key_frags * kFragBytes : 0;
     constexpr uint32_t values_at = head_at + Space::head_frags * kFragBytes;
 
@@ -901,10 +899,11 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
             }
         };
         auto request = [&](uint32_t c, uint8_t *to) {
+            const uint64_t entry = entry_of(p.a, rq, s_id, c);
             if constexpr (Space::keys) {
-                frags(keys + c * key_step, to, std::integral_constant<uint32_t, Space::key_frags>{});
+                frags(keys + entry * key_step, to, std::integral_constant<uint32_t, Space::key_frags>{});
             }
-            frags(heads + c * head_step, to + head_at, std::integral_constant<uint32_t, Space::head_frags>{});
+            frags(heads + entry * head_step, to + head_at, std::integral_constant<uint32_t, Space::head_frags>{});
             const uint32_t n = min(kChunk, rq.count - c * kChunk);
 #pragma unroll
             for (uint32_t i = 0; i < (lanes + WAVES - 1) / WAVES; ++i) {
@@ -972,9 +971,9 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
         const uint64_t row0 = static_cast<uint64_t>(rq.first) + c * kChunk;
         const uint32_t rows = with_out ? n : 0u;
         const uint8_t *here = lds + (Space::places == 2 ? (c & 1u) * Space::bytes : 0u);
-        const uint8_t *kp = keys + c * key_step;
-        if constexpr (Space::keys) {
-            kp = here;
+        const uint8_t *kp = here;
+        if constexpr (!Space::keys) {
+            kp = keys + entry_of(p.a, rq, s_id, c) * key_step;
         }
         const uint8_t *head = here + head_at;
         const ChunkHead *ch = reinterpret_cast<const ChunkHead *>(head);
