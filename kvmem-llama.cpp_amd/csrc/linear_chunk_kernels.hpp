@@ -61,8 +61,9 @@ __device__ inline uint64_t entry_of(const LinearParams &a, const Request &rq, ui
 }
 
 // The power of two that brings numbers whose largest magnitude has the bits `m`
-// into [2^14, 2^15): x * 2^-e.  At least -100, so that 2^-e is an fp32 number.
-__device__ inline int scale_exp(uint32_t m) { return max(static_cast<int>(m >> 23) - (127 + 14), -100); }
+// into [2^14, 2^15): x * 2^-e.  At least -127, so that 2^-e is an fp32 number: the
+// smallest normal ones still come to 2, 25 bits above what f16 can hold.
+__device__ inline int scale_exp(uint32_t m) { return max(static_cast<int>(m >> 23) - (127 + 14), -127); }
 __device__ inline float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 __device__ inline uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 constexpr uint32_t kInf = 0x7f800000u;

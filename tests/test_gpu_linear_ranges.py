@@ -74,3 +74,22 @@ def test_segments_from_a_state_of_zeros(ctx, type_, out, size):
             c.state.zero_()
         c.run()
         c.check()
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("type_,out", [("f32", "f32"), ("bf16", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("what", ["states", "values", "keys", "queries"])
+def test_numbers_near_the_smallest(ctx, what, type_, out, delta):
+    """A factor of a few steps above fp32's smallest normal number keeps its digits, whatever it meets."""
+    tiny, huge = 2.0 ** -118, 2.0 ** 100
+    c = Linear(ctx, Requests([150]), 1, 2, 64, 64, type_, out, delta, seed=6, rate=0.1)
+    if what == "states":
+        c.state.mul_(tiny), c.v.mul_(tiny)
+    elif what == "values":
+        c.v.mul_(tiny), c.state.zero_()
+    else:
+        (c.k if what == "keys" else c.q).mul_(tiny), c.v.mul_(huge), c.state.mul_(huge)
+    if what in ("states", "values"):
+        c.q.mul_(huge)
+    c.run()
+    c.check()
