@@ -1214,13 +1214,23 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (uint32_t k = 0; k < 2; ++k) {
+                half8_t second[4];
+                if constexpr (PARTS == 2) {
+                    // together: one by one each would wait for memory where keys are not in LDS
+                    // (F32, 256 x 256, without the delta rule: 2048 tokens of 8 heads 242 us, 170 so)
+#pragma unroll
+                    for (uint32_t t = 0; t < 4; ++t) {
+                        second[t] = get_frag(kp, frag_index(8 * KS, 2 * (t0 + t) + k, 1));
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
 #pragma unroll
                 for (uint32_t x = 0; x < (PARTS == 2 ? 3 : 2); ++x) {
 #pragma unroll
                     for (uint32_t t = 0; t < 4; ++t) {
                         half8_t a;
                         if (x == 2) {
-                            a = get_frag(kp, frag_index(8 * KS, 2 * (t0 + t) + k, 1));
+                            a = second[t];
                         } else {
                             a = kq[(T0 + t0 / 4) & 1][2 * t + k];
                         }

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from recurrent_helpers import Linear, Requests, close, half_step
+from recurrent_helpers import FILL, Linear, Requests, close, half_step
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +61,19 @@ def test_values_and_scores_that_cancel(ctx, dims, which):
         c.k.mul_(up)
     c.run()
     check(c)
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("type_", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("heads", [(1, 2, 64, 64), (2, 2, 128, 128), (1, 3, 128, 96), (1, 1, 256, 128), (1, 2, 64, 32)])
+def test_the_state_alone(ctx, heads, type_, delta):
+    """Without an out (and without queries) the state is the one that the call with an out stores, bit for bit."""
+    print(f"[linear] {heads} {type_} delta={delta}", flush=True)
+    c = Linear(ctx, Requests([150, 24, 64], use=[130, 24, 9], tail=1), *heads, type_, "f32", delta, seed=sum(heads))
+    c.run()
+    c.check()
+    want = c.state_out.clone()
+    c.out.fill_(FILL), c.state_out.fill_(FILL)
+    c.run(out=None, q=None)
+    c.check(out=False)
+    assert torch.equal(c.state_out, want)
