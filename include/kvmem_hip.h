@@ -752,9 +752,10 @@ KVMEM_HIP_API int kvmem_hip_attention(kvmem_hip_ctx *ctx, const kvmem_hip_pool *
  * Sums are fp32 whatever the rows' type (a run whose squares leave fp32's range
  * is summed in fp64; a run of zeros stays zero), each output is
  * rounded once (nearest even), and states are the rows' own values.
- * width 2 to 8; norm_dim 32, 64, 128, 256 or 512.  x is a strided view, element
- * (c, t) at c*size + t*x_nb bytes; rows, states and outputs that are 16-byte
- * aligned with n_channels a multiple of 8 are moved 16 bytes at a time. */
+ * width 2 to 8; norm_dim 32, 64, 128, 256 or 512; at most 2^24 channels, 65535
+ * requests and 2^26 tokens, and no more workgroups than one launch holds.  x is a
+ * strided view, element (c, t) at c*size + t*x_nb bytes; rows, states and outputs that
+ * are 16-byte aligned with n_channels a multiple of 8 are moved 16 bytes at a time. */
 typedef struct kvmem_hip_conv_args kvmem_hip_conv_args;
 struct kvmem_hip_conv_args {
     const void *x;
@@ -800,11 +801,14 @@ KVMEM_HIP_API int kvmem_hip_conv_rows(kvmem_hip_ctx *ctx, const kvmem_hip_conv_a
  * few tokens a request go token by token, longer ones by chunks of tokens on
  * the matrix cores: there every factor is scaled by a power of two (states,
  * values and their like column by column) and taken as two f16 parts of 22 bits
- * together, cut 2^-39 below the largest, whatever the type of out.
+ * together, cut 2^-39 below the largest (2^-25 where that is near fp32's smallest),
+ * whatever the type of out.
  * A value that is not finite reaches no earlier token, and where only a v is not
  * finite no other dim; what it reaches is not finite either (NaN, or the value).
- * head_dim_k 64, 128 or 256, head_dim_v a multiple of 32 up to 512; at most
- * 65535 requests and 2^26 tokens, and no more workgroups than one launch holds
+ * By chunks a d that leaves fp32's range takes its dim's other tokens of the same 64
+ * with it.
+ * head_dim_k 64, 128 or 256, head_dim_v a multiple of 32 up to 512; at most 4096
+ * heads, 65535 requests and 2^26 tokens, and no more workgroups than one launch holds
  * (KVMEM_HIP_ERR_INVALID otherwise).  Calls by chunks keep their chunks' factors
  * in a workspace: the caller's (kvmem_hip_linear_attention_workspace bytes,
  * 16-byte aligned, contents free) or, where it is NULL, one the context keeps

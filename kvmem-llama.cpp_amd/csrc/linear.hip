@@ -176,13 +176,16 @@ bool load_linear_kernels() {
 // token as for 64, and the chunks' kernels take longer to begin; token by token, a wave
 // alone on its SIMD needs 1.2 us a token, and many share the FMAs.  Measured, us by
 // chunks / by tokens, 48 heads of 128 x 128 (192 waves of states a request):
-//   bf16, 1 request    16 tokens 20.2 /  22.2    12 tokens  20.1 /  17.5
-//   bf16, 8 requests   24 tokens 40.4 /  37.7    32 tokens  40.8 /  47.1
-//   bf16, 64 requests  48 tokens 238  /  233     64 tokens  241  /  303
-//   F32, 1 request     16 tokens 23.5 /  22.1    24 tokens  23.9 /  31.5
-//   F32, 8 requests    32 tokens 61.8 /  47.3    48 tokens  62.5 /  67.2
-//   F32, 64 requests  128 tokens 687  /  599; a chunk of 64 more costs 219 / 284
-// 16 heads of 256 x 256 (64 requests: 56 tokens) and 8 of 64 x 64 cross near there.
+//   bf16, 1 request    16 tokens 17.6 /  20.9    12 tokens  17.6 /  16.6
+//   bf16, 8 requests   24 tokens 40.3 /  35.9    32 tokens  41.0 /  44.7
+//   bf16, 64 requests  56 tokens 296  /  283     64 tokens  298  /  318
+//   F32, 1 request     16 tokens 20.7 /  20.6    24 tokens  21.1 /  29.5
+//   F32, 8 requests    32 tokens 62.5 /  46.3    48 tokens  62.9 /  63.4
+//   F32, 64 requests  128 tokens 722  /  633    192 tokens  876  /  927
+// Heads of 64 x 64 cross near there (F16, 8 heads without the delta rule, 64 requests: 32
+// tokens 25.2 / 26.7; F32, 64 heads, 64 requests: 192 tokens 482 / 483).  16 heads of 256 x
+// 256 do for 8 requests (32 tokens 53.9 / 64.3), for 64 requests only from some 90 tokens
+// on (64 tokens 435 / 390, 80 tokens 497 / 474).
 static uint32_t chunk_from(const kvmem_hip_linear_args *a) {
     const uint64_t waves = static_cast<uint64_t>(a->n_seq) * a->n_head * (a->head_dim_v / kStepCols);
     const bool f32 = a->type == KVMEM_TYPE_F32;
@@ -208,10 +211,11 @@ static ChunkPlan plan_chunks(const kvmem_hip_linear_args *a, uint32_t max_q) {
     // what lies behind it is known, in a first pass, and a second one walks the segments
     // again.  Worth it where the CUs are a quarter full or less and segments hold enough
     // chunks to pay for their states' traffic.  One piece / segments, us: F16, heads of
-    // 64 x 64, 8 heads, 1024 tokens 42.9 / 25.1, 8192 tokens 265 / 48, eight requests of
-    // up to 4096 tokens 152 / 97; bf16, 32 heads of 128 x 128, 8192 tokens 326 / 217; F32,
-    // 8 heads of 256 x 256, 2048 tokens 376 / 210; bf16, 16 heads of 256 x 256, which the
-    // conditions leave whole, 1024 tokens 83.5 / 94.6 and 4096 tokens 290 / 307.
+    // 64 x 64, 8 heads, 1024 tokens 41.5 / 24.2, 8192 tokens 251 / 47, eight requests of
+    // up to 4096 tokens 145 / 96; bf16, 32 heads of 128 x 128, 8192 tokens 375 / 240; F32,
+    // 8 heads of 256 x 256, 2048 tokens 292 / 170; what the conditions leave whole: bf16, 16
+    // heads of 256 x 256, 1024 tokens 94.6 / 100 and 4096 tokens 333 / 340, 32 heads of
+    // 128 x 128, two requests of up to 2048 tokens 111 / 121.
     const bool narrow = a->head_dim_v % 64 || a->head_dim_k * float_type_size(a->type) > 256;  // 32 columns a workgroup
     const uint64_t groups = static_cast<uint64_t>(a->n_seq) * a->n_head * (a->head_dim_v / (narrow ? 32 : 64));
     const uint32_t segs = static_cast<uint32_t>(std::min<uint64_t>(256 / groups, pl.chunks / (a->head_dim_k / 32)));

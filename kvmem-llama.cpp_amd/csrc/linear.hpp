@@ -1,5 +1,5 @@
 // Linear attention's launches, shared by the token-by-token kernel and its entry
-// points (linear.hip) and the kernels that go by chunks (linear_chunk.hip).
+// points (linear.hip) and the kernels that go by chunks (linear_chunk_kernels.hpp).
 #pragma once
 
 #include "recurrent.hpp"
@@ -60,8 +60,9 @@ struct ChunkParams {
     float *seg_decays;  // [requests][segs][heads]
 };
 
-// Both launches of a call by chunks (the second only where the first was made), and
-// the loading of their code object, for rows of each type.
+// The launches of a call by chunks, each only where the one before was made (prepare and
+// walk; in segments also the scan and a second walk), and the loading of their code
+// object, for rows of each type.
 void launch_linear_chunks_f32(hipStream_t stream, const ChunkParams &p);
 void launch_linear_chunks_f16(hipStream_t stream, const ChunkParams &p);
 void launch_linear_chunks_bf16(hipStream_t stream, const ChunkParams &p);

@@ -279,9 +279,9 @@ __device__ inline float exp_diff(double x) {
 // 8, and then makes its column of blocks downwards by products.  Three workgroups share a
 // compute unit (35 KB of LDS, 168 registers; four would spill: 520 us for 405 of the
 // second call below). Bound by its chain of steps between barriers: waves wait half their
-// time, vector instructions take 40 %, matrix units 11 % of the busy cycles. 8192 tokens
-// of one bf16 request, 48 heads of 128 x 128: 87 us; eight of up to 4096 tokens, 32
-// heads: 140-148 us, 390 MB written.
+// time, vector instructions take 41 %, matrix units 10 % of the busy cycles. 8192 tokens
+// of one bf16 request, 48 heads of 128 x 128: 91-93 us; eight of up to 4096 tokens, 32
+// heads: 143-157 us, 408 MB written.
 template <typename T, int DK, bool DELTA>
 __global__ __launch_bounds__(kPrepThreads, DK <= 128 ? 3 : 1) void linear_prepare_kernel(const ChunkParams p,
                                                                                          const uint32_t heads) {
@@ -376,7 +376,7 @@ __global__ __launch_bounds__(kPrepThreads, DK <= 128 ? 3 : 1) void linear_prepar
             kk[j][r] = __builtin_amdgcn_ldexpf(kk[j][r], 2 * exp_k);
             qk[j][r] = __builtin_amdgcn_ldexpf(qk[j][r], exp_k + exp_q) * p.a.scale;
         }
-        __builtin_amdgcn_sched_barrier(0);  // a tile's operands at a time: registers for four waves a SIMD
+        __builtin_amdgcn_sched_barrier(0);  // a tile's operands at a time, to keep to the registers of three workgroups
     }
     float *tri_a = reinterpret_cast<float *>(lds);
     float *tri_t = tri_a + kChunk * kTriPitch;
@@ -815,7 +815,7 @@ static __global__ __launch_bounds__(kScanThreads) void linear_scan_kernel(const 
 
 // The request that the workgroups of `rank` take: the longest ones first, so that the
 // last to end are short (eight bf16 prompts of up to 4096 tokens, 32 heads of 128 x 128:
-// 378 us, 409 in their own order).  Beyond a wave's lanes of requests, in their own order.
+// 375-390 us, 430 in their own order).  Beyond a wave's lanes of requests, in their own order.
 __device__ inline uint32_t request_by_length(const LinearParams &a, uint32_t rank) {
     if (a.n_seq == 1 || a.n_seq > 64) {
         return rank;
@@ -835,10 +835,10 @@ __device__ inline uint32_t request_by_length(const LinearParams &a, uint32_t ran
 // computing ones a third of a chunk's time (8192 tokens, 48 heads of 128 x 128: 728 us
 // with loads of their own, 493 with these waves, at that step).
 //
-// Bound by one wave's instructions: a chunk of 128 x 128 takes it 104 matrix
-// instructions (1660 cycles) and 650 vector ones (2600), of which little overlaps, as
-// each product waits for the one before, 6400 cycles = 2.8 us in all.  8192 tokens take
-// 128 of these, one behind the other: 362-373 us on 96 compute units (a column of the
+// Bound by one wave's instructions: a chunk of 128 x 128 takes it 132 matrix
+// instructions (2110 cycles) and 690 vector ones (2750), of which little overlaps, as
+// each product waits for the one before, 7000 cycles = 3.1 us in all.  8192 tokens take
+// 128 of these, one behind the other: 401-417 us on 96 compute units (a column of the
 // state needs the whole chunk before it), 48 heads of 128 x 128.
 template <typename T, int DK, bool DELTA, bool OUT, int WAVES>
 __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const ChunkParams p) {
@@ -1276,8 +1276,8 @@ __global__ __launch_bounds__(128 * WAVES, 1) void linear_walk_kernel(const Chunk
 
 // A workgroup takes a chunk of one key head for all its heads where those fill the
 // CUs twice, else for one head.  48 heads of 16 key heads, the whole call: 1024 tokens
-// (256 chunks of key heads) 72.8 us together and 69.3 alone, 2048 tokens 120.6 and 125.3,
-// 8192 tokens 445.2 and 460.1.
+// (256 chunks of key heads) 79.8 us together and 75.4 alone, 2048 tokens 132 and 136,
+// 8192 tokens 486 and 502.
 constexpr uint32_t kPrepFull = 512;
 
 template <typename T, int DK>
@@ -1294,9 +1294,8 @@ static void prepare(hipStream_t stream, const ChunkParams &p) {
 
 // 64 columns a workgroup where a head has them and two chunks of that width fit into
 // LDS, else 32.  A chunk takes a wave the same time either way (one request of 8192
-// tokens, 48 heads of 128 x 128: 446 us, 443 by 32), and wide workgroups read the
-// operands half as often (eight of up to 4096 tokens, 32 heads, at an earlier step: 397
-// us, 553 by 32).
+// tokens, 48 heads of 128 x 128: 486 us, 485 by 32), and wide workgroups read the
+// operands half as often (eight of up to 4096 tokens, 32 heads: 385 us, 583 by 32).
 template <typename T, int DK, bool DELTA, bool OUT>
 static void walk_cols(hipStream_t stream, const ChunkParams &p) {
     constexpr bool wide = ChunkSpace<T, DK, DELTA, OUT, 4>::places == 2;

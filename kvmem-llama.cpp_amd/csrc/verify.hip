@@ -3,15 +3,15 @@
 // the next token is drawn from max(p - q, 0) at the first refusal, else from the
 // last row's p.
 //
-// Every logit is read once:
 //   parts    a workgroup per 2048 ids of a row: their maximum (with its lowest id) and
-//            the sum of exponentials relative to it
+//            the sum of exponentials relative to it: every logit, once
 //   decide   a workgroup per request: joins its rows' parts, tests its drafts in
 //            order, and draws the next token wherever p alone decides it, from the
-//            part sums first and then inside the one part that holds the border
+//            part sums first and then inside the one part that holds the border (read
+//            again, as are the drafts' logits and the part of a draft left out)
 //   rest     where a refused draft had probabilities, the parts' sums of
-//            max(p - q, 0), and
-//   draw     the draw from those
+//            max(p - q, 0): its row's logits again, and
+//   draw     the draw from those (the border's part once more)
 // Exponentials and sums are fp64: a draw compares a running sum with u times the
 // total, and of 10^5 ids' borders fp32 sums would misplace one in a few hundred
 // draws; a relative error of 10^-13, one in 10^7.
@@ -28,7 +28,7 @@ constexpr uint32_t kVerifyThreads = 256;
 constexpr uint32_t kVerifyMaxDraft = 127;
 constexpr uint32_t kPartIds = 8 * kVerifyThreads;
 // Parts from which a wave takes a whole one.  Rows of 152000 ids, by four waves / by one:
-// 64 rows (4800 parts) 26.0 / 25.4 us, 32 rows 21.6 / 21.9, 8 rows 16.8 / 18.3.
+// 64 rows (4800 parts) 25.8 / 25.3 us, 32 rows 21.5 / 21.9, 8 rows 16.6 / 18.2.
 constexpr uint64_t kManyParts = 4096;
 constexpr uint32_t kVerifyMaxVocab = 1u << 24;
 
@@ -233,11 +233,11 @@ __device__ inline void load_part(const uint8_t *row, uint32_t first, uint32_t en
 }
 
 // A thread has GROUPS groups of eight ids.  Each wave sums relative to its own maximum,
-// and the first joins them.  Bound by vector instructions, twelve fp64 ones and two more
+// and the first joins them.  Bound by vector instructions, thirteen fp64 ones and two more
 // an id and some ninety a wave to combine its lanes: with four groups a wave takes the
 // whole part and combines a quarter as often.  512 rows of 152000 bf16 ids, the whole
-// call: 78.3 us with one group, 71.7 with two, 67.9 with four (this kernel 49 us, 3.2
-// TB/s); 8 rows of 32000 ids: 13.1, 13.8, 16.4.
+// call: 80.1 us with one group, 73.6 with two, 68.0 with four (this kernel 49 us, 3.2
+// TB/s); 8 rows of 32000 ids: 14.1, 14.9, 15.7.
 template <typename T, int GROUPS>
 __global__ __launch_bounds__(kVerifyThreads / GROUPS) void verify_parts_kernel(const VerifyParams p) {
     constexpr uint32_t waves = 4 / GROUPS, threads = kVerifyThreads / GROUPS;
